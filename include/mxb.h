@@ -53,6 +53,10 @@ extern "C" {
 #define MXB_MODE_PARITY 0 /* fp32-faithful: |y - y_ref| <= 1e-5 * (|x| @ |W|) */
 #define MXB_MODE_FAST 1   /* weights rounded to bf16 once: ~4e-3 relative per weight */
 
+/* microscaled 4-bit formats (E2M1 codes) */
+#define MXB_FP4_MX 0 /* mxfp4: blocks of 32, E8M0 scales */
+#define MXB_FP4_NV 1 /* nvfp4: blocks of 16, E4M3 scales and one fp32 factor a tensor */
+
 /* Library version (major * 10000 + minor * 100 + patch). */
 int mxb_version(void);
 
@@ -368,6 +372,55 @@ int mxb_linear_wonly_kmajor(const void* x, int x_dtype, int64_t M, int64_t K,
 int mxb_linear_wonly_noalloc(const void* x, int x_dtype, int64_t M, int64_t K,
                              const void* w_packed, const float* w_scales, int64_t N, int bits,
                              int kind, int block, float* y, void* stream);
+
+/*
+ * Microscaled 4-bit floating point (no counterpart in the reference, whose
+ * float4 codes index a normalised grid under fp32 scales).  A matrix
+ * [rows, K] is stored as
+ *   codes   rows of ceil(K / 32) * 16 bytes, E2M1 bit patterns two a byte, low
+ *           first (0, .5, 1, 1.5, 2, 3, 4, 6; bit 3 the sign), zero past K;
+ *   scales  tiles of 128 rows x 4 blocks, tiles row-major, byte
+ *           ((r % 32) * 4 + r / 32) * 4 + c of a tile, zero past the matrix:
+ *           mxb_fp4_scale_bytes(rows, K, fmt) bytes, as the tensor cores
+ *           read them;
+ *   g       nvfp4 only: one fp32 factor.
+ * Value = code * scale (* g).
+ */
+size_t mxb_fp4_code_bytes(int64_t rows, int64_t K);
+size_t mxb_fp4_scale_bytes(int64_t rows, int64_t K, int fmt);
+
+/* Workspace bytes for mxb_fp4_quantize (0 unless derive is set). */
+size_t mxb_fp4_quantize_workspace_size(int64_t rows, int64_t K, int fmt, int derive);
+
+/*
+ * Quantize x [rows, K] (row stride ldx elements, x_dtype MXB_F32 / MXB_BF16).
+ *   mxfp4: scale 2^e, e = floor(log2(amax)) - 2 clamped to [-127, 127];
+ *   nvfp4: scale = e4m3(min(fl(amax / fl(6 g)), 448)); g is read from the
+ *     device word `global_scale`, or with derive != 0 computed first as
+ *     fl(amax(x) * fl(1 / 2688)) (1 where that amax is 0 or not finite) and written
+ *     there.
+ * Codes are x / scale rounded to the nearest E2M1 value, ties to even,
+ * saturating at 6.  A block with an infinity or NaN gets the NaN scale
+ * (0xFF / 0x7F) and zero codes.
+ */
+int mxb_fp4_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t ldx, int fmt,
+                     float* global_scale, int derive, void* codes, void* scales, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* out [rows, K] (contiguous, out_dtype MXB_F32 / MXB_BF16) = fl(code * fl(scale * g)). */
+int mxb_fp4_dequantize(const void* codes, const void* scales, const float* global_scale,
+                       int64_t rows, int64_t K, int fmt, void* out, int out_dtype, void* stream);
+
+/*
+ * C [M, N] = A [M, K] B [N, K]^T (+ bias [N], fp32, may be NULL), both operands
+ * in one format, fp32 accumulation on the block-scaled tcgen05 kinds,
+ * C (contiguous) rounded once to out_dtype.  a_global / b_global: the device
+ * words of nvfp4 operands (NULL for mxfp4).  codes and scales 16-byte aligned.
+ */
+int mxb_fp4_matmul(const void* a_codes, const void* a_scales, const float* a_global,
+                   const void* b_codes, const void* b_scales, const float* b_global, int64_t M,
+                   int64_t K, int64_t N, int fmt, const float* bias, void* out, int out_dtype,
+                   void* stream);
 
 #ifdef __cplusplus
 }

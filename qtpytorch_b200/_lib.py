@@ -28,6 +28,7 @@ F32, BF16 = 0, 1
 KIND_INT, KIND_FLOAT = 0, 1
 VAR_BASE, VAR_H = 0, 1
 MODE_PARITY, MODE_FAST = 0, 1
+FP4_MX, FP4_NV = 0, 1
 
 _i64, _int, _sz, _vp = C.c_int64, C.c_int, C.c_size_t, C.c_void_p
 
@@ -70,6 +71,14 @@ PROTOTYPES = {
     "mxb_hadamard_cross": (_int, [_vp, _i64, _i64, _int, _vp, _vp, _vp]),
     "mxb_linear_wonly_kmajor": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _i64, _int, _int, _int,
                                        _int, _vp, _vp]),
+    "mxb_fp4_code_bytes": (_sz, [_i64, _i64]),
+    "mxb_fp4_scale_bytes": (_sz, [_i64, _i64, _int]),
+    "mxb_fp4_quantize_workspace_size": (_sz, [_i64, _i64, _int, _int]),
+    "mxb_fp4_quantize": (_int, [_vp, _int, _i64, _i64, _i64, _int, _vp, _int, _vp, _vp, _vp, _sz,
+                                _vp]),
+    "mxb_fp4_dequantize": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _vp]),
+    "mxb_fp4_matmul": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _int,
+                              _vp]),
 }
 
 _lib = None

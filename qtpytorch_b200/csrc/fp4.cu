@@ -1,0 +1,393 @@
+// Microscaled 4-bit floating point: quantize, dequantize and the per-tensor
+// factor (mxfp4: E8M0 scales of 32 elements; nvfp4: E4M3 scales of 16 and one
+// fp32 factor g).  Layout and formulas: include/mxb.h.
+//
+// All three are one pass over HBM: a thread owns 16 consecutive elements of a
+// row (an nvfp4 block, half an mxfp4 block), so the block maximum costs no
+// shuffle (nvfp4) or one (mxfp4), the codes leave as one 8-byte store and the
+// scales of four blocks as one 32-bit store in the tensor-core tile order.
+#include "mxb_common.cuh"
+#include "mxb_internal.h"
+
+#include <cuda_fp16.h>
+
+using namespace mxb;
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kE = 16;  // elements per thread (quantize)
+
+__host__ __device__ inline int64_t fp4_blocks(int64_t K, int fmt) {
+  return fmt == MXB_FP4_NV ? cdiv(K, 16) : cdiv(K, 32);
+}
+__host__ __device__ inline int64_t fp4_row_bytes(int64_t K) { return cdiv(K, 32) * 16; }
+
+// byte offset of the first of the four scales (r, 4 * cg .. 4 * cg + 3)
+__device__ __forceinline__ size_t sf_offset(int64_t r, int64_t cg, int64_t groups) {
+  return ((size_t)(r >> 7) * groups + cg) * 512 + (size_t)(r & 31) * 16 + (size_t)((r >> 5) & 3) * 4;
+}
+
+// Eight floats -> eight E2M1 codes (round to nearest even, saturating), first
+// in the low nibble.
+__device__ __forceinline__ uint32_t e2m1x8(const float* q) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(w)
+      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
+  return w;
+}
+
+__device__ __forceinline__ uint32_t e4m3_of(float v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.0f), "f"(v));
+  return r & 0xFFu;
+}
+__device__ __forceinline__ float e4m3_value(uint32_t b) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)b));
+  return __half2float(__ushort_as_half((unsigned short)(h & 0xFFFFu)));
+}
+__device__ __forceinline__ float e8m0_value(uint32_t b) {
+  // 2^(b - 127); b = 0 is the subnormal 2^-127, 0xFF is NaN
+  return __uint_as_float(b == 0u ? 0x00400000u : b == 255u ? 0x7FC00000u : b << 23);
+}
+
+// The tensor's factor from its largest magnitude: amax * fl(1 / 2688), so
+// that the largest block's scale is e4m3's 448.
+__device__ __forceinline__ float factor_of(float amax) {
+  return (amax > 0.0f && amax <= 3.4028235e38f) ? __fmul_rn(amax, 1.0f / 2688.0f) : 1.0f;
+}
+
+// Up to 16 elements of a row from column c0 on; zero past K.
+template <typename InT>
+__device__ __forceinline__ void load16(const InT* __restrict__ row, int64_t c0, int64_t K, bool vec,
+                                       float (&v)[kE]) {
+  if (vec && c0 + kE <= K) {
+    if (sizeof(InT) == 4) {
+      const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + c0);
+      float4 t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = __ldg(p + i);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[4 * i] = t[i].x; v[4 * i + 1] = t[i].y; v[4 * i + 2] = t[i].z; v[4 * i + 3] = t[i].w;
+      }
+    } else {
+      const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(row) + c0);
+      const uint4 a = __ldg(p), b = __ldg(p + 1);
+      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kE; ++i) v[i] = c0 + i < K ? load_as_f32(row, c0 + i) : 0.0f;
+  }
+}
+
+// Largest |x| of the tensor as the bits of a non-negative float (which order
+// as integers, NaN last): the maximum does not depend on the order of the
+// atomics.
+template <typename InT>
+__global__ void __launch_bounds__(kThreads) fp4_amax_kernel(const InT* __restrict__ x, uint32_t rows,
+                                                            int64_t K, int64_t ldx, uint32_t gpr,
+                                                            uint32_t items, bool vec,
+                                                            uint32_t* __restrict__ out) {
+  float a = 0.0f;
+  for (uint64_t i = blockIdx.x * (uint64_t)kThreads + threadIdx.x; i < items;
+       i += (uint64_t)gridDim.x * kThreads) {
+    const uint32_t r = (uint32_t)i / gpr, c = (uint32_t)i - r * gpr;
+    float v[kE];
+    load16(x + (int64_t)r * ldx, (int64_t)c * kE, K, vec, v);
+#pragma unroll
+    for (int j = 0; j < kE; ++j) a = amax_step(a, v[j]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a = nan_max(a, __shfl_xor_sync(0xffffffffu, a, o));
+  __shared__ float s[kThreads / 32];
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = a;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < kThreads / 32; ++w) a = nan_max(a, s[w]);
+    atomicMax(out, __float_as_uint(a) & 0x7FFFFFFFu);
+  }
+}
+
+// gpr: 16-element groups per row, covering whole tiles of four scales;
+// items: rows * gpr groups, then one 32-bit word per four scales of each
+// padding row.  amax_bits: the tensor's maximum (derive), else null.
+template <typename InT, int FMT>
+__global__ void __launch_bounds__(kThreads)
+    fp4_quant_kernel(const InT* __restrict__ x, uint32_t rows, int64_t K, int64_t ldx, uint32_t gpr,
+                     uint32_t items, uint32_t pad_words, uint32_t groups, bool vec,
+                     const uint32_t* __restrict__ amax_bits, float* __restrict__ gscale,
+                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  const uint64_t i = blockIdx.x * (uint64_t)kThreads + threadIdx.x;
+  const bool mine = i < items;
+  if (!mine && i - items < pad_words) {
+    const uint32_t w = (uint32_t)(i - items);
+    const uint32_t r = rows + w / groups;
+    *reinterpret_cast<uint32_t*>(scales + sf_offset(r, w % groups, groups)) = 0u;
+  }
+  float g = 1.0f;
+  if (FMT == MXB_FP4_NV) {
+    if (amax_bits) {
+      g = factor_of(__uint_as_float(*amax_bits));
+      if (i == 0) *gscale = g;
+    } else {
+      g = *gscale;
+    }
+  }
+  const uint32_t r = mine ? (uint32_t)i / gpr : 0u, c = mine ? (uint32_t)i - r * gpr : 0u;
+  float v[kE];
+  if (mine) {
+    load16(x + (int64_t)r * ldx, (int64_t)c * kE, K, vec, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kE; ++j) v[j] = 0.0f;
+  }
+  float a = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kE; ++j) a = amax_step(a, v[j]);
+  if (FMT == MXB_FP4_MX) a = nan_max(a, __shfl_xor_sync(0xffffffffu, a, 1));
+  const bool finite = a <= 3.4028235e38f;
+  uint32_t sb;
+  float q[kE];
+  if (FMT == MXB_FP4_MX) {
+    // floor(log2(a)) is the exponent field; subnormals fall under the clamp
+    sb = (uint32_t)max((int)(__float_as_uint(a) >> 23) - 2, 0);
+    const float inv = __uint_as_float((254u - sb) << 23);  // exact: a power of two
+#pragma unroll
+    for (int j = 0; j < kE; ++j) q[j] = __fmul_rn(v[j], inv);
+    if (!finite) sb = 255u;
+  } else {
+    sb = e4m3_of(fminf(__fdiv_rn(a, __fmul_rn(6.0f, g)), 448.0f));
+    const float s = __fmul_rn(e4m3_value(sb), g);
+    if (s >= 7.9e-31f && s <= 1.2e30f) {
+      // x / s by Markstein's corrected product (r correctly rounded, the
+      // residual exact in an FMA): three operations instead of a division
+      const float rs = __frcp_rn(s);
+#pragma unroll
+      for (int j = 0; j < kE; ++j) {
+        const float q0 = __fmul_rn(v[j], rs);
+        q[j] = __fmaf_rn(__fmaf_rn(-q0, s, v[j]), rs, q0);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kE; ++j) q[j] = s > 0.0f ? __fdiv_rn(v[j], s) : __fmul_rn(v[j], 0.0f);
+    }
+    if (!finite) sb = 0x7Fu;
+  }
+  uint2 w = make_uint2(e2m1x8(q), e2m1x8(q + 8));
+  if (!finite) w = make_uint2(0u, 0u);
+  if (mine && (int64_t)c * 8 < fp4_row_bytes(K))
+    *reinterpret_cast<uint2*>(codes + (size_t)r * fp4_row_bytes(K) + (size_t)c * 8) = w;
+  // four scales -> one word.  A group of four blocks starts at a multiple of
+  // 8 (mxfp4) or 4 (nvfp4) items, and gpr is a multiple of that, so its lanes
+  // sit in one warp and one row.
+  constexpr int L = FMT == MXB_FP4_MX ? 2 : 1;
+  if ((int64_t)c * kE >= K) sb = 0u;  // blocks past the row
+  uint32_t word = sb;
+  word |= __shfl_down_sync(0xffffffffu, word, L) << 8;
+  word |= __shfl_down_sync(0xffffffffu, word, 2 * L) << 16;
+  if (mine && (c & (4 * L - 1)) == 0)
+    *reinterpret_cast<uint32_t*>(scales + sf_offset(r, c / (4 * L), groups)) = word;
+}
+
+// Two E2M1 codes (one byte) -> two floats.
+__device__ __forceinline__ float2 e2m1x2_value(uint32_t byte) {
+  uint32_t h;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}"
+      : "=r"(h)
+      : "r"(byte));
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
+}
+
+// A thread writes 16 bytes of output (4 fp32 or 8 bf16), so a warp's stores
+// are whole 512-byte runs; kU of them in flight.
+template <typename OutT, int FMT>
+__global__ void __launch_bounds__(kThreads)
+    fp4_dequant_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                       const float* __restrict__ gscale, uint32_t rows, int64_t K, uint32_t cpr,
+                       uint64_t items, uint32_t groups, bool vec, OutT* __restrict__ out) {
+  constexpr int E = 16 / sizeof(OutT), kU = 4;
+  constexpr int kBlk = FMT == MXB_FP4_NV ? 16 : 32;
+  const float g = FMT == MXB_FP4_NV ? *gscale : 1.0f;
+  const int64_t rb = fp4_row_bytes(K);
+  const uint64_t i0 = blockIdx.x * (uint64_t)(kThreads * kU) + threadIdx.x;
+  uint32_t w[kU], sb[kU], rr[kU], cc[kU];
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const uint64_t i = i0 + (uint64_t)u * kThreads;
+    w[u] = sb[u] = rr[u] = cc[u] = 0u;
+    if (i < items) {
+      const uint32_t r = (uint32_t)(i / cpr), c = (uint32_t)(i - (uint64_t)r * cpr);
+      const uint8_t* p = codes + (size_t)r * rb + (size_t)c * (E / 2);
+      w[u] = E == 8 ? __ldg(reinterpret_cast<const uint32_t*>(p))
+                    : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p));
+      const uint32_t blk = (c * E) / kBlk;
+      sb[u] = __ldg(scales + sf_offset(r, blk >> 2, groups) + (blk & 3));
+      rr[u] = r;
+      cc[u] = c;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const uint64_t i = i0 + (uint64_t)u * kThreads;
+    if (i >= items) continue;
+    const float s = FMT == MXB_FP4_NV ? __fmul_rn(e4m3_value(sb[u]), g) : e8m0_value(sb[u]);
+    float v[E];
+#pragma unroll
+    for (int j = 0; j < E / 2; ++j) {
+      const float2 t = e2m1x2_value((w[u] >> (8 * j)) & 0xFFu);
+      v[2 * j] = __fmul_rn(t.x, s);
+      v[2 * j + 1] = __fmul_rn(t.y, s);
+    }
+    const int64_t c0 = (int64_t)cc[u] * E;
+    OutT* o = out + (int64_t)rr[u] * K + c0;
+    if (sizeof(OutT) == 4) {
+      float* of = reinterpret_cast<float*>(o);
+      if (vec) {
+        __stcs(reinterpret_cast<float4*>(of), make_float4(v[0], v[1], v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (c0 + j < K) of[j] = v[j];
+      }
+    } else {
+      __nv_bfloat16* ob = reinterpret_cast<__nv_bfloat16*>(o);
+      if (vec) {
+        uint32_t p[E / 2];
+#pragma unroll
+        for (int j = 0; j < E / 2; ++j) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          p[j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        __stcs(reinterpret_cast<uint4*>(ob), make_uint4(p[0], p[1], p[2 % (E / 2)], p[3 % (E / 2)]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (c0 + j < K) ob[j] = __float2bfloat16_rn(v[j]);
+      }
+    }
+  }
+}
+
+template <typename InT>
+int quantize_t(const InT* x, int64_t rows, int64_t K, int64_t ldx, int fmt, float* g, int derive,
+               uint8_t* codes, uint8_t* scales, uint32_t* ws, cudaStream_t st) {
+  const int64_t groups = cdiv(fp4_blocks(K, fmt), 4);
+  const int64_t gpr = groups * (fmt == MXB_FP4_NV ? 4 : 8);
+  const int64_t items = rows * gpr, pad = (cdiv(rows, 128) * 128 - rows) * groups;
+  if (items + pad >= (int64_t)1 << 32) return MXB_E_SHAPE;
+  const bool vec = ((uintptr_t)x % 16) == 0 && (ldx * (int64_t)sizeof(InT)) % 16 == 0;
+  if (derive) {
+    MXB_CUDA_TRY(cudaMemsetAsync(ws, 0, sizeof(uint32_t), st));
+    const int64_t agpr = cdiv(K, kE), aitems = rows * agpr;
+    const int64_t blocks = cdiv(aitems, kThreads);
+    fp4_amax_kernel<InT><<<(unsigned)(blocks < 8 * kSMs ? blocks : 8 * kSMs), kThreads, 0, st>>>(
+        x, (uint32_t)rows, K, ldx, (uint32_t)agpr, (uint32_t)aitems, vec, ws);
+    MXB_LAUNCH_CHECK();
+  }
+  const unsigned grid = (unsigned)cdiv(items + pad, kThreads);
+  const uint32_t* am = derive ? ws : nullptr;
+  if (fmt == MXB_FP4_NV)
+    fp4_quant_kernel<InT, MXB_FP4_NV><<<grid, kThreads, 0, st>>>(
+        x, (uint32_t)rows, K, ldx, (uint32_t)gpr, (uint32_t)items, (uint32_t)pad, (uint32_t)groups,
+        vec, am, g, codes, scales);
+  else
+    fp4_quant_kernel<InT, MXB_FP4_MX><<<grid, kThreads, 0, st>>>(
+        x, (uint32_t)rows, K, ldx, (uint32_t)gpr, (uint32_t)items, (uint32_t)pad, (uint32_t)groups,
+        vec, nullptr, nullptr, codes, scales);
+  MXB_LAUNCH_CHECK();
+  return MXB_OK;
+}
+
+template <typename OutT>
+int dequantize_t(const uint8_t* codes, const uint8_t* scales, const float* g, int64_t rows,
+                 int64_t K, int fmt, OutT* out, cudaStream_t st) {
+  constexpr int E = 16 / sizeof(OutT);
+  const int64_t cpr = cdiv(K, E), items = rows * cpr;
+  const int64_t groups = cdiv(fp4_blocks(K, fmt), 4);
+  const int64_t grid = cdiv(items, 4 * kThreads);
+  if (rows >= (int64_t)1 << 32 || K >= (int64_t)1 << 31 || grid >= (int64_t)1 << 31)
+    return MXB_E_SHAPE;
+  const bool vec = K % E == 0 && ((uintptr_t)out % 16) == 0;
+  if (fmt == MXB_FP4_NV)
+    fp4_dequant_kernel<OutT, MXB_FP4_NV><<<(unsigned)grid, kThreads, 0, st>>>(
+        codes, scales, g, (uint32_t)rows, K, (uint32_t)cpr, (uint64_t)items, (uint32_t)groups, vec, out);
+  else
+    fp4_dequant_kernel<OutT, MXB_FP4_MX><<<(unsigned)grid, kThreads, 0, st>>>(
+        codes, scales, g, (uint32_t)rows, K, (uint32_t)cpr, (uint64_t)items, (uint32_t)groups, vec, out);
+  MXB_LAUNCH_CHECK();
+  return MXB_OK;
+}
+
+bool fmt_ok(int fmt) { return fmt == MXB_FP4_MX || fmt == MXB_FP4_NV; }
+bool io_ok(int dt) { return dt == MXB_F32 || dt == MXB_BF16; }
+
+}  // namespace
+
+extern "C" {
+
+size_t mxb_fp4_code_bytes(int64_t rows, int64_t K) {
+  return rows <= 0 || K <= 0 ? 0 : (size_t)rows * (size_t)fp4_row_bytes(K);
+}
+
+size_t mxb_fp4_scale_bytes(int64_t rows, int64_t K, int fmt) {
+  if (rows <= 0 || K <= 0 || !fmt_ok(fmt)) return 0;
+  return (size_t)cdiv(rows, 128) * (size_t)cdiv(fp4_blocks(K, fmt), 4) * 512;
+}
+
+size_t mxb_fp4_quantize_workspace_size(int64_t rows, int64_t K, int fmt, int derive) {
+  return rows > 0 && K > 0 && fmt == MXB_FP4_NV && derive ? 16 : 0;
+}
+
+int mxb_fp4_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t ldx, int fmt,
+                     float* global_scale, int derive, void* codes, void* scales, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  if (!fmt_ok(fmt) || !io_ok(x_dtype)) return MXB_E_DTYPE;
+  if (rows < 0 || K < 0 || (rows > 1 && ldx < K)) return MXB_E_SHAPE;
+  if (rows == 0 || K == 0) return MXB_OK;
+  if (!x || !codes || !scales || (fmt == MXB_FP4_NV) != (global_scale != nullptr)) return MXB_E_ARG;
+  if ((uintptr_t)codes % 16 || (uintptr_t)scales % 16) return MXB_E_ALIGN;
+  const bool d = fmt == MXB_FP4_NV && derive != 0;
+  if (d && (!workspace || workspace_bytes < mxb_fp4_quantize_workspace_size(rows, K, fmt, 1)))
+    return MXB_E_WORKSPACE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint32_t* ws = static_cast<uint32_t*>(workspace);
+  uint8_t* c = static_cast<uint8_t*>(codes);
+  uint8_t* s = static_cast<uint8_t*>(scales);
+  if (x_dtype == MXB_BF16)
+    return quantize_t(static_cast<const __nv_bfloat16*>(x), rows, K, ldx, fmt, global_scale, d, c, s,
+                      ws, st);
+  return quantize_t(static_cast<const float*>(x), rows, K, ldx, fmt, global_scale, d, c, s, ws, st);
+}
+
+int mxb_fp4_dequantize(const void* codes, const void* scales, const float* global_scale,
+                       int64_t rows, int64_t K, int fmt, void* out, int out_dtype, void* stream) {
+  if (!fmt_ok(fmt) || !io_ok(out_dtype)) return MXB_E_DTYPE;
+  if (rows < 0 || K < 0) return MXB_E_SHAPE;
+  if (rows == 0 || K == 0) return MXB_OK;
+  if (!codes || !scales || !out || (fmt == MXB_FP4_NV) != (global_scale != nullptr))
+    return MXB_E_ARG;
+  if ((uintptr_t)codes % 16 || (uintptr_t)scales % 16) return MXB_E_ALIGN;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const uint8_t* c = static_cast<const uint8_t*>(codes);
+  const uint8_t* s = static_cast<const uint8_t*>(scales);
+  if (out_dtype == MXB_BF16)
+    return dequantize_t(c, s, global_scale, rows, K, fmt, static_cast<__nv_bfloat16*>(out), st);
+  return dequantize_t(c, s, global_scale, rows, K, fmt, static_cast<float*>(out), st);
+}
+
+}  // extern "C"

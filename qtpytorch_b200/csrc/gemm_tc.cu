@@ -473,6 +473,13 @@ int make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dt, uint32_t esize, const
   return r == CUDA_SUCCESS ? MXB_OK : MXB_E_CUDA;
 }
 
+bool encode_tmap_2d(void* map, int dtype, uint32_t esize, const void* base, uint64_t cols,
+                    uint64_t rows, uint32_t box_cols, uint32_t box_rows, int swizzle) {
+  return make_tmap_2d(static_cast<CUtensorMap*>(map), static_cast<CUtensorMapDataType>(dtype),
+                      esize, base, cols, rows, box_cols, box_rows,
+                      static_cast<CUtensorMapSwizzle>(swizzle)) == MXB_OK;
+}
+
 int make_tmap_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
                  uint32_t box_cols, uint32_t box_rows) {
   return make_tmap_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, cols, rows, box_cols, box_rows,

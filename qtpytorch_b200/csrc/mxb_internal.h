@@ -69,6 +69,10 @@ int peer_barrier(unsigned long long* const* sync, int nranks, int rank, cudaStre
 // rank's call counter, [8 + r] the call counter rank r last signalled to
 // this rank.
 constexpr int kSyncWords = 16;
+// 2-D row-major matrix [rows][cols] of esize-byte elements -> tensor map
+// (dtype / swizzle: CUtensorMapDataType / CUtensorMapSwizzle values).
+bool encode_tmap_2d(void* map, int dtype, uint32_t esize, const void* base, uint64_t cols,
+                    uint64_t rows, uint32_t box_cols, uint32_t box_rows, int swizzle);
 bool tc_qgemm_eligible(int64_t M, int64_t K, int64_t N, int bits, int block, bool sa_ok,
                        bool sb_ok, const void* a, const void* b, const float* c);
 size_t tc_qgemm_workspace(int64_t M, int64_t K, int64_t N, int bits);

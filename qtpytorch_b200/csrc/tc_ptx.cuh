@@ -11,9 +11,11 @@
 
 namespace mxb {
 
-// The including translation unit defines the device-side error word
-// `__device__ int g_mxb_device_error` (0 = ok) before including this header;
-// mxb_device_error() reads and clears it.
+// gemm_tc.cu defines the device-side error word `__device__ int
+// g_mxb_device_error` (0 = ok) before including this header and uses mbar_wait;
+// mxb_device_error() reads and clears it.  Other translation units define
+// MXB_ERROR_WORD_BY_POINTER, get the word's address from device_error_ptr()
+// and pass it to mbar_wait_to.
 
 constexpr uint32_t kSpinLimit = 1u << 24;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s
@@ -26,6 +28,7 @@ enum DeviceError : int {
   kErrTimeoutDone = 5,
   kErrTimeoutPeer = 6,  // a peer rank never signalled the cross-rank barrier
   kErrTimeoutRowLoad = 7,  // a row's bulk copy into shared memory never completed (row transforms)
+  kErrIndex = 8,  // a slot or page number outside the paged cache (the access was skipped)
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -86,25 +89,36 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
 }
 
 // Bounded wait for the phase with the given parity to complete: gives up
-// after kWaitLimitNs of wall time (or kSpinLimit polls), records err_code and
-// returns false.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int err_code) {
+// after kWaitLimitNs of wall time (or kSpinLimit polls), records err_code in
+// *err and returns false.
+__device__ __forceinline__ bool mbar_wait_to(uint64_t* bar, uint32_t parity, int err_code,
+                                             int* err) {
   if (mbar_test_wait(bar, parity)) return true;  // already complete: no blocking probe
   const uint64_t t0 = globaltimer_ns();
   for (uint32_t i = 0; i < kSpinLimit; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((i & 15) == 15 && globaltimer_ns() - t0 > kWaitLimitNs) break;
   }
-  atomicCAS(&g_mxb_device_error, 0, err_code);
+  if (err) atomicCAS(err, 0, err_code);
   return false;
 }
 
 // Warp-uniform bounded wait: every lane polls; the warp proceeds only if all
 // lanes saw the phase complete, so `.aligned` tcgen05 ops stay converged.
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int err_code) {
-  bool ok = mbar_wait(bar, parity, err_code);
+__device__ __forceinline__ bool mbar_wait_warp_to(uint64_t* bar, uint32_t parity, int err_code,
+                                                  int* err) {
+  bool ok = mbar_wait_to(bar, parity, err_code, err);
   return __all_sync(0xffffffffu, ok);
 }
+
+#ifndef MXB_ERROR_WORD_BY_POINTER
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int err_code) {
+  return mbar_wait_to(bar, parity, err_code, &g_mxb_device_error);
+}
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int err_code) {
+  return mbar_wait_warp_to(bar, parity, err_code, &g_mxb_device_error);
+}
+#endif
 
 // 2-D tiled TMA load global -> shared, completion on `bar` (no multicast).
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar,
@@ -113,6 +127,17 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
       "[%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
+
+// Untiled bulk copy global -> shared, completion on `bar` (no multicast): both
+// addresses 16-byte aligned, bytes a multiple of 16.
+__device__ __forceinline__ void bulk_load_g2s(void* dst, const void* src, uint32_t bytes,
+                                              uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
 }
 
@@ -193,6 +218,39 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_
       : "memory");
 }
 
+// Block-scaled 4-bit products (E2M1 x E2M1, K = 64 a call): D[tmem] (+)=
+// (A * SFA) * (B * SFB), the scale factors read from TMEM at sfa / sfb.
+// kind::mxf4: one E8M0 scale per 32 elements; kind::mxf4nvf4 with 4X: one
+// E4M3 scale per 16.
+template <bool NV>
+__device__ __forceinline__ void mma_fp4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                        uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                        uint32_t accumulate) {
+  if constexpr (NV) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X "
+        "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X "
+        "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// 512 bytes of shared memory (32 rows x 16 bytes, unswizzled) -> 4 TMEM
+// columns, lanes 0..31, repeated in the other three lane quarters.  Ordered
+// before MMAs that the same thread issues later.
+__device__ __forceinline__ void tmem_cp_32x128(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+               : "memory");
+}
+
 // Arrive on `bar` when all previously issued MMAs of this thread complete.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile(
@@ -232,6 +290,22 @@ __device__ __forceinline__ uint64_t desc_kmajor_sw128(uint32_t saddr) {
 __device__ __forceinline__ uint64_t desc_mnmajor_sw128(uint32_t saddr, uint32_t mn_atom_stride) {
   return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)((mn_atom_stride >> 4) & 0x3FFF) << 16) |
          ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// Unswizzled rows of 16 bytes, 8-row core matrices 128 bytes apart (scale
+// factor blocks for tcgen05.cp).
+__device__ __forceinline__ uint64_t desc_rows16(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(128 >> 4) << 32) |
+         ((uint64_t)1 << 46);
+}
+
+// Instruction descriptor of the block-scaled 4-bit kinds, dense, K = 64, both
+// operands K-major E2M1; sf_id: first byte of the 32-bit scale column that
+// the call uses (0, or 2 for the second half of four E8M0 scales).
+__host__ __device__ constexpr uint32_t make_idesc_fp4(bool e8m0, uint32_t M, uint32_t N,
+                                                      uint32_t sf_id) {
+  return (sf_id << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((e8m0 ? 1u : 0u) << 23) |
+         ((M >> 7) << 27) | (sf_id << 29);
 }
 
 // Instruction descriptor (kind::i8 / kind::f16), dense, no negate.

@@ -1,0 +1,225 @@
+"""Microscaled 4-bit floating point: matrices of E2M1 codes with block scales
+along their rows, and their product on the block-scaled tensor-core kinds.
+
+Two formats:
+
+- ``"mxfp4"`` (the OCP microscaling format): blocks of 32, scales 2^e with
+  e = floor(log2(amax)) - 2;
+- ``"nvfp4"``: blocks of 16, E4M3 scales amax / (6 g) and one fp32 factor
+  g = amax(tensor) / 2688 a tensor.
+
+The reference has no counterpart: its ``float4d`` codes (mxtorch.py:1465-1528)
+index a normalised grid under fp32 scales, which no tensor core reads.
+
+    w = fp4_tensor.quantize(weight, "nvfp4")          # [N, K]
+    y = fp4_matmul(fp4_tensor.quantize(x, "nvfp4"), w)  # x @ w^T, bf16
+    layer = fp4_linear.from_linear(nn_linear, "mxfp4")
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+
+from . import _lib as L
+
+FORMATS = {"mxfp4": L.FP4_MX, "nvfp4": L.FP4_NV}
+BLOCK = {"mxfp4": 32, "nvfp4": 16}
+_IO = {torch.float32: L.F32, torch.bfloat16: L.BF16}
+
+
+def _fmt(fmt: str) -> int:
+    try:
+        return FORMATS[fmt]
+    except KeyError:
+        raise ValueError(f"Unknown 4-bit format {fmt!r}: one of {sorted(FORMATS)}") from None
+
+
+def code_row_bytes(K: int) -> int:
+    """Bytes of one row of codes: two a byte, whole groups of 32."""
+    return -(-K // 32) * 16
+
+
+def scale_bytes(rows: int, K: int, fmt: str) -> int:
+    """Bytes of the scale tiles (128 rows x 4 blocks, 512 bytes each)."""
+    return -(-rows // 128) * -(-(-(-K // BLOCK[fmt])) // 4) * 512
+
+
+class fp4_tensor:
+    """A matrix [..., K] of E2M1 codes; leading dims are rows.
+
+    ``codes``: uint8 [rows, ceil(K / 32) * 16], two codes a byte, low first,
+    zero past K.  ``scales``: uint8, tiles of 128 rows x 4 blocks, tiles
+    row-major, byte ((r % 32) * 4 + r // 32) * 4 + c of a tile, zero past the
+    matrix.  ``global_scale``: fp32 [1] on the device (nvfp4) or None."""
+
+    __slots__ = ("codes", "scales", "fmt", "shape", "global_scale")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str, shape,
+                 global_scale: Optional[torch.Tensor] = None):
+        _fmt(fmt)
+        shape = torch.Size(shape)
+        if len(shape) < 1:
+            raise ValueError("fp4_tensor: shape needs at least one dim")
+        rows, K = shape[:-1].numel(), shape[-1]
+        if (codes.dtype != torch.uint8 or scales.dtype != torch.uint8
+                or codes.numel() != rows * code_row_bytes(K)
+                or scales.numel() != scale_bytes(rows, K, fmt)
+                or not codes.is_contiguous() or not scales.is_contiguous()):
+            raise ValueError(
+                f"fp4_tensor {tuple(shape)} {fmt}: codes must be {rows * code_row_bytes(K)} and "
+                f"scales {scale_bytes(rows, K, fmt)} contiguous uint8 values")
+        if (fmt == "nvfp4") != (global_scale is not None):
+            raise ValueError("fp4_tensor: nvfp4 takes a global_scale, mxfp4 none")
+        if global_scale is not None and (global_scale.dtype != torch.float32
+                                         or global_scale.numel() != 1):
+            raise ValueError("fp4_tensor: global_scale must be one fp32 value")
+        if codes.device != scales.device or (global_scale is not None
+                                             and global_scale.device != codes.device):
+            raise ValueError("fp4_tensor: codes, scales and global_scale are on different devices")
+        self.codes, self.scales, self.fmt = codes, scales, fmt
+        self.shape, self.global_scale = shape, global_scale
+
+    @classmethod
+    def quantize(cls, x: torch.Tensor, fmt: str = "mxfp4",
+                 global_scale: Optional[torch.Tensor] = None) -> "fp4_tensor":
+        """Quantize along the last dim (fp32 and bf16 as they are, other types
+        through fp32).  ``global_scale`` (nvfp4): a positive fp32 factor to
+        use, e.g. a calibrated one; by default from the data."""
+        f = _fmt(fmt)
+        L.require_cuda(x, "fp4_tensor.quantize")
+        if x.dim() < 1:
+            raise ValueError("fp4_tensor.quantize: x needs at least one dim")
+        x = x.detach()
+        if x.dtype not in _IO:
+            x = x.float()
+        shape, K = x.shape, x.shape[-1]
+        rows = shape[:-1].numel()
+        if x.dim() != 2 or x.stride(1) != 1 or (rows > 1 and x.stride(0) < K):
+            x = x.reshape(rows, K).contiguous()
+        dev = x.device
+        lib = L.load()
+        codes = torch.empty(rows, code_row_bytes(K), dtype=torch.uint8, device=dev)
+        scales = torch.empty(scale_bytes(rows, K, fmt), dtype=torch.uint8, device=dev)
+        g, derive, ws, wsb = None, 0, None, 0
+        if f == L.FP4_NV:
+            derive = int(global_scale is None)
+            if derive:
+                g = (torch.empty if rows * K else torch.ones)(1, dtype=torch.float32, device=dev)
+                wsb = lib.mxb_fp4_quantize_workspace_size(rows, K, f, 1)
+                ws = L.workspace(wsb, dev)
+            else:
+                g = global_scale
+                if g.dtype != torch.float32 or g.numel() != 1 or g.device != dev:
+                    raise ValueError("quantize: global_scale must be one fp32 value on x's device")
+        elif global_scale is not None:
+            raise ValueError("quantize: mxfp4 takes no global_scale")
+        with torch.cuda.device(dev):
+            rc = lib.mxb_fp4_quantize(L.ptr(x), _IO[x.dtype], rows, K, x.stride(0) if rows else K,
+                                      f, L.ptr(g), derive, L.ptr(codes), L.ptr(scales), L.ptr(ws),
+                                      wsb, L.stream_of(dev))
+        L.check(rc, f"mxb_fp4_quantize({fmt}, {rows}x{K})")
+        return cls(codes, scales, fmt, shape, g)
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values, fp32 or bf16."""
+        if dtype not in _IO:
+            raise ValueError(f"dequantize: float32 or bfloat16, not {dtype}")
+        L.require_cuda(self.codes, "fp4_tensor.dequantize")
+        dev = self.codes.device
+        rows, K = self.shape[:-1].numel(), self.shape[-1]
+        out = torch.empty(self.shape, dtype=dtype, device=dev)
+        with torch.cuda.device(dev):
+            rc = L.load().mxb_fp4_dequantize(L.ptr(self.codes), L.ptr(self.scales),
+                                             L.ptr(self.global_scale), rows, K, FORMATS[self.fmt],
+                                             L.ptr(out), _IO[dtype], L.stream_of(dev))
+        L.check(rc, f"mxb_fp4_dequantize({self.fmt}, {rows}x{K})")
+        return out
+
+    def block_scales(self) -> torch.Tensor:
+        """The scale bytes in plain order, [rows, ceil(K / block)] (E8M0 or E4M3 bits)."""
+        rows, nb = self.shape[:-1].numel(), -(-self.shape[-1] // BLOCK[self.fmt])
+        t = self.scales.view(-(-rows // 128), -(-nb // 4), 32, 4, 4).permute(0, 3, 2, 1, 4)
+        return t.reshape(-(-rows // 128) * 128, -(-nb // 4) * 4)[:rows, :nb].contiguous()
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.nbytes + self.scales.nbytes + (4 if self.global_scale is not None else 0)
+
+    def __repr__(self):
+        return f"fp4_tensor({tuple(self.shape)}, {self.fmt}, {self.device})"
+
+
+def fp4_matmul(a: fp4_tensor, b: fp4_tensor, bias: Optional[torch.Tensor] = None,
+               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a [..., K] @ b [N, K]^T (+ bias [N]) of two matrices of one format, fp32
+    accumulation, rounded once to ``out_dtype`` (bf16 or fp32)."""
+    if not isinstance(a, fp4_tensor) or not isinstance(b, fp4_tensor):
+        raise TypeError("fp4_matmul takes two fp4_tensors")
+    if a.fmt != b.fmt:
+        raise ValueError(f"fp4_matmul: formats differ ({a.fmt}, {b.fmt})")
+    if len(b.shape) != 2 or a.shape[-1] != b.shape[1]:
+        raise ValueError(f"fp4_matmul: {tuple(a.shape)} @ {tuple(b.shape)}^T")
+    if out_dtype not in _IO:
+        raise ValueError(f"fp4_matmul: float32 or bfloat16 out, not {out_dtype}")
+    L.require_cuda(a.codes, "fp4_matmul")
+    dev = a.codes.device
+    if b.codes.device != dev:
+        raise ValueError("fp4_matmul: operands on different devices")
+    M, K, N = a.shape[:-1].numel(), a.shape[-1], b.shape[0]
+    if bias is not None:
+        if bias.shape != (N,) or bias.device != dev:
+            raise ValueError(f"fp4_matmul: bias must be [{N}] on {dev}")
+        bias = bias.detach().float().contiguous()
+    out = torch.empty(*a.shape[:-1], N, dtype=out_dtype, device=dev)
+    if K == 0:  # an empty sum
+        out.zero_()
+        return out if bias is None else out.add_(bias)
+    with torch.cuda.device(dev):
+        rc = L.load().mxb_fp4_matmul(L.ptr(a.codes), L.ptr(a.scales), L.ptr(a.global_scale),
+                                     L.ptr(b.codes), L.ptr(b.scales), L.ptr(b.global_scale),
+                                     M, K, N, FORMATS[a.fmt], L.ptr(bias), L.ptr(out),
+                                     _IO[out_dtype], L.stream_of(dev))
+    L.check(rc, f"mxb_fp4_matmul({M}x{K}x{N}, {a.fmt})")
+    return out
+
+
+class fp4_linear(nn.Module):
+    """nn.Linear with a microscaled 4-bit weight; the activations are quantized
+    to the same format on every call.  Inference only (no gradient)."""
+
+    def __init__(self, weight: fp4_tensor, bias: Optional[torch.Tensor] = None,
+                 out_dtype: torch.dtype = torch.bfloat16):
+        super().__init__()
+        self.out_features, self.in_features = weight.shape
+        self.fmt, self.out_dtype = weight.fmt, out_dtype
+        self.register_buffer("weight_codes", weight.codes)
+        self.register_buffer("weight_scales", weight.scales)
+        self.register_buffer("weight_global_scale", weight.global_scale)
+        self.register_buffer("bias", None if bias is None else bias.detach().float())
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, fmt: str = "mxfp4",
+                    out_dtype: torch.dtype = torch.bfloat16) -> "fp4_linear":
+        w = linear.weight.data
+        if not w.is_cuda:
+            w = w.cuda()
+        bias = None if linear.bias is None else linear.bias.data.to(w.device)
+        return cls(fp4_tensor.quantize(w, fmt), bias, out_dtype)
+
+    @property
+    def weight(self) -> fp4_tensor:
+        return fp4_tensor(self.weight_codes, self.weight_scales, self.fmt,
+                          (self.out_features, self.in_features), self.weight_global_scale)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return fp4_matmul(fp4_tensor.quantize(x, self.fmt), self.weight, self.bias, self.out_dtype)
+
+    def extra_repr(self):
+        return (f"in={self.in_features}, out={self.out_features}, fmt={self.fmt}, "
+                f"bias={self.bias is not None}")
