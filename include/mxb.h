@@ -422,6 +422,69 @@ int mxb_fp4_matmul(const void* a_codes, const void* a_scales, const float* a_glo
                    int64_t K, int64_t N, int fmt, const float* bias, void* out, int out_dtype,
                    void* stream);
 
+/*
+ * Paged quantized KV cache (the reference's kv_cache_quantizer,
+ * mxtorch.py:2998-3119, keeps one list entry a step for a whole batch; this
+ * one has no counterpart).  A pool of n_pages pages of `page` tokens (a power
+ * of two, 16..1024) for `heads` KV heads of `dim` (64 or 128) values:
+ *   codes   [n_pages][heads][page][dim * bits / 8], int8 or int4 (two's
+ *           complement, low nibble first);
+ *   scales  [n_pages][heads][page] fp32;
+ * one pair for K and one for V, 16-byte aligned, n_pages * heads * page < 2^31.
+ * A token's slot is page number * page + offset.
+ *
+ * mxb_kv_write quantizes T tokens of K and V (element [t][h][d] at
+ * t * token_stride + h * head_stride + d, x_dtype MXB_F32 / MXB_BF16) into
+ * their slots, each head row as mxb_quantize with block = dim does:
+ * si = fl(fl(1 / max(amax, 1e-12)) * m), code = rint(fl(x * si)),
+ * scale = fl(1 / si), m = 127 or 7.  slots[t] < 0 skips the token; a slot past
+ * the pool is skipped too and recorded (mxb_device_error: 8).  Slots of one
+ * call are distinct.
+ */
+int mxb_kv_write(const void* k, const void* v, int x_dtype, int64_t T, int heads, int dim,
+                 int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                 int64_t v_head_stride, const int64_t* slots, int64_t n_pages, int page, int bits,
+                 void* k_codes, float* k_scales, void* v_codes, float* v_scales, void* stream);
+
+/*
+ * Read histories back: out [B][max_len][heads][dim] (out_dtype MXB_F32 /
+ * MXB_BF16) of K and V, position p of sequence b from page
+ * table[b * width + p / page]; zero from lengths[b] on.  A page number outside
+ * the pool, or a length past the table, reads as zero and is recorded
+ * (mxb_device_error: 8).
+ */
+int mxb_kv_read(const void* k_codes, const float* k_scales, const void* v_codes,
+                const float* v_scales, int64_t n_pages, int heads, int page, int dim, int bits,
+                const int* table, int64_t width, const int* lengths, int64_t B, int64_t max_len,
+                void* k_out, void* v_out, int out_dtype, void* stream);
+
+/* Workspace bytes for mxb_paged_attention. */
+size_t mxb_paged_attention_workspace_size(int64_t B, int64_t T, int heads, int group, int dim,
+                                          int page, int64_t width, int64_t prefix_len);
+
+/*
+ * Attention of T query tokens a sequence over the paged cache.
+ *   q       [B][T][heads * group][dim] bf16; query heads h * group .. read KV head h
+ *   lengths[b]  keys of sequence b, its T newest tokens included: query t
+ *           sees keys j < lengths[b] - (T - 1 - t) through table
+ *           [B][width] (page numbers)
+ *   prefix_table, prefix_len  keys that every query of the batch sees in
+ *           front of its own, stored once (prefix_len 0: none)
+ *   out     [B][T][heads * group][dim] bf16 = softmax(scale q k) v over both,
+ *           zero for a row without keys
+ *   lse     [B][T][heads * group] fp32 log of the sum of exponentials (-inf
+ *           for a row without keys), or NULL
+ * A page number outside the pool reads page 0 and a length past the table is
+ * cut, both recorded (mxb_device_error: 8).
+ */
+int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim,
+                        const void* k_codes, const float* k_scales, const void* v_codes,
+                        const float* v_scales, int64_t n_pages, int page, int bits,
+                        const int* table, int64_t width, const int* lengths,
+                        const int* prefix_table, int64_t prefix_width, int64_t prefix_len,
+                        float scale, void* out, float* lse, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,7 @@ from .fused import fused_linear_relu, fused_silu_and_mul  # noqa: F401
 from .hadamard import sign_vector  # noqa: F401
 from .kv_cache import kv_cache_quantizer  # noqa: F401
 from .linear import mx_linear, to_mx  # noqa: F401
+from .paged import paged_attention, paged_kv_cache  # noqa: F401
 from .tensor import mx_matmul, mx_matmul_kmajor, mx_tensor, register_kernel  # noqa: F401
 
 __version__ = "0.1.0"

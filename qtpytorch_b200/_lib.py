@@ -71,6 +71,14 @@ PROTOTYPES = {
     "mxb_hadamard_cross": (_int, [_vp, _i64, _i64, _int, _vp, _vp, _vp]),
     "mxb_linear_wonly_kmajor": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _i64, _int, _int, _int,
                                        _int, _vp, _vp]),
+    "mxb_kv_write": (_int, [_vp, _vp, _int, _i64, _int, _int, _i64, _i64, _i64, _i64, _vp, _i64, _int,
+                            _int, _vp, _vp, _vp, _vp, _vp]),
+    "mxb_kv_read": (_int, [_vp, _vp, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _i64, _vp, _i64,
+                           _i64, _vp, _vp, _int, _vp]),
+    "mxb_paged_attention_workspace_size": (_sz, [_i64, _i64, _int, _int, _int, _int, _i64, _i64]),
+    "mxb_paged_attention": (_int, [_vp, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _vp, _i64, _int,
+                                   _int, _vp, _i64, _vp, _vp, _i64, _i64, C.c_float, _vp, _vp, _vp,
+                                   _sz, _vp]),
     "mxb_fp4_code_bytes": (_sz, [_i64, _i64]),
     "mxb_fp4_scale_bytes": (_sz, [_i64, _i64, _int]),
     "mxb_fp4_quantize_workspace_size": (_sz, [_i64, _i64, _int, _int]),

@@ -12,6 +12,10 @@ size_t mxb_requant_workspace_size(int64_t n, int block);
 
 namespace mxb {
 
+// kv_paged.cu: checks of a paged cache pool's geometry and pointers
+int kv_pool_check(int64_t n_pages, int heads, int page, int dim, int bits, const void* kc,
+                  const void* ks, const void* vc, const void* vs);
+
 // gemm_cuda_core.cu
 int qgemm_generic(const void* a, const float* sa, bool sa_ok, const void* b, const float* sb,
                   bool sb_ok, int64_t M, int64_t K, int64_t N, int bits, int block, float* C,
