@@ -131,6 +131,17 @@ def stream_of(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def call(name: str, dev: torch.device, *args) -> int:
+    """Status of the entry point ``name`` on ``dev``'s current stream (its last
+    argument).  The device guard and the stream object cost more than a short
+    launch, so the guard is taken only where another device is current."""
+    fn = getattr(_lib or load(), name)
+    if torch.cuda.current_device() == dev.index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    with torch.cuda.device(dev):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+
+
 def require_cuda(t: torch.Tensor, what: str) -> None:
     if not t.is_cuda:
         raise MxbError(f"{what}: tensor is on {t.device}; the mxb kernels run on CUDA only")

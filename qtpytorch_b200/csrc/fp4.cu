@@ -64,6 +64,19 @@ __device__ __forceinline__ float factor_of(float amax) {
   return (amax > 0.0f && amax <= 3.4028235e38f) ? __fmul_rn(amax, 1.0f / 2688.0f) : 1.0f;
 }
 
+// Maximum over the block (NaN kept), in every thread.
+__device__ __forceinline__ float block_max(float a) {
+  __shared__ float s[kThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a = nan_max(a, __shfl_xor_sync(0xffffffffu, a, o));
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = a;
+  __syncthreads();
+  a = s[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / 32; ++w) a = nan_max(a, s[w]);
+  return a;
+}
+
 // Up to 16 elements of a row from column c0 on; zero past K.
 template <typename InT>
 __device__ __forceinline__ void load16(const InT* __restrict__ row, int64_t c0, int64_t K, bool vec,
@@ -94,14 +107,17 @@ __device__ __forceinline__ void load16(const InT* __restrict__ row, int64_t c0, 
   }
 }
 
-// Largest |x| of the tensor as the bits of a non-negative float (which order
-// as integers, NaN last): the maximum does not depend on the order of the
-// atomics.
+// Largest |x| of each block's share of the tensor (NaN kept) -> part[block].
+// The quantize kernel reduces the at most kAmaxBlocks values, so there is no
+// atomic and nothing to clear.
+constexpr int kAmaxBlocks = 4 * kSMs;
 template <typename InT>
-__global__ void __launch_bounds__(kThreads) fp4_amax_kernel(const InT* __restrict__ x, uint32_t rows,
-                                                            int64_t K, int64_t ldx, uint32_t gpr,
+__global__ void __launch_bounds__(kThreads) fp4_amax_kernel(const InT* __restrict__ x, int64_t K,
+                                                            int64_t ldx, uint32_t gpr,
                                                             uint32_t items, bool vec,
-                                                            uint32_t* __restrict__ out) {
+                                                            float* __restrict__ part) {
+  pdl_trigger();
+  pdl_wait();
   float a = 0.0f;
   for (uint64_t i = blockIdx.x * (uint64_t)kThreads + threadIdx.x; i < items;
        i += (uint64_t)gridDim.x * kThreads) {
@@ -111,28 +127,24 @@ __global__ void __launch_bounds__(kThreads) fp4_amax_kernel(const InT* __restric
 #pragma unroll
     for (int j = 0; j < kE; ++j) a = amax_step(a, v[j]);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) a = nan_max(a, __shfl_xor_sync(0xffffffffu, a, o));
-  __shared__ float s[kThreads / 32];
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = a;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-#pragma unroll
-    for (int w = 1; w < kThreads / 32; ++w) a = nan_max(a, s[w]);
-    atomicMax(out, __float_as_uint(a) & 0x7FFFFFFFu);
-  }
+  a = block_max(a);
+  if (threadIdx.x == 0) part[blockIdx.x] = a;
 }
 
 // gpr: 16-element groups per row, covering whole tiles of four scales;
 // items: rows * gpr groups, then one 32-bit word per four scales of each
-// padding row.  amax_bits: the tensor's maximum (derive), else null.
+// padding row.  part: the blocks' maxima (derive), else null; the blocks then run
+// from the end of the tensor, whose rows the maximum pass left in L2.
 template <typename InT, int FMT>
 __global__ void __launch_bounds__(kThreads)
     fp4_quant_kernel(const InT* __restrict__ x, uint32_t rows, int64_t K, int64_t ldx, uint32_t gpr,
                      uint32_t items, uint32_t pad_words, uint32_t groups, bool vec,
-                     const uint32_t* __restrict__ amax_bits, float* __restrict__ gscale,
+                     const float* __restrict__ part, int parts, float* __restrict__ gscale,
                      uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const uint64_t i = blockIdx.x * (uint64_t)kThreads + threadIdx.x;
+  pdl_trigger();
+  pdl_wait();
+  const uint32_t blk = part ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const uint64_t i = blk * (uint64_t)kThreads + threadIdx.x;
   const bool mine = i < items;
   if (!mine && i - items < pad_words) {
     const uint32_t w = (uint32_t)(i - items);
@@ -141,8 +153,10 @@ __global__ void __launch_bounds__(kThreads)
   }
   float g = 1.0f;
   if (FMT == MXB_FP4_NV) {
-    if (amax_bits) {
-      g = factor_of(__uint_as_float(*amax_bits));
+    if (part) {
+      float a = 0.0f;
+      for (int p = threadIdx.x; p < parts; p += kThreads) a = nan_max(a, part[p]);
+      g = factor_of(block_max(a));
       if (i == 0) *gscale = g;
     } else {
       g = *gscale;
@@ -219,19 +233,21 @@ template <typename OutT, int FMT>
 __global__ void __launch_bounds__(kThreads)
     fp4_dequant_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                        const float* __restrict__ gscale, uint32_t rows, int64_t K, uint32_t cpr,
-                       uint64_t items, uint32_t groups, bool vec, OutT* __restrict__ out) {
+                       uint32_t items, uint32_t groups, bool vec, OutT* __restrict__ out) {
   constexpr int E = 16 / sizeof(OutT), kU = 4;
   constexpr int kBlk = FMT == MXB_FP4_NV ? 16 : 32;
+  pdl_trigger();
+  pdl_wait();
   const float g = FMT == MXB_FP4_NV ? *gscale : 1.0f;
   const int64_t rb = fp4_row_bytes(K);
-  const uint64_t i0 = blockIdx.x * (uint64_t)(kThreads * kU) + threadIdx.x;
+  const uint64_t i0 = blockIdx.x * (uint64_t)(kThreads * kU) + threadIdx.x;  // may pass 32 bits
   uint32_t w[kU], sb[kU], rr[kU], cc[kU];
 #pragma unroll
   for (int u = 0; u < kU; ++u) {
     const uint64_t i = i0 + (uint64_t)u * kThreads;
     w[u] = sb[u] = rr[u] = cc[u] = 0u;
     if (i < items) {
-      const uint32_t r = (uint32_t)(i / cpr), c = (uint32_t)(i - (uint64_t)r * cpr);
+      const uint32_t r = (uint32_t)i / cpr, c = (uint32_t)i - r * cpr;
       const uint8_t* p = codes + (size_t)r * rb + (size_t)c * (E / 2);
       w[u] = E == 8 ? __ldg(reinterpret_cast<const uint32_t*>(p))
                     : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p));
@@ -285,30 +301,25 @@ __global__ void __launch_bounds__(kThreads)
 
 template <typename InT>
 int quantize_t(const InT* x, int64_t rows, int64_t K, int64_t ldx, int fmt, float* g, int derive,
-               uint8_t* codes, uint8_t* scales, uint32_t* ws, cudaStream_t st) {
+               uint8_t* codes, uint8_t* scales, float* part, cudaStream_t st) {
   const int64_t groups = cdiv(fp4_blocks(K, fmt), 4);
   const int64_t gpr = groups * (fmt == MXB_FP4_NV ? 4 : 8);
   const int64_t items = rows * gpr, pad = (cdiv(rows, 128) * 128 - rows) * groups;
   if (items + pad >= (int64_t)1 << 32) return MXB_E_SHAPE;
   const bool vec = ((uintptr_t)x % 16) == 0 && (ldx * (int64_t)sizeof(InT)) % 16 == 0;
+  int parts = 0;
   if (derive) {
-    MXB_CUDA_TRY(cudaMemsetAsync(ws, 0, sizeof(uint32_t), st));
     const int64_t agpr = cdiv(K, kE), aitems = rows * agpr;
     const int64_t blocks = cdiv(aitems, kThreads);
-    fp4_amax_kernel<InT><<<(unsigned)(blocks < 8 * kSMs ? blocks : 8 * kSMs), kThreads, 0, st>>>(
-        x, (uint32_t)rows, K, ldx, (uint32_t)agpr, (uint32_t)aitems, vec, ws);
+    parts = (int)(blocks < kAmaxBlocks ? blocks : kAmaxBlocks);
+    MXB_CUDA_TRY(launch_pdl(fp4_amax_kernel<InT>, dim3((unsigned)parts), kThreads, 0, st, x, K, ldx,
+                            (uint32_t)agpr, (uint32_t)aitems, vec, part));
     MXB_LAUNCH_CHECK();
   }
-  const unsigned grid = (unsigned)cdiv(items + pad, kThreads);
-  const uint32_t* am = derive ? ws : nullptr;
-  if (fmt == MXB_FP4_NV)
-    fp4_quant_kernel<InT, MXB_FP4_NV><<<grid, kThreads, 0, st>>>(
-        x, (uint32_t)rows, K, ldx, (uint32_t)gpr, (uint32_t)items, (uint32_t)pad, (uint32_t)groups,
-        vec, am, g, codes, scales);
-  else
-    fp4_quant_kernel<InT, MXB_FP4_MX><<<grid, kThreads, 0, st>>>(
-        x, (uint32_t)rows, K, ldx, (uint32_t)gpr, (uint32_t)items, (uint32_t)pad, (uint32_t)groups,
-        vec, nullptr, nullptr, codes, scales);
+  auto kern = fmt == MXB_FP4_NV ? fp4_quant_kernel<InT, MXB_FP4_NV> : fp4_quant_kernel<InT, MXB_FP4_MX>;
+  MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)cdiv(items + pad, kThreads)), kThreads, 0, st, x,
+                          (uint32_t)rows, K, ldx, (uint32_t)gpr, (uint32_t)items, (uint32_t)pad,
+                          (uint32_t)groups, vec, derive ? part : nullptr, parts, g, codes, scales));
   MXB_LAUNCH_CHECK();
   return MXB_OK;
 }
@@ -320,15 +331,12 @@ int dequantize_t(const uint8_t* codes, const uint8_t* scales, const float* g, in
   const int64_t cpr = cdiv(K, E), items = rows * cpr;
   const int64_t groups = cdiv(fp4_blocks(K, fmt), 4);
   const int64_t grid = cdiv(items, 4 * kThreads);
-  if (rows >= (int64_t)1 << 32 || K >= (int64_t)1 << 31 || grid >= (int64_t)1 << 31)
-    return MXB_E_SHAPE;
+  if (items >= (int64_t)1 << 32) return MXB_E_SHAPE;
   const bool vec = K % E == 0 && ((uintptr_t)out % 16) == 0;
-  if (fmt == MXB_FP4_NV)
-    fp4_dequant_kernel<OutT, MXB_FP4_NV><<<(unsigned)grid, kThreads, 0, st>>>(
-        codes, scales, g, (uint32_t)rows, K, (uint32_t)cpr, (uint64_t)items, (uint32_t)groups, vec, out);
-  else
-    fp4_dequant_kernel<OutT, MXB_FP4_MX><<<(unsigned)grid, kThreads, 0, st>>>(
-        codes, scales, g, (uint32_t)rows, K, (uint32_t)cpr, (uint64_t)items, (uint32_t)groups, vec, out);
+  auto kern = fmt == MXB_FP4_NV ? fp4_dequant_kernel<OutT, MXB_FP4_NV>
+                                : fp4_dequant_kernel<OutT, MXB_FP4_MX>;
+  MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)grid), kThreads, 0, st, codes, scales, g, (uint32_t)rows,
+                          K, (uint32_t)cpr, (uint32_t)items, (uint32_t)groups, vec, out));
   MXB_LAUNCH_CHECK();
   return MXB_OK;
 }
@@ -350,7 +358,7 @@ size_t mxb_fp4_scale_bytes(int64_t rows, int64_t K, int fmt) {
 }
 
 size_t mxb_fp4_quantize_workspace_size(int64_t rows, int64_t K, int fmt, int derive) {
-  return rows > 0 && K > 0 && fmt == MXB_FP4_NV && derive ? 16 : 0;
+  return rows > 0 && K > 0 && fmt == MXB_FP4_NV && derive ? kAmaxBlocks * sizeof(float) : 0;
 }
 
 int mxb_fp4_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t ldx, int fmt,
@@ -365,7 +373,7 @@ int mxb_fp4_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int64_
   if (d && (!workspace || workspace_bytes < mxb_fp4_quantize_workspace_size(rows, K, fmt, 1)))
     return MXB_E_WORKSPACE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  uint32_t* ws = static_cast<uint32_t*>(workspace);
+  float* ws = static_cast<float*>(workspace);
   uint8_t* c = static_cast<uint8_t*>(codes);
   uint8_t* s = static_cast<uint8_t*>(scales);
   if (x_dtype == MXB_BF16)

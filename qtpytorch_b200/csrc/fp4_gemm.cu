@@ -160,6 +160,8 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = bars->tmem_base;
+  pdl_trigger();
+  pdl_wait();  // the setup above overlaps the end of the quantize kernel
 
   if (warp == 0) {
     if (lane == 0) {
@@ -317,13 +319,15 @@ int launch(const CUtensorMap& tf, const CUtensorMap& tt, const Args& a, cudaStre
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)a.splits;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   MXB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tf, tt, a));
   MXB_LAUNCH_CHECK();
   return MXB_OK;

@@ -50,18 +50,21 @@ template <typename InT, int BITS, int D>
 __global__ void __launch_bounds__(kThreads)
     kv_write_kernel(const InT* __restrict__ k, const InT* __restrict__ v, int64_t T, int H,
                     int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs, bool vec,
-                    const int64_t* __restrict__ slots, int64_t n_slots, int page,
+                    const int64_t* __restrict__ slots, int64_t n_slots, int page_shift,
                     uint8_t* __restrict__ kc, float* __restrict__ ks, uint8_t* __restrict__ vc,
                     float* __restrict__ vs, int* __restrict__ err) {
   constexpr int L = D / 8;
   constexpr float m = BITS == 8 ? 127.0f : 7.0f;
+  pdl_trigger();
+  pdl_wait();
   const bool val = blockIdx.y != 0;
-  const int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x;
-  const int64_t row = i / L;
-  const int part = (int)(i % L);
-  const bool live = row < T * H;
-  const int64_t t = live ? row / H : 0;
-  const int h = live ? (int)(row - t * H) : 0;
+  // 32-bit index: T * H < 2^32 (checked at the launch)
+  const uint32_t row = blockIdx.x * (uint32_t)(kThreads / L) + threadIdx.x / L;
+  const int part = threadIdx.x % L;
+  const bool live = row < (uint32_t)(T * H);
+  const uint32_t t32 = live ? row / (uint32_t)H : 0u;
+  const int64_t t = t32;
+  const int h = live ? (int)(row - t32 * (uint32_t)H) : 0;
   float x[8];
   int64_t slot = -1;
   if (live) {
@@ -92,8 +95,8 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int j = 0; j < 8; ++j) c[j] = 0u;
   }
-  const int64_t pg = slot / page;
-  const int64_t r = (pg * H + h) * page + (slot - pg * page);
+  const int64_t pg = slot >> page_shift;
+  const int64_t r = ((pg * H + h) << page_shift) + (slot & ((1 << page_shift) - 1));
   uint8_t* dst = (val ? vc : kc) + r * (D * BITS / 8) + part * BITS;
   if (BITS == 8) {
     *reinterpret_cast<uint2*>(dst) = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24,
@@ -114,33 +117,36 @@ __global__ void __launch_bounds__(kThreads)
     kv_read_kernel(const uint8_t* __restrict__ kc, const float* __restrict__ ks,
                    const uint8_t* __restrict__ vc, const float* __restrict__ vs,
                    const int* __restrict__ table, int width, const int* __restrict__ lengths,
-                   int64_t n_pages, int H, int page, int64_t max_len, OutT* __restrict__ ko,
+                   int64_t n_pages, int H, int page_shift, uint32_t max_len, OutT* __restrict__ ko,
                    OutT* __restrict__ vo, int* __restrict__ err) {
   constexpr int E = 16 / sizeof(OutT), C = D / E, kU = 4;
+  pdl_trigger();
+  pdl_wait();
   const int b = blockIdx.y;
   const bool val = blockIdx.z != 0;
   const uint8_t* codes = val ? vc : kc;
   const float* scales = val ? vs : ks;
   OutT* out = (val ? vo : ko) + (int64_t)b * max_len * H * D;
-  const int64_t len = lengths[b], items = max_len * H * C;
-  const int64_t i0 = blockIdx.x * (int64_t)(kThreads * kU) + threadIdx.x;
+  const uint32_t len = (uint32_t)max(lengths[b], 0), rows = max_len * (uint32_t)H;
+  constexpr uint32_t kRows = kThreads / C;  // head rows per block and step
+  const uint32_t row0 = blockIdx.x * (kRows * kU) + threadIdx.x / C;
+  const int part = threadIdx.x % C;
   uint64_t w[kU];
   float s[kU];
 #pragma unroll
   for (int u = 0; u < kU; ++u) {
-    const int64_t i = i0 + u * kThreads;
+    const uint32_t row = row0 + u * kRows;
     w[u] = 0;
     s[u] = 0.0f;
-    if (i < items) {
-      const int part = (int)(i % C);
-      const int64_t row = i / C;
-      const int64_t pos = row / H;
-      const int h = (int)(row - pos * H);
+    if (row < rows) {
+      const uint32_t pos = row / (uint32_t)H;
+      const int h = (int)(row - pos * (uint32_t)H);
       if (pos < len) {
-        const int64_t at = pos / page;
-        const int pg = at < width ? table[(int64_t)b * width + at] : -1;
+        const uint32_t at = pos >> page_shift;
+        const int pg = at < (uint32_t)width ? table[(int64_t)b * width + at] : -1;
         if (pg >= 0 && pg < n_pages) {
-          const int64_t r = ((int64_t)pg * H + h) * page + (pos - at * page);
+          const int64_t r =
+              (((int64_t)pg * H + h) << page_shift) + (pos & ((1u << page_shift) - 1u));
           const uint8_t* p = codes + r * (D * BITS / 8) + part * (E * BITS / 8);
           if (E * BITS == 64) w[u] = __ldg(reinterpret_cast<const unsigned long long*>(p));
           else if (E * BITS == 32) w[u] = __ldg(reinterpret_cast<const uint32_t*>(p));
@@ -154,13 +160,13 @@ __global__ void __launch_bounds__(kThreads)
   }
 #pragma unroll
   for (int u = 0; u < kU; ++u) {
-    const int64_t i = i0 + u * kThreads;
-    if (i >= items) continue;
+    const uint32_t row = row0 + u * kRows;
+    if (row >= rows) continue;
     float v[E];
 #pragma unroll
     for (int j = 0; j < E; ++j)
       v[j] = __fmul_rn((float)sext((uint32_t)(w[u] >> (j * BITS)), BITS), s[u]);
-    OutT* o = out + i * E;
+    OutT* o = out + (int64_t)row * D + part * E;
     if (sizeof(OutT) == 4) {
       __stcs(reinterpret_cast<float4*>(o), make_float4(v[0], v[1], v[2], v[3]));
     } else {
@@ -174,6 +180,8 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
 }
+
+int shift_of(int page) { return 31 - __builtin_clz((unsigned)page); }
 
 struct WriteArgs {
   int64_t T;
@@ -189,13 +197,14 @@ struct WriteArgs {
 template <typename InT, int BITS, int D>
 int write_t(const void* k, const void* v, const WriteArgs& a, cudaStream_t st) {
   const int64_t blocks = cdiv(a.T * a.H * (D / 8), kThreads);
-  if (blocks >= (int64_t)1 << 31) return MXB_E_SHAPE;
+  if (a.T * a.H >= (int64_t)1 << 31) return MXB_E_SHAPE;
   const int64_t per = 16 / sizeof(InT);
   const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && a.k_ts % per == 0 &&
                    a.k_hs % per == 0 && a.v_ts % per == 0 && a.v_hs % per == 0;
-  kv_write_kernel<InT, BITS, D><<<dim3((unsigned)blocks, 2), kThreads, 0, st>>>(
-      static_cast<const InT*>(k), static_cast<const InT*>(v), a.T, a.H, a.k_ts, a.k_hs, a.v_ts,
-      a.v_hs, vec, a.slots, a.n_slots, a.page, a.kc, a.ks, a.vc, a.vs, device_error_ptr());
+  MXB_CUDA_TRY(launch_pdl(kv_write_kernel<InT, BITS, D>, dim3((unsigned)blocks, 2), kThreads, 0, st,
+                          static_cast<const InT*>(k), static_cast<const InT*>(v), a.T, a.H, a.k_ts,
+                          a.k_hs, a.v_ts, a.v_hs, vec, a.slots, a.n_slots, shift_of(a.page), a.kc,
+                          a.ks, a.vc, a.vs, device_error_ptr()));
   MXB_LAUNCH_CHECK();
   return MXB_OK;
 }
@@ -213,11 +222,12 @@ struct ReadArgs {
 
 template <typename OutT, int BITS, int D>
 int read_t(const ReadArgs& a, void* ko, void* vo, cudaStream_t st) {
-  const int64_t blocks = cdiv(a.max_len * a.H * (D / (16 / (int64_t)sizeof(OutT))), kThreads * 4);
-  if (blocks >= (int64_t)1 << 31) return MXB_E_SHAPE;
-  kv_read_kernel<OutT, BITS, D><<<dim3((unsigned)blocks, (unsigned)a.B, 2), kThreads, 0, st>>>(
-      a.kc, a.ks, a.vc, a.vs, a.table, a.width, a.lengths, a.n_pages, a.H, a.page, a.max_len,
-      static_cast<OutT*>(ko), static_cast<OutT*>(vo), device_error_ptr());
+  const int64_t rows = a.max_len * a.H, blocks = cdiv(rows * (D / (16 / (int64_t)sizeof(OutT))), kThreads * 4);
+  if (rows >= (int64_t)1 << 31) return MXB_E_SHAPE;
+  MXB_CUDA_TRY(launch_pdl(kv_read_kernel<OutT, BITS, D>, dim3((unsigned)blocks, (unsigned)a.B, 2),
+                          kThreads, 0, st, a.kc, a.ks, a.vc, a.vs, a.table, a.width, a.lengths,
+                          a.n_pages, a.H, shift_of(a.page), (uint32_t)a.max_len,
+                          static_cast<OutT*>(ko), static_cast<OutT*>(vo), device_error_ptr()));
   MXB_LAUNCH_CHECK();
   return MXB_OK;
 }

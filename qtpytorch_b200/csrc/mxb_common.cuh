@@ -197,6 +197,34 @@ __device__ __forceinline__ void decode_word2(uint32_t w, uint64_t* out) {
   }
 }
 
+// Programmatic dependent launch.  A kernel launched by launch_pdl may be
+// scheduled while its predecessor on the stream drains, so every thread of it
+// calls pdl_wait() before its first access to global memory (the predecessor,
+// and with it everything before, is then complete and visible), and
+// pdl_trigger() lets its own successor be scheduled early.
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_trigger() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <typename... P, typename... A>
+inline cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, int threads, size_t smem,
+                              cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+}
+
 __device__ __forceinline__ float load_as_f32(const float* p, int64_t i) { return __ldg(p + i); }
 __device__ __forceinline__ float load_as_f32(const __nv_bfloat16* p, int64_t i) {
   return __bfloat162float(p[i]);

@@ -156,6 +156,8 @@ __global__ void __launch_bounds__(kThreads)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
 
+  pdl_trigger();
+  pdl_wait();
   const int split = blockIdx.x;
   const int h = blockIdx.y / a.row_tiles, r0 = (blockIdx.y % a.row_tiles) * R;
   const int unit = blockIdx.z;
@@ -482,6 +484,8 @@ __global__ void __launch_bounds__(128)
                       int64_t n_rows, __nv_bfloat16* __restrict__ out, float* __restrict__ lse) {
   const int64_t row = blockIdx.x * (int64_t)4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
+  pdl_trigger();
+  pdl_wait();
   if (row >= n_rows) return;
   constexpr int V = D / 32;
   float mx = -INFINITY;
@@ -516,8 +520,8 @@ int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int unit
   constexpr size_t join = (size_t)kWarps * 8 * NT * (D + 4) * 4;
   constexpr size_t smem = 1024 + (ring > join ? ring : join);
   MXB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kern<<<dim3((unsigned)a.splits, (unsigned)(a.row_tiles * a.H), (unsigned)units), kThreads, smem, st>>>(
-      tk, tv, a);
+  MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)a.splits, (unsigned)(a.row_tiles * a.H), (unsigned)units),
+                          kThreads, smem, st, tk, tv, a));
   MXB_LAUNCH_CHECK();
   return MXB_OK;
 }
@@ -668,12 +672,9 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
   }
   if (!direct) {
     const unsigned grid = (unsigned)cdiv(a.n_rows, 4);
-    if (dim == 128)
-      pattn::paged_join_kernel<128><<<grid, 128, 0, st>>>(a.po, a.pml, p.parts(), a.n_rows,
-                                                         static_cast<__nv_bfloat16*>(out), lse);
-    else
-      pattn::paged_join_kernel<64><<<grid, 128, 0, st>>>(a.po, a.pml, p.parts(), a.n_rows,
-                                                        static_cast<__nv_bfloat16*>(out), lse);
+    MXB_CUDA_TRY(launch_pdl(dim == 128 ? pattn::paged_join_kernel<128> : pattn::paged_join_kernel<64>,
+                            dim3(grid), 128, 0, st, a.po, a.pml, p.parts(), a.n_rows,
+                            static_cast<__nv_bfloat16*>(out), lse));
     MXB_LAUNCH_CHECK();
   }
   return MXB_OK;

@@ -91,23 +91,29 @@ class fp4_tensor:
         L.require_cuda(x, "fp4_tensor.quantize")
         if x.dim() < 1:
             raise ValueError("fp4_tensor.quantize: x needs at least one dim")
-        x = x.detach()
-        if x.dtype not in _IO:
-            x = x.float()
-        shape, K = x.shape, x.shape[-1]
-        rows = shape[:-1].numel()
-        if x.dim() != 2 or x.stride(1) != 1 or (rows > 1 and x.stride(0) < K):
-            x = x.reshape(rows, K).contiguous()
+        io = _IO.get(x.dtype)
+        if io is None:
+            x, io = x.float(), L.F32
+        shape = x.shape
+        if len(shape) == 2:
+            rows, K = shape
+        else:
+            rows, K = shape[:-1].numel(), shape[-1]
+            x = x.reshape(rows, K)
+        ldx = x.stride(0) if rows > 1 else K
+        if x.stride(1) != 1 or ldx < K:
+            x, ldx = x.contiguous(), K
         dev = x.device
-        lib = L.load()
         codes = torch.empty(rows, code_row_bytes(K), dtype=torch.uint8, device=dev)
         scales = torch.empty(scale_bytes(rows, K, fmt), dtype=torch.uint8, device=dev)
         g, derive, ws, wsb = None, 0, None, 0
         if f == L.FP4_NV:
-            derive = int(global_scale is None)
-            if derive:
-                g = (torch.empty if rows * K else torch.ones)(1, dtype=torch.float32, device=dev)
-                wsb = lib.mxb_fp4_quantize_workspace_size(rows, K, f, 1)
+            if global_scale is None:
+                derive = 1
+                # the factor, and behind it the workspace
+                wsb = L.load().mxb_fp4_quantize_workspace_size(rows, K, f, 1)
+                g = torch.empty(1, dtype=torch.float32, device=dev) if wsb else torch.ones(
+                    1, dtype=torch.float32, device=dev)
                 ws = L.workspace(wsb, dev)
             else:
                 g = global_scale
@@ -115,26 +121,27 @@ class fp4_tensor:
                     raise ValueError("quantize: global_scale must be one fp32 value on x's device")
         elif global_scale is not None:
             raise ValueError("quantize: mxfp4 takes no global_scale")
-        with torch.cuda.device(dev):
-            rc = lib.mxb_fp4_quantize(L.ptr(x), _IO[x.dtype], rows, K, x.stride(0) if rows else K,
-                                      f, L.ptr(g), derive, L.ptr(codes), L.ptr(scales), L.ptr(ws),
-                                      wsb, L.stream_of(dev))
-        L.check(rc, f"mxb_fp4_quantize({fmt}, {rows}x{K})")
-        return cls(codes, scales, fmt, shape, g)
+        rc = L.call("mxb_fp4_quantize", dev, x.data_ptr(), io, rows, K, ldx, f, L.ptr(g), derive,
+                    codes.data_ptr(), scales.data_ptr(), L.ptr(ws), wsb)
+        if rc:
+            L.check(rc, f"mxb_fp4_quantize({fmt}, {rows}x{K})")
+        self = cls.__new__(cls)
+        self.codes, self.scales, self.fmt, self.shape, self.global_scale = codes, scales, fmt, shape, g
+        return self
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values, fp32 or bf16."""
-        if dtype not in _IO:
+        io = _IO.get(dtype)
+        if io is None:
             raise ValueError(f"dequantize: float32 or bfloat16, not {dtype}")
         L.require_cuda(self.codes, "fp4_tensor.dequantize")
-        dev = self.codes.device
-        rows, K = self.shape[:-1].numel(), self.shape[-1]
-        out = torch.empty(self.shape, dtype=dtype, device=dev)
-        with torch.cuda.device(dev):
-            rc = L.load().mxb_fp4_dequantize(L.ptr(self.codes), L.ptr(self.scales),
-                                             L.ptr(self.global_scale), rows, K, FORMATS[self.fmt],
-                                             L.ptr(out), _IO[dtype], L.stream_of(dev))
-        L.check(rc, f"mxb_fp4_dequantize({self.fmt}, {rows}x{K})")
+        dev, shape = self.codes.device, self.shape
+        rows, K = shape[:-1].numel(), shape[-1]
+        out = torch.empty(shape, dtype=dtype, device=dev)
+        rc = L.call("mxb_fp4_dequantize", dev, self.codes.data_ptr(), self.scales.data_ptr(),
+                    L.ptr(self.global_scale), rows, K, FORMATS[self.fmt], out.data_ptr(), io)
+        if rc:
+            L.check(rc, f"mxb_fp4_dequantize({self.fmt}, {rows}x{K})")
         return out
 
     def block_scales(self) -> torch.Tensor:
@@ -175,17 +182,17 @@ def fp4_matmul(a: fp4_tensor, b: fp4_tensor, bias: Optional[torch.Tensor] = None
     if bias is not None:
         if bias.shape != (N,) or bias.device != dev:
             raise ValueError(f"fp4_matmul: bias must be [{N}] on {dev}")
-        bias = bias.detach().float().contiguous()
-    out = torch.empty(*a.shape[:-1], N, dtype=out_dtype, device=dev)
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.float().contiguous()
+    out = torch.empty((M, N) if len(a.shape) == 2 else (*a.shape[:-1], N), dtype=out_dtype, device=dev)
     if K == 0:  # an empty sum
         out.zero_()
         return out if bias is None else out.add_(bias)
-    with torch.cuda.device(dev):
-        rc = L.load().mxb_fp4_matmul(L.ptr(a.codes), L.ptr(a.scales), L.ptr(a.global_scale),
-                                     L.ptr(b.codes), L.ptr(b.scales), L.ptr(b.global_scale),
-                                     M, K, N, FORMATS[a.fmt], L.ptr(bias), L.ptr(out),
-                                     _IO[out_dtype], L.stream_of(dev))
-    L.check(rc, f"mxb_fp4_matmul({M}x{K}x{N}, {a.fmt})")
+    rc = L.call("mxb_fp4_matmul", dev, a.codes.data_ptr(), a.scales.data_ptr(), L.ptr(a.global_scale),
+                b.codes.data_ptr(), b.scales.data_ptr(), L.ptr(b.global_scale), M, K, N,
+                FORMATS[a.fmt], L.ptr(bias), out.data_ptr(), _IO[out_dtype])
+    if rc:
+        L.check(rc, f"mxb_fp4_matmul({M}x{K}x{N}, {a.fmt})")
     return out
 
 

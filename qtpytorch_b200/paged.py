@@ -94,21 +94,20 @@ class paged_kv_cache:
                              f"{tuple(k.shape)}, {tuple(v.shape)}, {tuple(slots.shape)}")
         if k.device != dev or v.device != dev or slots.device != dev:
             raise ValueError(f"write: k, v and slots must be on {dev}")
-        k, v = k.detach(), v.detach()
         if k.dtype != v.dtype or k.dtype not in _IO:
             k, v = k.float(), v.float()
         if k.stride(2) != 1:
             k = k.contiguous()
         if v.stride(2) != 1:
             v = v.contiguous()
-        slots = slots.to(torch.int64).contiguous()
-        with torch.cuda.device(dev):
-            rc = L.load().mxb_kv_write(
-                L.ptr(k), L.ptr(v), _IO[k.dtype], k.shape[0], H, D, k.stride(0), k.stride(1),
-                v.stride(0), v.stride(1), L.ptr(slots), self.n_pages, self.page_size,
-                self.dtype.bits, L.ptr(self.k_codes), L.ptr(self.k_scales), L.ptr(self.v_codes),
-                L.ptr(self.v_scales), L.stream_of(dev))
-        L.check(rc, f"mxb_kv_write({self.dtype.name}, T={k.shape[0]})")
+        if slots.dtype != torch.int64 or not slots.is_contiguous():
+            slots = slots.to(torch.int64).contiguous()
+        rc = L.call("mxb_kv_write", dev, k.data_ptr(), v.data_ptr(), _IO[k.dtype], k.shape[0], H, D,
+                    k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(),
+                    self.n_pages, self.page_size, self.dtype.bits, self.k_codes.data_ptr(),
+                    self.k_scales.data_ptr(), self.v_codes.data_ptr(), self.v_scales.data_ptr())
+        if rc:
+            L.check(rc, f"mxb_kv_write({self.dtype.name}, T={k.shape[0]})")
 
     def read(self, table: torch.Tensor, lengths: torch.Tensor, max_len: int,
              dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -122,14 +121,14 @@ class paged_kv_cache:
             raise ValueError("read: max_len must not be negative")
         B = table.shape[0]
         shape = (B, max_len, self.n_heads, self.head_dim)
-        k, v = (torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
-        with torch.cuda.device(dev):
-            rc = L.load().mxb_kv_read(
-                L.ptr(self.k_codes), L.ptr(self.k_scales), L.ptr(self.v_codes), L.ptr(self.v_scales),
-                self.n_pages, self.n_heads, self.page_size, self.head_dim, self.dtype.bits,
-                L.ptr(table), table.shape[1], L.ptr(lengths), B, max_len, L.ptr(k), L.ptr(v),
-                _IO[dtype], L.stream_of(dev))
-        L.check(rc, f"mxb_kv_read({self.dtype.name}, B={B}, max_len={max_len})")
+        k = torch.empty(shape, dtype=dtype, device=dev)
+        v = torch.empty(shape, dtype=dtype, device=dev)
+        rc = L.call("mxb_kv_read", dev, self.k_codes.data_ptr(), self.k_scales.data_ptr(),
+                    self.v_codes.data_ptr(), self.v_scales.data_ptr(), self.n_pages, self.n_heads,
+                    self.page_size, self.head_dim, self.dtype.bits, table.data_ptr(), table.shape[1],
+                    lengths.data_ptr(), B, max_len, k.data_ptr(), v.data_ptr(), _IO[dtype])
+        if rc:
+            L.check(rc, f"mxb_kv_read({self.dtype.name}, B={B}, max_len={max_len})")
         return k, v
 
     @property
@@ -149,7 +148,11 @@ def _tables(table: torch.Tensor, lengths: torch.Tensor, dev, what: str):
         raise ValueError(f"{what}: table and lengths must be on {dev}")
     if table.is_floating_point() or lengths.is_floating_point():
         raise ValueError(f"{what}: table and lengths hold integers")
-    return table.to(torch.int32).contiguous(), lengths.to(torch.int32).contiguous()
+    if table.dtype != torch.int32 or not table.is_contiguous():
+        table = table.to(torch.int32).contiguous()
+    if lengths.dtype != torch.int32 or not lengths.is_contiguous():
+        lengths = lengths.to(torch.int32).contiguous()
+    return table, lengths
 
 
 def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
@@ -191,7 +194,7 @@ def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
             raise ValueError(f"paged_attention: prefix_len {prefix_len} needs more than the "
                              f"{width} pages of prefix_table")
         prefix_table = prefix_table.to(torch.int32).contiguous()
-    q = q.detach().contiguous()
+    q = q.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
     out = torch.empty_like(q)
@@ -200,13 +203,13 @@ def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
     wsb = lib.mxb_paged_attention_workspace_size(B, T, H, Hq // H, D, cache.page_size,
                                                  table.shape[1], prefix_len)
     ws = L.workspace(wsb, dev)
-    with torch.cuda.device(dev):
-        rc = lib.mxb_paged_attention(
-            L.ptr(q), B, T, H, Hq // H, D, L.ptr(cache.k_codes), L.ptr(cache.k_scales),
-            L.ptr(cache.v_codes), L.ptr(cache.v_scales), cache.n_pages, cache.page_size,
-            cache.dtype.bits, L.ptr(table), table.shape[1], L.ptr(lengths),
-            L.ptr(prefix_table) if prefix_len else 0, width, prefix_len,
-            1.0 / math.sqrt(D) if scale is None else float(scale), L.ptr(out), L.ptr(lse),
-            L.ptr(ws), wsb, L.stream_of(dev))
-    L.check(rc, f"mxb_paged_attention(B={B}, T={T}, heads={H}x{Hq // H}, dim={D})")
+    rc = L.call("mxb_paged_attention", dev, q.data_ptr(), B, T, H, Hq // H, D,
+                cache.k_codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(),
+                cache.v_scales.data_ptr(), cache.n_pages, cache.page_size, cache.dtype.bits,
+                table.data_ptr(), table.shape[1], lengths.data_ptr(),
+                prefix_table.data_ptr() if prefix_len else 0, width, prefix_len,
+                1.0 / math.sqrt(D) if scale is None else float(scale), out.data_ptr(), L.ptr(lse),
+                L.ptr(ws), wsb)
+    if rc:
+        L.check(rc, f"mxb_paged_attention(B={B}, T={T}, heads={H}x{Hq // H}, dim={D})")
     return (out, lse) if return_lse else out
