@@ -460,7 +460,7 @@ int mxb_kv_read(const void* k_codes, const float* k_scales, const void* v_codes,
 
 /* Workspace bytes for mxb_paged_attention. */
 size_t mxb_paged_attention_workspace_size(int64_t B, int64_t T, int heads, int group, int dim,
-                                          int page, int64_t width, int64_t prefix_len);
+                                          int bits, int page, int64_t width, int64_t prefix_len);
 
 /*
  * Attention of T query tokens a sequence over the paged cache.

@@ -75,7 +75,8 @@ PROTOTYPES = {
                             _int, _vp, _vp, _vp, _vp, _vp]),
     "mxb_kv_read": (_int, [_vp, _vp, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _i64, _vp, _i64,
                            _i64, _vp, _vp, _int, _vp]),
-    "mxb_paged_attention_workspace_size": (_sz, [_i64, _i64, _int, _int, _int, _int, _i64, _i64]),
+    "mxb_paged_attention_workspace_size": (_sz, [_i64, _i64, _int, _int, _int, _int, _int, _i64,
+                                                 _i64]),
     "mxb_paged_attention": (_int, [_vp, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _vp, _i64, _int,
                                    _int, _vp, _i64, _vp, _vp, _i64, _i64, C.c_float, _vp, _vp, _vp,
                                    _sz, _vp]),
@@ -136,7 +137,7 @@ def call(name: str, dev: torch.device, *args) -> int:
     argument).  The device guard and the stream object cost more than a short
     launch, so the guard is taken only where another device is current."""
     fn = getattr(_lib or load(), name)
-    if torch.cuda.current_device() == dev.index:
+    if torch._C._cuda_getDevice() == dev.index:
         return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     with torch.cuda.device(dev):
         return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))

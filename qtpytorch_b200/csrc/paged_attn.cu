@@ -3,30 +3,43 @@
 //
 //   s_j = scale * sk_j (q . kc_j),  o = sum_j exp(s_j - m) sv_j vc_j / sum_j exp(s_j - m)
 //
-// with int8 / int4 codes kc, vc and one scale per key and head.  The codes are
-// small integers, exact in bf16: they go to the MMAs as they are, sk_j
-// multiplies a score and sv_j a probability, so a key costs two fp32
-// multiplies a row instead of 2 D.  One pass with a running maximum and sum;
-// both, and the outputs, are fp32.  Probabilities are rounded to bf16 for
-// their product (2^-9 relative each, as the output itself is).
+// with int8 / int4 codes kc, vc and one scale per key and head.  One pass with
+// a running maximum and sum; both, and the outputs, are fp32.
 //
-// The problem is bound by the bytes of the codes for few query rows.  A warp
-// is on its own: it walks tiles of 32 keys through a private ring of shared
-// memory that its own lanes fill by TMA (the pool is a matrix of head rows, a
-// box never leaves a page), so there is no block-wide barrier in the loop and
-// all of a CTA's rings are in flight at once.  The products run transposed,
-// S^T = K Q^T and O^T = V^T P^T: keys (then head dims) take the 16 rows of the
-// MMA and query rows its 8 columns, so 8 grouped heads waste nothing.  K rows
-// and V columns come from ldmatrix as 16-bit pairs of codes, and the order of
-// the contraction index is permuted (the same for Q) to what the byte order of
-// the codes gives, so that unpacking is two or three instructions a pair.
+// The codes are small integers and go to the MMAs as such (bf16 or fp16, both
+// exact): sk_j multiplies a score, and sv_j joins the exponent of the weight
+// of the second product, exp2(s_j + log2 sv_j - m'), with a running maximum m'
+// of its own.  The weights are then at most 1 with a 1 in every row's range,
+// so fp16 (11 bits) holds them whatever the scales are, and a key costs a few
+// fp32 operations a row instead of 2 D.
 //
-// Work is split over keys when there are few rows; partial results (m, l, O)
-// are joined by a second kernel, as are the prefix's and the sequences' own.
+// For few query rows the bytes of the codes are the bound.  A warp is on its
+// own: it walks tiles of 32 keys through a private ring of shared memory that
+// its own lanes fill by TMA (the pool is a matrix of head rows, a box never
+// leaves a page), so there is no block-wide barrier in the loop and all of a
+// CTA's rings are in flight at once.  The products run transposed, S^T = K Q^T
+// and O^T = V^T P^T: keys (then head dims) take the 16 rows of the MMA and
+// query rows its 8 columns, so 8 grouped heads waste nothing.  K rows and V
+// columns come from ldmatrix as 16-bit pairs of codes, and the order of the
+// contraction index is permuted (the same for Q) to what the byte order of the
+// codes gives.  Unpacking: a mask and an exclusive or put a code under a fixed
+// exponent, which leaves code + offset; for K the offset is taken out once, in
+// the accumulator's start -offset * sum(q) (eight products deep, so the
+// cancellation costs under 2^-14 of a score's own rounding to bf16 inputs),
+// for V by one packed subtraction.
+//
+// Work: the tiles of all sequences, heads and row groups form one list, which
+// the CTAs share out in equal runs (lengths are known on the device only), so
+// a batch of very different lengths keeps every SM busy to the end.  A run may
+// hold several units or a part of one; a unit's first part goes to a row
+// buffer, a later part to its CTA's buffer, and a second kernel joins them
+// with the parts of the shared prefix.  Rows with a single part are written
+// directly.
 #include "mxb_common.cuh"
 #include "mxb_internal.h"
 
 #include <cuda.h>
+#include <cuda_fp16.h>
 
 #define MXB_ERROR_WORD_BY_POINTER
 #include "tc_ptx.cuh"
@@ -39,21 +52,34 @@ namespace pattn {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 32;    // keys per warp tile
-constexpr int kStages = 3;
 
-template <int BITS, int D>
+template <int BITS, int D, int NT>
 struct Geo {
   static constexpr int RB = D * BITS / 8;       // bytes of a head row: 128, 64 or 32
   static constexpr int kTileBytes = kTile * RB;
-  static constexpr int kRing = kStages * (2 * kTileBytes + 2 * kTile * 4);
-  static constexpr CUtensorMapSwizzle kSwz = RB == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-                                             : RB == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                        : CU_TENSOR_MAP_SWIZZLE_32B;
+  // ring depth and CTAs per SM: about 150 KB in flight an SM
+  static constexpr int kStages = RB == 128 ? 3 : RB == 64 ? 4 : 6;
+  static constexpr int kCtas = NT >= 2 ? 2 : RB == 128 ? 2 : RB == 64 ? 3 : 4;
+  static constexpr int R = 8 * NT;              // query rows per CTA
+  static constexpr int kPitch = D + 4;          // floats of a row in the join buffer
+  static constexpr size_t kRing = (size_t)kWarps * kStages * (2 * kTileBytes + 2 * kTile * 4);
+  static constexpr size_t kJoin = (size_t)kWarps * R * kPitch * 4;
+  // with few rows the join buffer lies beside the ring, so the next unit's
+  // loads start before the join
+  static constexpr bool kApart = NT <= 2;
+  static constexpr size_t kSmem = 1024 + (kApart ? kRing + kJoin : kRing > kJoin ? kRing : kJoin);
   // byte offset of 16-byte chunk c of row r in a tile (the TMA swizzle)
   __device__ static uint32_t at(int r, int c) {
     const int x = RB == 128 ? (r & 7) : RB == 64 ? ((r >> 1) & 3) : ((r >> 2) & 1);
     return (uint32_t)(r * RB + ((c ^ x) << 4));
   }
+};
+
+// Results of a key range: [rows][D] weighted sums relative to 2^m', and
+// (m, l, m', 0) per row.
+struct Part {
+  float* o;
+  float4* ml;
 };
 
 struct Args {
@@ -68,14 +94,14 @@ struct Args {
   int prefix_len;
   int rows;                // query rows per unit (T * G, or B * T * G for the prefix)
   int row_tiles;           // per unit and KV head
-  int splits;
+  int splits;              // prefix: CTAs over the keys
   float scale_log2;
-  // outputs: partials [part][row][D] / [part][row][2], or the result itself
-  float* po;
-  float* pml;
-  int part0;
+  Part main, cta;          // sequences: by output row / by CTA; prefix: main by split and row
+  int64_t* plan;           // [0] tiles per CTA, [1 + b] first tile of sequence b
   int64_t n_rows;          // B * T * Hq
-  __nv_bfloat16* out;      // direct result (one part), else null
+  bool whole;              // one unit per CTA, no plan
+  bool direct;             // rows with one part go straight to out
+  __nv_bfloat16* out;
   float* lse;
   int* err;
 };
@@ -97,21 +123,33 @@ __device__ __forceinline__ uint32_t movm(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
+template <bool HALF>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if constexpr (HALF)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t bsub2(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t hsub2u(uint32_t a, uint32_t b) {
   uint32_t d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 __device__ __forceinline__ uint32_t bf2(float lo, float hi) {
   const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+__device__ __forceinline__ uint32_t hf2(float lo, float hi) {
+  const __half2 t = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&t);
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -119,85 +157,177 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-
-// Bytes 0 and 2 of w, two's complement int8 -> bf16 pair: with u the low seven
-// bits and s the sign, (128 + u) - (128 + 128 s), all three exact in bf16.
-__device__ __forceinline__ uint32_t i8pair(uint32_t w) {
-  return bsub2((w & 0x007F007Fu) | 0x43004300u, (w & 0x00800080u) | 0x43004300u);
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-// Low nibbles of both halves of w, two's complement int4 -> bf16 pair:
-// (128 + (code + 8)) - 136.
-__device__ __forceinline__ uint32_t i4pair(uint32_t w) {
-  return bsub2((w & 0x000F000Fu) ^ 0x43084308u, 0x43084308u);
-}
+// 2^(x - ref) of a running maximum; nothing seen yet gives 0
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
 
-// Index within a 16-value contraction step of the pairs that the code bytes
-// give: the k-th value (0..7 of the lane's eight a 32-value chunk, 0..3 of the
-// four a 16-value chunk) that pair p (b0 / b1 of step st) holds.
+// Two codes as 16-bit floats.  int8: bytes 0 and 2 of w, fp16 1152 + code
+// ((code + 128) in the mantissa of 1024).  int4: low nibbles of both halves;
+// for K bf16 136 + code ((code + 8) in the mantissa of 128), for V fp16
+// 1032 + code.
 template <int BITS>
-__device__ __forceinline__ int qdim(int step, int c, int pair, int e) {
-  if (BITS == 8) return step * 16 + 4 * c + pair + 2 * e;  // bytes (0, 2), then (1, 3)
-  const int i = (step & 1) * 2 + pair;                     // nibbles (i, i + 4)
-  return (step >> 1) * 32 + 8 * c + i + 4 * e;
+struct Codes;
+template <>
+struct Codes<8> {
+  static constexpr float kOffset = 1152.0f;
+  static constexpr bool kHalfQ = true;
+  __device__ static uint32_t k(uint32_t w) { return (w & 0x00FF00FFu) ^ 0x64806480u; }
+  __device__ static uint32_t v(uint32_t w) { return hsub2u(k(w), 0x64806480u); }
+};
+template <>
+struct Codes<4> {
+  static constexpr float kOffset = 136.0f;
+  static constexpr bool kHalfQ = false;
+  __device__ static uint32_t k(uint32_t w) { return (w & 0x000F000Fu) ^ 0x43084308u; }
+  __device__ static uint32_t v(uint32_t w) {
+    return hsub2u((w & 0x000F000Fu) ^ 0x64086408u, 0x64086408u);
+  }
+};
+
+// Sum over the block (kThreads) of one value a thread, and its exclusive prefix.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& before, int64_t* sm) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += t;
+  }
+  if (lane == 31) sm[warp] = inc;
+  __syncthreads();
+  int64_t total = 0, pre = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) pre += sm[w];
+    total += sm[w];
+  }
+  __syncthreads();
+  before = pre + inc - v;
+  return total;
 }
 
 template <int BITS, int D, int NT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
     paged_attn_kernel(const __grid_constant__ CUtensorMap tmap_k,
                       const __grid_constant__ CUtensorMap tmap_v, const Args a) {
-  using Ge = Geo<BITS, D>;
-  constexpr int kSteps = D / 16, kMT = D / 16;
-  constexpr int R = 8 * NT;  // query rows per CTA
+  using Ge = Geo<BITS, D, NT>;
+  using Cd = Codes<BITS>;
+  constexpr int kSteps = D / 16, kMT = D / 16, kStages = Ge::kStages;
+  constexpr int R = Ge::R;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   __shared__ uint64_t full[kWarps][kStages];
-  __shared__ float sm_m[kWarps][R], sm_l[kWarps][R];
+  __shared__ float sm_m[kWarps][R], sm_l[kWarps][R], sm_v[kWarps][R];
+  __shared__ int64_t sm_scan[kWarps], sm_off;
+  __shared__ int sm_b;
+  // with many rows the query fragments, the same for all warps, live in
+  // shared memory: in registers they would spill
+  constexpr bool kQs = NT >= 3 && D == 128;
+  __shared__ uint2 sq[kQs ? NT * kSteps * 32 : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-
-  pdl_trigger();
-  pdl_wait();
-  const int split = blockIdx.x;
-  const int h = blockIdx.y / a.row_tiles, r0 = (blockIdx.y % a.row_tiles) * R;
-  const int unit = blockIdx.z;
-  const bool own = a.lengths != nullptr;
-  int len = own ? a.lengths[unit] : a.prefix_len;
-  const int64_t cap = (int64_t)a.width << a.page_shift;
-  if (len > cap) {
-    if (threadIdx.x == 0 && a.err) atomicCAS(a.err, 0, kErrIndex);
-    len = (int)cap;
-  }
-  len = max(len, 0);
-  const int tiles = (len + kTile - 1) / kTile;
-  const int per = (tiles + a.splits - 1) / a.splits;
-  const int t_lo = min(split * per, tiles), t_hi = min(t_lo + per, tiles);
-  const int* table = a.table + (own ? (int64_t)unit * a.width : 0);
 
   // ring of this warp: [stages][K tile][V tile], then the scales
   uint8_t* ring = smem + warp * (kStages * 2 * Ge::kTileBytes);
   float* rs = reinterpret_cast<float*>(smem + kWarps * kStages * 2 * Ge::kTileBytes) +
               warp * (kStages * 2 * kTile);
+  float* join = reinterpret_cast<float*>(smem + (Ge::kApart ? Ge::kRing : 0));
   const int boxes = kTile / a.box;
   if (lane == 0) {
     for (int s = 0; s < kStages; ++s) mbar_init(&full[warp][s], boxes);
     fence_barrier_init();
   }
   __syncwarp();
+  pdl_trigger();
+  pdl_wait();
+
+  const bool own = a.lengths != nullptr;
+  const int hr = a.H * a.row_tiles;  // units per sequence
+  const int64_t cap = (int64_t)a.width << a.page_shift;
+  auto len_of = [&](int b) -> int {
+    int n = own ? __ldg(a.lengths + b) : a.prefix_len;
+    return (int)min((int64_t)max(n, 0), cap);
+  };
+  auto tiles_of = [&](int n) { return (n + kTile - 1) / kTile; };
+
+  // ── this CTA's run of the tile list ──
+  int b = 0, u = 0;             // sequence, unit within it
+  int t_lo = 0, t_hi = 0;       // tiles of the current segment
+  int64_t left = 0;             // tiles of the run, the segment's included
+  int len, n_tiles;
+  if (!own) {  // prefix: blockIdx.x = split, blockIdx.y = unit
+    u = blockIdx.y;
+    len = len_of(0);
+    n_tiles = tiles_of(len);
+    const int per = (n_tiles + a.splits - 1) / a.splits;
+    t_lo = min((int)blockIdx.x * per, n_tiles);
+    t_hi = min(t_lo + per, n_tiles);
+    left = t_hi - t_lo;
+  } else if (a.whole) {
+    b = blockIdx.x / hr;
+    u = blockIdx.x - b * hr;
+    len = len_of(b);
+    n_tiles = tiles_of(len);
+    t_hi = n_tiles;
+    left = n_tiles;
+  } else {
+    int64_t total = 0, before;
+    for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+      const int i = b0 + threadIdx.x;
+      int n = 0;
+      if (i < a.B) {
+        n = __ldg(a.lengths + i);
+        if (n > cap && blockIdx.x == 0 && a.err) atomicCAS(a.err, 0, kErrIndex);
+        n = tiles_of((int)min((int64_t)max(n, 0), cap));
+      }
+      total += block_scan((int64_t)n * hr, before, sm_scan);
+    }
+    // equal runs, at least a tile a warp
+    const int64_t per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kWarps);
+    const int64_t lo = blockIdx.x * per, hi = min(lo + per, total);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = per;
+    int64_t base = 0;
+    for (int b0 = 0; b0 < a.B && (blockIdx.x == 0 || base <= lo); b0 += kThreads) {
+      const int i = b0 + threadIdx.x;
+      const int64_t n = i < a.B ? (int64_t)tiles_of(len_of(i)) * hr : 0;
+      const int64_t sum = block_scan(n, before, sm_scan);
+      before += base;
+      if (i < a.B && blockIdx.x == 0) a.plan[1 + i] = before;
+      if (lo < hi && lo >= before && lo < before + n) {
+        sm_b = i;
+        sm_off = before;
+      }
+      base += sum;
+    }
+    __syncthreads();
+    if (lo >= hi) return;
+    b = sm_b;
+    len = len_of(b);
+    n_tiles = tiles_of(len);
+    u = (int)((lo - sm_off) / n_tiles);
+    t_lo = (int)((lo - sm_off) - (int64_t)u * n_tiles);
+    left = hi - lo;
+    t_hi = (int)min((int64_t)n_tiles, t_lo + left);
+  }
 
   const int page_mask = (1 << a.page_shift) - 1;
   // page numbers are fetched one tile before the copies that need them
   auto page_of = [&](int tile) -> int {
     const int pos = tile * kTile + lane * a.box;
     if (lane >= boxes || tile >= t_hi || pos >= len) return -1;
-    int p = __ldg(table + (pos >> a.page_shift));
+    int p = __ldg(a.table + (own ? (int64_t)b * a.width : 0) + (pos >> a.page_shift));
     if (p < 0 || p >= a.n_pages) {
       if (a.err) atomicCAS(a.err, 0, kErrIndex);
       p = 0;
     }
     return p;
   };
-  auto issue = [&](int tile, int s, int p) {
+  auto issue = [&](int tile, int h, int s, int p) {
     if (lane < boxes) {
       if (p >= 0) {
         const int pos = tile * kTile + lane * a.box;
@@ -216,296 +346,448 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
   };
-
-  // fill the ring
   int next_page = -1;
-  {
+  uint32_t it = 0;  // tiles consumed by this warp: stage it % kStages, round it / kStages
+  auto fill = [&]() {
     int pg[kStages];
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) pg[s] = page_of(t_lo + warp + s * kWarps);
+    for (int i = 0; i < kStages; ++i) pg[i] = page_of(t_lo + warp + i * kWarps);
 #pragma unroll
-    for (int s = 0; s < kStages; ++s)
-      if (t_lo + warp + s * kWarps < t_hi) issue(t_lo + warp + s * kWarps, s, pg[s]);
+    for (int i = 0; i < kStages; ++i)
+      if (t_lo + warp + i * kWarps < t_hi)
+        issue(t_lo + warp + i * kWarps, u / a.row_tiles, (it + i) % kStages, pg[i]);
     next_page = page_of(t_lo + warp + kStages * kWarps);
-  }
-
-  // query rows as B fragments (columns = rows r0 + 8 n + g), and the number
-  // of keys that each of this lane's two columns per n-tile sees
-  uint32_t qf[NT][kSteps][2];
-  int limit[NT][2];
-  int lim_min = len;
-  auto row_id = [&](int r, int& t) -> int64_t {  // row of the unit -> row of the output
-    int b = unit, rr = r;
-    if (!own) {
-      b = r / (a.T * a.G);
-      rr = r - b * a.T * a.G;
-    }
-    t = rr / a.G;
-    return ((int64_t)b * a.T + t) * ((int64_t)a.H * a.G) + (int64_t)h * a.G + (rr - t * a.G);
   };
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r = r0 + 8 * n + g;
-    int t;
-    const bool live = r < a.rows;
-    const __nv_bfloat16* qp = a.q + (live ? row_id(r, t) : 0) * D;
-#pragma unroll
-    for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const uint16_t lo = live ? __bfloat16_as_ushort(qp[qdim<BITS>(st, c, p, 0)]) : 0;
-        const uint16_t hi = live ? __bfloat16_as_ushort(qp[qdim<BITS>(st, c, p, 1)]) : 0;
-        qf[n][st][p] = (uint32_t)lo | ((uint32_t)hi << 16);
-      }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int rr = r0 + 8 * n + 2 * c + e;
-      limit[n][e] = len;
-      if (own && rr < a.rows) limit[n][e] = len - (a.T - 1 - rr / a.G);
-    }
-  }
-  if (own) lim_min = len - (a.T - 1);
-
-  float o[kMT][NT][4];
-  float m[NT][2], l[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int j = 0; j < kMT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[j][n][e] = 0.0f;
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n][0] = l[n][1] = 0.0f;
-  }
+  fill();
 
   bool ok = true;
-  int it = 0;
-  for (int tile = t_lo + warp; tile < t_hi; tile += kWarps, ++it) {
-    const int s = it % kStages;
-    ok = mbar_wait_warp_to(&full[warp][s], (it / kStages) & 1, kErrTimeoutFull, a.err);
-    if (!ok) break;
-    const uint32_t kt = smem_u32(ring + s * 2 * Ge::kTileBytes);
-    const uint32_t vt = kt + Ge::kTileBytes;
-    const float* sc = rs + s * 2 * kTile;
+  while (true) {
+    const int h = u / a.row_tiles, r0 = (u - h * a.row_tiles) * R;
+    const bool first = t_lo == 0, last = t_hi == n_tiles;
+    auto row_id = [&](int r) -> int64_t {  // row of the unit -> row of the output
+      int bb = b, rr = r;
+      if (!own) {
+        bb = r / (a.T * a.G);
+        rr = r - bb * a.T * a.G;
+      }
+      const int t = rr / a.G;
+      return ((int64_t)bb * a.T + t) * ((int64_t)a.H * a.G) + (int64_t)h * a.G + (rr - t * a.G);
+    };
 
-    // ── S^T = K Q^T: 32 keys x R rows ──
-    float sa[2][NT][4];
+    // query rows as B fragments (columns = rows r0 + 8 n + g), the sum that
+    // takes the codes' offset out, and how many keys each of this lane's two
+    // columns per n-tile sees
+    uint32_t qf[NT][kSteps][2];
+    float start[NT][2], cfac[NT][2];
+    int limit[NT][2];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+    for (int n = 0; n < NT; ++n) {
+      const int r = r0 + 8 * n + g;
+      const bool live = r < a.rows;
+      const uint4* qp = reinterpret_cast<const uint4*>(a.q + (live ? row_id(r) : 0) * D);
+      uint32_t raw[kSteps][2];  // bf16 pairs in memory order, 4 values a step
+      if (BITS == 8) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sa[mt][n][e] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < Ge::RB / 16; ++j) {
-      uint32_t w[4];
-      ldsm4(kt + Ge::at(lane, j), w);
-      if constexpr (BITS == 8) {
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const uint32_t a0 = i8pair(w[2 * mt]), a1 = i8pair(w[2 * mt + 1]);
-          const uint32_t a2 = i8pair(w[2 * mt] >> 8), a3 = i8pair(w[2 * mt + 1] >> 8);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816(sa[mt][n], a0, a1, a2, a3, qf[n][j][0], qf[n][j][1]);
+        for (int st = 0; st < kSteps; ++st) {  // values 16 st + 4 c ..
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(qp) + st * 4 + c);
+          raw[st][0] = w.x;
+          raw[st][1] = w.y;
         }
       } else {
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const uint32_t a0 = i4pair(w[2 * mt] >> (8 * z)), a1 = i4pair(w[2 * mt + 1] >> (8 * z));
-            const uint32_t a2 = i4pair(w[2 * mt] >> (8 * z + 4));
-            const uint32_t a3 = i4pair(w[2 * mt + 1] >> (8 * z + 4));
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              mma16816(sa[mt][n], a0, a1, a2, a3, qf[n][2 * j + z][0], qf[n][2 * j + z][1]);
-          }
-      }
-    }
-    // ── scores, running maximum ──
-    float kscale[4], vscale[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      kscale[i] = sc[8 * i + g] * a.scale_log2;
-      vscale[i] = sc[kTile + 8 * i + g];
-    }
-    const int key0 = tile * kTile + g;
-    const bool ragged = (tile + 1) * kTile > lim_min;  // some key is hidden from some row
-    uint32_t pb[2][NT][2];
-    bool grew = false;
-    float alpha[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float& v = sa[i >> 1][n][(i & 1) * 2 + e];
-          v *= kscale[i];
-          if (ragged && key0 + 8 * i >= limit[n][e]) v = -INFINITY;
-          mx[e] = fmaxf(mx[e], v);
+        for (int j = 0; j < kSteps / 2; ++j) {  // values 32 j + 8 c ..
+          const uint4 w = __ldg(qp + j * 4 + c);
+          raw[2 * j][0] = w.x;
+          raw[2 * j][1] = w.y;
+          raw[2 * j + 1][0] = w.z;
+          raw[2 * j + 1][1] = w.w;
         }
+      }
+      float sum = 0.0f, fac = 1.0f;
+      if constexpr (BITS == 8) {
+        // bf16 -> fp16 under a power of two that puts the row's largest value
+        // into [2^14, 2^15): eight bits of every value down to 2^-29 of it
+        float top = 0.0f;
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            if (!live) raw[st][p] = 0u;
+            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(raw[st][p] << 16)),
+                                   fabsf(__uint_as_float(raw[st][p] & 0xffff0000u))));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int ex = (int)(__float_as_uint(top) >> 23);  // biased
+        // 2^(14 - (ex - 127)), at most 2^100
+        const int up = ex == 0 || ex == 255 ? 127 : min(127 + 14 + 127 - ex, 227);
+        const float f = __uint_as_float((uint32_t)up << 23);
+        fac = __uint_as_float((uint32_t)(254 - up) << 23);  // its inverse
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+          const float v0 = __uint_as_float(raw[st][0] << 16) * f;
+          const float v1 = __uint_as_float(raw[st][0] & 0xffff0000u) * f;
+          const float v2 = __uint_as_float(raw[st][1] << 16) * f;
+          const float v3 = __uint_as_float(raw[st][1] & 0xffff0000u) * f;
+          qf[n][st][0] = hf2(v0, v2);  // bytes 0, 2 of a code word, then 1, 3
+          qf[n][st][1] = hf2(v1, v3);
+          const float2 s0 = __half22float2(*reinterpret_cast<__half2*>(&qf[n][st][0]));
+          const float2 s1 = __half22float2(*reinterpret_cast<__half2*>(&qf[n][st][1]));
+          sum += (s0.x + s0.y) + (s1.x + s1.y);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kSteps / 2; ++j) {
+          uint32_t x[4] = {raw[2 * j][0], raw[2 * j][1], raw[2 * j + 1][0], raw[2 * j + 1][1]};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (!live) x[i] = 0u;
+            sum += __uint_as_float(x[i] << 16) + __uint_as_float(x[i] & 0xffff0000u);
+          }
+          // values (i, i + 4): nibbles i of the two halves of a code word
+          qf[n][2 * j][0] = __byte_perm(x[0], x[2], 0x5410);
+          qf[n][2 * j][1] = __byte_perm(x[0], x[2], 0x7632);
+          qf[n][2 * j + 1][0] = __byte_perm(x[1], x[3], 0x5410);
+          qf[n][2 * j + 1][1] = __byte_perm(x[1], x[3], 0x7632);
+        }
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum *= -Cd::kOffset;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int w = 4; w < 32; w <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], w));
-        const float mn = fmaxf(m[n][e], mx[e]);
-        const float mu = mn == -INFINITY ? 0.0f : mn;  // no key yet: every weight is 0
-        alpha[n][e] = ex2(m[n][e] - mu);
-        grew |= mn != m[n][e];
-        m[n][e] = mn;
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float& v = sa[i >> 1][n][(i & 1) * 2 + e];
-          const float p = ex2(v - mu);
-          sum += p;
-          // a hidden key's scale may be anything, NaN included
-          v = (ragged && key0 + 8 * i >= limit[n][e]) ? 0.0f : p * vscale[i];
-        }
-        l[n][e] = l[n][e] * alpha[n][e] + sum;
+        start[n][e] = __shfl_sync(0xffffffffu, sum, (2 * c + e) * 4);
+        cfac[n][e] = __shfl_sync(0xffffffffu, fac, (2 * c + e) * 4);
+        const int rr = r0 + 8 * n + 2 * c + e;
+        limit[n][e] = len;
+        if (own && rr < a.rows) limit[n][e] = len - (a.T - 1 - rr / a.G);
       }
-      // keys x rows -> rows x keys: the B fragment of the second product
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        pb[i >> 1][n][i & 1] = movm(bf2(sa[i >> 1][n][(i & 1) * 2], sa[i >> 1][n][(i & 1) * 2 + 1]));
     }
-    if (__any_sync(0xffffffffu, grew)) {
+    const int lim_min = own ? len - (a.T - 1) : len;
+    if constexpr (kQs) {
+      if (warp == 0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st)
+            sq[(n * kSteps + st) * 32 + lane] = make_uint2(qf[n][st][0], qf[n][st][1]);
+      }
+      __syncthreads();
+    }
+    auto q_of = [&](int n, int st) -> uint2 {
+      if constexpr (kQs) return sq[(n * kSteps + st) * 32 + lane];
+      else return make_uint2(qf[n][st][0], qf[n][st][1]);
+    };
+
+    float o[kMT][NT][4];
+    float m[NT][2], l[NT][2], mv[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int j = 0; j < kMT; ++j)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          o[j][n][0] *= alpha[n][0];
-          o[j][n][1] *= alpha[n][1];
-          o[j][n][2] *= alpha[n][0];
-          o[j][n][3] *= alpha[n][1];
-        }
+        for (int e = 0; e < 4; ++e) o[j][n][e] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[n][e] = mv[n][e] = -INFINITY;
+        l[n][e] = 0.0f;
+      }
     }
-    // ── O^T += V^T P^T ──
+
+    for (int tile = t_lo + warp; tile < t_hi; tile += kWarps, ++it) {
+      const int s = it % kStages;
+      ok = ok && mbar_wait_warp_to(&full[warp][s], (it / kStages) & 1, kErrTimeoutFull, a.err);
+      const uint32_t kt = smem_u32(ring + s * 2 * Ge::kTileBytes);
+      const uint32_t vt = kt + Ge::kTileBytes;
+      const float* sc = rs + s * 2 * kTile;
+
+      // ── S^T = K Q^T: 32 keys x R rows ──
+      float sa[2][NT][4];
 #pragma unroll
-    for (int j = 0; j < Ge::RB / 16; ++j) {
-      uint32_t w[4];
-      ldsm4t(vt + Ge::at(lane, j), w);
-      if constexpr (BITS == 8) {
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const uint32_t a0 = i8pair(w[2 * mt]), a1 = i8pair(w[2 * mt] >> 8);
-          const uint32_t a2 = i8pair(w[2 * mt + 1]), a3 = i8pair(w[2 * mt + 1] >> 8);
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816(o[j][n], a0, a1, a2, a3, pb[mt][n][0], pb[mt][n][1]);
+          for (int e = 0; e < 4; ++e) sa[mt][n][e] = start[n][e & 1];
+#pragma unroll
+      for (int j = 0; j < Ge::RB / 16; ++j) {
+        uint32_t w[4];
+        ldsm4(kt + Ge::at(lane, j), w);
+        constexpr int Z = BITS == 8 ? 1 : 2, SH = BITS;  // steps a chunk; shift to the second pair
+#pragma unroll
+        for (int z = 0; z < Z; ++z) {
+          uint32_t f[2][4];
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            f[mt][0] = Cd::k(w[2 * mt] >> (8 * z));
+            f[mt][1] = Cd::k(w[2 * mt + 1] >> (8 * z));
+            f[mt][2] = Cd::k(w[2 * mt] >> (8 * z + SH));
+            f[mt][3] = Cd::k(w[2 * mt + 1] >> (8 * z + SH));
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint2 qv = q_of(n, Z * j + z);
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+              mma16816<Cd::kHalfQ>(sa[mt][n], f[mt][0], f[mt][1], f[mt][2], f[mt][3], qv.x, qv.y);
+          }
         }
-      } else {
+      }
+      // ── scores, running maxima, weights ──
+      float kscale[4], lv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        kscale[i] = sc[8 * i + g] * a.scale_log2;
+        lv[i] = lg2(sc[kTile + 8 * i + g]);
+      }
+      const int key0 = tile * kTile + g;
+      const bool ragged = (tile + 1) * kTile > lim_min;  // some key is hidden from some row
+      uint32_t pb[2][NT][2];
+      bool grew = false;
+      float alpha[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float wv[4][2];  // s + log2 sv
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = -INFINITY, mw = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float v = sa[i >> 1][n][(i & 1) * 2 + e] * kscale[i];
+            if (BITS == 8) v *= cfac[n][e];
+            float w = v + lv[i];
+            if (ragged && key0 + 8 * i >= limit[n][e]) v = w = -INFINITY;  // whatever its scales hold
+            sa[i >> 1][n][(i & 1) * 2 + e] = v;
+            wv[i][e] = w;
+            mx = fmaxf(mx, v);
+            mw = fmaxf(mw, w);
+          }
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) {
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, x));
+          }
+          mx = fmaxf(m[n][e], mx);
+          mw = fmaxf(mv[n][e], mw);
+          const float mu = base_of(mx), wu = base_of(mw);
+          alpha[n][e] = ex2(mv[n][e] - wu);
+          grew |= mw != mv[n][e];
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sum += ex2(sa[i >> 1][n][(i & 1) * 2 + e] - mu);
+            wv[i][e] = ex2(wv[i][e] - wu);
+          }
+          l[n][e] = l[n][e] * ex2(m[n][e] - mu) + sum;
+          m[n][e] = mx;
+          mv[n][e] = mw;
+        }
+        // keys x rows -> rows x keys: the B fragment of the second product
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pb[i >> 1][n][i & 1] = movm(hf2(wv[i][0], wv[i][1]));
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int j = 0; j < kMT; ++j)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][n][e] *= alpha[n][e & 1];
+      }
+      // ── O^T += V^T P^T ──
+#pragma unroll
+      for (int j = 0; j < Ge::RB / 16; ++j) {
+        uint32_t w[4];
+        ldsm4t(vt + Ge::at(lane, j), w);
+        constexpr int Z = BITS == 8 ? 1 : 2, SH = BITS;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const uint32_t a0 = i4pair(w[2 * mt] >> (8 * z)), a1 = i4pair(w[2 * mt] >> (8 * z + 4));
-            const uint32_t a2 = i4pair(w[2 * mt + 1] >> (8 * z));
-            const uint32_t a3 = i4pair(w[2 * mt + 1] >> (8 * z + 4));
+          for (int z = 0; z < Z; ++z) {
+            const uint32_t a0 = Cd::v(w[2 * mt] >> (8 * z)), a1 = Cd::v(w[2 * mt] >> (8 * z + SH));
+            const uint32_t a2 = Cd::v(w[2 * mt + 1] >> (8 * z));
+            const uint32_t a3 = Cd::v(w[2 * mt + 1] >> (8 * z + SH));
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-              mma16816(o[2 * j + z][n], a0, a1, a2, a3, pb[mt][n][0], pb[mt][n][1]);
+              mma16816<true>(o[Z * j + z][n], a0, a1, a2, a3, pb[mt][n][0], pb[mt][n][1]);
           }
       }
-    }
-    __syncwarp();  // the stage is read
-    const int nt = tile + kStages * kWarps;
-    if (nt < t_hi) {
-      issue(nt, s, next_page);
-      next_page = page_of(nt + kWarps);
-    }
-  }
-
-  // ── join the warps ──
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
-      if (g == 0) {
-        sm_m[warp][8 * n + 2 * c + e] = m[n][e];
-        sm_l[warp][8 * n + 2 * c + e] = l[n][e];
+      __syncwarp();  // the stage is read
+      const int nt = tile + kStages * kWarps;
+      if (nt < t_hi) {
+        issue(nt, h, s, next_page);
+        next_page = page_of(nt + kWarps);
       }
     }
-  __syncthreads();  // every ring is idle
-  constexpr int P = D + 4;  // row pitch in floats
-  float* so = reinterpret_cast<float*>(smem) + warp * R * P;
-#pragma unroll
-  for (int j = 0; j < kMT; ++j) {
-    // dims of this lane's accumulator rows g and g + 8
-    const int d = BITS == 8 ? 16 * j + 2 * g : 32 * (j >> 1) + 4 * g + 2 * (j & 1);
+
+    // ── the next segment, its loads already in flight during the join ──
+    const int cb = b, cu = u;
+    left -= t_hi - t_lo;
+    const bool more = left > 0;
+    if (more) {
+      t_lo = 0;
+      if (++u == hr) {
+        u = 0;
+        do {  // sequences without keys have no tiles
+          ++b;
+          len = len_of(b);
+        } while (len == 0);
+        n_tiles = tiles_of(len);
+      }
+      t_hi = (int)min((int64_t)n_tiles, left);
+      if (Ge::kApart) fill();
+    }
+
+    // ── join the warps ──
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        *reinterpret_cast<float2*>(so + (8 * n + 2 * c + e) * P + d) =
-            make_float2(o[j][n][e], o[j][n][2 + e]);
-  }
-  __syncthreads();
-  const float* s0 = reinterpret_cast<const float*>(smem);
-  for (int u = threadIdx.x; u < R * (D / 4); u += kThreads) {
-    const int r = u / (D / 4), d = (u % (D / 4)) * 4;
-    if (r0 + r >= a.rows) break;
-    float mx = -INFINITY;
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm_m[w][r]);
-    const float mu = mx == -INFINITY ? 0.0f : mx;
-    float sum = 0.0f;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
+        if (g == 0) {
+          sm_m[warp][8 * n + 2 * c + e] = m[n][e];
+          sm_l[warp][8 * n + 2 * c + e] = l[n][e];
+          sm_v[warp][8 * n + 2 * c + e] = mv[n][e];
+        }
+      }
+    if (!Ge::kApart) __syncthreads();  // every ring is idle
+    constexpr int P = Ge::kPitch;
+    float* so = join + warp * R * P;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2(sm_m[w][r] - mu);
-      const float4 x = *reinterpret_cast<const float4*>(s0 + (w * R + r) * P + d);
-      sum += f * sm_l[w][r];
-      v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w;
+    for (int j = 0; j < kMT; ++j) {
+      // dims of this lane's accumulator rows g and g + 8
+      const int d = BITS == 8 ? 16 * j + 2 * g : 32 * (j >> 1) + 4 * g + 2 * (j & 1);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<float2*>(so + (8 * n + 2 * c + e) * P + d) =
+              make_float2(o[j][n][e], o[j][n][2 + e]);
     }
-    int t;
-    const int64_t id = row_id(r0 + r, t);
-    if (a.out) {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      *reinterpret_cast<uint2*>(a.out + id * D + d) =
-          make_uint2(bf2(v.x * inv, v.y * inv), bf2(v.z * inv, v.w * inv));
-      if (a.lse && d == 0)
-        a.lse[id] = sum == 0.0f ? -INFINITY : (mu + __log2f(sum)) * 0.69314718055994531f;
-    } else {
-      const int64_t pr = (int64_t)(a.part0 + split) * a.n_rows + id;
-      *reinterpret_cast<float4*>(a.po + pr * D + d) = v;
-      if (d == 0) *reinterpret_cast<float2*>(a.pml + pr * 2) = make_float2(mx, sum);
+    __syncthreads();
+    const bool direct = a.direct && first && last;
+    for (int i = threadIdx.x; i < R * (D / 4); i += kThreads) {
+      const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+      if (r0 + r >= a.rows) break;
+      float mx = -INFINITY, mw = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        mx = fmaxf(mx, sm_m[w][r]);
+        mw = fmaxf(mw, sm_v[w][r]);
+      }
+      const float mu = base_of(mx), wu = base_of(mw);
+      float sum = 0.0f;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = ex2(sm_v[w][r] - wu);
+        const float4 x = *reinterpret_cast<const float4*>(join + (w * R + r) * P + d);
+        sum += ex2(sm_m[w][r] - mu) * sm_l[w][r];
+        v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w;
+      }
+      // row of the output: the unit's h and b are those before the advance
+      int bb = cb, rr = r0 + r;
+      if (!own) {
+        bb = rr / (a.T * a.G);
+        rr -= bb * a.T * a.G;
+      }
+      const int t = rr / a.G, hh = cu / a.row_tiles;
+      const int64_t id = ((int64_t)bb * a.T + t) * ((int64_t)a.H * a.G) + (int64_t)hh * a.G + (rr - t * a.G);
+      if (direct) {
+        const float inv = sum == 0.0f ? 0.0f : ex2(wu - mu) / sum;
+        *reinterpret_cast<uint2*>(a.out + id * D + d) =
+            make_uint2(bf2(v.x * inv, v.y * inv), bf2(v.z * inv, v.w * inv));
+        if (a.lse && d == 0)
+          a.lse[id] = sum == 0.0f ? -INFINITY : (mu + __log2f(sum)) * 0.69314718055994531f;
+      } else {
+        const Part& p = own && !first ? a.cta : a.main;
+        const int64_t pr = own ? (first ? id : (int64_t)blockIdx.x * R + r)
+                               : (int64_t)blockIdx.x * a.n_rows + id;
+        *reinterpret_cast<float4*>(p.o + pr * D + d) = v;
+        if (d == 0) p.ml[pr] = make_float4(mx, sum, mw, 0.0f);
+      }
     }
+    if (!more) break;
+    __syncthreads();  // the join buffer is read
+    if (!Ge::kApart) fill();
   }
 }
 
-// One warp a row: joins the parts in order.
+// One warp a row: joins its parts in order (the sequence's own, by CTA, then
+// the prefix's, by split).
 template <int D>
 __global__ void __launch_bounds__(128)
-    paged_join_kernel(const float* __restrict__ po, const float* __restrict__ pml, int parts,
-                      int64_t n_rows, __nv_bfloat16* __restrict__ out, float* __restrict__ lse) {
+    paged_join_kernel(const Part main, const Part cta, const Part pre, const int64_t* __restrict__ plan,
+                      const int* __restrict__ lengths, int64_t cap, int pre_parts, int64_t n_rows,
+                      int T, int H, int G, int row_tiles, int R, bool direct,
+                      __nv_bfloat16* __restrict__ out, float* __restrict__ lse) {
   const int64_t row = blockIdx.x * (int64_t)4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   pdl_trigger();
   pdl_wait();
   if (row >= n_rows) return;
   constexpr int V = D / 32;
-  float mx = -INFINITY;
-  for (int p = lane; p < parts; p += 32) mx = fmaxf(mx, pml[((int64_t)p * n_rows + row) * 2]);
+  const int64_t bt = row / ((int64_t)H * G);
+  const int hq = (int)(row - bt * ((int64_t)H * G)), h = hq / G;
+  const int b = (int)(bt / T), rr = (int)(bt - (int64_t)b * T) * G + (hq - h * G);
+  int own = 0;
+  int64_t c0 = 0;
+  if (lengths) {
+    const int64_t n = (min((int64_t)max(lengths[b], 0), cap) + kTile - 1) / kTile;
+    if (n > 0) {
+      const int64_t per = plan[0];
+      const int64_t f0 = plan[1 + b] + ((int64_t)h * row_tiles + rr / R) * n;
+      c0 = f0 / per;
+      own = (int)((f0 + n - 1) / per - c0) + 1;
+    }
+  }
+  if (direct && own == 1) return;  // written already
+  const int parts = own + pre_parts;
+  auto at = [&](int p, const Part*& q) -> int64_t {
+    if (p >= own) {
+      q = &pre;
+      return (int64_t)(p - own) * n_rows + row;
+    }
+    q = p == 0 ? &main : &cta;
+    return p == 0 ? row : (c0 + p) * R + rr % R;
+  };
+  float mx = -INFINITY, mw = -INFINITY;
+  for (int p = lane; p < parts; p += 32) {
+    const Part* q;
+    const int64_t i = at(p, q);
+    const float4 ml = q->ml[i];
+    mx = fmaxf(mx, ml.x);
+    mw = fmaxf(mw, ml.z);
+  }
 #pragma unroll
-  for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-  const float mu = mx == -INFINITY ? 0.0f : mx;
+  for (int w = 16; w > 0; w >>= 1) {
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+    mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, w));
+  }
+  const float mu = base_of(mx), wu = base_of(mw);
   float sum = 0.0f, v[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = 0.0f;
+#pragma unroll 4
   for (int p = 0; p < parts; ++p) {
-    const int64_t pr = (int64_t)p * n_rows + row;
-    const float2 ml = *reinterpret_cast<const float2*>(pml + pr * 2);
-    const float f = ex2(ml.x - mu);
-    sum += f * ml.y;
-    if (f == 0.0f && ml.y == ml.y) continue;  // an empty or vanishing part
+    const Part* q;
+    const int64_t i = at(p, q);
+    const float4 ml = q->ml[i];
+    float x[V];
+    if constexpr (V == 4) {
+      const float4 t = *reinterpret_cast<const float4*>(q->o + i * D + lane * V);
+      x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
+    } else {
+      const float2 t = *reinterpret_cast<const float2*>(q->o + i * D + lane * V);
+      x[0] = t.x; x[1] = t.y;
+    }
+    sum += ex2(ml.x - mu) * ml.y;
+    const float f = ex2(ml.z - wu);
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] += f * po[pr * D + lane * V + i];
+    for (int k = 0; k < V; ++k) v[k] += f * x[k];
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inv = sum == 0.0f ? 0.0f : ex2(wu - mu) / sum;
   __nv_bfloat16* o = out + row * D + lane * V;
 #pragma unroll
   for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(o + i) = bf2(v[i] * inv, v[i + 1] * inv);
@@ -513,69 +795,95 @@ __global__ void __launch_bounds__(128)
     lse[row] = sum == 0.0f ? -INFINITY : (mu + __log2f(sum)) * 0.69314718055994531f;
 }
 
+// How a call is cut: column tiles of 8 query rows per CTA, CTAs for the
+// sequences' own keys and splits of the prefix.
+struct Plan {
+  int nt_own, tiles_own, ctas_own;        // ctas_own 0: no own keys possible
+  bool whole;                             // a unit per CTA, nothing to join
+  int nt_pre, tiles_pre, splits_pre;      // splits_pre 0: no prefix
+  size_t o_plan, o_main, o_cta, o_pre, bytes;  // workspace offsets
+};
+
+int nt_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4; }
+
+// CTAs that fit an SM (Geo::kCtas)
+int ctas_per_sm(int nt, int rb) { return nt >= 2 ? 2 : rb == 128 ? 2 : rb == 64 ? 3 : 4; }
+
+Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, int64_t max_keys,
+               int64_t prefix) {
+  Plan p = {};
+  const int64_t n_rows = B * T * H * G;
+  const int rb = dim * bits / 8;
+  p.nt_own = nt_of(T * G);
+  p.tiles_own = (int)cdiv(T * G, 8 * p.nt_own);
+  const int64_t units = B * H * p.tiles_own;
+  // Up to two tiles a warp a unit is not worth a second part: one CTA each
+  // and no join.
+  p.whole = prefix == 0 && max_keys <= 2 * kTile * kWarps;
+  if (p.whole) {
+    p.ctas_own = (int)units;
+  } else if (max_keys > 0) {
+    const int64_t most = units * cdiv(max_keys, kTile * kWarps), fit = kSMs * ctas_per_sm(p.nt_own, rb);
+    p.ctas_own = (int)(most < fit ? most : fit);
+  }
+  if (prefix > 0) {
+    p.nt_pre = nt_of(B * T * G);
+    p.tiles_pre = (int)cdiv(B * T * G, 8 * p.nt_pre);
+    const int64_t most = cdiv(prefix, kTile * kWarps);
+    int64_t s = cdiv(kSMs * ctas_per_sm(p.nt_pre, rb), H * p.tiles_pre);
+    s = s < most ? s : most;
+    p.splits_pre = (int)(s < 1 ? 1 : s);
+  }
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t o = at;
+    at += (n + 255) & ~(size_t)255;
+    return o;
+  };
+  const size_t row = (size_t)dim * 4 + 16;
+  if (!p.whole) {
+    p.o_plan = take((size_t)(B + 1) * 8);
+    p.o_main = take(p.ctas_own ? (size_t)n_rows * row : 0);
+    p.o_cta = take((size_t)p.ctas_own * 8 * p.nt_own * row);
+    p.o_pre = take((size_t)p.splits_pre * n_rows * row);
+  }
+  p.bytes = at;
+  return p;
+}
+
 template <int BITS, int D, int NT>
-int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int units, cudaStream_t st) {
+int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, dim3 grid, cudaStream_t st) {
   auto kern = paged_attn_kernel<BITS, D, NT>;
-  constexpr size_t ring = (size_t)kWarps * Geo<BITS, D>::kRing;
-  constexpr size_t join = (size_t)kWarps * 8 * NT * (D + 4) * 4;
-  constexpr size_t smem = 1024 + (ring > join ? ring : join);
+  constexpr size_t smem = Geo<BITS, D, NT>::kSmem;
   MXB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)a.splits, (unsigned)(a.row_tiles * a.H), (unsigned)units),
-                          kThreads, smem, st, tk, tv, a));
+  MXB_CUDA_TRY(launch_pdl(kern, grid, kThreads, smem, st, tk, tv, a));
   MXB_LAUNCH_CHECK();
   return MXB_OK;
 }
 
 template <int BITS, int D>
-int launch_nt(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int nt, int units,
+int launch_nt(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int nt, dim3 grid,
               cudaStream_t st) {
   switch (nt) {
-    case 1: return launch<BITS, D, 1>(tk, tv, a, units, st);
-    case 2: return launch<BITS, D, 2>(tk, tv, a, units, st);
-    default: return launch<BITS, D, 4>(tk, tv, a, units, st);
+    case 1: return launch<BITS, D, 1>(tk, tv, a, grid, st);
+    case 2: return launch<BITS, D, 2>(tk, tv, a, grid, st);
+    case 3: return launch<BITS, D, 3>(tk, tv, a, grid, st);
+    default: return launch<BITS, D, 4>(tk, tv, a, grid, st);
   }
 }
 
 int launch_any(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int bits, int dim,
-               int nt, int units, cudaStream_t st) {
+               int nt, dim3 grid, cudaStream_t st) {
   if (bits == 8)
-    return dim == 128 ? launch_nt<8, 128>(tk, tv, a, nt, units, st)
-                      : launch_nt<8, 64>(tk, tv, a, nt, units, st);
-  return dim == 128 ? launch_nt<4, 128>(tk, tv, a, nt, units, st)
-                    : launch_nt<4, 64>(tk, tv, a, nt, units, st);
+    return dim == 128 ? launch_nt<8, 128>(tk, tv, a, nt, grid, st)
+                      : launch_nt<8, 64>(tk, tv, a, nt, grid, st);
+  return dim == 128 ? launch_nt<4, 128>(tk, tv, a, nt, grid, st)
+                    : launch_nt<4, 64>(tk, tv, a, nt, grid, st);
 }
 
-// How a call is cut: column tiles of 8 query rows per CTA, CTAs per unit over
-// the keys.
-struct Plan {
-  int nt_own, tiles_own, splits_own;  // the sequences' own keys (0 splits: none)
-  int nt_pre, tiles_pre, splits_pre;  // the shared prefix
-  int parts() const { return splits_own + splits_pre; }
-};
-
-int nt_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
-
-// Splits over the keys until two CTAs an SM are busy, each with at least one
-// tile a warp.
-int splits_of(int64_t units, int64_t keys) {
-  const int64_t most = cdiv(keys, kTile * kWarps);
-  int64_t s = cdiv(2 * kSMs, units);
-  s = s < most ? s : most;
-  return (int)(s < 1 ? 1 : s > 128 ? 128 : s);
-}
-
-Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int64_t max_keys, int64_t prefix) {
-  Plan p = {};
-  p.nt_own = nt_of(T * G);
-  p.tiles_own = (int)cdiv(T * G, 8 * p.nt_own);
-  // with no own keys possible the sequences' launch still writes the empty rows
-  if (max_keys > 0 || prefix == 0) p.splits_own = splits_of(B * H * p.tiles_own, max_keys);
-  if (prefix > 0) {
-    p.nt_pre = nt_of(B * T * G);
-    p.tiles_pre = (int)cdiv(B * T * G, 8 * p.nt_pre);
-    p.splits_pre = splits_of(H * p.tiles_pre, prefix);
-  }
-  return p;
+Part part_at(void* ws, size_t off, size_t rows, int dim) {
+  char* p = static_cast<char*>(ws) + off;
+  return {reinterpret_cast<float*>(p), reinterpret_cast<float4*>(p + rows * dim * 4)};
 }
 
 }  // namespace pattn
@@ -584,11 +892,9 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int64_t max_keys, int
 extern "C" {
 
 size_t mxb_paged_attention_workspace_size(int64_t B, int64_t T, int heads, int group, int dim,
-                                          int page, int64_t width, int64_t prefix_len) {
-  if (B <= 0 || T <= 0 || heads <= 0 || group <= 0 || dim <= 0 || page <= 0) return 0;
-  const pattn::Plan p = pattn::make_plan(B, T, heads, group, width * page, prefix_len);
-  if (p.parts() <= 1) return 0;
-  return (size_t)p.parts() * (size_t)(B * T * heads * group) * (size_t)(dim + 2) * sizeof(float);
+                                          int bits, int page, int64_t width, int64_t prefix_len) {
+  if (B <= 0 || T <= 0 || heads <= 0 || group <= 0 || dim <= 0 || page <= 0 || bits <= 0) return 0;
+  return pattn::make_plan(B, T, heads, group, dim, bits, width * page, prefix_len).bytes;
 }
 
 int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim,
@@ -601,20 +907,20 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
   const int rc = kv_pool_check(n_pages, heads, page, dim, bits, k_codes, k_scales, v_codes, v_scales);
   if (rc != MXB_OK) return rc;
   if (B < 0 || B > 65535 || T < 0 || T > 65535 || group <= 0 || group > 1024 || width < 0 ||
-      prefix_len < 0 || width * page > INT32_MAX - 64 || prefix_len > INT32_MAX - 64 ||
-      prefix_len > prefix_width * page || B * T * group > INT32_MAX / 2)
+      prefix_len < 0 || width > (INT32_MAX - 64) / page || prefix_len > INT32_MAX - 64 ||
+      prefix_width < 0 || prefix_width > INT32_MAX || prefix_len > prefix_width * page ||
+      B * T * group > INT32_MAX / 2)
     return MXB_E_SHAPE;
   if (B == 0 || T == 0) return MXB_OK;
   if (!q || !out || !lengths || (width > 0 && !table) || (prefix_len > 0 && !prefix_table))
     return MXB_E_ARG;
-  if (((uintptr_t)q | (uintptr_t)out) % 16) return MXB_E_ALIGN;
-  const pattn::Plan p = pattn::make_plan(B, T, heads, group, width * page, prefix_len);
-  if ((int64_t)p.tiles_own * heads > 65535 || (int64_t)p.tiles_pre * heads > 65535)
+  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) % 16) return MXB_E_ALIGN;
+  const pattn::Plan p =
+      pattn::make_plan(B, T, heads, group, dim, bits, width * page, prefix_len);
+  if ((int64_t)p.tiles_own * heads > 65535 || (int64_t)p.tiles_pre * heads > 65535 ||
+      B * heads * p.tiles_own > INT32_MAX)
     return MXB_E_SHAPE;
-  const size_t need =
-      mxb_paged_attention_workspace_size(B, T, heads, group, dim, page, width, prefix_len);
-  if (need > 0 && (!workspace || workspace_bytes < need)) return MXB_E_WORKSPACE;
-  if ((uintptr_t)workspace % 16) return MXB_E_ALIGN;
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return MXB_E_WORKSPACE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 
   CUtensorMap tk, tv;
@@ -640,41 +946,48 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
   a.G = group;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.n_rows = B * T * heads * group;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.lse = lse;
   a.err = device_error_ptr();
-  const bool direct = p.parts() == 1;
-  a.out = direct ? static_cast<__nv_bfloat16*>(out) : nullptr;
-  a.lse = direct ? lse : nullptr;
-  a.po = static_cast<float*>(workspace);
-  a.pml = a.po ? a.po + (size_t)p.parts() * a.n_rows * dim : nullptr;
+  pattn::Part pre = {}, own = {}, cta = {};
   if (p.splits_pre > 0) {
+    pre = pattn::part_at(workspace, p.o_pre, (size_t)p.splits_pre * a.n_rows, dim);
     a.table = prefix_table;
-    a.lengths = nullptr;
     a.width = (int)prefix_width;
     a.prefix_len = (int)prefix_len;
     a.rows = (int)(B * T * group);
     a.row_tiles = p.tiles_pre;
     a.splits = p.splits_pre;
-    a.part0 = p.splits_own;
-    const int r = pattn::launch_any(tk, tv, a, bits, dim, p.nt_pre, 1, st);
+    a.main = pre;
+    const int r = pattn::launch_any(tk, tv, a, bits, dim, p.nt_pre,
+                                    dim3((unsigned)p.splits_pre, (unsigned)(p.tiles_pre * heads)), st);
     if (r != MXB_OK) return r;
   }
-  if (p.splits_own > 0) {
-    a.table = table;
-    a.lengths = lengths;
-    a.width = (int)width;
-    a.prefix_len = 0;
-    a.rows = (int)(T * group);
-    a.row_tiles = p.tiles_own;
-    a.splits = p.splits_own;
-    a.part0 = 0;
-    const int r = pattn::launch_any(tk, tv, a, bits, dim, p.nt_own, (int)B, st);
+  a.lengths = lengths;
+  a.table = table;
+  a.width = (int)width;
+  a.rows = (int)(T * group);
+  a.row_tiles = p.tiles_own;
+  a.whole = p.whole;
+  a.direct = p.splits_pre == 0;
+  if (p.ctas_own > 0) {
+    if (!p.whole) {
+      own = pattn::part_at(workspace, p.o_main, (size_t)a.n_rows, dim);
+      cta = pattn::part_at(workspace, p.o_cta, (size_t)p.ctas_own * 8 * p.nt_own, dim);
+      a.plan = reinterpret_cast<int64_t*>(static_cast<char*>(workspace) + p.o_plan);
+    }
+    a.main = own;
+    a.cta = cta;
+    const int r =
+        pattn::launch_any(tk, tv, a, bits, dim, p.nt_own, dim3((unsigned)p.ctas_own), st);
     if (r != MXB_OK) return r;
   }
-  if (!direct) {
-    const unsigned grid = (unsigned)cdiv(a.n_rows, 4);
-    MXB_CUDA_TRY(launch_pdl(dim == 128 ? pattn::paged_join_kernel<128> : pattn::paged_join_kernel<64>,
-                            dim3(grid), 128, 0, st, a.po, a.pml, p.parts(), a.n_rows,
-                            static_cast<__nv_bfloat16*>(out), lse));
+  if (!p.whole) {
+    MXB_CUDA_TRY(launch_pdl(
+        dim == 128 ? pattn::paged_join_kernel<128> : pattn::paged_join_kernel<64>,
+        dim3((unsigned)cdiv(a.n_rows, 4)), 128, 0, st, own, cta, pre, a.plan,
+        p.ctas_own > 0 ? lengths : nullptr, width * page, p.splits_pre, a.n_rows, (int)T, heads,
+        group, p.tiles_own, 8 * p.nt_own, a.direct, a.out, lse));
     MXB_LAUNCH_CHECK();
   }
   return MXB_OK;

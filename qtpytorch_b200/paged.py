@@ -200,8 +200,8 @@ def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
     out = torch.empty_like(q)
     lse = torch.empty(B, T, Hq, dtype=torch.float32, device=dev) if return_lse else None
     lib = L.load()
-    wsb = lib.mxb_paged_attention_workspace_size(B, T, H, Hq // H, D, cache.page_size,
-                                                 table.shape[1], prefix_len)
+    wsb = lib.mxb_paged_attention_workspace_size(B, T, H, Hq // H, D, cache.dtype.bits,
+                                                 cache.page_size, table.shape[1], prefix_len)
     ws = L.workspace(wsb, dev)
     rc = L.call("mxb_paged_attention", dev, q.data_ptr(), B, T, H, Hq // H, D,
                 cache.k_codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(),
