@@ -57,17 +57,19 @@ template <int BITS, int D, int NT>
 struct Geo {
   static constexpr int RB = D * BITS / 8;       // bytes of a head row: 128, 64 or 32
   static constexpr int kTileBytes = kTile * RB;
-  // ring depth and CTAs per SM: about 150 KB in flight an SM
-  static constexpr int kStages = RB == 128 ? 3 : RB == 64 ? 4 : 6;
-  static constexpr int kCtas = NT >= 2 ? 2 : RB == 128 ? 2 : RB == 64 ? 3 : 4;
+  // CTAs per SM (registers bound them from 9 rows on) and ring depth: 100 to
+  // 200 KB in flight an SM
+  static constexpr int kCtas = NT >= 2 ? 2 : RB == 32 ? 4 : 3;
+  static constexpr int kStages = RB == 128 ? (NT >= 2 ? 3 : 2) : RB == 64 ? (NT >= 2 ? 4 : 3) : 4;
   static constexpr int R = 8 * NT;              // query rows per CTA
   static constexpr int kPitch = D + 4;          // floats of a row in the join buffer
   static constexpr size_t kRing = (size_t)kWarps * kStages * (2 * kTileBytes + 2 * kTile * 4);
   static constexpr size_t kJoin = (size_t)kWarps * R * kPitch * 4;
-  // with few rows the join buffer lies beside the ring, so the next unit's
+  // where it fits the join buffer lies beside the ring, so the next unit's
   // loads start before the join
-  static constexpr bool kApart = NT <= 2;
+  static constexpr bool kApart = NT <= 2 && RB < 128;
   static constexpr size_t kSmem = 1024 + (kApart ? kRing + kJoin : kRing > kJoin ? kRing : kJoin);
+  static_assert(kCtas * (kSmem + 2048 + (NT >= 3 ? 9 * 1024 : 0)) <= 228 * 1024, "CTAs fit an SM");
   // byte offset of 16-byte chunk c of row r in a tile (the TMA swizzle)
   __device__ static uint32_t at(int r, int c) {
     const int x = RB == 128 ? (r & 7) : RB == 64 ? ((r >> 1) & 3) : ((r >> 2) & 1);
@@ -807,7 +809,7 @@ struct Plan {
 int nt_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4; }
 
 // CTAs that fit an SM (Geo::kCtas)
-int ctas_per_sm(int nt, int rb) { return nt >= 2 ? 2 : rb == 128 ? 2 : rb == 64 ? 3 : 4; }
+int ctas_per_sm(int nt, int rb) { return nt >= 2 ? 2 : rb == 32 ? 4 : 3; }
 
 Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, int64_t max_keys,
                int64_t prefix) {
