@@ -70,10 +70,11 @@ struct Geo {
   static constexpr bool kApart = NT <= 2 && RB < 128;
   static constexpr size_t kSmem = 1024 + (kApart ? kRing + kJoin : kRing > kJoin ? kRing : kJoin);
   static_assert(kCtas * (kSmem + 2048 + (NT >= 3 ? 9 * 1024 : 0)) <= 228 * 1024, "CTAs fit an SM");
-  // byte offset of 16-byte chunk c of row r in a tile (the TMA swizzle)
-  __device__ static uint32_t at(int r, int c) {
+  // byte offset of 16-byte chunk 0 of row r in a tile (the TMA swizzle); chunk c
+  // lies at that address ^ (c << 4)
+  __device__ static uint32_t at(int r) {
     const int x = RB == 128 ? (r & 7) : RB == 64 ? ((r >> 1) & 3) : ((r >> 2) & 1);
-    return (uint32_t)(r * RB + ((c ^ x) << 4));
+    return (uint32_t)(r * RB + (x << 4));
   }
 };
 
@@ -167,26 +168,34 @@ __device__ __forceinline__ float lg2(float x) {
 // 2^(x - ref) of a running maximum; nothing seen yet gives 0
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
 
-// Two codes as 16-bit floats.  int8: bytes 0 and 2 of w, fp16 1152 + code
-// ((code + 128) in the mantissa of 1024).  int4: low nibbles of both halves;
-// for K bf16 136 + code ((code + 8) in the mantissa of 128), for V fp16
-// 1032 + code.
+// Two codes as 16-bit floats.  K: int8 bytes 0 and 2 of w -> fp16 1152 + code
+// ((code + 128) in the mantissa of 1024); int4 low nibbles of both halves ->
+// bf16 136 + code ((code + 8) in the mantissa of 128).  V: exact fp16 codes;
+// int4 nibble 1 (HI) stays where it is in the mantissa, 16 times its code,
+// which saves its shift: the factor leaves with the result.
 template <int BITS>
 struct Codes;
 template <>
 struct Codes<8> {
   static constexpr float kOffset = 1152.0f;
   static constexpr bool kHalfQ = true;
+  static constexpr float kHiScale = 1.0f;
   __device__ static uint32_t k(uint32_t w) { return (w & 0x00FF00FFu) ^ 0x64806480u; }
-  __device__ static uint32_t v(uint32_t w) { return hsub2u(k(w), 0x64806480u); }
+  template <bool HI>
+  __device__ static uint32_t v(uint32_t w) {
+    return hsub2u(k(HI ? w >> 8 : w), 0x64806480u);
+  }
 };
 template <>
 struct Codes<4> {
   static constexpr float kOffset = 136.0f;
   static constexpr bool kHalfQ = false;
+  static constexpr float kHiScale = 1.0f / 16.0f;
   __device__ static uint32_t k(uint32_t w) { return (w & 0x000F000Fu) ^ 0x43084308u; }
+  template <bool HI>
   __device__ static uint32_t v(uint32_t w) {
-    return hsub2u((w & 0x000F000Fu) ^ 0x64086408u, 0x64086408u);
+    return HI ? hsub2u((w & 0x00F000F0u) ^ 0x64806480u, 0x64806480u)
+              : hsub2u((w & 0x000F000Fu) ^ 0x64086408u, 0x64086408u);
   }
 };
 
@@ -349,7 +358,9 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
     }
   };
   int next_page = -1;
-  uint32_t it = 0;  // tiles consumed by this warp: stage it % kStages, round it / kStages
+  int stage = 0;  // ring position of the warp's next tile, and its parity
+  uint32_t round = 0;
+  const uint32_t lane_at = smem_u32(ring) + Ge::at(lane);
   auto fill = [&]() {
     int pg[kStages];
 #pragma unroll
@@ -357,7 +368,8 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
 #pragma unroll
     for (int i = 0; i < kStages; ++i)
       if (t_lo + warp + i * kWarps < t_hi)
-        issue(t_lo + warp + i * kWarps, u / a.row_tiles, (it + i) % kStages, pg[i]);
+        issue(t_lo + warp + i * kWarps, u / a.row_tiles,
+              stage + i < kStages ? stage + i : stage + i - kStages, pg[i]);
     next_page = page_of(t_lo + warp + kStages * kWarps);
   };
   fill();
@@ -482,7 +494,9 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
     };
 
     float o[kMT][NT][4];
-    float m[NT][2], l[NT][2], mv[NT][2];
+    // references of the sums and of the weights, and the values beyond which
+    // they move (-inf: nothing seen)
+    float mu[NT][2], l[NT][2], wu[NT][2], m_top[NT][2], w_top[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -491,15 +505,19 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
         for (int e = 0; e < 4; ++e) o[j][n][e] = 0.0f;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        m[n][e] = mv[n][e] = -INFINITY;
-        l[n][e] = 0.0f;
+        m_top[n][e] = w_top[n][e] = -INFINITY;
+        mu[n][e] = wu[n][e] = l[n][e] = 0.0f;
       }
     }
 
-    for (int tile = t_lo + warp; tile < t_hi; tile += kWarps, ++it) {
-      const int s = it % kStages;
-      ok = ok && mbar_wait_warp_to(&full[warp][s], (it / kStages) & 1, kErrTimeoutFull, a.err);
-      const uint32_t kt = smem_u32(ring + s * 2 * Ge::kTileBytes);
+    for (int tile = t_lo + warp; tile < t_hi; tile += kWarps) {
+      const int s = stage;
+      ok = ok && mbar_wait_warp_to(&full[warp][s], round, kErrTimeoutFull, a.err);
+      if (++stage == kStages) {
+        stage = 0;
+        round ^= 1u;
+      }
+      const uint32_t kt = lane_at + s * 2 * Ge::kTileBytes;
       const uint32_t vt = kt + Ge::kTileBytes;
       const float* sc = rs + s * 2 * kTile;
 
@@ -514,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
 #pragma unroll
       for (int j = 0; j < Ge::RB / 16; ++j) {
         uint32_t w[4];
-        ldsm4(kt + Ge::at(lane, j), w);
+        ldsm4(kt ^ (j << 4), w);
         constexpr int Z = BITS == 8 ? 1 : 2, SH = BITS;  // steps a chunk; shift to the second pair
 #pragma unroll
         for (int z = 0; z < Z; ++z) {
@@ -535,80 +553,107 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
           }
         }
       }
-      // ── scores, running maxima, weights ──
+      // ── scores and the weights' exponents ──
       float kscale[4], lv[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         kscale[i] = sc[8 * i + g] * a.scale_log2;
         lv[i] = lg2(sc[kTile + 8 * i + g]);
       }
-      const int key0 = tile * kTile + g;
-      const bool ragged = (tile + 1) * kTile > lim_min;  // some key is hidden from some row
-      uint32_t pb[2][NT][2];
-      bool grew = false;
-      float alpha[NT][2];
+      float wv[NT][4][2];  // s + log2 sv
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float wv[4][2];  // s + log2 sv
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& v = sa[i >> 1][n][(i & 1) * 2 + e];
+            v *= kscale[i];
+            if (BITS == 8) v *= cfac[n][e];
+            wv[n][i][e] = v + lv[i];
+          }
+      if ((tile + 1) * kTile > lim_min) {  // some key is hidden from some row
+        const int key0 = tile * kTile + g;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (key0 + 8 * i >= limit[n][e])  // whatever its scales hold
+                sa[i >> 1][n][(i & 1) * 2 + e] = wv[n][i][e] = -INFINITY;
+      }
+      // ── the references: moved only when a sum's terms pass 2^64 or a weight
+      // 2^8 (fp16 holds 2^15), so most tiles need no exchange between lanes ──
+      bool move = false;
+      float mx[NT][2], mw[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = -INFINITY, mw = -INFINITY;
+          mx[n][e] = fmaxf(fmaxf(sa[0][n][e], sa[0][n][2 + e]), fmaxf(sa[1][n][e], sa[1][n][2 + e]));
+          mw[n][e] = fmaxf(fmaxf(wv[n][0][e], wv[n][1][e]), fmaxf(wv[n][2][e], wv[n][3][e]));
+          move |= mx[n][e] > m_top[n][e] || mw[n][e] > w_top[n][e];
+        }
+      if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float v = sa[i >> 1][n][(i & 1) * 2 + e] * kscale[i];
-            if (BITS == 8) v *= cfac[n][e];
-            float w = v + lv[i];
-            if (ragged && key0 + 8 * i >= limit[n][e]) v = w = -INFINITY;  // whatever its scales hold
-            sa[i >> 1][n][(i & 1) * 2 + e] = v;
-            wv[i][e] = w;
-            mx = fmaxf(mx, v);
-            mw = fmaxf(mw, w);
+        for (int n = 0; n < NT; ++n) {
+          float alpha[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+              mx[n][e] = fmaxf(mx[n][e], __shfl_xor_sync(0xffffffffu, mx[n][e], x));
+              mw[n][e] = fmaxf(mw[n][e], __shfl_xor_sync(0xffffffffu, mw[n][e], x));
+            }
+            // the larger of the reference (where there is one) and the tile's
+            const float m0 = m_top[n][e] == -INFINITY ? -INFINITY : mu[n][e];
+            const float w0 = w_top[n][e] == -INFINITY ? -INFINITY : wu[n][e];
+            const float m1 = fmaxf(m0, mx[n][e]), w1 = fmaxf(w0, mw[n][e]);
+            mu[n][e] = base_of(m1);
+            wu[n][e] = base_of(w1);
+            l[n][e] *= ex2(m0 - mu[n][e]);
+            alpha[e] = ex2(w0 - wu[n][e]);
+            m_top[n][e] = m1 + 64.0f;
+            w_top[n][e] = w1 + 8.0f;
           }
 #pragma unroll
-          for (int x = 4; x < 32; x <<= 1) {
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, x));
-          }
-          mx = fmaxf(m[n][e], mx);
-          mw = fmaxf(mv[n][e], mw);
-          const float mu = base_of(mx), wu = base_of(mw);
-          alpha[n][e] = ex2(mv[n][e] - wu);
-          grew |= mw != mv[n][e];
+          for (int j = 0; j < kMT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][n][e] *= alpha[e & 1];
+        }
+      }
+      // ── weights: keys x rows -> rows x keys, the B fragment of the second
+      // product ──
+      uint32_t pb[2][NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
           float sum = 0.0f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            sum += ex2(sa[i >> 1][n][(i & 1) * 2 + e] - mu);
-            wv[i][e] = ex2(wv[i][e] - wu);
+            sum += ex2(sa[i >> 1][n][(i & 1) * 2 + e] - mu[n][e]);
+            wv[n][i][e] = ex2(wv[n][i][e] - wu[n][e]);
           }
-          l[n][e] = l[n][e] * ex2(m[n][e] - mu) + sum;
-          m[n][e] = mx;
-          mv[n][e] = mw;
+          l[n][e] += sum;
         }
-        // keys x rows -> rows x keys: the B fragment of the second product
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pb[i >> 1][n][i & 1] = movm(hf2(wv[i][0], wv[i][1]));
-      }
-      if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-        for (int j = 0; j < kMT; ++j)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][n][e] *= alpha[n][e & 1];
+        for (int i = 0; i < 4; ++i) pb[i >> 1][n][i & 1] = movm(hf2(wv[n][i][0], wv[n][i][1]));
       }
       // ── O^T += V^T P^T ──
 #pragma unroll
       for (int j = 0; j < Ge::RB / 16; ++j) {
         uint32_t w[4];
-        ldsm4t(vt + Ge::at(lane, j), w);
-        constexpr int Z = BITS == 8 ? 1 : 2, SH = BITS;
+        ldsm4t(vt ^ (j << 4), w);
+        constexpr int Z = BITS == 8 ? 1 : 2;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int z = 0; z < Z; ++z) {
-            const uint32_t a0 = Cd::v(w[2 * mt] >> (8 * z)), a1 = Cd::v(w[2 * mt] >> (8 * z + SH));
-            const uint32_t a2 = Cd::v(w[2 * mt + 1] >> (8 * z));
-            const uint32_t a3 = Cd::v(w[2 * mt + 1] >> (8 * z + SH));
+            const uint32_t w0 = w[2 * mt] >> (8 * z), w1 = w[2 * mt + 1] >> (8 * z);
+            const uint32_t a0 = Cd::template v<false>(w0), a1 = Cd::template v<true>(w0);
+            const uint32_t a2 = Cd::template v<false>(w1), a3 = Cd::template v<true>(w1);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
               mma16816<true>(o[Z * j + z][n], a0, a1, a2, a3, pb[mt][n][0], pb[mt][n][1]);
@@ -648,9 +693,9 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
         if (g == 0) {
-          sm_m[warp][8 * n + 2 * c + e] = m[n][e];
+          sm_m[warp][8 * n + 2 * c + e] = m_top[n][e] == -INFINITY ? -INFINITY : mu[n][e];
           sm_l[warp][8 * n + 2 * c + e] = l[n][e];
-          sm_v[warp][8 * n + 2 * c + e] = mv[n][e];
+          sm_v[warp][8 * n + 2 * c + e] = w_top[n][e] == -INFINITY ? -INFINITY : wu[n][e];
         }
       }
     if (!Ge::kApart) __syncthreads();  // every ring is idle
@@ -665,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           *reinterpret_cast<float2*>(so + (8 * n + 2 * c + e) * P + d) =
-              make_float2(o[j][n][e], o[j][n][2 + e]);
+              make_float2(o[j][n][e], o[j][n][2 + e] * Cd::kHiScale);
     }
     __syncthreads();
     const bool direct = a.direct && first && last;
