@@ -160,6 +160,13 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// Arrive on bar (one of its counted arrivals) when this thread's cp.async are done.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ float lg2(float x) {
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -250,7 +257,8 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
   float* join = reinterpret_cast<float*>(smem + (Ge::kApart ? Ge::kRing : 0));
   const int boxes = kTile / a.box;
   if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&full[warp][s], boxes);
+    // one arrival a box (its copies' bytes), one a lane (its scales)
+    for (int s = 0; s < kStages; ++s) mbar_init(&full[warp][s], boxes + 32);
     fence_barrier_init();
   }
   __syncwarp();
@@ -339,23 +347,30 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
     return p;
   };
   auto issue = [&](int tile, int h, int s, int p) {
+    uint64_t* bar = &full[warp][s];
     if (lane < boxes) {
       if (p >= 0) {
         const int pos = tile * kTile + lane * a.box;
         const int row = ((p * a.H + h) << a.page_shift) + (pos & page_mask);
-        const uint32_t bytes = (uint32_t)a.box * (2 * Ge::RB + 8);
         uint8_t* k = ring + s * 2 * Ge::kTileBytes + lane * a.box * Ge::RB;
-        float* sc = rs + s * 2 * kTile + lane * a.box;
-        uint64_t* bar = &full[warp][s];
-        mbar_expect_tx(bar, bytes);
+        mbar_expect_tx(bar, (uint32_t)a.box * 2 * Ge::RB);
         tma_load_2d(k, &tmap_k, bar, 0, row);
         tma_load_2d(k + Ge::kTileBytes, &tmap_v, bar, 0, row);
-        bulk_load_g2s(sc, a.ks + row, (uint32_t)a.box * 4, bar);
-        bulk_load_g2s(sc + kTile, a.vs + row, (uint32_t)a.box * 4, bar);
       } else {
-        mbar_arrive(&full[warp][s]);
+        mbar_arrive(bar);
       }
     }
+    // a lane's two scales: a bulk copy each would cost the TMA unit as much as
+    // a tile of codes (attend_long without them 8 us shorter)
+    const int kp = __shfl_sync(0xffffffffu, p, lane / a.box);
+    const int pos = tile * kTile + lane;
+    if (kp >= 0) {
+      const int row = ((kp * a.H + h) << a.page_shift) + (pos & page_mask);
+      float* sc = rs + s * 2 * kTile + lane;
+      cp_async4(sc, a.ks + row);
+      cp_async4(sc + kTile, a.vs + row);
+    }
+    cp_async_arrive(bar);
   };
   int next_page = -1;
   int stage = 0;  // ring position of the warp's next tile, and its parity
@@ -761,23 +776,23 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
   }
 }
 
-// One warp a row: joins its parts in order (the sequence's own, by CTA, then
-// the prefix's, by split).
+// A block per row joins its parts (the sequence's own, by CTA, then the
+// prefix's, by split): warp w the parts w, w + 4, .., then the warps in order.
 template <int D>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kThreads)
     paged_join_kernel(const Part main, const Part cta, const Part pre, const int64_t* __restrict__ plan,
                       const int* __restrict__ lengths, int64_t cap, int pre_parts, int64_t n_rows,
                       int T, int H, int G, int row_tiles, int R, bool direct,
                       __nv_bfloat16* __restrict__ out, float* __restrict__ lse) {
-  const int64_t row = blockIdx.x * (int64_t)4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  const uint32_t row = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ float sv[kWarps][D], sm[kWarps], ss[kWarps], sw[kWarps];
   pdl_trigger();
   pdl_wait();
-  if (row >= n_rows) return;
   constexpr int V = D / 32;
-  const int64_t bt = row / ((int64_t)H * G);
-  const int hq = (int)(row - bt * ((int64_t)H * G)), h = hq / G;
-  const int b = (int)(bt / T), rr = (int)(bt - (int64_t)b * T) * G + (hq - h * G);
+  const uint32_t bt = row / (uint32_t)(H * G);
+  const int hq = (int)(row - bt * (uint32_t)(H * G)), h = hq / G;
+  const int b = (int)(bt / (uint32_t)T), rr = (int)(bt - (uint32_t)b * T) * G + (hq - h * G);
   int own = 0;
   int64_t c0 = 0;
   if (lengths) {
@@ -791,55 +806,90 @@ __global__ void __launch_bounds__(128)
   }
   if (direct && own == 1) return;  // written already
   const int parts = own + pre_parts;
-  auto at = [&](int p, const Part*& q) -> int64_t {
+  const int64_t c_at = c0 * R + rr % R;
+  auto part_of = [&](int p, int64_t& i) -> const Part& {
     if (p >= own) {
-      q = &pre;
-      return (int64_t)(p - own) * n_rows + row;
+      i = (int64_t)(p - own) * n_rows + row;
+      return pre;
     }
-    q = p == 0 ? &main : &cta;
-    return p == 0 ? row : (c0 + p) * R + rr % R;
+    i = p == 0 ? (int64_t)row : c_at + (int64_t)p * R;
+    return p == 0 ? main : cta;
   };
-  float mx = -INFINITY, mw = -INFINITY;
-  for (int p = lane; p < parts; p += 32) {
-    const Part* q;
-    const int64_t i = at(p, q);
-    const float4 ml = q->ml[i];
-    mx = fmaxf(mx, ml.x);
-    mw = fmaxf(mw, ml.z);
-  }
+  float mu = -INFINITY, wu = -INFINITY, sum = 0.0f, v[V];
 #pragma unroll
-  for (int w = 16; w > 0; w >>= 1) {
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-    mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, w));
-  }
-  const float mu = base_of(mx), wu = base_of(mw);
-  float sum = 0.0f, v[V];
+  for (int k = 0; k < V; ++k) v[k] = 0.0f;
+  constexpr int U = 4;  // parts in flight a warp
+  for (int p0 = warp; p0 < parts; p0 += kWarps * U) {
+    float4 ml[U];
+    float x[U][V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = 0.0f;
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
-    const Part* q;
-    const int64_t i = at(p, q);
-    const float4 ml = q->ml[i];
-    float x[V];
-    if constexpr (V == 4) {
-      const float4 t = *reinterpret_cast<const float4*>(q->o + i * D + lane * V);
-      x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
-    } else {
-      const float2 t = *reinterpret_cast<const float2*>(q->o + i * D + lane * V);
-      x[0] = t.x; x[1] = t.y;
+    for (int i = 0; i < U; ++i) {
+      const int p = p0 + i * kWarps;
+      ml[i] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[i][k] = 0.0f;
+      if (p < parts) {
+        int64_t at;
+        const Part& q = part_of(p, at);
+        ml[i] = q.ml[at];
+        if constexpr (V == 4) {
+          const float4 t = *reinterpret_cast<const float4*>(q.o + at * D + lane * V);
+          x[i][0] = t.x; x[i][1] = t.y; x[i][2] = t.z; x[i][3] = t.w;
+        } else {
+          const float2 t = *reinterpret_cast<const float2*>(q.o + at * D + lane * V);
+          x[i][0] = t.x; x[i][1] = t.y;
+        }
+      }
     }
-    sum += ex2(ml.x - mu) * ml.y;
-    const float f = ex2(ml.z - wu);
+    float m1 = mu, w1 = wu;
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] += f * x[k];
+    for (int i = 0; i < U; ++i) {
+      m1 = fmaxf(m1, ml[i].x);
+      w1 = fmaxf(w1, ml[i].z);
+    }
+    const float fm = ex2(mu - base_of(m1)), fw = ex2(wu - base_of(w1));
+    sum *= fm;
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] *= fw;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      sum += ex2(ml[i].x - base_of(m1)) * ml[i].y;
+      const float f = ex2(ml[i].z - base_of(w1));
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] += f * x[i][k];
+    }
+    mu = m1;
+    wu = w1;
   }
-  const float inv = sum == 0.0f ? 0.0f : ex2(wu - mu) / sum;
-  __nv_bfloat16* o = out + row * D + lane * V;
+  if (lane == 0) {
+    sm[warp] = mu;
+    ss[warp] = sum;
+    sw[warp] = wu;
+  }
 #pragma unroll
-  for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(o + i) = bf2(v[i] * inv, v[i + 1] * inv);
-  if (lse && lane == 0)
-    lse[row] = sum == 0.0f ? -INFINITY : (mu + __log2f(sum)) * 0.69314718055994531f;
+  for (int k = 0; k < V; ++k) sv[warp][lane * V + k] = v[k];
+  __syncthreads();
+  if (threadIdx.x >= D / 2) return;
+  float mx = -INFINITY, mw = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    mx = fmaxf(mx, sm[w]);
+    mw = fmaxf(mw, sw[w]);
+  }
+  mx = base_of(mx);
+  mw = base_of(mw);
+  float total = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    total += ex2(sm[w] - mx) * ss[w];
+    const float f = ex2(sw[w] - mw);
+    o0 += f * sv[w][2 * threadIdx.x];
+    o1 += f * sv[w][2 * threadIdx.x + 1];
+  }
+  const float inv = total == 0.0f ? 0.0f : ex2(mw - mx) / total;
+  reinterpret_cast<uint32_t*>(out + (int64_t)row * D)[threadIdx.x] = bf2(o0 * inv, o1 * inv);
+  if (lse && threadIdx.x == 0)
+    lse[row] = total == 0.0f ? -INFINITY : (mx + __log2f(total)) * 0.69314718055994531f;
 }
 
 // How a call is cut: column tiles of 8 query rows per CTA, CTAs for the
@@ -965,7 +1015,7 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
   const pattn::Plan p =
       pattn::make_plan(B, T, heads, group, dim, bits, width * page, prefix_len);
   if ((int64_t)p.tiles_own * heads > 65535 || (int64_t)p.tiles_pre * heads > 65535 ||
-      B * heads * p.tiles_own > INT32_MAX)
+      B * heads * p.tiles_own > INT32_MAX || B * T * heads * group > INT32_MAX)
     return MXB_E_SHAPE;
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return MXB_E_WORKSPACE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -1032,7 +1082,7 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
   if (!p.whole) {
     MXB_CUDA_TRY(launch_pdl(
         dim == 128 ? pattn::paged_join_kernel<128> : pattn::paged_join_kernel<64>,
-        dim3((unsigned)cdiv(a.n_rows, 4)), 128, 0, st, own, cta, pre, a.plan,
+        dim3((unsigned)a.n_rows), pattn::kThreads, 0, st, own, cta, pre, a.plan,
         p.ctas_own > 0 ? lengths : nullptr, width * page, p.splits_pre, a.n_rows, (int)T, heads,
         group, p.tiles_own, 8 * p.nt_own, a.direct, a.out, lse));
     MXB_LAUNCH_CHECK();

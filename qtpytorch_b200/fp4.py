@@ -36,6 +36,11 @@ def _fmt(fmt: str) -> int:
         raise ValueError(f"Unknown 4-bit format {fmt!r}: one of {sorted(FORMATS)}") from None
 
 
+def _require_cuda(dev: torch.device, what: str) -> None:
+    if dev.type != "cuda":
+        raise L.MxbError(f"{what}: tensor is on {dev}; the mxb kernels run on CUDA only")
+
+
 def code_row_bytes(K: int) -> int:
     """Bytes of one row of codes: two a byte, whole groups of 32."""
     return -(-K // 32) * 16
@@ -54,7 +59,7 @@ class fp4_tensor:
     row-major, byte ((r % 32) * 4 + r // 32) * 4 + c of a tile, zero past the
     matrix.  ``global_scale``: fp32 [1] on the device (nvfp4) or None."""
 
-    __slots__ = ("codes", "scales", "fmt", "shape", "global_scale")
+    __slots__ = ("fmt", "shape", "device", "_parts", "_ptrs")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str, shape,
                  global_scale: Optional[torch.Tensor] = None):
@@ -78,8 +83,9 @@ class fp4_tensor:
         if codes.device != scales.device or (global_scale is not None
                                              and global_scale.device != codes.device):
             raise ValueError("fp4_tensor: codes, scales and global_scale are on different devices")
-        self.codes, self.scales, self.fmt = codes, scales, fmt
-        self.shape, self.global_scale = shape, global_scale
+        self.fmt, self.shape, self.device = fmt, shape, codes.device
+        self._parts = (codes, scales, global_scale)
+        self._ptrs = (codes.data_ptr(), scales.data_ptr(), L.ptr(global_scale))
 
     @classmethod
     def quantize(cls, x: torch.Tensor, fmt: str = "mxfp4",
@@ -104,42 +110,68 @@ class fp4_tensor:
         if x.stride(1) != 1 or ldx < K:
             x, ldx = x.contiguous(), K
         dev = x.device
-        codes = torch.empty(rows, code_row_bytes(K), dtype=torch.uint8, device=dev)
-        scales = torch.empty(scale_bytes(rows, K, fmt), dtype=torch.uint8, device=dev)
-        g, derive, ws, wsb = None, 0, None, 0
-        if f == L.FP4_NV:
-            if global_scale is None:
-                derive = 1
-                # the factor, and behind it the workspace
-                wsb = L.load().mxb_fp4_quantize_workspace_size(rows, K, f, 1)
-                g = torch.empty(1, dtype=torch.float32, device=dev) if wsb else torch.ones(
-                    1, dtype=torch.float32, device=dev)
-                ws = L.workspace(wsb, dev)
-            else:
-                g = global_scale
-                if g.dtype != torch.float32 or g.numel() != 1 or g.device != dev:
-                    raise ValueError("quantize: global_scale must be one fp32 value on x's device")
+        # one allocation: [codes][scales][factor, workspace]; the views are made
+        # when they are asked for
+        cb, sb = rows * code_row_bytes(K), scale_bytes(rows, K, fmt)
+        at_s = -(-cb // 256) * 256
+        at_g = at_s + sb
+        derive = wsb = 0
+        if f == L.FP4_NV and global_scale is None:
+            derive, wsb = 1, L.load().mxb_fp4_quantize_workspace_size(rows, K, f, 1)
+        elif f == L.FP4_NV:
+            if (global_scale.dtype != torch.float32 or global_scale.numel() != 1
+                    or global_scale.device != dev):
+                raise ValueError("quantize: global_scale must be one fp32 value on x's device")
         elif global_scale is not None:
             raise ValueError("quantize: mxfp4 takes no global_scale")
-        rc = L.call("mxb_fp4_quantize", dev, x.data_ptr(), io, rows, K, ldx, f, L.ptr(g), derive,
-                    codes.data_ptr(), scales.data_ptr(), L.ptr(ws), wsb)
-        if rc:
-            L.check(rc, f"mxb_fp4_quantize({fmt}, {rows}x{K})")
+        buf = torch.empty(at_g + (16 + wsb if derive else 0), dtype=torch.uint8, device=dev)
+        base = buf.data_ptr()
+        gp = base + at_g if derive else L.ptr(global_scale)
+        if rows * K:
+            rc = L.call("mxb_fp4_quantize", dev, x.data_ptr(), io, rows, K, ldx, f, gp, derive, base,
+                        base + at_s, base + at_g + 16 if wsb else 0, wsb)
+            if rc:
+                L.check(rc, f"mxb_fp4_quantize({fmt}, {rows}x{K})")
+        elif derive:
+            buf[at_g:at_g + 4].view(torch.float32).fill_(1.0)
         self = cls.__new__(cls)
-        self.codes, self.scales, self.fmt, self.shape, self.global_scale = codes, scales, fmt, shape, g
+        self.fmt, self.shape, self.device = fmt, shape, dev
+        self._parts = (buf, rows, cb, at_s, sb, at_g if derive else global_scale)
+        self._ptrs = (base, base + at_s, gp)
         return self
+
+    def _views(self):
+        if len(self._parts) != 3:
+            buf, rows, cb, at_s, sb, g = self._parts
+            if isinstance(g, int):
+                g = buf[g:g + 4].view(torch.float32)
+            self._parts = (buf[:cb].view(rows, -1) if cb else buf[:0].view(rows, 0),
+                           buf[at_s:at_s + sb], g)
+        return self._parts
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._views()[0]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._views()[1]
+
+    @property
+    def global_scale(self) -> Optional[torch.Tensor]:
+        return self._views()[2]
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values, fp32 or bf16."""
         io = _IO.get(dtype)
         if io is None:
             raise ValueError(f"dequantize: float32 or bfloat16, not {dtype}")
-        L.require_cuda(self.codes, "fp4_tensor.dequantize")
-        dev, shape = self.codes.device, self.shape
+        dev, shape = self.device, self.shape
+        _require_cuda(dev, "fp4_tensor.dequantize")
         rows, K = shape[:-1].numel(), shape[-1]
         out = torch.empty(shape, dtype=dtype, device=dev)
-        rc = L.call("mxb_fp4_dequantize", dev, self.codes.data_ptr(), self.scales.data_ptr(),
-                    L.ptr(self.global_scale), rows, K, FORMATS[self.fmt], out.data_ptr(), io)
+        rc = L.call("mxb_fp4_dequantize", dev, *self._ptrs, rows, K, FORMATS[self.fmt],
+                    out.data_ptr(), io)
         if rc:
             L.check(rc, f"mxb_fp4_dequantize({self.fmt}, {rows}x{K})")
         return out
@@ -149,10 +181,6 @@ class fp4_tensor:
         rows, nb = self.shape[:-1].numel(), -(-self.shape[-1] // BLOCK[self.fmt])
         t = self.scales.view(-(-rows // 128), -(-nb // 4), 32, 4, 4).permute(0, 3, 2, 1, 4)
         return t.reshape(-(-rows // 128) * 128, -(-nb // 4) * 4)[:rows, :nb].contiguous()
-
-    @property
-    def device(self):
-        return self.codes.device
 
     @property
     def nbytes(self) -> int:
@@ -174,9 +202,9 @@ def fp4_matmul(a: fp4_tensor, b: fp4_tensor, bias: Optional[torch.Tensor] = None
         raise ValueError(f"fp4_matmul: {tuple(a.shape)} @ {tuple(b.shape)}^T")
     if out_dtype not in _IO:
         raise ValueError(f"fp4_matmul: float32 or bfloat16 out, not {out_dtype}")
-    L.require_cuda(a.codes, "fp4_matmul")
-    dev = a.codes.device
-    if b.codes.device != dev:
+    dev = a.device
+    _require_cuda(dev, "fp4_matmul")
+    if b.device != dev:
         raise ValueError("fp4_matmul: operands on different devices")
     M, K, N = a.shape[:-1].numel(), a.shape[-1], b.shape[0]
     if bias is not None:
@@ -188,9 +216,8 @@ def fp4_matmul(a: fp4_tensor, b: fp4_tensor, bias: Optional[torch.Tensor] = None
     if K == 0:  # an empty sum
         out.zero_()
         return out if bias is None else out.add_(bias)
-    rc = L.call("mxb_fp4_matmul", dev, a.codes.data_ptr(), a.scales.data_ptr(), L.ptr(a.global_scale),
-                b.codes.data_ptr(), b.scales.data_ptr(), L.ptr(b.global_scale), M, K, N,
-                FORMATS[a.fmt], L.ptr(bias), out.data_ptr(), _IO[out_dtype])
+    rc = L.call("mxb_fp4_matmul", dev, *a._ptrs, *b._ptrs, M, K, N, FORMATS[a.fmt], L.ptr(bias),
+                out.data_ptr(), _IO[out_dtype])
     if rc:
         L.check(rc, f"mxb_fp4_matmul({M}x{K}x{N}, {a.fmt})")
     return out
