@@ -16,6 +16,32 @@ namespace mxb {
 int kv_pool_check(int64_t n_pages, int heads, int page, int dim, int bits, const void* kc,
                   const void* ks, const void* vc, const void* vs);
 
+// prefix_attn.cu: tcgen05 attention of all query rows of a batch over a
+// prefix that they share.  Partial results by split and output row:
+// o [splits][n_rows][dim] relative to 2^m', ml (m, l, m', 0).
+struct PrefixArgs {
+  const void* q;  // bf16 [B][T][H * G][dim]
+  int B, T, H, G, dim, bits;
+  const void *k_codes, *v_codes;
+  const float *k_scales, *v_scales;
+  int64_t n_pages;
+  int page_shift;
+  const int* table;
+  int len;
+  int splits;
+  float scale_log2;
+  int64_t n_rows;
+  float* o;
+  float* ml;
+  int* err;
+};
+// Rows per CTA, the least query rows a KV head that pay for the tensor cores'
+// 128-row tiles, and keys per tile.
+constexpr int kPrefixMinRows = 48;
+int prefix_rows_per_cta(int64_t rows);
+constexpr int kPrefixKeys = 64;
+int prefix_attention(const PrefixArgs& a, cudaStream_t st);
+
 // gemm_cuda_core.cu
 int qgemm_generic(const void* a, const float* sa, bool sa_ok, const void* b, const float* sb,
                   bool sb_ok, int64_t M, int64_t K, int64_t N, int bits, int block, float* C,

@@ -897,7 +897,7 @@ __global__ void __launch_bounds__(kThreads)
 struct Plan {
   int nt_own, tiles_own, ctas_own;        // ctas_own 0: no own keys possible
   bool whole;                             // a unit per CTA, nothing to join
-  int nt_pre, tiles_pre, splits_pre;      // splits_pre 0: no prefix
+  int nt_pre, tiles_pre, splits_pre;      // splits_pre 0: no prefix; nt_pre 0: prefix_attn.cu
   size_t o_plan, o_main, o_cta, o_pre, bytes;  // workspace offsets
 };
 
@@ -923,7 +923,14 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, in
     const int64_t most = units * cdiv(max_keys, kTile * kWarps), fit = kSMs * ctas_per_sm(p.nt_own, rb);
     p.ctas_own = (int)(most < fit ? most : fit);
   }
-  if (prefix > 0) {
+  if (prefix > 0 && B * T * G >= kPrefixMinRows) {
+    // many rows: 128-row tensor-core tiles, one CTA an SM
+    const int64_t units = H * cdiv(B * T * G, prefix_rows_per_cta(B * T * G));
+    const int64_t most = cdiv(prefix, 2 * kPrefixKeys);
+    int64_t s = kSMs / units;
+    s = s < most ? s : most;
+    p.splits_pre = (int)(s < 1 ? 1 : s);
+  } else if (prefix > 0) {
     p.nt_pre = nt_of(B * T * G);
     p.tiles_pre = (int)cdiv(B * T * G, 8 * p.nt_pre);
     const int64_t most = cdiv(prefix, kTile * kWarps);
@@ -1056,8 +1063,35 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
     a.row_tiles = p.tiles_pre;
     a.splits = p.splits_pre;
     a.main = pre;
-    const int r = pattn::launch_any(tk, tv, a, bits, dim, p.nt_pre,
-                                    dim3((unsigned)p.splits_pre, (unsigned)(p.tiles_pre * heads)), st);
+    int r;
+    if (p.nt_pre == 0) {
+      PrefixArgs x = {};
+      x.q = q;
+      x.B = (int)B;
+      x.T = (int)T;
+      x.H = heads;
+      x.G = group;
+      x.dim = dim;
+      x.bits = bits;
+      x.k_codes = k_codes;
+      x.v_codes = v_codes;
+      x.k_scales = k_scales;
+      x.v_scales = v_scales;
+      x.n_pages = n_pages;
+      x.page_shift = a.page_shift;
+      x.table = prefix_table;
+      x.len = (int)prefix_len;
+      x.splits = p.splits_pre;
+      x.scale_log2 = a.scale_log2;
+      x.n_rows = a.n_rows;
+      x.o = pre.o;
+      x.ml = reinterpret_cast<float*>(pre.ml);
+      x.err = a.err;
+      r = prefix_attention(x, st);
+    } else {
+      r = pattn::launch_any(tk, tv, a, bits, dim, p.nt_pre,
+                            dim3((unsigned)p.splits_pre, (unsigned)(p.tiles_pre * heads)), st);
+    }
     if (r != MXB_OK) return r;
   }
   a.lengths = lengths;

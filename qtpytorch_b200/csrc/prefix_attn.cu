@@ -1,0 +1,539 @@
+// Attention of every query row of a batch over a prefix that they share, on
+// tcgen05 (paged_attn.cu describes the cache and the parts that it joins).
+//
+// With all B * T * G rows of a KV head taken together the prefix is a product
+// of two matrices, bound by arithmetic: 4 * rows * keys * dim operations, and
+// the work around it, one exponential a score and the unpacking of the codes.
+// A CTA owns 128 rows (two groups of 128 from 129 rows on, so that a key is
+// unpacked once for 256 rows) and a run of the keys, in tiles of 64:
+//   warp 0        TMA producer: raw codes and scales, ring of kStages tiles;
+//   warp 1        TMEM allocation, MMA issue: S = Q K^T (fp16 x fp16), two
+//                 buffers a row group; O += P V with P read from TMEM;
+//   warps 2-5     unpack codes to exact fp16 (K and V tiles have one layout:
+//                 K-major for the first product, MN-major for the second),
+//                 and lay out the tile's scales;
+//   warps 6-..    softmax, a thread a row: S from TMEM, running maximum, sum,
+//                 weights back to TMEM over S.
+// Scores: Q is fp16 under a power of two per row that puts its largest value
+// into [2^14, 2^15), the codes are exact.  Weights: p_j = exp2(s_j - m) times
+// sv_j / c, c a power of two of at least the largest value scale so far; with
+// 2^6 of room above and m following the maximum within 2^8, fp16 keeps 11 bits
+// of every weight down to 2^-20 of the largest possible one.  m, sums and
+// outputs are fp32; O is rescaled in TMEM only when m or c moves.
+// Pairs of codes unpack out of order; Q's columns are stored in the same
+// order and O's columns are put back when they are written.
+#include "mxb_common.cuh"
+#include "mxb_internal.h"
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#define MXB_ERROR_WORD_BY_POINTER
+#include "tc_ptx.cuh"
+
+using namespace mxb;
+
+namespace mxb {
+namespace pfx {
+
+constexpr int KT = kPrefixKeys;
+constexpr int kStages = 3;
+constexpr int kSlots = 4;  // scale slots: softmax may lag the unpacking by two tiles
+constexpr int kConvWarps = 4;
+constexpr float kRoom = 64.0f;  // 2^6
+
+template <int BITS, int D, int MT>
+struct Cfg {
+  static constexpr int RB = D * BITS / 8;
+  static constexpr int kRaw = KT * RB;
+  static constexpr int kAtom = KT * 128;           // 64 dims of every key
+  static constexpr int kPlane = kAtom * (D / 64);  // 16 or 8 KB
+  static constexpr int kQAtom = 128 * 128;
+  static constexpr int kQ = kQAtom * (D / 64);
+  static constexpr int kThreads = 64 + 32 * kConvWarps + 128 * MT;
+  static constexpr size_t oK = (size_t)MT * kQ, oV = oK + 2 * kPlane, oRaw = oV + 2 * kPlane;
+  static constexpr size_t oRawS = oRaw + (size_t)kStages * 2 * kRaw;
+  static constexpr size_t oSc = oRawS + (size_t)kStages * 2 * KT * 4;
+  static constexpr size_t oBars = oSc + (size_t)kSlots * (2 * KT + 4) * 4;
+  static constexpr size_t kSmem = 1024 + oBars + 512;
+  // TMEM: per row group two S buffers of 64 columns, then O
+  static constexpr int kCols = MT == 2 ? 512 : 256;
+};
+
+struct Bars {
+  uint64_t raw_full[kStages], raw_empty[kStages];
+  uint64_t kready[2], kfree[2], vready[2], vfree[2];
+  uint64_t sready[2][2], pready[2][2], pvdone[2];
+  uint64_t scready[kSlots];
+  uint64_t qready;
+  uint32_t tmem_base;
+};
+static_assert(sizeof(Bars) <= 512, "barrier block overflows its slot");
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t hsub2u(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t hf2(float lo, float hi) {
+  const __half2 t = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+
+// Position p of a group of unpacked codes holds dim order(p) of the group: int8
+// words give (0, 2), (1, 3); int4 words (0, 4), (1, 5), (2, 6), (3, 7).
+template <int BITS>
+__host__ __device__ constexpr int order(int p) {
+  return BITS == 8 ? ((p & 4) | ((p & 1) << 1) | ((p & 2) >> 1))
+                   : ((p & 1) << 2) | (p >> 1);
+}
+
+// 16 bytes of codes -> 16 (int8) or 32 (int4) exact fp16 values as 16-byte
+// chunks of eight.
+template <int BITS>
+__device__ __forceinline__ void unpack16(uint4 r, uint4 (&o)[BITS == 8 ? 2 : 4]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  if constexpr (BITS == 8) {
+    uint32_t v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = hsub2u((w[i] & 0x00FF00FFu) ^ 0x64806480u, 0x64806480u);
+      v[2 * i + 1] = hsub2u(((w[i] >> 8) & 0x00FF00FFu) ^ 0x64806480u, 0x64806480u);
+    }
+    o[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    o[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        v[k] = hsub2u(((w[i] >> (4 * k)) & 0x000F000Fu) ^ 0x64086408u, 0x64086408u);
+      o[i] = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+  }
+}
+
+// One raw tile [KT][RB] -> fp16 plane, rows of 128 bytes per 64-dim atom,
+// 128-byte swizzle (thread t of the 128 unpackers).
+template <int BITS, int D>
+__device__ __forceinline__ void unpack_tile(const uint8_t* raw, uint8_t* plane, int t) {
+  constexpr int RB = D * BITS / 8, C = RB / 16, N = BITS == 8 ? 2 : 4;  // chunks a row, out per chunk
+  constexpr int kAtom = KT * 128;
+#pragma unroll
+  for (int i = t; i < KT * C; i += 32 * kConvWarps) {
+    const int row = i / C, c = i % C;
+    const uint4 r = *reinterpret_cast<const uint4*>(raw + row * RB + c * 16);
+    uint4 o[N];
+    unpack16<BITS>(r, o);
+    // lanes of the second atom start at the next chunk, so a store's lanes
+    // cover all banks
+    const int first = (c * N) >> 3;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int kk = (k + first) % N;
+      const int ch = c * N + kk;
+      uint4 v = o[0];
+#pragma unroll
+      for (int x = 1; x < N; ++x)
+        if (kk == x) v = o[x];
+      *reinterpret_cast<uint4*>(plane + (ch >> 3) * kAtom + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v;
+    }
+  }
+}
+
+template <int BITS, int D, int MT>
+__global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
+    prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_k,
+                       const __grid_constant__ CUtensorMap tmap_v, const PrefixArgs a, int box) {
+  using C = Cfg<BITS, D, MT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  Bars* bars = reinterpret_cast<Bars*>(smem + C::oBars);
+  float* sc_slots = reinterpret_cast<float*>(smem + C::oSc);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int boxes = KT / box;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&bars->raw_full[s], boxes);
+      mbar_init(&bars->raw_empty[s], kConvWarps);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars->kready[b], kConvWarps);
+      mbar_init(&bars->kfree[b], 1);
+      mbar_init(&bars->vready[b], kConvWarps);
+      mbar_init(&bars->vfree[b], 1);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&bars->sready[x][b], 1);
+        mbar_init(&bars->pready[x][b], 4);
+      }
+      mbar_init(&bars->pvdone[b], 1);
+    }
+    for (int s = 0; s < kSlots; ++s) mbar_init(&bars->scready[s], kConvWarps);
+    mbar_init(&bars->qready, 4 * MT);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_base, C::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = bars->tmem_base;
+  pdl_trigger();
+  pdl_wait();
+
+  const int h = blockIdx.z, r0 = blockIdx.y * 128 * MT;
+  const int rows = a.B * a.T * a.G;
+  const int tiles = (a.len + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
+  const int t_lo = min((int)blockIdx.x * per, tiles), n = min(per, tiles - t_lo);
+  auto t_s = [&](int x, int b) { return tbase + (uint32_t)(x * (128 + D) + b * 64); };
+  auto t_o = [&](int x) { return tbase + (uint32_t)(x * (128 + D) + 128); };
+
+  if (warp == 0) {
+    const int page_mask = (1 << a.page_shift) - 1;
+    for (int i = 0; i < n; ++i) {
+      const int s = i % kStages, round = i / kStages;
+      const int pos = (t_lo + i) * KT + lane * box;
+      int p = -1;
+      if (lane < boxes && pos < a.len) {
+        p = __ldg(a.table + (pos >> a.page_shift));
+        if (p < 0 || p >= a.n_pages) {
+          if (a.err) atomicCAS(a.err, 0, kErrIndex);
+          p = 0;
+        }
+      }
+      if (round > 0 && !mbar_wait_warp_to(&bars->raw_empty[s], (round - 1) & 1, kErrTimeoutEmpty, a.err))
+        break;
+      if (lane < boxes) {
+        uint64_t* bar = &bars->raw_full[s];
+        if (p >= 0) {
+          const int row = ((p * a.H + h) << a.page_shift) + (pos & page_mask);
+          uint8_t* dst = smem + C::oRaw + (size_t)s * 2 * C::kRaw + lane * box * C::RB;
+          float* sc = reinterpret_cast<float*>(smem + C::oRawS) + s * 2 * KT + lane * box;
+          mbar_expect_tx(bar, (uint32_t)box * (2 * C::RB + 8));
+          tma_load_2d(dst, &tmap_k, bar, 0, row);
+          tma_load_2d(dst + C::kRaw, &tmap_v, bar, 0, row);
+          bulk_load_g2s(sc, a.k_scales + row, (uint32_t)box * 4, bar);
+          bulk_load_g2s(sc + KT, a.v_scales + row, (uint32_t)box * 4, bar);
+        } else {
+          mbar_arrive(bar);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      constexpr uint32_t id_s = make_idesc(/*F32*/ 1, /*F16*/ 0, 0, 0, 128, KT);
+      constexpr uint32_t id_o = make_idesc(1, 0, 0, /*B MN-major*/ 1, 128, D);
+      const uint32_t sq = smem_u32(smem), sk = smem_u32(smem + C::oK), sv = smem_u32(smem + C::oV);
+      bool ok = mbar_wait_to(&bars->qready, 0, kErrTimeoutFull, a.err);
+      auto issue_s = [&](int t) {
+        const int b = t & 1;
+        ok = ok && mbar_wait_to(&bars->kready[b], (t >> 1) & 1, kErrTimeoutFull, a.err);
+        if (!ok) return;
+        tc_fence_after();
+        for (int x = 0; x < MT; ++x) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_f16(t_s(x, b),
+                    desc_kmajor_sw128(sq + x * C::kQ + (kk >> 2) * C::kQAtom + (kk & 3) * 32),
+                    desc_kmajor_sw128(sk + b * C::kPlane + (kk >> 2) * C::kAtom + (kk & 3) * 32),
+                    id_s, kk > 0 ? 1u : 0u);
+          mma_commit(&bars->sready[x][b]);
+        }
+        mma_commit(&bars->kfree[b]);
+      };
+      issue_s(0);
+      if (n > 1) issue_s(1);
+      for (int t = 0; t < n && ok; ++t) {
+        const int b = t & 1;
+        ok = ok && mbar_wait_to(&bars->vready[b], (t >> 1) & 1, kErrTimeoutFull, a.err);
+        for (int x = 0; x < MT && ok; ++x) {
+          ok = mbar_wait_to(&bars->pready[x][b], (t >> 1) & 1, kErrTimeoutTmemFull, a.err);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < KT / 16; ++kk)
+            mma_f16_ts(t_o(x), t_s(x, b) + kk * 8,
+                       desc_mnmajor_sw128(sv + b * C::kPlane + kk * 16 * 128, C::kAtom), id_o,
+                       (t > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(&bars->pvdone[x]);
+        }
+        if (!ok) break;
+        mma_commit(&bars->vfree[b]);
+        // P of tile t has been consumed by the products issued above, which
+        // run in issue order: its buffer takes S of tile t + 2
+        if (t + 2 < n) issue_s(t + 2);
+      }
+    }
+  } else if (warp < 2 + kConvWarps) {
+    const int t = threadIdx.x - 64;
+    float c = 0.0f;  // power of two above every value scale so far (0: none)
+    for (int i = 0; i < n; ++i) {
+      const int s = i % kStages, b = i & 1, slot = i % kSlots;
+      if (!mbar_wait_warp_to(&bars->raw_full[s], (i / kStages) & 1, kErrTimeoutFull, a.err)) break;
+      const uint8_t* raw = smem + C::oRaw + (size_t)s * 2 * C::kRaw;
+      const float* rsc = reinterpret_cast<const float*>(smem + C::oRawS) + s * 2 * KT;
+      if (i >= 2 && !mbar_wait_warp_to(&bars->kfree[b], ((i >> 1) - 1) & 1, kErrTimeoutEmpty, a.err)) break;
+      {
+        // scales: every warp finds the tile's largest value scale for itself
+        const int valid = a.len - (t_lo + i) * KT;
+        const float v0 = lane < valid ? rsc[KT + lane] : 0.0f;
+        const float v1 = lane + 32 < valid ? rsc[KT + lane + 32] : 0.0f;
+        float mx = fmaxf(v0, v1);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        if (mx > c || c == 0.0f) {
+          // four times the next power of two, between 2^-100 and 2^100
+          const int ex = min(max((int)(__float_as_uint(mx) >> 23) + 3, 27), 227);
+          c = __uint_as_float((uint32_t)ex << 23);
+        }
+        float* sl = sc_slots + slot * (2 * KT + 4);
+        if (warp < 4) {  // warps 2 and 3: 32 keys each
+          const int j = (warp - 2) * 32 + lane;
+          sl[j] = j < valid ? rsc[j] * a.scale_log2 : 0.0f;
+          sl[KT + j] = (warp == 2 ? v0 : v1) * (kRoom / c);
+        } else if (warp == 4 && lane == 0) {
+          sl[2 * KT] = c;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->scready[slot]);
+      }
+      unpack_tile<BITS, D>(raw, smem + C::oK + b * C::kPlane, t);
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->kready[b]);
+      if (i >= 2 && !mbar_wait_warp_to(&bars->vfree[b], ((i >> 1) - 1) & 1, kErrTimeoutEmpty, a.err)) break;
+      unpack_tile<BITS, D>(raw + C::kRaw, smem + C::oV + b * C::kPlane, t);
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bars->vready[b]);
+        mbar_arrive(&bars->raw_empty[s]);
+      }
+    }
+  } else {
+    const int x = (warp - 2 - kConvWarps) >> 2, q4 = warp & 3;
+    const int lr = q4 * 32 + lane, row = r0 + x * 128 + lr;
+    const uint32_t lane_sel = (uint32_t)(q4 * 32) << 16;
+    const bool live = row < rows;
+    int64_t id = 0;  // output row
+    if (live) {
+      const int b = row / (a.T * a.G), rr = row - b * a.T * a.G, t = rr / a.G;
+      id = ((int64_t)b * a.T + t) * ((int64_t)a.H * a.G) + (int64_t)h * a.G + (rr - t * a.G);
+    }
+    // ── Q row: bf16 -> fp16 under a power of two, columns in unpack order ──
+    float rowf;
+    {
+      const uint4* qp = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + id * D);
+      float top = 0.0f;
+#pragma unroll 4
+      for (int ch = 0; ch < D / 8; ++ch) {
+        const uint4 r = __ldg(qp + ch);
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)),
+                                 fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+      }
+      const int ex = (int)(__float_as_uint(top) >> 23);
+      const int up = !live || ex == 0 || ex == 255 ? 127 : min(127 + 14 + 127 - ex, 227);
+      const float f = live ? __uint_as_float((uint32_t)up << 23) : 0.0f;
+      rowf = __uint_as_float((uint32_t)(254 - up) << 23);
+      uint8_t* dst = smem + (size_t)x * C::kQ;
+#pragma unroll 4
+      for (int ch = 0; ch < D / 8; ++ch) {
+        const uint4 r = __ldg(qp + ch);
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[2 * i] = live ? __uint_as_float(w[i] << 16) * f : 0.0f;
+          v[2 * i + 1] = live ? __uint_as_float(w[i] & 0xffff0000u) * f : 0.0f;
+        }
+        const uint4 o = make_uint4(hf2(v[order<BITS>(0)], v[order<BITS>(1)]),
+                                   hf2(v[order<BITS>(2)], v[order<BITS>(3)]),
+                                   hf2(v[order<BITS>(4)], v[order<BITS>(5)]),
+                                   hf2(v[order<BITS>(6)], v[order<BITS>(7)]));
+        *reinterpret_cast<uint4*>(dst + (ch >> 3) * C::kQAtom + lr * 128 + (((ch & 7) ^ (lr & 7)) << 4)) = o;
+      }
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->qready);
+    }
+    float mu = 0.0f, m_top = -INFINITY, l = 0.0f, c = 1.0f;
+    bool ok = true;
+    for (int t = 0; t < n; ++t) {
+      const int b = t & 1, slot = t % kSlots;
+      ok = mbar_wait_warp_to(&bars->scready[slot], (t / kSlots) & 1, kErrTimeoutFull, a.err) &&
+           mbar_wait_warp_to(&bars->sready[x][b], (t >> 1) & 1, kErrTimeoutTmemFull, a.err);
+      if (!ok) break;
+      tc_fence_after();
+      float v[KT];
+      {
+        uint32_t r0v[32], r1v[32];
+        tmem_ld32(t_s(x, b) + lane_sel, r0v);
+        tmem_ld32(t_s(x, b) + lane_sel + 32, r1v);
+        tmem_wait_ld();
+        const float4* ks = reinterpret_cast<const float4*>(sc_slots + slot * (2 * KT + 4));
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 k0 = ks[j / 4], k1 = ks[8 + j / 4];
+          v[j] = __uint_as_float(r0v[j]) * k0.x;
+          v[j + 1] = __uint_as_float(r0v[j + 1]) * k0.y;
+          v[j + 2] = __uint_as_float(r0v[j + 2]) * k0.z;
+          v[j + 3] = __uint_as_float(r0v[j + 3]) * k0.w;
+          v[32 + j] = __uint_as_float(r1v[j]) * k1.x;
+          v[33 + j] = __uint_as_float(r1v[j + 1]) * k1.y;
+          v[34 + j] = __uint_as_float(r1v[j + 2]) * k1.z;
+          v[35 + j] = __uint_as_float(r1v[j + 3]) * k1.w;
+        }
+      }
+      const int valid = a.len - (t_lo + t) * KT;
+      if (valid < KT) {
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+          if (j >= valid) v[j] = -INFINITY;
+      }
+      float mx = v[0];
+#pragma unroll
+      for (int j = 1; j < KT; ++j) mx = fmaxf(mx, v[j]);
+      mx *= rowf;
+      const float cn = sc_slots[slot * (2 * KT + 4) + 2 * KT];
+      if (__any_sync(0xffffffffu, mx > m_top || cn != c)) {
+        const float m0 = m_top == -INFINITY ? -INFINITY : mu;
+        const float m1 = fmaxf(m0, mx);
+        mu = m1 == -INFINITY ? 0.0f : m1;
+        const float am = ex2(m0 - mu);
+        l *= am;
+        if (t > 0) {
+          // O of the tiles before is complete, and the next product waits for
+          // this tile's weights
+          ok = mbar_wait_warp_to(&bars->pvdone[x], (t - 1) & 1, kErrTimeoutTmemEmpty, a.err);
+          if (!ok) break;
+          tc_fence_after();
+          const float alpha = am * (c / cn);
+#pragma unroll 1
+          for (int d = 0; d < D; d += 32) {
+            uint32_t r[32];
+            tmem_ld32(t_o(x) + lane_sel + d, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+            tmem_st32(t_o(x) + lane_sel + d, r);
+          }
+        }
+        m_top = m1 + 8.0f;
+        c = cn;
+      }
+      const float4* vs = reinterpret_cast<const float4*>(sc_slots + slot * (2 * KT + 4) + KT);
+      uint32_t pk[32];
+      float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+      for (int j = 0; j < KT; j += 4) {
+        const float4 w = vs[j / 4];
+        const float p0 = ex2(__fmaf_rn(v[j], rowf, -mu)), p1 = ex2(__fmaf_rn(v[j + 1], rowf, -mu));
+        const float p2 = ex2(__fmaf_rn(v[j + 2], rowf, -mu)), p3 = ex2(__fmaf_rn(v[j + 3], rowf, -mu));
+        s0 += p0 + p2;
+        s1 += p1 + p3;
+        pk[j / 2] = hf2(p0 * w.x, p1 * w.y);
+        pk[j / 2 + 1] = hf2(p2 * w.z, p3 * w.w);
+      }
+      l += s0 + s1;
+      tmem_st32(t_s(x, b) + lane_sel, pk);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->pready[x][b]);
+    }
+    // ── this split's part ──
+    if (ok && n > 0) ok = mbar_wait_warp_to(&bars->pvdone[x], (n - 1) & 1, kErrTimeoutDone, a.err);
+    tc_fence_after();
+    const int64_t pr = (int64_t)blockIdx.x * a.n_rows + id;
+#pragma unroll 1
+    for (int d = 0; d < D; d += 32) {
+      uint32_t r[32];
+      if (n > 0) {
+        tmem_ld32(t_o(x) + lane_sel + d, r);
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[i] = 0u;
+      }
+      if (live) {
+#pragma unroll
+        for (int g8 = 0; g8 < 32; g8 += 8) {
+          float o[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[order<BITS>(i)] = __uint_as_float(r[g8 + i]);
+          float4* dst = reinterpret_cast<float4*>(a.o + pr * D + d + g8);
+          dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+          dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+        }
+      }
+    }
+    if (live) {
+      // O = 2^m' sum: m' = m + log2(c / room), c a power of two
+      const float lc = (float)((int)(__float_as_uint(c) >> 23) - 127) - 6.0f;
+      reinterpret_cast<float4*>(a.ml)[pr] =
+          m_top == -INFINITY ? make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f)
+                             : make_float4(mu, l, mu + lc, 0.0f);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    // every product issued is complete once the last commits are (they were
+    // waited for by the softmax warps)
+    tc_fence_after();
+    tmem_dealloc(tbase, C::kCols);
+  }
+}
+
+template <int BITS, int D, int MT>
+int launch(const CUtensorMap& tk, const CUtensorMap& tv, const PrefixArgs& a, int box, cudaStream_t st) {
+  using C = Cfg<BITS, D, MT>;
+  auto kern = prefix_attn_kernel<BITS, D, MT>;
+  static_assert(C::kSmem <= 227 * 1024, "shared memory");
+  MXB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem));
+  const dim3 grid((unsigned)a.splits, (unsigned)cdiv((int64_t)a.B * a.T * a.G, 128 * MT), (unsigned)a.H);
+  MXB_CUDA_TRY(launch_pdl(kern, grid, C::kThreads, C::kSmem, st, tk, tv, a, box));
+  MXB_LAUNCH_CHECK();
+  return MXB_OK;
+}
+
+template <int BITS, int D>
+int launch_mt(const CUtensorMap& tk, const CUtensorMap& tv, const PrefixArgs& a, int box, cudaStream_t st) {
+  return prefix_rows_per_cta((int64_t)a.B * a.T * a.G) == 256 ? launch<BITS, D, 2>(tk, tv, a, box, st)
+                                                              : launch<BITS, D, 1>(tk, tv, a, box, st);
+}
+
+}  // namespace pfx
+
+int prefix_rows_per_cta(int64_t rows) { return rows > 128 ? 256 : 128; }
+
+int prefix_attention(const PrefixArgs& a, cudaStream_t st) {
+  CUtensorMap tk, tv;
+  const int page = 1 << a.page_shift, box = page < pfx::KT ? page : pfx::KT;
+  const uint64_t rb = (uint64_t)a.dim * a.bits / 8, rows = (uint64_t)a.n_pages * a.H * page;
+  if (!encode_tmap_2d(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.k_codes, rb, rows, (uint32_t)rb, box,
+                      CU_TENSOR_MAP_SWIZZLE_NONE) ||
+      !encode_tmap_2d(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.v_codes, rb, rows, (uint32_t)rb, box,
+                      CU_TENSOR_MAP_SWIZZLE_NONE))
+    return MXB_E_CUDA;
+  if (a.bits == 8)
+    return a.dim == 128 ? pfx::launch_mt<8, 128>(tk, tv, a, box, st)
+                        : pfx::launch_mt<8, 64>(tk, tv, a, box, st);
+  return a.dim == 128 ? pfx::launch_mt<4, 128>(tk, tv, a, box, st)
+                      : pfx::launch_mt<4, 64>(tk, tv, a, box, st);
+}
+
+}  // namespace mxb
