@@ -252,6 +252,7 @@ __global__ void __launch_bounds__(kThreads)
         uint32_t r[32];
         tmem_ld32(tbase + ((uint32_t)(q * 32) << 16) + c0, r);
         tmem_wait_ld();
+        tmem_landed(r);
         if (n < a.N) {
           OutT* o = out + (size_t)(m0 + c0) * a.N + n;
 #pragma unroll
@@ -273,6 +274,7 @@ __global__ void __launch_bounds__(kThreads)
         uint32_t r[32];
         tmem_ld32(tbase + ((uint32_t)(q * 32) << 16) + c0, r);
         tmem_wait_ld();
+        tmem_landed(r);
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
           part[(c0 + j) * BM + q * 32 + lane] = __uint_as_float(r[j]);

@@ -9,10 +9,10 @@
 //   warp 0        TMA producer: raw codes and scales, ring of kStages tiles;
 //   warp 1        TMEM allocation, MMA issue: S = Q K^T (fp16 x fp16), two
 //                 buffers a row group; O += P V with P read from TMEM;
-//   warps 2-5     unpack codes to exact fp16 (K and V tiles have one layout:
+//   warps 2-9     unpack codes to exact fp16 (K and V tiles have one layout:
 //                 K-major for the first product, MN-major for the second),
 //                 and lay out the tile's scales;
-//   warps 6-..    softmax, a thread a row: S from TMEM, running maximum, sum,
+//   warps 10-..   softmax, a thread a row: S from TMEM, running maximum, sum,
 //                 weights back to TMEM over S.
 // Scores: Q is fp16 under a power of two per row that puts its largest value
 // into [2^14, 2^15), the codes are exact.  Weights: p_j = exp2(s_j - m) times
@@ -39,7 +39,7 @@ namespace pfx {
 constexpr int KT = kPrefixKeys;
 constexpr int kStages = 3;
 constexpr int kSlots = 4;  // scale slots: softmax may lag the unpacking by two tiles
-constexpr int kConvWarps = 4;
+constexpr int kConvWarps = 8;
 constexpr float kRoom = 64.0f;  // 2^6
 
 template <int BITS, int D, int MT>
@@ -120,29 +120,35 @@ __device__ __forceinline__ void unpack16(uint4 r, uint4 (&o)[BITS == 8 ? 2 : 4])
 }
 
 // One raw tile [KT][RB] -> fp16 plane, rows of 128 bytes per 64-dim atom,
-// 128-byte swizzle (thread t of the 128 unpackers).
+// 128-byte swizzle (thread t of the unpackers).  Eight neighbouring lanes take
+// chunks of one atom from two (four) rows, so that their 16-byte stores cover
+// all banks.
 template <int BITS, int D>
 __device__ __forceinline__ void unpack_tile(const uint8_t* raw, uint8_t* plane, int t) {
   constexpr int RB = D * BITS / 8, C = RB / 16, N = BITS == 8 ? 2 : 4;  // chunks a row, out per chunk
-  constexpr int kAtom = KT * 128;
+  constexpr int kAtom = KT * 128, kThr = 32 * kConvWarps;
 #pragma unroll
-  for (int i = t; i < KT * C; i += 32 * kConvWarps) {
-    const int row = i / C, c = i % C;
+  for (int i0 = 0; i0 < KT * C; i0 += kThr) {
+    const int i = i0 + t;
+    if (KT * C < kThr && i >= KT * C) break;
+    int row, c;
+    if (C == 8) {
+      c = (i & 3) | (((i >> 3) & 1) << 2);
+      row = ((i >> 4) << 1) | ((i >> 2) & 1);
+    } else if (C == 4 && BITS == 4) {
+      c = (i & 1) | (((i >> 3) & 1) << 1);
+      row = ((i >> 4) << 2) | ((i >> 1) & 3);
+    } else {
+      c = i % C;
+      row = i / C;
+    }
     const uint4 r = *reinterpret_cast<const uint4*>(raw + row * RB + c * 16);
     uint4 o[N];
     unpack16<BITS>(r, o);
-    // lanes of the second atom start at the next chunk, so a store's lanes
-    // cover all banks
-    const int first = (c * N) >> 3;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int kk = (k + first) % N;
-      const int ch = c * N + kk;
-      uint4 v = o[0];
-#pragma unroll
-      for (int x = 1; x < N; ++x)
-        if (kk == x) v = o[x];
-      *reinterpret_cast<uint4*>(plane + (ch >> 3) * kAtom + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v;
+      const int ch = c * N + k;
+      *reinterpret_cast<uint4*>(plane + (ch >> 3) * kAtom + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = o[k];
     }
   }
 }
@@ -252,9 +258,15 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
         mma_commit(&bars->kfree[b]);
       };
       issue_s(0);
-      if (n > 1) issue_s(1);
       for (int t = 0; t < n && ok; ++t) {
         const int b = t & 1;
+        if (t + 1 < n) {
+          // S of the next tile goes over P of the last one: that product has to
+          // be complete, since MMAs of different shapes need not run in the
+          // order they are issued (the softmax of tile t runs meanwhile)
+          if (t > 0) ok = mbar_wait_to(&bars->pvdone[MT - 1], (t - 1) & 1, kErrTimeoutTmemEmpty, a.err);
+          if (ok) issue_s(t + 1);
+        }
         ok = ok && mbar_wait_to(&bars->vready[b], (t >> 1) & 1, kErrTimeoutFull, a.err);
         for (int x = 0; x < MT && ok; ++x) {
           ok = mbar_wait_to(&bars->pready[x][b], (t >> 1) & 1, kErrTimeoutTmemFull, a.err);
@@ -267,11 +279,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
                        (t > 0 || kk > 0) ? 1u : 0u);
           mma_commit(&bars->pvdone[x]);
         }
-        if (!ok) break;
-        mma_commit(&bars->vfree[b]);
-        // P of tile t has been consumed by the products issued above, which
-        // run in issue order: its buffer takes S of tile t + 2
-        if (t + 2 < n) issue_s(t + 2);
+        if (ok) mma_commit(&bars->vfree[b]);
       }
     }
   } else if (warp < 2 + kConvWarps) {
@@ -297,7 +305,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
           c = __uint_as_float((uint32_t)ex << 23);
         }
         float* sl = sc_slots + slot * (2 * KT + 4);
-        if (warp < 4) {  // warps 2 and 3: 32 keys each
+        if (warp < 4) {  // the first two of these warps: 32 keys each
           const int j = (warp - 2) * 32 + lane;
           sl[j] = j < valid ? rsc[j] * a.scale_log2 : 0.0f;
           sl[KT + j] = (warp == 2 ? v0 : v1) * (kRoom / c);
@@ -334,11 +342,13 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
     float rowf;
     {
       const uint4* qp = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + id * D);
+      uint4 raw[D / 8];
+#pragma unroll
+      for (int ch = 0; ch < D / 8; ++ch) raw[ch] = __ldg(qp + ch);
       float top = 0.0f;
-#pragma unroll 4
+#pragma unroll
       for (int ch = 0; ch < D / 8; ++ch) {
-        const uint4 r = __ldg(qp + ch);
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+        const uint32_t w[4] = {raw[ch].x, raw[ch].y, raw[ch].z, raw[ch].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)),
@@ -349,10 +359,9 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
       const float f = live ? __uint_as_float((uint32_t)up << 23) : 0.0f;
       rowf = __uint_as_float((uint32_t)(254 - up) << 23);
       uint8_t* dst = smem + (size_t)x * C::kQ;
-#pragma unroll 4
+#pragma unroll
       for (int ch = 0; ch < D / 8; ++ch) {
-        const uint4 r = __ldg(qp + ch);
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+        const uint32_t w[4] = {raw[ch].x, raw[ch].y, raw[ch].z, raw[ch].w};
         float v[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -383,6 +392,8 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
         tmem_ld32(t_s(x, b) + lane_sel, r0v);
         tmem_ld32(t_s(x, b) + lane_sel + 32, r1v);
         tmem_wait_ld();
+        tmem_landed(r0v);
+        tmem_landed(r1v);
         const float4* ks = reinterpret_cast<const float4*>(sc_slots + slot * (2 * KT + 4));
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
@@ -403,11 +414,12 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
         for (int j = 0; j < KT; ++j)
           if (j >= valid) v[j] = -INFINITY;
       }
-      float mx = v[0];
+      float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-      for (int j = 1; j < KT; ++j) mx = fmaxf(mx, v[j]);
-      mx *= rowf;
+      for (int j = 4; j < KT; ++j) m4[j & 3] = fmaxf(m4[j & 3], v[j]);
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * rowf;
       const float cn = sc_slots[slot * (2 * KT + 4) + 2 * KT];
+      bool waited = t == 0;
       if (__any_sync(0xffffffffu, mx > m_top || cn != c)) {
         const float m0 = m_top == -INFINITY ? -INFINITY : mu;
         const float m1 = fmaxf(m0, mx);
@@ -415,10 +427,11 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
         const float am = ex2(m0 - mu);
         l *= am;
         if (t > 0) {
-          // O of the tiles before is complete, and the next product waits for
-          // this tile's weights
+          // O of the tiles before has to be complete; the next product waits
+          // for this tile's weights
           ok = mbar_wait_warp_to(&bars->pvdone[x], (t - 1) & 1, kErrTimeoutTmemEmpty, a.err);
           if (!ok) break;
+          waited = true;
           tc_fence_after();
           const float alpha = am * (c / cn);
 #pragma unroll 1
@@ -426,6 +439,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
             uint32_t r[32];
             tmem_ld32(t_o(x) + lane_sel + d, r);
             tmem_wait_ld();
+            tmem_landed(r);
 #pragma unroll
             for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
             tmem_st32(t_o(x) + lane_sel + d, r);
@@ -448,6 +462,12 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
         pk[j / 2 + 1] = hf2(p2 * w.z, p3 * w.w);
       }
       l += s0 + s1;
+      // every phase of pvdone is waited for in turn: a parity tells only the
+      // last completed phase from the one before it
+      if (!waited) {
+        ok = mbar_wait_warp_to(&bars->pvdone[x], (t - 1) & 1, kErrTimeoutTmemEmpty, a.err);
+        if (!ok) break;
+      }
       tmem_st32(t_s(x, b) + lane_sel, pk);
       tmem_wait_st();
       tc_fence_before();
@@ -464,6 +484,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
       if (n > 0) {
         tmem_ld32(t_o(x) + lane_sel + d, r);
         tmem_wait_ld();
+        tmem_landed(r);
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) r[i] = 0u;
