@@ -9,10 +9,10 @@
 //   warp 0        TMA producer: raw codes and scales, ring of kStages tiles;
 //   warp 1        TMEM allocation, MMA issue: S = Q K^T (fp16 x fp16), two
 //                 buffers a row group; O += P V with P read from TMEM;
-//   warps 2-9     unpack codes to exact fp16 (K and V tiles have one layout:
+//   warps 2-5     unpack codes to exact fp16 (K and V tiles have one layout:
 //                 K-major for the first product, MN-major for the second),
 //                 and lay out the tile's scales;
-//   warps 10-..   softmax, a thread a row: S from TMEM, running maximum, sum,
+//   warps 6-..    softmax, a thread a row: S from TMEM, running maximum, sum,
 //                 weights back to TMEM over S.
 // Scores: Q is fp16 under a power of two per row that puts its largest value
 // into [2^14, 2^15), the codes are exact.  Weights: p_j = exp2(s_j - m) times
@@ -39,7 +39,7 @@ namespace pfx {
 constexpr int KT = kPrefixKeys;
 constexpr int kStages = 3;
 constexpr int kSlots = 4;  // scale slots: softmax may lag the unpacking by two tiles
-constexpr int kConvWarps = 8;
+constexpr int kConvWarps = 4;
 constexpr float kRoom = 64.0f;  // 2^6
 
 template <int BITS, int D, int MT>
@@ -495,9 +495,12 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
           float o[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) o[order<BITS>(i)] = __uint_as_float(r[g8 + i]);
-          float4* dst = reinterpret_cast<float4*>(a.o + pr * D + d + g8);
-          dst[0] = make_float4(o[0], o[1], o[2], o[3]);
-          dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+          // a whole 32-byte sector a lane
+          asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(
+                           a.o + pr * D + d + g8),
+                       "f"(o[0]), "f"(o[1]), "f"(o[2]), "f"(o[3]), "f"(o[4]), "f"(o[5]), "f"(o[6]),
+                       "f"(o[7])
+                       : "memory");
         }
       }
     }
