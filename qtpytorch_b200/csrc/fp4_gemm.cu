@@ -13,12 +13,18 @@
 // of it; the S CTAs form a cluster, leave their partial tiles in shared memory
 // and add them over distributed shared memory in rank order, so the result
 // does not depend on timing and one launch does it all.
-//   warp 0     TMA producer: codes of 128 features and NT tokens (256 K values
-//              = 128 bytes a row, 128-byte swizzle) and their scale tiles
-//              (bulk copies; the stored order is the tensor core's) a stage;
-//   warp 1     TMEM allocation; per stage copies the scale tiles to TMEM
-//              (tcgen05.cp) and issues 4 MMAs of K = 64;
-//   warps 2-9  epilogue: tcgen05.ld, factor, bias, rounding, store.
+//   warp 0       TMA producer: codes of 128 features and NT tokens (256 K values
+//                = 128 bytes a row, 128-byte swizzle) a stage;
+//   warp 1       TMEM allocation, 4 MMAs of K = 64 a stage;
+//   warps 2-9    epilogue: tcgen05.ld, factor, bias, rounding, store;
+//   warps 10-13  scales: the stored order is the tensor core's, so they go by
+//                cp.async into a ring and with one or two tcgen05.st a stage to
+//                TMEM.  tcgen05.cp would stand in line with the MMAs (about 65
+//                cycles a 512-byte tile measured, so 520 beside 256 of MMAs for
+//                nvfp4), and bulk copies would cost the TMA unit as much as a
+//                box of codes each (14 of 100 us at 4096 x 8192 x 8192).
+// Two CTAs an SM: one alone draws 73 KB/us of operands through its ring, two
+// 121, and each covers the other's start and epilogue.
 #include "mxb_common.cuh"
 #include "mxb_internal.h"
 
@@ -35,7 +41,8 @@ namespace fp4g {
 constexpr int BM = 128;       // features per tile
 constexpr int BK = 256;       // K values per stage (128 bytes of codes)
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kSfWarps = 4;
+constexpr int kThreads = 64 + 32 * (kEpiWarps + kSfWarps);
 constexpr int kMaxSplit = 8;  // portable cluster size
 
 constexpr int kTileF = BM * BK / 2;  // 16 KB of feature codes
@@ -44,30 +51,34 @@ template <int FMT>
 constexpr int groups() { return FMT == MXB_FP4_NV ? 4 : 2; }  // scale tiles per stage and 128 rows
 template <int NT>
 constexpr int tok_blocks() { return (NT + 127) / 128; }
-template <int FMT, int NT>
-constexpr int stage_bytes() {
-  return kTileF + (NT < 8 ? 8 : NT) * BK / 2 + (1 + tok_blocks<NT>()) * groups<FMT>() * 512;
-}
 template <int NT>
-constexpr int stages() { return NT >= 256 ? 4 : NT >= 128 ? 5 : 6; }
+constexpr int stage_bytes() { return kTileF + NT * BK / 2; }
+template <int NT>
+constexpr int stages() { return NT >= 128 ? 3 : 4; }
 template <int NT>
 constexpr int acc_cols() { return NT < 32 ? 32 : NT; }
-// scale columns: per group 4 for the features, 4 per 128 tokens
+// scale tiles of a stage (features and tokens), their ring, and their two sets
+// of TMEM columns, four a tile
 template <int FMT, int NT>
-constexpr int sf_cols() { return groups<FMT>() * 4 * (1 + tok_blocks<NT>()); }
+constexpr int sf_tiles() { return groups<FMT>() * (1 + tok_blocks<NT>()); }
+constexpr int kSfRing = 3;
+template <int FMT, int NT>
+constexpr int sf_cols() { return 4 * sf_tiles<FMT, NT>(); }
 constexpr int pow2_cols(int c) { return c <= 64 ? 64 : c <= 128 ? 128 : c <= 256 ? 256 : 512; }
 template <int FMT, int NT>
-constexpr int tmem_cols() { return pow2_cols(acc_cols<NT>() + sf_cols<FMT, NT>()); }
+constexpr int tmem_cols() { return pow2_cols(acc_cols<NT>() + 2 * sf_cols<FMT, NT>()); }
 
 constexpr int kBarBytes = 256;
 template <int FMT, int NT>
 constexpr size_t smem_bytes() {
-  return 1024 + (size_t)stages<NT>() * stage_bytes<FMT, NT>() + kBarBytes;
+  return 1024 + (size_t)stages<NT>() * stage_bytes<NT>() + kSfRing * sf_tiles<FMT, NT>() * 512 +
+         kBarBytes;
 }
 
 struct Bars {
-  uint64_t full[6];
-  uint64_t empty[6];
+  uint64_t full[4];
+  uint64_t empty[4];
+  uint64_t sf_ready[2], sf_free[2];  // a stage's scales in TMEM
   uint64_t acc;
   uint32_t tmem_base;
 };
@@ -108,6 +119,15 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t saddr, uint32_t rank) {
   return v;
 }
 
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 template <typename OutT>
 __device__ __forceinline__ void store1(OutT* p, float v) {
   if constexpr (sizeof(OutT) == 2) *p = __float2bfloat16_rn(v);
@@ -115,22 +135,21 @@ __device__ __forceinline__ void store1(OutT* p, float v) {
 }
 
 template <int FMT, int NT, typename OutT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_f,
                     const __grid_constant__ CUtensorMap tmap_t, const Args a) {
   constexpr int S = stages<NT>(), G = groups<FMT>(), TB = tok_blocks<NT>();
   constexpr int kTileT = NT * BK / 2;
-  constexpr int kStage = stage_bytes<FMT, NT>();
   constexpr int kAcc = acc_cols<NT>(), kCols = tmem_cols<FMT, NT>();
+  constexpr int kSfTiles = sf_tiles<FMT, NT>(), kSfCols = sf_cols<FMT, NT>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  // [S feature tiles][S token tiles][S scale tiles][barriers]
+  // [S feature tiles][S token tiles][scale ring][barriers]
   uint8_t* sF = smem;
   uint8_t* sT = sF + S * kTileF;
   uint8_t* sS = sT + S * kTileT;
-  Bars* bars = reinterpret_cast<Bars*>(smem + S * kStage);
-  constexpr int kScaleStage = (1 + TB) * G * 512;
+  Bars* bars = reinterpret_cast<Bars*>(sS + kSfRing * kSfTiles * 512);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = a.splits > 1 ? (int)(blockIdx.x % a.splits) : 0;
@@ -144,6 +163,10 @@ __global__ void __launch_bounds__(kThreads)
     for (int s = 0; s < S; ++s) {
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->sf_ready[i], kSfWarps);
+      mbar_init(&bars->sf_free[i], 1);
     }
     mbar_init(&bars->acc, 1);
     fence_barrier_init();
@@ -165,59 +188,37 @@ __global__ void __launch_bounds__(kThreads)
 
   if (warp == 0) {
     if (lane == 0) {
-      const int frb = n0 >> 7, trb = m0 >> 7;
       for (int i = 0; i < nk; ++i) {
         const int s = i % S, round = i / S, ks = k_lo + i;
         if (round > 0 && !mbar_wait_to(&bars->empty[s], (round - 1) & 1, kErrTimeoutEmpty, a.err))
           break;
-        const int ng = min(G, a.kgroups - ks * G);              // scale tiles of this stage
-        const int tb = min(TB, a.tok_rblocks - trb);            // existing token scale blocks
-        mbar_expect_tx(&bars->full[s], kTileF + kTileT + (uint32_t)(1 + tb) * ng * 512);
+        mbar_expect_tx(&bars->full[s], kTileF + kTileT);
         tma_load_2d(sF + s * kTileF, &tmap_f, &bars->full[s], ks * (BK / 2), n0);
         tma_load_2d(sT + s * kTileT, &tmap_t, &bars->full[s], ks * (BK / 2), m0);
-        uint8_t* sc = sS + s * kScaleStage;
-        bulk_load_g2s(sc, a.fs + ((size_t)frb * a.kgroups + (size_t)ks * G) * 512, ng * 512,
-                      &bars->full[s]);
-        for (int b = 0; b < tb; ++b)
-          bulk_load_g2s(sc + (1 + b) * G * 512,
-                        a.ts + ((size_t)(trb + b) * a.kgroups + (size_t)ks * G) * 512, ng * 512,
-                        &bars->full[s]);
       }
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t sf0 = tbase + kAcc;
+      constexpr uint32_t i0 = make_idesc_fp4(FMT == MXB_FP4_MX, BM, NT, 0);
+      constexpr uint32_t i2 = make_idesc_fp4(FMT == MXB_FP4_MX, BM, NT, 2);
       bool ok = true;
       for (int i = 0; i < nk; ++i) {
         const int s = i % S, round = i / S, ks = k_lo + i;
-        if (!mbar_wait_to(&bars->full[s], round & 1, kErrTimeoutFull, a.err)) {
-          ok = false;
-          break;
-        }
+        const uint32_t sf0 = tbase + kAcc + (i & 1) * kSfCols;
+        ok = mbar_wait_to(&bars->sf_ready[i & 1], (i >> 1) & 1, kErrTimeoutTmemFull, a.err) &&
+             mbar_wait_to(&bars->full[s], round & 1, kErrTimeoutFull, a.err);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t sc = smem_u32(sS + s * kScaleStage);
         const uint32_t pf = smem_u32(sF + s * kTileF), pt = smem_u32(sT + s * kTileT);
         const int ng = min(G, a.kgroups - ks * G);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          if (g < ng) {
-            const uint32_t c = sf0 + g * 4 * (1 + TB);
-            tmem_cp_32x128(c, desc_rows16(sc + g * 512));
-#pragma unroll
-            for (int b = 0; b < TB; ++b)
-              tmem_cp_32x128(c + 4 * (1 + b), desc_rows16(sc + ((1 + b) * G + g) * 512));
-          }
-        }
         // K slices of 64 values = 32 bytes; those past the last scale tile
         // hold only padding
 #pragma unroll
         for (int kk = 0; kk < BK / 64; ++kk) {
           const int g = kk * G / 4;
           if (g < ng) {
-            const uint32_t c = sf0 + g * 4 * (1 + TB);
             // mxfp4: a tile of four scales serves two slices
-            constexpr uint32_t i0 = make_idesc_fp4(FMT == MXB_FP4_MX, BM, NT, 0);
-            constexpr uint32_t i2 = make_idesc_fp4(FMT == MXB_FP4_MX, BM, NT, 2);
+            const uint32_t c = sf0 + g * 4 * (1 + TB);
             mma_fp4<FMT == MXB_FP4_NV>(tbase, desc_kmajor_sw128(pf + kk * 32),
                                        desc_kmajor_sw128(pt + kk * 32),
                                        (FMT == MXB_FP4_MX && (kk & 1)) ? i2 : i0, c, c + 4,
@@ -225,15 +226,72 @@ __global__ void __launch_bounds__(kThreads)
           }
         }
         mma_commit(&bars->empty[s]);
+        mma_commit(&bars->sf_free[i & 1]);
       }
       if (ok) mma_commit(&bars->acc);
     }
+  } else if (warp >= 2 + kEpiWarps) {
+    // Scales: every warp fills the lane quarter of TMEM that it may write (each
+    // quarter holds all 32 rows of a scale column).
+    const int t = threadIdx.x - 32 * (2 + kEpiWarps);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int frb = n0 >> 7, trb = m0 >> 7;
+    constexpr int kChunks = kSfTiles * 32;  // 16-byte pieces of a stage
+    auto fetch = [&](int i) {  // stage i -> its slot; tile order [group][features, token blocks]
+      if (i < nk) {
+        const int ks = k_lo + i;
+        uint8_t* dst = sS + (i % kSfRing) * kSfTiles * 512;
+#pragma unroll
+        for (int x0 = 0; x0 < kChunks; x0 += 32 * kSfWarps) {
+          const int x = x0 + t, tile = x >> 5, g = tile / (1 + TB), b = tile % (1 + TB);
+          const int64_t rb = b == 0 ? frb : trb + b - 1;
+          if ((kChunks % (32 * kSfWarps) == 0 || x < kChunks) && ks * G + g < a.kgroups &&
+              (b == 0 || rb < a.tok_rblocks))
+            cp_async16(dst + x * 16, (b == 0 ? a.fs : a.ts) +
+                                         ((size_t)rb * a.kgroups + (size_t)ks * G + g) * 512 + (x & 31) * 16);
+        }
+      }
+      cp_async_commit();
+    };
+    bool ok = true;
+#pragma unroll
+    for (int i = 0; i < kSfRing - 1; ++i) fetch(i);
+    for (int i = 0; i < nk; ++i) {
+      cp_async_wait<kSfRing - 2>();
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kSfWarps) : "memory");
+      // all warps are past stage i - 1: its slot takes stage i + kSfRing - 1
+      fetch(i + kSfRing - 1);
+      // after a wait that gave up the loop runs on (the block barrier above
+      // needs every warp), without further waits
+      if (i >= 2)
+        ok = ok && mbar_wait_warp_to(&bars->sf_free[i & 1], ((i >> 1) - 1) & 1, kErrTimeoutTmemEmpty, a.err);
+      tc_fence_after();
+      const uint8_t* src = sS + (i % kSfRing) * kSfTiles * 512 + lane * 16;
+      const uint32_t dst = tbase + kAcc + (i & 1) * kSfCols + lanes;
+#pragma unroll
+      for (int x = 0; x < kSfTiles; x += 4) {  // four tiles = 16 columns a store
+        uint32_t r[16];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint4 v = *reinterpret_cast<const uint4*>(src + (x + k) * 512);
+          r[4 * k] = v.x;
+          r[4 * k + 1] = v.y;
+          r[4 * k + 2] = v.z;
+          r[4 * k + 3] = v.w;
+        }
+        tmem_st16(dst + x * 4, r);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->sf_ready[i & 1]);
+    }
+    cp_async_wait<0>();
   }
-
   __syncwarp();  // warps 0 and 1 ran on one lane
 
   // ── epilogue ──
-  const bool epi = warp >= 2;
+  const bool epi = warp >= 2 && warp < 2 + kEpiWarps;
   const int q = warp & 3, half = (warp - 2) >> 2;  // TMEM lane quarter, column half
   constexpr int kPer = NT >= 64 ? 32 : NT / 2;     // columns per tcgen05.ld
   float factor = 1.0f;
@@ -337,29 +395,30 @@ int launch(const CUtensorMap& tf, const CUtensorMap& tt, const Args& a, cudaStre
 
 template <int FMT, typename OutT>
 int dispatch(const void* fcodes, const void* tcodes, Args& a, cudaStream_t st) {
-  // Tokens per tile: the smallest that holds them all, so a step of few
-  // tokens pays an MMA of that width; from 129 tokens on 256 where that still
-  // fills the SMs, else 128.
   const int64_t ft = cdiv(a.N, BM);
-  int nt = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
-  if (a.M > 128 && ft * cdiv(a.M, 256) >= kSMs) nt = 256;
-  // K splits: while the tiles leave half of the SMs idle, at least two stages each
-  const int64_t tiles = ft * cdiv(a.M, nt);
-  int splits = 1;
-  while (splits < kMaxSplit && tiles * splits * 2 <= kSMs && a.ksteps >= splits * 4) splits *= 2;
-  a.splits = splits;
   CUtensorMap tf, tt;
-  if (!encode_tmap_2d(&tf, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, fcodes, (uint64_t)a.kbytes,
-                      (uint64_t)a.N, BK / 2, BM, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !encode_tmap_2d(&tt, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, tcodes, (uint64_t)a.kbytes,
-                      (uint64_t)a.M, BK / 2, nt, CU_TENSOR_MAP_SWIZZLE_128B))
-    return MXB_E_CUDA;
+  auto maps = [&](int rows_f, int rows_t) {
+    return encode_tmap_2d(&tf, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, fcodes, (uint64_t)a.kbytes,
+                          (uint64_t)a.N, BK / 2, rows_f, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           encode_tmap_2d(&tt, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, tcodes, (uint64_t)a.kbytes,
+                          (uint64_t)a.M, BK / 2, rows_t, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  // Tokens per tile: the smallest that holds them all, so a step of few
+  // tokens pays an MMA of that width
+  const int nt = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+  // K splits while they fill the SMs (two CTAs each for narrow tiles; a wide
+  // tile's partial sums cost more than the second CTA saves: 128 x 4096 x 4096
+  // 8.1 us with 4 splits, 11.3 with 8), at least two stages each
+  const int64_t tiles = ft * cdiv(a.M, nt);
+  int64_t splits = (nt >= 128 ? kSMs : 2 * kSMs) / tiles;
+  if (splits > a.ksteps / 2) splits = a.ksteps / 2;
+  a.splits = (int)(splits < 1 ? 1 : splits > kMaxSplit ? kMaxSplit : splits);
+  if (!maps(BM, nt)) return MXB_E_CUDA;
   switch (nt) {
     case 16: return launch<FMT, 16, OutT>(tf, tt, a, st);
     case 32: return launch<FMT, 32, OutT>(tf, tt, a, st);
     case 64: return launch<FMT, 64, OutT>(tf, tt, a, st);
-    case 128: return launch<FMT, 128, OutT>(tf, tt, a, st);
-    default: return launch<FMT, 256, OutT>(tf, tt, a, st);
+    default: return launch<FMT, 128, OutT>(tf, tt, a, st);
   }
 }
 
