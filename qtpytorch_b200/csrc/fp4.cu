@@ -77,24 +77,33 @@ __device__ __forceinline__ float block_max(float a) {
   return a;
 }
 
-// Up to 16 elements of a row from column c0 on; zero past K.
+// 32 bytes: a whole sector a lane, so that a warp's lanes, 16 elements apart,
+// use all that they touch.
+__device__ __forceinline__ void ld32b(const void* p, uint32_t (&r)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+                 "=r"(r[7])
+               : "l"(p));
+}
+
+// Up to 16 elements of a row from column c0 on; zero past K.  vec: rows are
+// 32-byte aligned.
 template <typename InT>
 __device__ __forceinline__ void load16(const InT* __restrict__ row, int64_t c0, int64_t K, bool vec,
                                        float (&v)[kE]) {
   if (vec && c0 + kE <= K) {
-    if (sizeof(InT) == 4) {
-      const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + c0);
-      float4 t[4];
+    if constexpr (sizeof(InT) == 4) {
+      uint32_t a[8], b[8];
+      ld32b(row + c0, a);
+      ld32b(row + c0 + 8, b);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) t[i] = __ldg(p + i);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[4 * i] = t[i].x; v[4 * i + 1] = t[i].y; v[4 * i + 2] = t[i].z; v[4 * i + 3] = t[i].w;
+      for (int i = 0; i < 8; ++i) {
+        v[i] = __uint_as_float(a[i]);
+        v[8 + i] = __uint_as_float(b[i]);
       }
     } else {
-      const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(row) + c0);
-      const uint4 a = __ldg(p), b = __ldg(p + 1);
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      uint32_t w[8];
+      ld32b(row + c0, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         v[2 * i] = __uint_as_float(w[i] << 16);
@@ -110,7 +119,7 @@ __device__ __forceinline__ void load16(const InT* __restrict__ row, int64_t c0, 
 // Largest |x| of each block's share of the tensor (NaN kept) -> part[block].
 // The quantize kernel reduces the at most kAmaxBlocks values, so there is no
 // atomic and nothing to clear.
-constexpr int kAmaxBlocks = 4 * kSMs;
+constexpr int kAmaxBlocks = 6 * kSMs;
 template <typename InT>
 __global__ void __launch_bounds__(kThreads) fp4_amax_kernel(const InT* __restrict__ x, int64_t K,
                                                             int64_t ldx, uint32_t gpr,
@@ -119,13 +128,17 @@ __global__ void __launch_bounds__(kThreads) fp4_amax_kernel(const InT* __restric
   pdl_trigger();
   pdl_wait();
   float a = 0.0f;
-  for (uint64_t i = blockIdx.x * (uint64_t)kThreads + threadIdx.x; i < items;
-       i += (uint64_t)gridDim.x * kThreads) {
-    const uint32_t r = (uint32_t)i / gpr, c = (uint32_t)i - r * gpr;
-    float v[kE];
-    load16(x + (int64_t)r * ldx, (int64_t)c * kE, K, vec, v);
+  const uint64_t step = (uint64_t)gridDim.x * kThreads;
+  for (uint64_t i = blockIdx.x * (uint64_t)kThreads + threadIdx.x; i < items; i += 2 * step) {
+    float v[2][kE];
 #pragma unroll
-    for (int j = 0; j < kE; ++j) a = amax_step(a, v[j]);
+    for (int h = 0; h < 2; ++h) {  // two in flight
+      const uint64_t j = i + h * step < items ? i + h * step : i;
+      const uint32_t r = (uint32_t)j / gpr, c = (uint32_t)j - r * gpr;
+      load16(x + (int64_t)r * ldx, (int64_t)c * kE, K, vec, v[h]);
+    }
+#pragma unroll
+    for (int j = 0; j < kE; ++j) a = nan_max(a, nan_max(fabsf(v[0][j]), fabsf(v[1][j])));
   }
   a = block_max(a);
   if (threadIdx.x == 0) part[blockIdx.x] = a;
@@ -143,79 +156,83 @@ __global__ void __launch_bounds__(kThreads)
                      uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   pdl_trigger();
   pdl_wait();
-  const uint32_t blk = part ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-  const uint64_t i = blk * (uint64_t)kThreads + threadIdx.x;
-  const bool mine = i < items;
-  if (!mine && i - items < pad_words) {
-    const uint32_t w = (uint32_t)(i - items);
-    const uint32_t r = rows + w / groups;
-    *reinterpret_cast<uint32_t*>(scales + sf_offset(r, w % groups, groups)) = 0u;
-  }
   float g = 1.0f;
   if (FMT == MXB_FP4_NV) {
     if (part) {
       float a = 0.0f;
       for (int p = threadIdx.x; p < parts; p += kThreads) a = nan_max(a, part[p]);
       g = factor_of(block_max(a));
-      if (i == 0) *gscale = g;
+      if (blockIdx.x == 0 && threadIdx.x == 0) *gscale = g;
     } else {
       g = *gscale;
     }
   }
-  const uint32_t r = mine ? (uint32_t)i / gpr : 0u, c = mine ? (uint32_t)i - r * gpr : 0u;
-  float v[kE];
-  if (mine) {
-    load16(x + (int64_t)r * ldx, (int64_t)c * kE, K, vec, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kE; ++j) v[j] = 0.0f;
-  }
-  float a = 0.0f;
-#pragma unroll
-  for (int j = 0; j < kE; ++j) a = amax_step(a, v[j]);
-  if (FMT == MXB_FP4_MX) a = nan_max(a, __shfl_xor_sync(0xffffffffu, a, 1));
-  const bool finite = a <= 3.4028235e38f;
-  uint32_t sb;
-  float q[kE];
-  if (FMT == MXB_FP4_MX) {
-    // floor(log2(a)) is the exponent field; subnormals fall under the clamp
-    sb = (uint32_t)max((int)(__float_as_uint(a) >> 23) - 2, 0);
-    const float inv = __uint_as_float((254u - sb) << 23);  // exact: a power of two
-#pragma unroll
-    for (int j = 0; j < kE; ++j) q[j] = __fmul_rn(v[j], inv);
-    if (!finite) sb = 255u;
-  } else {
-    sb = e4m3_of(fminf(__fdiv_rn(a, __fmul_rn(6.0f, g)), 448.0f));
-    const float s = __fmul_rn(e4m3_value(sb), g);
-    if (s >= 7.9e-31f && s <= 1.2e30f) {
-      // x / s by Markstein's corrected product (r correctly rounded, the
-      // residual exact in an FMA): three operations instead of a division
-      const float rs = __frcp_rn(s);
-#pragma unroll
-      for (int j = 0; j < kE; ++j) {
-        const float q0 = __fmul_rn(v[j], rs);
-        q[j] = __fmaf_rn(__fmaf_rn(-q0, s, v[j]), rs, q0);
-      }
+  const int64_t rb = fp4_row_bytes(K);
+  const uint32_t blocks = (uint32_t)(((uint64_t)items + pad_words + kThreads - 1) / kThreads);
+  for (uint32_t blk0 = blockIdx.x; blk0 < blocks; blk0 += gridDim.x) {
+    const uint32_t blk = part ? blocks - 1 - blk0 : blk0;
+    const uint64_t i = blk * (uint64_t)kThreads + threadIdx.x;
+    const bool mine = i < items;
+    if (!mine && i - items < pad_words) {
+      const uint32_t w = (uint32_t)(i - items);
+      const uint32_t r = rows + w / groups;
+      *reinterpret_cast<uint32_t*>(scales + sf_offset(r, w % groups, groups)) = 0u;
+    }
+    const uint32_t r = mine ? (uint32_t)i / gpr : 0u, c = mine ? (uint32_t)i - r * gpr : 0u;
+    float v[kE];
+    if (mine) {
+      load16(x + (int64_t)r * ldx, (int64_t)c * kE, K, vec, v);
     } else {
 #pragma unroll
-      for (int j = 0; j < kE; ++j) q[j] = s > 0.0f ? __fdiv_rn(v[j], s) : __fmul_rn(v[j], 0.0f);
+      for (int j = 0; j < kE; ++j) v[j] = 0.0f;
     }
-    if (!finite) sb = 0x7Fu;
+    float a = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kE; ++j) a = amax_step(a, v[j]);
+    if (FMT == MXB_FP4_MX) a = nan_max(a, __shfl_xor_sync(0xffffffffu, a, 1));
+    const bool finite = a <= 3.4028235e38f;
+    uint32_t sb;
+    float q[kE];
+    if (FMT == MXB_FP4_MX) {
+      // floor(log2(a)) is the exponent field; subnormals fall under the clamp
+      sb = (uint32_t)max((int)(__float_as_uint(a) >> 23) - 2, 0);
+      const float inv = __uint_as_float((254u - sb) << 23);  // exact: a power of two
+#pragma unroll
+      for (int j = 0; j < kE; ++j) q[j] = __fmul_rn(v[j], inv);
+      if (!finite) sb = 255u;
+    } else {
+      sb = e4m3_of(fminf(__fdiv_rn(a, __fmul_rn(6.0f, g)), 448.0f));
+      const float s = __fmul_rn(e4m3_value(sb), g);
+      if (s >= 7.9e-31f && s <= 1.2e30f) {
+        // x / s by Markstein's corrected product (r correctly rounded, the
+        // residual exact in an FMA): three operations instead of a division
+        const float rs = __frcp_rn(s);
+#pragma unroll
+        for (int j = 0; j < kE; ++j) {
+          const float q0 = __fmul_rn(v[j], rs);
+          q[j] = __fmaf_rn(__fmaf_rn(-q0, s, v[j]), rs, q0);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kE; ++j) q[j] = s > 0.0f ? __fdiv_rn(v[j], s) : __fmul_rn(v[j], 0.0f);
+      }
+      if (!finite) sb = 0x7Fu;
+    }
+    uint2 w = make_uint2(e2m1x8(q), e2m1x8(q + 8));
+    if (!finite) w = make_uint2(0u, 0u);
+    if (mine && (int64_t)c * 8 < rb)
+      *reinterpret_cast<uint2*>(codes + (size_t)r * rb + (size_t)c * 8) = w;
+    // four scales -> one word.  A group of four blocks starts at a multiple of
+    // 8 (mxfp4) or 4 (nvfp4) items, and gpr is a multiple of that, so its lanes
+    // sit in one warp and one row.
+    constexpr int L = FMT == MXB_FP4_MX ? 2 : 1;
+    if ((int64_t)c * kE >= K) sb = 0u;  // blocks past the row
+    uint32_t word = sb;
+    word |= __shfl_down_sync(0xffffffffu, word, L) << 8;
+    word |= __shfl_down_sync(0xffffffffu, word, 2 * L) << 16;
+    if (mine && (c & (4 * L - 1)) == 0)
+      *reinterpret_cast<uint32_t*>(scales + sf_offset(r, c / (4 * L), groups)) = word;
   }
-  uint2 w = make_uint2(e2m1x8(q), e2m1x8(q + 8));
-  if (!finite) w = make_uint2(0u, 0u);
-  if (mine && (int64_t)c * 8 < fp4_row_bytes(K))
-    *reinterpret_cast<uint2*>(codes + (size_t)r * fp4_row_bytes(K) + (size_t)c * 8) = w;
-  // four scales -> one word.  A group of four blocks starts at a multiple of
-  // 8 (mxfp4) or 4 (nvfp4) items, and gpr is a multiple of that, so its lanes
-  // sit in one warp and one row.
-  constexpr int L = FMT == MXB_FP4_MX ? 2 : 1;
-  if ((int64_t)c * kE >= K) sb = 0u;  // blocks past the row
-  uint32_t word = sb;
-  word |= __shfl_down_sync(0xffffffffu, word, L) << 8;
-  word |= __shfl_down_sync(0xffffffffu, word, 2 * L) << 16;
-  if (mine && (c & (4 * L - 1)) == 0)
-    *reinterpret_cast<uint32_t*>(scales + sf_offset(r, c / (4 * L), groups)) = word;
 }
 
 // Two E2M1 codes (one byte) -> two floats.
@@ -306,7 +323,7 @@ int quantize_t(const InT* x, int64_t rows, int64_t K, int64_t ldx, int fmt, floa
   const int64_t gpr = groups * (fmt == MXB_FP4_NV ? 4 : 8);
   const int64_t items = rows * gpr, pad = (cdiv(rows, 128) * 128 - rows) * groups;
   if (items + pad >= (int64_t)1 << 32) return MXB_E_SHAPE;
-  const bool vec = ((uintptr_t)x % 16) == 0 && (ldx * (int64_t)sizeof(InT)) % 16 == 0;
+  const bool vec = ((uintptr_t)x % 32) == 0 && (ldx * (int64_t)sizeof(InT)) % 32 == 0;
   int parts = 0;
   if (derive) {
     const int64_t agpr = cdiv(K, kE), aitems = rows * agpr;
@@ -317,7 +334,11 @@ int quantize_t(const InT* x, int64_t rows, int64_t K, int64_t ldx, int fmt, floa
     MXB_LAUNCH_CHECK();
   }
   auto kern = fmt == MXB_FP4_NV ? fp4_quant_kernel<InT, MXB_FP4_NV> : fp4_quant_kernel<InT, MXB_FP4_MX>;
-  MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)cdiv(items + pad, kThreads)), kThreads, 0, st, x,
+  // with a factor to find every block first reduces the maxima, so there are
+  // only as many blocks as fit
+  int64_t blocks = cdiv(items + pad, kThreads);
+  if (derive && blocks > 6 * kSMs) blocks = 6 * kSMs;
+  MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)blocks), kThreads, 0, st, x,
                           (uint32_t)rows, K, ldx, (uint32_t)gpr, (uint32_t)items, (uint32_t)pad,
                           (uint32_t)groups, vec, derive ? part : nullptr, parts, g, codes, scales));
   MXB_LAUNCH_CHECK();

@@ -45,46 +45,11 @@ __device__ __forceinline__ void load8v(const __nv_bfloat16* p, bool vec, float (
   }
 }
 
-// blockIdx.y: 0 the keys, 1 the values
-template <typename InT, int BITS, int D>
-__global__ void __launch_bounds__(kThreads)
-    kv_write_kernel(const InT* __restrict__ k, const InT* __restrict__ v, int64_t T, int H,
-                    int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs, bool vec,
-                    const int64_t* __restrict__ slots, int64_t n_slots, int page_shift,
-                    uint8_t* __restrict__ kc, float* __restrict__ ks, uint8_t* __restrict__ vc,
-                    float* __restrict__ vs, int* __restrict__ err) {
-  constexpr int L = D / 8;
+// One head row's eight values of this lane -> codes and scale in the slot.
+template <int BITS, int D>
+__device__ __forceinline__ void put_row(const float (&x)[8], float a, int64_t r, int part,
+                                        uint8_t* __restrict__ codes, float* __restrict__ scales) {
   constexpr float m = BITS == 8 ? 127.0f : 7.0f;
-  pdl_trigger();
-  pdl_wait();
-  const bool val = blockIdx.y != 0;
-  // 32-bit index: T * H < 2^32 (checked at the launch)
-  const uint32_t row = blockIdx.x * (uint32_t)(kThreads / L) + threadIdx.x / L;
-  const int part = threadIdx.x % L;
-  const bool live = row < (uint32_t)(T * H);
-  const uint32_t t32 = live ? row / (uint32_t)H : 0u;
-  const int64_t t = t32;
-  const int h = live ? (int)(row - t32 * (uint32_t)H) : 0;
-  float x[8];
-  int64_t slot = -1;
-  if (live) {
-    slot = slots[t];
-    const InT* src = val ? v + t * v_ts + h * v_hs : k + t * k_ts + h * k_hs;
-    load8v(src + part * 8, vec, x);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.0f;
-  }
-  float a = 0.0f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) a = amax_step(a, x[j]);
-#pragma unroll
-  for (int o = L >> 1; o > 0; o >>= 1) a = nan_max(a, __shfl_xor_sync(0xffffffffu, a, o));
-  if (slot < 0) return;  // padding token
-  if (slot >= n_slots) {
-    if (part == 0 && err) atomicCAS(err, 0, kErrIndexCode);
-    return;
-  }
   // the integer quantizer's order of roundings (quantize.cu block_factor)
   const float si = __fmul_rn(__frcp_rn(nan_max(a, 1e-12f)), m);
   uint32_t c[8];
@@ -95,9 +60,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int j = 0; j < 8; ++j) c[j] = 0u;
   }
-  const int64_t pg = slot >> page_shift;
-  const int64_t r = ((pg * H + h) << page_shift) + (slot & ((1 << page_shift) - 1));
-  uint8_t* dst = (val ? vc : kc) + r * (D * BITS / 8) + part * BITS;
+  uint8_t* dst = codes + r * (D * BITS / 8) + part * BITS;
   if (BITS == 8) {
     *reinterpret_cast<uint2*>(dst) = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24,
                                                 c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
@@ -107,7 +70,58 @@ __global__ void __launch_bounds__(kThreads)
     for (int j = 0; j < 8; ++j) w |= c[j] << (4 * j);
     *reinterpret_cast<uint32_t*>(dst) = w;
   }
-  if (part == 0) (val ? vs : ks)[r] = __frcp_rn(si);
+  if (part == 0) scales[r] = __frcp_rn(si);
+}
+
+// A lane takes its eight values of a key and of the value beside it: two loads
+// in flight, and the slot's address once for both.
+template <typename InT, int BITS, int D>
+__global__ void __launch_bounds__(kThreads)
+    kv_write_kernel(const InT* __restrict__ k, const InT* __restrict__ v, int64_t T, int H,
+                    int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs, bool vec,
+                    const int64_t* __restrict__ slots, int64_t n_slots, int page_shift,
+                    uint8_t* __restrict__ kc, float* __restrict__ ks, uint8_t* __restrict__ vc,
+                    float* __restrict__ vs, int* __restrict__ err) {
+  constexpr int L = D / 8;
+  pdl_trigger();
+  pdl_wait();
+  // 32-bit index: T * H < 2^31 (checked at the launch)
+  const uint32_t row = blockIdx.x * (uint32_t)(kThreads / L) + threadIdx.x / L;
+  const int part = threadIdx.x % L;
+  const bool live = row < (uint32_t)(T * H);
+  const uint32_t t32 = live ? row / (uint32_t)H : 0u;
+  const int64_t t = t32;
+  const int h = live ? (int)(row - t32 * (uint32_t)H) : 0;
+  float x[8], y[8];
+  int64_t slot = -1;
+  if (live) {
+    slot = slots[t];
+    load8v(k + t * k_ts + h * k_hs + part * 8, vec, x);
+    load8v(v + t * v_ts + h * v_hs + part * 8, vec, y);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = y[j] = 0.0f;
+  }
+  float a = 0.0f, b = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    a = amax_step(a, x[j]);
+    b = amax_step(b, y[j]);
+  }
+#pragma unroll
+  for (int o = L >> 1; o > 0; o >>= 1) {
+    a = nan_max(a, __shfl_xor_sync(0xffffffffu, a, o));
+    b = nan_max(b, __shfl_xor_sync(0xffffffffu, b, o));
+  }
+  if (slot < 0) return;  // padding token
+  if (slot >= n_slots) {
+    if (part == 0 && err) atomicCAS(err, 0, kErrIndexCode);
+    return;
+  }
+  const int64_t pg = slot >> page_shift;
+  const int64_t r = ((pg * H + h) << page_shift) + (slot & ((1 << page_shift) - 1));
+  put_row<BITS, D>(x, a, r, part, kc, ks);
+  put_row<BITS, D>(y, b, r, part, vc, vs);
 }
 
 // blockIdx.y: sequence, blockIdx.z: 0 the keys, 1 the values.  A thread makes
@@ -201,7 +215,7 @@ int write_t(const void* k, const void* v, const WriteArgs& a, cudaStream_t st) {
   const int64_t per = 16 / sizeof(InT);
   const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && a.k_ts % per == 0 &&
                    a.k_hs % per == 0 && a.v_ts % per == 0 && a.v_hs % per == 0;
-  MXB_CUDA_TRY(launch_pdl(kv_write_kernel<InT, BITS, D>, dim3((unsigned)blocks, 2), kThreads, 0, st,
+  MXB_CUDA_TRY(launch_pdl(kv_write_kernel<InT, BITS, D>, dim3((unsigned)blocks), kThreads, 0, st,
                           static_cast<const InT*>(k), static_cast<const InT*>(v), a.T, a.H, a.k_ts,
                           a.k_hs, a.v_ts, a.v_hs, vec, a.slots, a.n_slots, shift_of(a.page), a.kc,
                           a.ks, a.vc, a.vs, device_error_ptr()));
