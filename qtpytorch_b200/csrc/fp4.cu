@@ -169,9 +169,23 @@ __global__ void __launch_bounds__(kThreads)
   }
   const int64_t rb = fp4_row_bytes(K);
   const uint32_t blocks = (uint32_t)(((uint64_t)items + pad_words + kThreads - 1) / kThreads);
+  auto item_of = [&](uint32_t blk0) -> uint64_t {
+    return (part ? blocks - 1 - blk0 : blk0) * (uint64_t)kThreads + threadIdx.x;
+  };
+  float next[kE];
+  auto fetch = [&](uint32_t blk0) {  // the values of a later item
+    const uint64_t i = blk0 < blocks ? item_of(blk0) : items;
+    if (i < items) {
+      const uint32_t r = (uint32_t)i / gpr, c = (uint32_t)i - r * gpr;
+      load16(x + (int64_t)r * ldx, (int64_t)c * kE, K, vec, next);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kE; ++j) next[j] = 0.0f;
+    }
+  };
+  fetch(blockIdx.x);
   for (uint32_t blk0 = blockIdx.x; blk0 < blocks; blk0 += gridDim.x) {
-    const uint32_t blk = part ? blocks - 1 - blk0 : blk0;
-    const uint64_t i = blk * (uint64_t)kThreads + threadIdx.x;
+    const uint64_t i = item_of(blk0);
     const bool mine = i < items;
     if (!mine && i - items < pad_words) {
       const uint32_t w = (uint32_t)(i - items);
@@ -180,12 +194,9 @@ __global__ void __launch_bounds__(kThreads)
     }
     const uint32_t r = mine ? (uint32_t)i / gpr : 0u, c = mine ? (uint32_t)i - r * gpr : 0u;
     float v[kE];
-    if (mine) {
-      load16(x + (int64_t)r * ldx, (int64_t)c * kE, K, vec, v);
-    } else {
 #pragma unroll
-      for (int j = 0; j < kE; ++j) v[j] = 0.0f;
-    }
+    for (int j = 0; j < kE; ++j) v[j] = next[j];
+    fetch(blk0 + gridDim.x);
     float a = 0.0f;
 #pragma unroll
     for (int j = 0; j < kE; ++j) a = amax_step(a, v[j]);
@@ -244,31 +255,37 @@ __device__ __forceinline__ float2 e2m1x2_value(uint32_t byte) {
   return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
 
-// A thread writes 16 bytes of output (4 fp32 or 8 bf16), so a warp's stores
-// are whole 512-byte runs; kU of them in flight.
+__device__ __forceinline__ void st32b(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// A thread makes 16 values of one scale (8 bytes of codes) and writes them in
+// whole sectors; kU of them in flight.  vec: rows of out are 32-byte aligned.
 template <typename OutT, int FMT>
 __global__ void __launch_bounds__(kThreads)
     fp4_dequant_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                       const float* __restrict__ gscale, uint32_t rows, int64_t K, uint32_t cpr,
-                       uint32_t items, uint32_t groups, bool vec, OutT* __restrict__ out) {
-  constexpr int E = 16 / sizeof(OutT), kU = 4;
-  constexpr int kBlk = FMT == MXB_FP4_NV ? 16 : 32;
+                       const float* __restrict__ gscale, int64_t K, uint32_t cpr, uint32_t items,
+                       uint32_t groups, bool vec, OutT* __restrict__ out) {
+  constexpr int kU = 2;
+  constexpr int kPerBlk = FMT == MXB_FP4_NV ? 1 : 2;  // items per scale
   pdl_trigger();
   pdl_wait();
   const float g = FMT == MXB_FP4_NV ? *gscale : 1.0f;
   const int64_t rb = fp4_row_bytes(K);
   const uint64_t i0 = blockIdx.x * (uint64_t)(kThreads * kU) + threadIdx.x;  // may pass 32 bits
-  uint32_t w[kU], sb[kU], rr[kU], cc[kU];
+  uint2 w[kU];
+  uint32_t sb[kU], rr[kU], cc[kU];
 #pragma unroll
   for (int u = 0; u < kU; ++u) {
     const uint64_t i = i0 + (uint64_t)u * kThreads;
-    w[u] = sb[u] = rr[u] = cc[u] = 0u;
+    w[u] = make_uint2(0u, 0u);
+    sb[u] = rr[u] = cc[u] = 0u;
     if (i < items) {
       const uint32_t r = (uint32_t)i / cpr, c = (uint32_t)i - r * cpr;
-      const uint8_t* p = codes + (size_t)r * rb + (size_t)c * (E / 2);
-      w[u] = E == 8 ? __ldg(reinterpret_cast<const uint32_t*>(p))
-                    : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p));
-      const uint32_t blk = (c * E) / kBlk;
+      w[u] = __ldg(reinterpret_cast<const uint2*>(codes + (size_t)r * rb + (size_t)c * 8));
+      const uint32_t blk = c / kPerBlk;
       sb[u] = __ldg(scales + sf_offset(r, blk >> 2, groups) + (blk & 3));
       rr[u] = r;
       cc[u] = c;
@@ -276,41 +293,40 @@ __global__ void __launch_bounds__(kThreads)
   }
 #pragma unroll
   for (int u = 0; u < kU; ++u) {
-    const uint64_t i = i0 + (uint64_t)u * kThreads;
-    if (i >= items) continue;
+    if (i0 + (uint64_t)u * kThreads >= items) continue;
     const float s = FMT == MXB_FP4_NV ? __fmul_rn(e4m3_value(sb[u]), g) : e8m0_value(sb[u]);
-    float v[E];
+    float v[kE];
 #pragma unroll
-    for (int j = 0; j < E / 2; ++j) {
-      const float2 t = e2m1x2_value((w[u] >> (8 * j)) & 0xFFu);
+    for (int j = 0; j < kE / 2; ++j) {
+      const float2 t = e2m1x2_value(((j < 4 ? w[u].x : w[u].y) >> (8 * (j & 3))) & 0xFFu);
       v[2 * j] = __fmul_rn(t.x, s);
       v[2 * j + 1] = __fmul_rn(t.y, s);
     }
-    const int64_t c0 = (int64_t)cc[u] * E;
+    const int64_t c0 = (int64_t)cc[u] * kE;
     OutT* o = out + (int64_t)rr[u] * K + c0;
-    if (sizeof(OutT) == 4) {
-      float* of = reinterpret_cast<float*>(o);
-      if (vec) {
-        __stcs(reinterpret_cast<float4*>(of), make_float4(v[0], v[1], v[2], v[3]));
+    if (vec && c0 + kE <= K) {
+      uint32_t p[8];
+      if constexpr (sizeof(OutT) == 4) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[j] = __float_as_uint(v[8 * h + j]);
+          st32b(o + 8 * h, p);
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (c0 + j < K) of[j] = v[j];
+        for (int j = 0; j < 8; ++j) {
+          const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          p[j] = *reinterpret_cast<const uint32_t*>(&t);
+        }
+        st32b(o, p);
       }
     } else {
-      __nv_bfloat16* ob = reinterpret_cast<__nv_bfloat16*>(o);
-      if (vec) {
-        uint32_t p[E / 2];
 #pragma unroll
-        for (int j = 0; j < E / 2; ++j) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-          p[j] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        __stcs(reinterpret_cast<uint4*>(ob), make_uint4(p[0], p[1], p[2 % (E / 2)], p[3 % (E / 2)]));
-      } else {
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (c0 + j < K) ob[j] = __float2bfloat16_rn(v[j]);
+      for (int j = 0; j < kE; ++j) {
+        if (c0 + j >= K) break;
+        if constexpr (sizeof(OutT) == 4) o[j] = v[j];
+        else o[j] = __float2bfloat16_rn(v[j]);
       }
     }
   }
@@ -337,7 +353,7 @@ int quantize_t(const InT* x, int64_t rows, int64_t K, int64_t ldx, int fmt, floa
   // with a factor to find every block first reduces the maxima, so there are
   // only as many blocks as fit
   int64_t blocks = cdiv(items + pad, kThreads);
-  if (derive && blocks > 6 * kSMs) blocks = 6 * kSMs;
+  if (derive && blocks > 4 * kSMs) blocks = 4 * kSMs;
   MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)blocks), kThreads, 0, st, x,
                           (uint32_t)rows, K, ldx, (uint32_t)gpr, (uint32_t)items, (uint32_t)pad,
                           (uint32_t)groups, vec, derive ? part : nullptr, parts, g, codes, scales));
@@ -348,16 +364,15 @@ int quantize_t(const InT* x, int64_t rows, int64_t K, int64_t ldx, int fmt, floa
 template <typename OutT>
 int dequantize_t(const uint8_t* codes, const uint8_t* scales, const float* g, int64_t rows,
                  int64_t K, int fmt, OutT* out, cudaStream_t st) {
-  constexpr int E = 16 / sizeof(OutT);
-  const int64_t cpr = cdiv(K, E), items = rows * cpr;
+  const int64_t cpr = cdiv(K, kE), items = rows * cpr;
   const int64_t groups = cdiv(fp4_blocks(K, fmt), 4);
-  const int64_t grid = cdiv(items, 4 * kThreads);
+  const int64_t grid = cdiv(items, 2 * kThreads);
   if (items >= (int64_t)1 << 32) return MXB_E_SHAPE;
-  const bool vec = K % E == 0 && ((uintptr_t)out % 16) == 0;
+  const bool vec = ((uintptr_t)out % 32) == 0 && (K * (int64_t)sizeof(OutT)) % 32 == 0;
   auto kern = fmt == MXB_FP4_NV ? fp4_dequant_kernel<OutT, MXB_FP4_NV>
                                 : fp4_dequant_kernel<OutT, MXB_FP4_MX>;
-  MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)grid), kThreads, 0, st, codes, scales, g, (uint32_t)rows,
-                          K, (uint32_t)cpr, (uint32_t)items, (uint32_t)groups, vec, out));
+  MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)grid), kThreads, 0, st, codes, scales, g, K,
+                          (uint32_t)cpr, (uint32_t)items, (uint32_t)groups, vec, out));
   MXB_LAUNCH_CHECK();
   return MXB_OK;
 }
