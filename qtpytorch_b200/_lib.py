@@ -7,6 +7,7 @@ is missing or a call fails, an exception says why.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 import threading
 
@@ -132,15 +133,27 @@ def stream_of(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_fns: dict = {}
+
+
 def call(name: str, dev: torch.device, *args) -> int:
     """Status of the entry point ``name`` on ``dev``'s current stream (its last
     argument).  The device guard and the stream object cost more than a short
     launch, so the guard is taken only where another device is current."""
-    fn = getattr(_lib or load(), name)
-    if torch._C._cuda_getDevice() == dev.index:
-        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(load(), name)
+    i = dev.index
+    if torch._C._cuda_getDevice() == i:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(i))
     with torch.cuda.device(dev):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        return fn(*args, torch._C._cuda_getCurrentRawStream(i))
+
+
+@functools.lru_cache(maxsize=4096)
+def size(name: str, *args) -> int:
+    """A byte count of the library, a function of its arguments alone."""
+    return getattr(load(), name)(*args)
 
 
 def require_cuda(t: torch.Tensor, what: str) -> None:

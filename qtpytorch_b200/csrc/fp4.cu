@@ -144,9 +144,49 @@ __global__ void __launch_bounds__(kThreads) fp4_amax_kernel(const InT* __restric
   if (threadIdx.x == 0) part[blockIdx.x] = a;
 }
 
+// Largest |x| of a small tensor, found by every cluster of kSmallCluster blocks
+// for itself: a launch less than with fp4_amax_kernel, which costs a call of
+// this size more than the extra reads from L2.
+constexpr int kSmallCluster = 8;
+constexpr int64_t kSmallItems = (int64_t)kSmallCluster * kThreads * 8;
+template <typename InT>
+__device__ __forceinline__ float cluster_amax(const InT* __restrict__ x, uint32_t rows, int64_t K,
+                                              int64_t ldx, bool vec) {
+  __shared__ float mine;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const uint32_t gpr = (uint32_t)((K + kE - 1) / kE), items = rows * gpr;
+  float a = 0.0f;
+  for (uint32_t i = rank * kThreads + threadIdx.x; i < items; i += kSmallCluster * kThreads) {
+    const uint32_t r = i / gpr, c = i - r * gpr;
+    float v[kE];
+    load16(x + (int64_t)r * ldx, (int64_t)c * kE, K, vec, v);
+#pragma unroll
+    for (int j = 0; j < kE; ++j) a = amax_step(a, v[j]);
+  }
+  a = block_max(a);
+  if (threadIdx.x == 0) mine = a;
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(&mine));
+#pragma unroll
+  for (int p = 0; p < kSmallCluster; ++p) {
+    uint32_t ra;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(at), "r"(p));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ra));
+    a = nan_max(a, v);
+  }
+  // no block leaves while another may still read its value
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+  return a;
+}
+
 // gpr: 16-element groups per row, covering whole tiles of four scales;
 // items: rows * gpr groups, then one 32-bit word per four scales of each
-// padding row.  part: the blocks' maxima (derive), else null; the blocks then run
+// padding row.  parts: -1 the factor from the cluster's own pass over x, 0 given.
+// part: the blocks' maxima (parts > 0), else null; the blocks then run
 // from the end of the tensor, whose rows the maximum pass left in L2.
 template <typename InT, int FMT>
 __global__ void __launch_bounds__(kThreads)
@@ -162,6 +202,9 @@ __global__ void __launch_bounds__(kThreads)
       float a = 0.0f;
       for (int p = threadIdx.x; p < parts; p += kThreads) a = nan_max(a, part[p]);
       g = factor_of(block_max(a));
+      if (blockIdx.x == 0 && threadIdx.x == 0) *gscale = g;
+    } else if (parts < 0) {
+      g = factor_of(cluster_amax(x, rows, K, ldx, vec));
       if (blockIdx.x == 0 && threadIdx.x == 0) *gscale = g;
     } else {
       g = *gscale;
@@ -341,7 +384,8 @@ int quantize_t(const InT* x, int64_t rows, int64_t K, int64_t ldx, int fmt, floa
   if (items + pad >= (int64_t)1 << 32) return MXB_E_SHAPE;
   const bool vec = ((uintptr_t)x % 32) == 0 && (ldx * (int64_t)sizeof(InT)) % 32 == 0;
   int parts = 0;
-  if (derive) {
+  const bool small = derive && rows * cdiv(K, kE) <= kSmallItems;
+  if (derive && !small) {
     const int64_t agpr = cdiv(K, kE), aitems = rows * agpr;
     const int64_t blocks = cdiv(aitems, kThreads);
     parts = (int)(blocks < kAmaxBlocks ? blocks : kAmaxBlocks);
@@ -353,10 +397,27 @@ int quantize_t(const InT* x, int64_t rows, int64_t K, int64_t ldx, int fmt, floa
   // with a factor to find every block first reduces the maxima, so there are
   // only as many blocks as fit
   int64_t blocks = cdiv(items + pad, kThreads);
-  if (derive && blocks > 4 * kSMs) blocks = 4 * kSMs;
-  MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)blocks), kThreads, 0, st, x,
-                          (uint32_t)rows, K, ldx, (uint32_t)gpr, (uint32_t)items, (uint32_t)pad,
-                          (uint32_t)groups, vec, derive ? part : nullptr, parts, g, codes, scales));
+  if (derive && !small && blocks > 4 * kSMs) blocks = 4 * kSMs;
+  if (small) {
+    blocks = cdiv(blocks, kSmallCluster) * kSmallCluster;
+    parts = -1;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kSmallCluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = small ? 2 : 1;
+  MXB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, x, (uint32_t)rows, K, ldx, (uint32_t)gpr, (uint32_t)items,
+                                  (uint32_t)pad, (uint32_t)groups, vec,
+                                  (const float*)(derive && !small ? part : nullptr), parts, g, codes,
+                                  scales));
   MXB_LAUNCH_CHECK();
   return MXB_OK;
 }

@@ -117,7 +117,7 @@ class fp4_tensor:
         at_g = at_s + sb
         derive = wsb = 0
         if f == L.FP4_NV and global_scale is None:
-            derive, wsb = 1, L.load().mxb_fp4_quantize_workspace_size(rows, K, f, 1)
+            derive, wsb = 1, L.size("mxb_fp4_quantize_workspace_size", rows, K, f, 1)
         elif f == L.FP4_NV:
             if (global_scale.dtype != torch.float32 or global_scale.numel() != 1
                     or global_scale.device != dev):

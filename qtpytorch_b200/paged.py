@@ -64,6 +64,8 @@ class paged_kv_cache:
         if (kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or ks.dtype != torch.float32
                 or vs.dtype != torch.float32):
             raise ValueError("paged_kv_cache: codes are uint8, scales fp32")
+        if not kc.device == ks.device == vc.device == vs.device:
+            raise ValueError("paged_kv_cache: buffers are on different devices")
         if not (kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
             raise ValueError("paged_kv_cache: buffers must be contiguous")
         n_pages, heads, page, row = kc.shape
@@ -78,6 +80,7 @@ class paged_kv_cache:
         self.dtype, self.n_pages, self.n_heads = dt, n_pages, heads
         self.page_size, self.head_dim = page, dim
         self.device = kc.device
+        self._pool = (kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr())
 
     def _cuda(self, what: str) -> torch.device:
         L.require_cuda(self.k_codes, what)
@@ -104,8 +107,7 @@ class paged_kv_cache:
             slots = slots.to(torch.int64).contiguous()
         rc = L.call("mxb_kv_write", dev, k.data_ptr(), v.data_ptr(), _IO[k.dtype], k.shape[0], H, D,
                     k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(),
-                    self.n_pages, self.page_size, self.dtype.bits, self.k_codes.data_ptr(),
-                    self.k_scales.data_ptr(), self.v_codes.data_ptr(), self.v_scales.data_ptr())
+                    self.n_pages, self.page_size, self.dtype.bits, *self._pool)
         if rc:
             L.check(rc, f"mxb_kv_write({self.dtype.name}, T={k.shape[0]})")
 
@@ -120,12 +122,9 @@ class paged_kv_cache:
         if max_len < 0:
             raise ValueError("read: max_len must not be negative")
         B = table.shape[0]
-        shape = (B, max_len, self.n_heads, self.head_dim)
-        k = torch.empty(shape, dtype=dtype, device=dev)
-        v = torch.empty(shape, dtype=dtype, device=dev)
-        rc = L.call("mxb_kv_read", dev, self.k_codes.data_ptr(), self.k_scales.data_ptr(),
-                    self.v_codes.data_ptr(), self.v_scales.data_ptr(), self.n_pages, self.n_heads,
-                    self.page_size, self.head_dim, self.dtype.bits, table.data_ptr(), table.shape[1],
+        k, v = torch.empty((2, B, max_len, self.n_heads, self.head_dim), dtype=dtype, device=dev).unbind()
+        rc = L.call("mxb_kv_read", dev, *self._pool, self.n_pages, self.n_heads, self.page_size,
+                    self.head_dim, self.dtype.bits, table.data_ptr(), table.shape[1],
                     lengths.data_ptr(), B, max_len, k.data_ptr(), v.data_ptr(), _IO[dtype])
         if rc:
             L.check(rc, f"mxb_kv_read({self.dtype.name}, B={B}, max_len={max_len})")
@@ -199,13 +198,11 @@ def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
         q = q.clone()
     out = torch.empty_like(q)
     lse = torch.empty(B, T, Hq, dtype=torch.float32, device=dev) if return_lse else None
-    lib = L.load()
-    wsb = lib.mxb_paged_attention_workspace_size(B, T, H, Hq // H, D, cache.dtype.bits,
-                                                 cache.page_size, table.shape[1], prefix_len)
+    wsb = L.size("mxb_paged_attention_workspace_size", B, T, H, Hq // H, D, cache.dtype.bits,
+                 cache.page_size, table.shape[1], prefix_len)
     ws = L.workspace(wsb, dev)
     rc = L.call("mxb_paged_attention", dev, q.data_ptr(), B, T, H, Hq // H, D,
-                cache.k_codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(),
-                cache.v_scales.data_ptr(), cache.n_pages, cache.page_size, cache.dtype.bits,
+                *cache._pool, cache.n_pages, cache.page_size, cache.dtype.bits,
                 table.data_ptr(), table.shape[1], lengths.data_ptr(),
                 prefix_table.data_ptr() if prefix_len else 0, width, prefix_len,
                 1.0 / math.sqrt(D) if scale is None else float(scale), out.data_ptr(), L.ptr(lse),

@@ -169,7 +169,7 @@ def special(rows, K, seed):
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,K", [(1, 1), (1, 32), (3, 17), (5, 100), (129, 250), (128, 256), (33, 4097)])
+@pytest.mark.parametrize("rows,K", [(1, 1), (1, 32), (3, 17), (5, 100), (129, 250), (128, 256), (33, 4097), (300, 1500)])
 def test_quantize_codes_scales_values(fmt, dtype, rows, K):
     x = special(rows, K, rows * 7919 + K).to(dtype)
     if fmt == "nvfp4" and rows > 3:
