@@ -53,28 +53,36 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 32;    // keys per warp tile
 
+// CTAs per SM, by what their registers and rings leave room for
+__host__ __device__ constexpr int ctas(int nt, int rb, int dim) {
+  return nt == 1 ? (rb == 32 ? 4 : 3) : (dim == 64 && nt <= 3) ? 3 : 2;
+}
+
 template <int BITS, int D, int NT>
 struct Geo {
   static constexpr int RB = D * BITS / 8;       // bytes of a head row: 128, 64 or 32
   static constexpr int kTileBytes = kTile * RB;
-  // CTAs per SM (registers bound them from 9 rows on) and ring depth: 100 to
-  // 200 KB in flight an SM
-  static constexpr int kCtas = NT >= 2 ? 2 : RB == 32 ? 4 : 3;
-  static constexpr int kStages = RB == 128 ? (NT >= 2 ? 3 : 2) : RB == 64 ? (NT >= 2 ? 4 : 3) : 4;
+  // ring depth: 100 to 200 KB in flight an SM
+  static constexpr int kCtas = ctas(NT, RB, D);
+  static constexpr int kStages = RB == 128 ? (NT >= 2 ? 3 : 2) : RB == 64 ? (kCtas == 2 ? 4 : 3) : 4;
   static constexpr int R = 8 * NT;              // query rows per CTA
   static constexpr int kPitch = D + 4;          // floats of a row in the join buffer
   static constexpr size_t kRing = (size_t)kWarps * kStages * (2 * kTileBytes + 2 * kTile * 4);
   static constexpr size_t kJoin = (size_t)kWarps * R * kPitch * 4;
   // where it fits the join buffer lies beside the ring, so the next unit's
   // loads start before the join
-  static constexpr bool kApart = NT <= 2 && RB < 128;
+  static constexpr size_t kStatic = 2048 + (NT >= 3 && D == 128 ? 9 * 1024 : 0);
+  static constexpr bool kApart = kCtas * (1024 + kRing + kJoin + kStatic) <= 228 * 1024;
   static constexpr size_t kSmem = 1024 + (kApart ? kRing + kJoin : kRing > kJoin ? kRing : kJoin);
-  static_assert(kCtas * (kSmem + 2048 + (NT >= 3 ? 9 * 1024 : 0)) <= 228 * 1024, "CTAs fit an SM");
-  // byte offset of 16-byte chunk 0 of row r in a tile (the TMA swizzle); chunk c
-  // lies at that address ^ (c << 4)
+  static_assert(kCtas * (kSmem + kStatic) <= 228 * 1024, "CTAs fit an SM");
+  // The pool is copied as lines of 128 bytes (one, two or four head rows): the
+  // TMA unit takes its time by the line, so 32-byte rows one by one held int4
+  // tiles of 64 dims to 285 cycles each.  Byte offset of 16-byte chunk 0 of
+  // head row r in a tile under the 128-byte swizzle; chunk c lies at that
+  // address ^ (c << 4).
   __device__ static uint32_t at(int r) {
-    const int x = RB == 128 ? (r & 7) : RB == 64 ? ((r >> 1) & 3) : ((r >> 2) & 1);
-    return (uint32_t)(r * RB + (x << 4));
+    const uint32_t byte = (uint32_t)(r * RB), line = byte >> 7;
+    return (line << 7) | ((((byte >> 4) & 7) ^ (line & 7)) << 4);
   }
 };
 
@@ -92,7 +100,7 @@ struct Args {
   const int* table;        // [B][width] (sequences) or [width] (prefix)
   const int* lengths;      // null: the prefix
   int64_t n_pages;
-  int width, page_shift, box;
+  int width, page_shift, box_shift;  // box: keys per copy, a page's or a tile's
   int B, T, H, G;
   int prefix_len;
   int rows;                // query rows per unit (T * G, or B * T * G for the prefix)
@@ -255,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
   float* rs = reinterpret_cast<float*>(smem + kWarps * kStages * 2 * Ge::kTileBytes) +
               warp * (kStages * 2 * kTile);
   float* join = reinterpret_cast<float*>(smem + (Ge::kApart ? Ge::kRing : 0));
-  const int boxes = kTile / a.box;
+  const int box = 1 << a.box_shift, boxes = kTile >> a.box_shift;
   if (lane == 0) {
     // one arrival a box (its copies' bytes), one a lane (its scales)
     for (int s = 0; s < kStages; ++s) mbar_init(&full[warp][s], boxes + 32);
@@ -335,11 +343,12 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
   }
 
   const int page_mask = (1 << a.page_shift) - 1;
+  const int* table = a.table + (own ? (int64_t)b * a.width : 0);
   // page numbers are fetched one tile before the copies that need them
   auto page_of = [&](int tile) -> int {
-    const int pos = tile * kTile + lane * a.box;
+    const int pos = tile * kTile + (lane << a.box_shift);
     if (lane >= boxes || tile >= t_hi || pos >= len) return -1;
-    int p = __ldg(a.table + (own ? (int64_t)b * a.width : 0) + (pos >> a.page_shift));
+    int p = __ldg(table + (pos >> a.page_shift));
     if (p < 0 || p >= a.n_pages) {
       if (a.err) atomicCAS(a.err, 0, kErrIndex);
       p = 0;
@@ -350,19 +359,20 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
     uint64_t* bar = &full[warp][s];
     if (lane < boxes) {
       if (p >= 0) {
-        const int pos = tile * kTile + lane * a.box;
+        const int pos = tile * kTile + (lane << a.box_shift);
         const int row = ((p * a.H + h) << a.page_shift) + (pos & page_mask);
-        uint8_t* k = ring + s * 2 * Ge::kTileBytes + lane * a.box * Ge::RB;
-        mbar_expect_tx(bar, (uint32_t)a.box * 2 * Ge::RB);
-        tma_load_2d(k, &tmap_k, bar, 0, row);
-        tma_load_2d(k + Ge::kTileBytes, &tmap_v, bar, 0, row);
+        uint8_t* k = ring + s * 2 * Ge::kTileBytes + (lane << a.box_shift) * Ge::RB;
+        mbar_expect_tx(bar, (uint32_t)box * 2 * Ge::RB);
+        const int line = row / (128 / Ge::RB);
+        tma_load_2d(k, &tmap_k, bar, 0, line);
+        tma_load_2d(k + Ge::kTileBytes, &tmap_v, bar, 0, line);
       } else {
         mbar_arrive(bar);
       }
     }
     // a lane's two scales: a bulk copy each would cost the TMA unit as much as
     // a tile of codes (attend_long without them 8 us shorter)
-    const int kp = __shfl_sync(0xffffffffu, p, lane / a.box);
+    const int kp = __shfl_sync(0xffffffffu, p, lane >> a.box_shift);
     const int pos = tile * kTile + lane;
     if (kp >= 0) {
       const int row = ((kp * a.H + h) << a.page_shift) + (pos & page_mask);
@@ -575,56 +585,55 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
         kscale[i] = sc[8 * i + g] * a.scale_log2;
         lv[i] = lg2(sc[kTile + 8 * i + g]);
       }
-      float wv[NT][4][2];  // s + log2 sv
+      // One column tile after the other, to keep few values alive; the two
+      // columns of an accumulator pair go through packed operations.
+      const int key0 = tile * kTile + g;
+      const bool ragged = (tile + 1) * kTile > lim_min;  // some key is hidden from some row
+      uint32_t pb[2][NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        uint64_t v2[4], w2[4];  // s, s + log2 sv
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+          uint64_t f = pack2(kscale[i], kscale[i]);
+          if (BITS == 8) f = fmul2(f, pack2(cfac[n][0], cfac[n][1]));
+          v2[i] = fmul2(pack2(sa[i >> 1][n][(i & 1) * 2], sa[i >> 1][n][(i & 1) * 2 + 1]), f);
+          w2[i] = fadd2(v2[i], pack2(lv[i], lv[i]));
+        }
+        if (ragged) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& v = sa[i >> 1][n][(i & 1) * 2 + e];
-            v *= kscale[i];
-            if (BITS == 8) v *= cfac[n][e];
-            wv[n][i][e] = v + lv[i];
+          for (int i = 0; i < 4; ++i) {
+            float2 v = unpack2(v2[i]), w = unpack2(w2[i]);
+            if (key0 + 8 * i >= limit[n][0]) v.x = w.x = -INFINITY;  // whatever its scales hold
+            if (key0 + 8 * i >= limit[n][1]) v.y = w.y = -INFINITY;
+            v2[i] = pack2(v.x, v.y);
+            w2[i] = pack2(w.x, w.y);
           }
-      if ((tile + 1) * kTile > lim_min) {  // some key is hidden from some row
-        const int key0 = tile * kTile + g;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (key0 + 8 * i >= limit[n][e])  // whatever its scales hold
-                sa[i >> 1][n][(i & 1) * 2 + e] = wv[n][i][e] = -INFINITY;
-      }
-      // ── the references: moved only when a sum's terms pass 2^64 or a weight
-      // 2^8 (fp16 holds 2^15), so most tiles need no exchange between lanes ──
-      bool move = false;
-      float mx[NT][2], mw[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
+        }
+        // the references move only when a sum's terms pass 2^64 or a weight 2^8
+        // (fp16 holds 2^15), so most tiles need no exchange between lanes
+        float mx[2], mw[2];
+        bool move = false;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          mx[n][e] = fmaxf(fmaxf(sa[0][n][e], sa[0][n][2 + e]), fmaxf(sa[1][n][e], sa[1][n][2 + e]));
-          mw[n][e] = fmaxf(fmaxf(wv[n][0][e], wv[n][1][e]), fmaxf(wv[n][2][e], wv[n][3][e]));
-          move |= mx[n][e] > m_top[n][e] || mw[n][e] > w_top[n][e];
+          auto of = [&](uint64_t p) { return e ? unpack2(p).y : unpack2(p).x; };
+          mx[e] = fmaxf(fmaxf(of(v2[0]), of(v2[1])), fmaxf(of(v2[2]), of(v2[3])));
+          mw[e] = fmaxf(fmaxf(of(w2[0]), of(w2[1])), fmaxf(of(w2[2]), of(w2[3])));
+          move |= mx[e] > m_top[n][e] || mw[e] > w_top[n][e];
         }
-      if (__any_sync(0xffffffffu, move)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
+        if (__any_sync(0xffffffffu, move)) {
           float alpha[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) {
-              mx[n][e] = fmaxf(mx[n][e], __shfl_xor_sync(0xffffffffu, mx[n][e], x));
-              mw[n][e] = fmaxf(mw[n][e], __shfl_xor_sync(0xffffffffu, mw[n][e], x));
+              mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
+              mw[e] = fmaxf(mw[e], __shfl_xor_sync(0xffffffffu, mw[e], x));
             }
             // the larger of the reference (where there is one) and the tile's
             const float m0 = m_top[n][e] == -INFINITY ? -INFINITY : mu[n][e];
             const float w0 = w_top[n][e] == -INFINITY ? -INFINITY : wu[n][e];
-            const float m1 = fmaxf(m0, mx[n][e]), w1 = fmaxf(w0, mw[n][e]);
+            const float m1 = fmaxf(m0, mx[e]), w1 = fmaxf(w0, mw[e]);
             mu[n][e] = base_of(m1);
             wu[n][e] = base_of(w1);
             l[n][e] *= ex2(m0 - mu[n][e]);
@@ -637,24 +646,17 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[j][n][e] *= alpha[e & 1];
         }
-      }
-      // ── weights: keys x rows -> rows x keys, the B fragment of the second
-      // product ──
-      uint32_t pb[2][NT][2];
+        // weights: keys x rows -> rows x keys, the B fragment of the second product
+        const uint64_t mu2 = pack2(mu[n][0], mu[n][1]), wu2 = pack2(wu[n][0], wu[n][1]);
+        uint64_t sum = pack2(0.0f, 0.0f);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float sum = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sum += ex2(sa[i >> 1][n][(i & 1) * 2 + e] - mu[n][e]);
-            wv[n][i][e] = ex2(wv[n][i][e] - wu[n][e]);
-          }
-          l[n][e] += sum;
+        for (int i = 0; i < 4; ++i) {
+          const float2 v = unpack2(fsub2(v2[i], mu2)), w = unpack2(fsub2(w2[i], wu2));
+          sum = fadd2(sum, pack2(ex2(v.x), ex2(v.y)));
+          pb[i >> 1][n][i & 1] = movm(hf2(ex2(w.x), ex2(w.y)));
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pb[i >> 1][n][i & 1] = movm(hf2(wv[n][i][0], wv[n][i][1]));
+        l[n][0] += unpack2(sum).x;
+        l[n][1] += unpack2(sum).y;
       }
       // ── O^T += V^T P^T ──
 #pragma unroll
@@ -694,6 +696,7 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
           ++b;
           len = len_of(b);
         } while (len == 0);
+        table = a.table + (int64_t)b * a.width;
         n_tiles = tiles_of(len);
       }
       t_hi = (int)min((int64_t)n_tiles, left);
@@ -903,9 +906,6 @@ struct Plan {
 
 int nt_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4; }
 
-// CTAs that fit an SM (Geo::kCtas)
-int ctas_per_sm(int nt, int rb) { return nt >= 2 ? 2 : rb == 32 ? 4 : 3; }
-
 Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, int64_t max_keys,
                int64_t prefix) {
   Plan p = {};
@@ -920,7 +920,7 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, in
   if (p.whole) {
     p.ctas_own = (int)units;
   } else if (max_keys > 0) {
-    const int64_t most = units * cdiv(max_keys, kTile * kWarps), fit = kSMs * ctas_per_sm(p.nt_own, rb);
+    const int64_t most = units * cdiv(max_keys, kTile * kWarps), fit = kSMs * ctas(p.nt_own, rb, dim);
     p.ctas_own = (int)(most < fit ? most : fit);
   }
   if (prefix > 0 && B * T * G >= kPrefixMinRows) {
@@ -934,7 +934,7 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, in
     p.nt_pre = nt_of(B * T * G);
     p.tiles_pre = (int)cdiv(B * T * G, 8 * p.nt_pre);
     const int64_t most = cdiv(prefix, kTile * kWarps);
-    int64_t s = cdiv(kSMs * ctas_per_sm(p.nt_pre, rb), H * p.tiles_pre);
+    int64_t s = cdiv(kSMs * ctas(p.nt_pre, rb, dim), H * p.tiles_pre);
     s = s < most ? s : most;
     p.splits_pre = (int)(s < 1 ? 1 : s);
   }
@@ -1029,12 +1029,12 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
 
   CUtensorMap tk, tv;
   const int box = page < pattn::kTile ? page : pattn::kTile;
-  const uint64_t rb = (uint64_t)dim * bits / 8, rows = (uint64_t)n_pages * heads * page;
-  const int swz = rb == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-                  : rb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                             : CU_TENSOR_MAP_SWIZZLE_32B;
-  if (!encode_tmap_2d(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, k_codes, rb, rows, (uint32_t)rb, box, swz) ||
-      !encode_tmap_2d(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, v_codes, rb, rows, (uint32_t)rb, box, swz))
+  const uint64_t rb = (uint64_t)dim * bits / 8, lines = (uint64_t)n_pages * heads * page * rb / 128;
+  const uint32_t box_lines = (uint32_t)(box * rb / 128);
+  if (!encode_tmap_2d(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, k_codes, 128, lines, 128, box_lines,
+                      CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !encode_tmap_2d(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, v_codes, 128, lines, 128, box_lines,
+                      CU_TENSOR_MAP_SWIZZLE_128B))
     return MXB_E_CUDA;
 
   pattn::Args a = {};
@@ -1043,7 +1043,7 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
   a.vs = v_scales;
   a.n_pages = n_pages;
   a.page_shift = 31 - __builtin_clz((unsigned)page);
-  a.box = box;
+  a.box_shift = 31 - __builtin_clz((unsigned)box);
   a.B = (int)B;
   a.T = (int)T;
   a.H = heads;

@@ -226,8 +226,9 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
           uint8_t* dst = smem + C::oRaw + (size_t)s * 2 * C::kRaw + lane * box * C::RB;
           float* sc = reinterpret_cast<float*>(smem + C::oRawS) + s * 2 * KT + lane * box;
           mbar_expect_tx(bar, (uint32_t)box * (2 * C::RB + 8));
-          tma_load_2d(dst, &tmap_k, bar, 0, row);
-          tma_load_2d(dst + C::kRaw, &tmap_v, bar, 0, row);
+          const int line = (int)((int64_t)row * C::RB / 128);  // lines of 128 bytes
+          tma_load_2d(dst, &tmap_k, bar, 0, line);
+          tma_load_2d(dst + C::kRaw, &tmap_v, bar, 0, line);
           bulk_load_g2s(sc, a.k_scales + row, (uint32_t)box * 4, bar);
           bulk_load_g2s(sc + KT, a.v_scales + row, (uint32_t)box * 4, bar);
         } else {
@@ -547,10 +548,11 @@ int prefix_rows_per_cta(int64_t rows) { return rows > 128 ? 256 : 128; }
 int prefix_attention(const PrefixArgs& a, cudaStream_t st) {
   CUtensorMap tk, tv;
   const int page = 1 << a.page_shift, box = page < pfx::KT ? page : pfx::KT;
-  const uint64_t rb = (uint64_t)a.dim * a.bits / 8, rows = (uint64_t)a.n_pages * a.H * page;
-  if (!encode_tmap_2d(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.k_codes, rb, rows, (uint32_t)rb, box,
+  const uint64_t rb = (uint64_t)a.dim * a.bits / 8, lines = (uint64_t)a.n_pages * a.H * page * rb / 128;
+  const uint32_t box_lines = (uint32_t)(box * rb / 128);
+  if (!encode_tmap_2d(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.k_codes, 128, lines, 128, box_lines,
                       CU_TENSOR_MAP_SWIZZLE_NONE) ||
-      !encode_tmap_2d(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.v_codes, rb, rows, (uint32_t)rb, box,
+      !encode_tmap_2d(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.v_codes, 128, lines, 128, box_lines,
                       CU_TENSOR_MAP_SWIZZLE_NONE))
     return MXB_E_CUDA;
   if (a.bits == 8)
