@@ -249,8 +249,8 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
                                              ~static_cast<uintptr_t>(1023));
   __shared__ uint64_t full[kWarps][kStages];
   __shared__ float sm_m[kWarps][R], sm_l[kWarps][R], sm_v[kWarps][R];
-  __shared__ int64_t sm_scan[kWarps], sm_off;
-  __shared__ int sm_b;
+  __shared__ int64_t sm_scan[kWarps];
+  __shared__ int sm_b, sm_off;
   // with many rows the query fragments, the same for all warps, live in
   // shared memory: in registers they would spill
   constexpr bool kQs = NT >= 3 && D == 128;
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
     t_hi = n_tiles;
     left = n_tiles;
   } else {
-    int64_t total = 0, before;
+    int64_t total = 0, before, n0 = 0, before0 = 0;
     for (int b0 = 0; b0 < a.B; b0 += kThreads) {
       const int i = b0 + threadIdx.x;
       int n = 0;
@@ -313,31 +313,41 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
         n = tiles_of((int)min((int64_t)max(n, 0), cap));
       }
       total += block_scan((int64_t)n * hr, before, sm_scan);
+      if (b0 == 0) {
+        n0 = (int64_t)n * hr;
+        before0 = before;
+      }
     }
     // equal runs, at least a tile a warp
-    const int64_t per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kWarps);
+    const int64_t per = max((int64_t)(total >> 31 ? (total + gridDim.x - 1) / gridDim.x
+                                                  : ((uint32_t)total + gridDim.x - 1) / gridDim.x),
+                            (int64_t)kWarps);
     const int64_t lo = blockIdx.x * per, hi = min(lo + per, total);
     if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = per;
     int64_t base = 0;
     for (int b0 = 0; b0 < a.B && (blockIdx.x == 0 || base <= lo); b0 += kThreads) {
       const int i = b0 + threadIdx.x;
-      const int64_t n = i < a.B ? (int64_t)tiles_of(len_of(i)) * hr : 0;
-      const int64_t sum = block_scan(n, before, sm_scan);
-      before += base;
+      int64_t n = n0;
+      before = before0;
+      if (a.B > kThreads) {  // one scan was not all
+        n = i < a.B ? (int64_t)tiles_of(len_of(i)) * hr : 0;
+        const int64_t sum = block_scan(n, before, sm_scan);
+        before += base;
+        base += sum;
+      }
       if (i < a.B && blockIdx.x == 0) a.plan[1 + i] = before;
       if (lo < hi && lo >= before && lo < before + n) {
         sm_b = i;
-        sm_off = before;
+        sm_off = (int)(lo - before);
       }
-      base += sum;
     }
     __syncthreads();
     if (lo >= hi) return;
     b = sm_b;
     len = len_of(b);
     n_tiles = tiles_of(len);
-    u = (int)((lo - sm_off) / n_tiles);
-    t_lo = (int)((lo - sm_off) - (int64_t)u * n_tiles);
+    u = sm_off / n_tiles;  // a sequence has fewer than 2^31 tiles (checked at the launch)
+    t_lo = sm_off - u * n_tiles;
     left = hi - lo;
     t_hi = (int)min((int64_t)n_tiles, t_lo + left);
   }
@@ -1022,7 +1032,8 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
   const pattn::Plan p =
       pattn::make_plan(B, T, heads, group, dim, bits, width * page, prefix_len);
   if ((int64_t)p.tiles_own * heads > 65535 || (int64_t)p.tiles_pre * heads > 65535 ||
-      B * heads * p.tiles_own > INT32_MAX || B * T * heads * group > INT32_MAX)
+      B * heads * p.tiles_own > INT32_MAX || B * T * heads * group > INT32_MAX ||
+      (int64_t)heads * p.tiles_own * (width * page / pattn::kTile + 1) > INT32_MAX)
     return MXB_E_SHAPE;
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return MXB_E_WORKSPACE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

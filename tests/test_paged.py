@@ -486,3 +486,11 @@ def test_serving_example_matches_the_dequantized_layer():
     o = mxb.paged_attention(q, c, table, n, prefix_table=doc, prefix_len=300)
     check_attention(o, None, q, c, table, [6] * 6, doc, 300)
     assert torch.equal(got, layer.out(o.reshape(6, 1, 1024)))
+
+
+@pytest.mark.gpu
+def test_attention_of_a_batch_wider_than_a_block():
+    """More sequences than threads in a CTA: the shared list is scanned in steps."""
+    lengths = [(37 * i) % 300 for i in range(301)]
+    run_attention("int8d", 64, 16, 2, 2, 1, lengths, 0)
+    run_attention("int4d", 128, 64, 1, 4, 1, lengths[:129], 70)
