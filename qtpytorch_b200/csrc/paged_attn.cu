@@ -30,7 +30,8 @@
 //
 // Work: the tiles of all sequences, heads and row groups form one list, which
 // the CTAs share out in equal runs (lengths are known on the device only), so
-// a batch of very different lengths keeps every SM busy to the end.  A run may
+// a batch of very different lengths keeps every SM busy to the end; short units
+// (make_plan) get a CTA each instead.  A run may
 // hold several units or a part of one; a unit's first part goes to a row
 // buffer, a later part to its CTA's buffer, and a second kernel joins them
 // with the parts of the shared prefix.  Rows with a single part are written
@@ -299,6 +300,8 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
     b = blockIdx.x / hr;
     u = blockIdx.x - b * hr;
     len = len_of(b);
+    if (u == 0 && threadIdx.x == 0 && a.err && __ldg(a.lengths + b) > cap)
+      atomicCAS(a.err, 0, kErrIndex);
     n_tiles = tiles_of(len);
     t_hi = n_tiles;
     left = n_tiles;
@@ -318,10 +321,12 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
         before0 = before;
       }
     }
-    // equal runs, at least a tile a warp
-    const int64_t per = max((int64_t)(total >> 31 ? (total + gridDim.x - 1) / gridDim.x
-                                                  : ((uint32_t)total + gridDim.x - 1) / gridDim.x),
-                            (int64_t)kWarps);
+    // equal runs, of a tile a warp or a unit's average length at least: a CTA
+    // takes about 5 us a unit, so short units are not put one after another
+    auto share = [&](uint32_t n) {
+      return (int64_t)(total >> 31 ? (total + n - 1) / n : ((uint32_t)total + n - 1) / n);
+    };
+    const int64_t per = max(share(gridDim.x), min(share((uint32_t)(a.B * hr)), (int64_t)kWarps));
     const int64_t lo = blockIdx.x * per, hi = min(lo + per, total);
     if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = per;
     int64_t base = 0;
@@ -811,10 +816,13 @@ __global__ void __launch_bounds__(kThreads)
   if (lengths) {
     const int64_t n = (min((int64_t)max(lengths[b], 0), cap) + kTile - 1) / kTile;
     if (n > 0) {
-      const int64_t per = plan[0];
-      const int64_t f0 = plan[1 + b] + ((int64_t)h * row_tiles + rr / R) * n;
-      c0 = f0 / per;
-      own = (int)((f0 + n - 1) / per - c0) + 1;
+      own = 1;
+      if (plan) {
+        const int64_t per = plan[0];
+        const int64_t f0 = plan[1 + b] + ((int64_t)h * row_tiles + rr / R) * n;
+        c0 = f0 / per;
+        own = (int)((f0 + n - 1) / per - c0) + 1;
+      }
     }
   }
   if (direct && own == 1) return;  // written already
@@ -909,7 +917,8 @@ __global__ void __launch_bounds__(kThreads)
 // sequences' own keys and splits of the prefix.
 struct Plan {
   int nt_own, tiles_own, ctas_own;        // ctas_own 0: no own keys possible
-  bool whole;                             // a unit per CTA, nothing to join
+  bool whole;                             // a unit per CTA
+  bool join;                              // rows may have several parts
   int nt_pre, tiles_pre, splits_pre;      // splits_pre 0: no prefix; nt_pre 0: prefix_attn.cu
   size_t o_plan, o_main, o_cta, o_pre, bytes;  // workspace offsets
 };
@@ -924,14 +933,21 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, in
   p.nt_own = nt_of(T * G);
   p.tiles_own = (int)cdiv(T * G, 8 * p.nt_own);
   const int64_t units = B * H * p.tiles_own;
-  // Up to two tiles a warp a unit is not worth a second part: one CTA each
-  // and no join.
-  p.whole = prefix == 0 && max_keys <= 2 * kTile * kWarps;
+  // Short units: one CTA each, and the hardware shares them out.  The list's
+  // even runs cost a plan, a second unit's start in most CTAs (5 us) and a
+  // join, and pay only where a unit is long beside that or too few units fill
+  // the SMs.  Microseconds, a CTA a unit against the list, 8 heads of 128 dims
+  // in int8, lengths uniform up to the width: 64 x 512 keys 19 / 52, 256 x 1024
+  // 69 / 126, 64 x 4096 71 / 87 (all full 113 / 108), 16 x 2048 24 / 24 (27 /
+  // 31), 16 x 4096 45 / 37, 4 x 2048 18.5 / 15.8, 1 x 1024 11.6 / 13.0.
+  const int64_t slots = kSMs * ctas(p.nt_own, rb, dim);
+  const int64_t whole_keys = units >= slots ? 4096 : units >= kSMs * 3 / 4 ? 2048 : 1024;
+  p.whole = max_keys <= whole_keys && (max_keys > 0 || prefix == 0);
   if (p.whole) {
     p.ctas_own = (int)units;
   } else if (max_keys > 0) {
-    const int64_t most = units * cdiv(max_keys, kTile * kWarps), fit = kSMs * ctas(p.nt_own, rb, dim);
-    p.ctas_own = (int)(most < fit ? most : fit);
+    const int64_t most = units * cdiv(max_keys, kTile * kWarps);
+    p.ctas_own = (int)(most < slots ? most : slots);
   }
   if (prefix > 0 && B * T * G >= kPrefixMinRows) {
     // many rows: 128-row tensor-core tiles, one CTA an SM
@@ -955,10 +971,11 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, in
     return o;
   };
   const size_t row = (size_t)dim * 4 + 16;
-  if (!p.whole) {
-    p.o_plan = take((size_t)(B + 1) * 8);
+  p.join = !p.whole || prefix > 0;
+  if (p.join) {
+    p.o_plan = take(p.whole ? 0 : (size_t)(B + 1) * 8);
     p.o_main = take(p.ctas_own ? (size_t)n_rows * row : 0);
-    p.o_cta = take((size_t)p.ctas_own * 8 * p.nt_own * row);
+    p.o_cta = take(p.whole ? 0 : (size_t)p.ctas_own * 8 * p.nt_own * row);
     p.o_pre = take((size_t)p.splits_pre * n_rows * row);
   }
   p.bytes = at;
@@ -1113,8 +1130,8 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
   a.whole = p.whole;
   a.direct = p.splits_pre == 0;
   if (p.ctas_own > 0) {
+    if (p.join) own = pattn::part_at(workspace, p.o_main, (size_t)a.n_rows, dim);
     if (!p.whole) {
-      own = pattn::part_at(workspace, p.o_main, (size_t)a.n_rows, dim);
       cta = pattn::part_at(workspace, p.o_cta, (size_t)p.ctas_own * 8 * p.nt_own, dim);
       a.plan = reinterpret_cast<int64_t*>(static_cast<char*>(workspace) + p.o_plan);
     }
@@ -1124,7 +1141,7 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
         pattn::launch_any(tk, tv, a, bits, dim, p.nt_own, dim3((unsigned)p.ctas_own), st);
     if (r != MXB_OK) return r;
   }
-  if (!p.whole) {
+  if (p.join) {
     MXB_CUDA_TRY(launch_pdl(
         dim == 128 ? pattn::paged_join_kernel<128> : pattn::paged_join_kernel<64>,
         dim3((unsigned)a.n_rows), pattn::kThreads, 0, st, own, cta, pre, a.plan,

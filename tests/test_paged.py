@@ -325,6 +325,16 @@ def test_attention_long_skewed_batch(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["int8d", "int4d"])
+@pytest.mark.parametrize("T,group,prefix", [(1, 4, 0), (3, 8, 0), (1, 4, 100)])
+def test_attention_of_short_sequences_beside_a_long_one(dtype, T, group, prefix):
+    """A table wide enough for 4200 keys, nearly all of it unused: many units of a
+    tile or two in a CTA's run, empty ones between them."""
+    run_attention(dtype, 64, 32, 2, group, T, [4200] + [0, 1, 31, 32, 33, 0, 65, 100] * 17, prefix)
+    run_attention(dtype, 128, 64, 3, group, T, [1, 0, 40, 0, 4160, 64, 2], prefix)
+
+
+@pytest.mark.gpu
 def test_attention_scores_that_grow_and_values_of_any_scale():
     """Keys whose scores rise along the sequence move the running maximum again
     and again; value scales over six decades stay exact beside one another."""
