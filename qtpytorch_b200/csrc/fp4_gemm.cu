@@ -25,6 +25,12 @@
 //                box of codes each (14 of 100 us at 4096 x 8192 x 8192).
 // Two CTAs an SM: one alone draws 73 KB/us of operands through its ring, two
 // 121, and each covers the other's start and epilogue.
+//
+// Few tokens are bound by the weight's bytes and the start of a launch (1 token,
+// 4096 -> 11008: 8.0 us for 24 MB), many by the operands' way from L2 and then by
+// power: 4096 tokens, 8192 -> 8192 138 us = 4.0 PFLOP/s in mxfp4, 160 us where the
+// clock has fallen to 1.58 GHz at 986 W; 2048 tokens, 4096 -> 11008 in nvfp4 62 and
+// 70 us.
 #include "mxb_common.cuh"
 #include "mxb_internal.h"
 
@@ -404,15 +410,22 @@ int dispatch(const void* fcodes, const void* tcodes, Args& a, cudaStream_t st) {
                           (uint64_t)a.M, BK / 2, rows_t, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   // Tokens per tile: the smallest that holds them all, so a step of few
-  // tokens pays an MMA of that width
+  // tokens pays an MMA of that width (1 x 4096 x 11008 8.0 us, 13.3 with 128
+  // columns; 32 x 8192 x 8192 10.6, 12.8)
   const int nt = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
   // K splits while they fill the SMs (two CTAs each for narrow tiles; a wide
   // tile's partial sums cost more than the second CTA saves: 128 x 4096 x 4096
-  // 8.1 us with 4 splits, 11.3 with 8), at least two stages each
+  // 8.1 us with 4 splits, 11.3 with 8), at least two stages each.  More splits
+  // shorten the stages' time / splits and lengthen the sum, so that the best is
+  // near the root of the stages: tokens x K x features 16 x 4096 x 4096 takes
+  // 6.7 us with 8, 5.8 with 4 or 5, 8.7 with one; 8 x 2048 x 1000 4.1 with 4, 4.6
+  // with 2, 5.3 with one.
   const int64_t tiles = ft * cdiv(a.M, nt);
   int64_t splits = (nt >= 128 ? kSMs : 2 * kSMs) / tiles;
   if (splits > a.ksteps / 2) splits = a.ksteps / 2;
-  a.splits = (int)(splits < 1 ? 1 : splits > kMaxSplit ? kMaxSplit : splits);
+  if (splits > kMaxSplit) splits = kMaxSplit;
+  while (splits * splits > 2 * (int64_t)a.ksteps) --splits;
+  a.splits = (int)(splits < 1 ? 1 : splits);
   if (!maps(BM, nt)) return MXB_E_CUDA;
   switch (nt) {
     case 16: return launch<FMT, 16, OutT>(tf, tt, a, st);
