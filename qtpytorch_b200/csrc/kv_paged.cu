@@ -8,6 +8,8 @@
 // Both kernels are one pass over HBM.  Write: D / 8 lanes own a head row (one
 // 16-byte load of bf16 each), so the row maximum is 3 or 4 shuffles and a
 // row's codes leave as one run.  Read: a thread produces 16 bytes of output.
+// At 4 x 4096 tokens of 8 heads of 128 dims in int4 (85 MB either way) they are
+// bound by HBM, 17 us = 5 TB/s each; a step's 32 tokens by the launch.
 #include "mxb_common.cuh"
 #include "mxb_internal.h"
 

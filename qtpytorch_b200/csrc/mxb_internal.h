@@ -35,9 +35,7 @@ struct PrefixArgs {
   float* ml;
   int* err;
 };
-// Rows per CTA, the least query rows a KV head that pay for the tensor cores'
-// 128-row tiles, and keys per tile.
-constexpr int kPrefixMinRows = 48;
+// Rows per CTA and keys per tile.
 int prefix_rows_per_cta(int64_t rows);
 constexpr int kPrefixKeys = 64;
 int prefix_attention(const PrefixArgs& a, cudaStream_t st);

@@ -24,18 +24,22 @@
 // contraction index is permuted (the same for Q) to what the byte order of the
 // codes gives.  Unpacking: a mask and an exclusive or put a code under a fixed
 // exponent, which leaves code + offset; for K the offset is taken out once, in
-// the accumulator's start -offset * sum(q) (eight products deep, so the
-// cancellation costs under 2^-14 of a score's own rounding to bf16 inputs),
-// for V by one packed subtraction.
+// the accumulator's start -offset * sum(q) (in fp32: the D / 16 + 4 additions may
+// each be off by 2^-23 of (offset + code) sum|q| sk, offset 1152 or 136), for V by
+// one packed subtraction.
 //
 // Work: the tiles of all sequences, heads and row groups form one list, which
 // the CTAs share out in equal runs (lengths are known on the device only), so
 // a batch of very different lengths keeps every SM busy to the end; short units
-// (make_plan) get a CTA each instead.  A run may
-// hold several units or a part of one; a unit's first part goes to a row
-// buffer, a later part to its CTA's buffer, and a second kernel joins them
-// with the parts of the shared prefix.  Rows with a single part are written
-// directly.
+// (make_plan) get a CTA each instead.  A run may hold several units or a part of
+// one; a unit's first part goes to a row buffer, a later part to its CTA's
+// buffer, and a second kernel joins them with the parts of the shared prefix.
+// Rows with a single part are written directly.
+//
+// 2 x 131072 keys and less, 4 rows of each of 8 heads of 128 dims in int8 (346 MB):
+// 71 us = 4.9 TB/s, 62 without any arithmetic.  24 rows of 64 dims in int4 take
+// about 1080 instructions a tile for 2 KB of codes and are bound by their latency
+// (0.43 issued a cycle with 8 warps an SM): 50 us for 48 x up to 6000 keys.
 #include "mxb_common.cuh"
 #include "mxb_internal.h"
 
@@ -949,9 +953,14 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, in
     const int64_t most = units * cdiv(max_keys, kTile * kWarps);
     p.ctas_own = (int)(most < slots ? most : slots);
   }
-  if (prefix > 0 && B * T * G >= kPrefixMinRows) {
-    // many rows: 128-row tensor-core tiles, one CTA an SM
-    const int64_t units = H * cdiv(B * T * G, prefix_rows_per_cta(B * T * G));
+  // Many rows: 128-row tensor-core tiles, one CTA an SM.  Microseconds of a
+  // call, tiles against groups of up to 32 rows, 8 heads of 128 dims in int8
+  // (64 in int4): 24 rows over 512 keys 16.5 / 20.5 (15 / 18.5), over 8192
+  // 28 / 25; 28 rows over 512 16.4 / 25.7 (15.6 / 19.5), over 8192 28 / 33
+  // (26 / 24.5), over 32768 58 / 62 (51 / 33); 48 rows over 32768 65 / 138.
+  const int64_t pre_rows = B * T * G;
+  if (prefix > 0 && (pre_rows >= 48 || (pre_rows > 24 && prefix <= 8192))) {
+    const int64_t units = H * cdiv(pre_rows, prefix_rows_per_cta(pre_rows));
     const int64_t most = cdiv(prefix, 2 * kPrefixKeys);
     int64_t s = kSMs / units;
     s = s < most ? s : most;
