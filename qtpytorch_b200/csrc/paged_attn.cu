@@ -798,123 +798,186 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
   }
 }
 
-// A block per row joins its parts (the sequence's own, by CTA, then the
-// prefix's, by split): warp w the parts w, w + 4, .., then the warps in order.
+// Joins the parts of rows: the sequence's own, by CTA, then the prefix's, by split.
+struct JoinArgs {
+  Part main, cta, pre;
+  const int64_t* plan;  // null: a unit has one part
+  const int* lengths;   // null: no keys of its own
+  int64_t cap, n_rows;
+  int pre_parts, T, H, G, row_tiles, R;
+  bool direct;  // rows with one part of their own are written already
+  __nv_bfloat16* out;
+  float* lse;
+};
+
+// A row's parts p0, p0 + step, .. summed, lane l with dims l * D / 32 on.
 template <int D>
-__global__ void __launch_bounds__(kThreads)
-    paged_join_kernel(const Part main, const Part cta, const Part pre, const int64_t* __restrict__ plan,
-                      const int* __restrict__ lengths, int64_t cap, int pre_parts, int64_t n_rows,
-                      int T, int H, int G, int row_tiles, int R, bool direct,
-                      __nv_bfloat16* __restrict__ out, float* __restrict__ lse) {
-  const uint32_t row = blockIdx.x;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __shared__ float sv[kWarps][D], sm[kWarps], ss[kWarps], sw[kWarps];
-  pdl_trigger();
-  pdl_wait();
-  constexpr int V = D / 32;
-  const uint32_t bt = row / (uint32_t)(H * G);
-  const int hq = (int)(row - bt * (uint32_t)(H * G)), h = hq / G;
-  const int b = (int)(bt / (uint32_t)T), rr = (int)(bt - (uint32_t)b * T) * G + (hq - h * G);
-  int own = 0;
-  int64_t c0 = 0;
-  if (lengths) {
-    const int64_t n = (min((int64_t)max(lengths[b], 0), cap) + kTile - 1) / kTile;
-    if (n > 0) {
-      own = 1;
-      if (plan) {
-        const int64_t per = plan[0];
-        const int64_t f0 = plan[1 + b] + ((int64_t)h * row_tiles + rr / R) * n;
-        c0 = f0 / per;
-        own = (int)((f0 + n - 1) / per - c0) + 1;
-      }
-    }
-  }
-  if (direct && own == 1) return;  // written already
-  const int parts = own + pre_parts;
-  const int64_t c_at = c0 * R + rr % R;
-  auto part_of = [&](int p, int64_t& i) -> const Part& {
-    if (p >= own) {
-      i = (int64_t)(p - own) * n_rows + row;
-      return pre;
-    }
-    i = p == 0 ? (int64_t)row : c_at + (int64_t)p * R;
-    return p == 0 ? main : cta;
-  };
+struct RowSum {
+  static constexpr int V = D / 32, U = 4;  // U parts in flight
   float mu = -INFINITY, wu = -INFINITY, sum = 0.0f, v[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) v[k] = 0.0f;
-  constexpr int U = 4;  // parts in flight a warp
-  for (int p0 = warp; p0 < parts; p0 += kWarps * U) {
-    float4 ml[U];
-    float x[U][V];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int p = p0 + i * kWarps;
-      ml[i] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
-#pragma unroll
-      for (int k = 0; k < V; ++k) x[i][k] = 0.0f;
-      if (p < parts) {
-        int64_t at;
-        const Part& q = part_of(p, at);
-        ml[i] = q.ml[at];
-        if constexpr (V == 4) {
-          const float4 t = *reinterpret_cast<const float4*>(q.o + at * D + lane * V);
-          x[i][0] = t.x; x[i][1] = t.y; x[i][2] = t.z; x[i][3] = t.w;
-        } else {
-          const float2 t = *reinterpret_cast<const float2*>(q.o + at * D + lane * V);
-          x[i][0] = t.x; x[i][1] = t.y;
+
+  // parts of a row, of them its own, and where the CTAs' buffers hold those
+  __device__ static int count(const JoinArgs& a, uint32_t row, int& own, int64_t& c_at) {
+    const uint32_t bt = row / (uint32_t)(a.H * a.G);
+    const int hq = (int)(row - bt * (uint32_t)(a.H * a.G)), h = hq / a.G;
+    const int b = (int)(bt / (uint32_t)a.T), rr = (int)(bt - (uint32_t)b * a.T) * a.G + (hq - h * a.G);
+    own = 0;
+    c_at = 0;
+    if (a.lengths) {
+      const int64_t n = (min((int64_t)max(__ldg(a.lengths + b), 0), a.cap) + kTile - 1) / kTile;
+      if (n > 0) {
+        own = 1;
+        if (a.plan) {
+          const int64_t per = a.plan[0];
+          const int64_t f0 = a.plan[1 + b] + ((int64_t)h * a.row_tiles + rr / a.R) * n;
+          const int64_t c0 = f0 / per;
+          own = (int)((f0 + n - 1) / per - c0) + 1;
+          c_at = c0 * a.R + rr % a.R;
         }
       }
     }
-    float m1 = mu, w1 = wu;
+    return own + a.pre_parts;
+  }
+
+  __device__ void add(const JoinArgs& a, uint32_t row, int own, int64_t c_at, int parts, int p0, int step) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      m1 = fmaxf(m1, ml[i].x);
-      w1 = fmaxf(w1, ml[i].z);
+    for (int k = 0; k < V; ++k) v[k] = 0.0f;
+    for (; p0 < parts; p0 += step * U) {
+      float4 ml[U];
+      float x[U][V];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int p = p0 + i * step;
+        ml[i] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[i][k] = 0.0f;
+        if (p < parts) {
+          const bool pre = p >= own;
+          const Part& q = pre ? a.pre : p == 0 ? a.main : a.cta;
+          const int64_t at = pre ? (int64_t)(p - own) * a.n_rows + row
+                                 : p == 0 ? (int64_t)row : c_at + (int64_t)p * a.R;
+          ml[i] = q.ml[at];
+          if constexpr (V == 4) {
+            const float4 t = *reinterpret_cast<const float4*>(q.o + at * D + lane * V);
+            x[i][0] = t.x; x[i][1] = t.y; x[i][2] = t.z; x[i][3] = t.w;
+          } else {
+            const float2 t = *reinterpret_cast<const float2*>(q.o + at * D + lane * V);
+            x[i][0] = t.x; x[i][1] = t.y;
+          }
+        }
+      }
+      float m1 = mu, w1 = wu;
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        m1 = fmaxf(m1, ml[i].x);
+        w1 = fmaxf(w1, ml[i].z);
+      }
+      const float mb = base_of(m1), wb = base_of(w1), fm = ex2(mu - mb), fw = ex2(wu - wb);
+      sum *= fm;
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] *= fw;
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        sum += ex2(ml[i].x - mb) * ml[i].y;
+        const float f = ex2(ml[i].z - wb);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] += f * x[i][k];
+      }
+      mu = m1;
+      wu = w1;
     }
-    const float fm = ex2(mu - base_of(m1)), fw = ex2(wu - base_of(w1));
-    sum *= fm;
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] *= fw;
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      sum += ex2(ml[i].x - base_of(m1)) * ml[i].y;
-      const float f = ex2(ml[i].z - base_of(w1));
-#pragma unroll
-      for (int k = 0; k < V; ++k) v[k] += f * x[i][k];
+  }
+};
+
+__device__ __forceinline__ float lse_of(float mx, float sum) {
+  return sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * 0.69314718055994531f;
+}
+
+// RPB rows a block.  One: all warps share its parts, then add up in order.
+// kWarps: a warp a row, which needs no second step; a row of more than
+// kJoinAlone parts (one long sequence in a batch) still gets the whole block.
+// Many rows have few parts and cost instructions: 4096 rows of 10 parts take
+// 5 us less with a warp each (4608 rows of 7 to 10 parts the same).  Few rows
+// cost the chain of their parts: 64 rows of 28 parts 12 us more with a warp each.
+constexpr int kJoinAlone = 32;
+constexpr int64_t kJoinManyRows = 1024;
+template <int D, int RPB>
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(const JoinArgs a) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int V = D / 32;
+  __shared__ float sv[kWarps][D], sm[kWarps], ss[kWarps], sw[kWarps];
+  pdl_trigger();
+  pdl_wait();
+  int own;
+  int64_t c_at;
+  auto together = [&](uint32_t row, int parts) {
+    RowSum<D> r;
+    r.add(a, row, own, c_at, parts, warp, kWarps);
+    if (lane == 0) {
+      sm[warp] = r.mu;
+      ss[warp] = r.sum;
+      sw[warp] = r.wu;
     }
-    mu = m1;
-    wu = w1;
-  }
-  if (lane == 0) {
-    sm[warp] = mu;
-    ss[warp] = sum;
-    sw[warp] = wu;
-  }
 #pragma unroll
-  for (int k = 0; k < V; ++k) sv[warp][lane * V + k] = v[k];
-  __syncthreads();
-  if (threadIdx.x >= D / 2) return;
-  float mx = -INFINITY, mw = -INFINITY;
+    for (int k = 0; k < V; ++k) sv[warp][lane * V + k] = r.v[k];
+    __syncthreads();
+    if (threadIdx.x >= D / 2) return;
+    float mx = -INFINITY, mw = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    mx = fmaxf(mx, sm[w]);
-    mw = fmaxf(mw, sw[w]);
-  }
-  mx = base_of(mx);
-  mw = base_of(mw);
-  float total = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    for (int w = 0; w < kWarps; ++w) {
+      mx = fmaxf(mx, sm[w]);
+      mw = fmaxf(mw, sw[w]);
+    }
+    mx = base_of(mx);
+    mw = base_of(mw);
+    float total = 0.0f, o0 = 0.0f, o1 = 0.0f;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    total += ex2(sm[w] - mx) * ss[w];
-    const float f = ex2(sw[w] - mw);
-    o0 += f * sv[w][2 * threadIdx.x];
-    o1 += f * sv[w][2 * threadIdx.x + 1];
+    for (int w = 0; w < kWarps; ++w) {
+      total += ex2(sm[w] - mx) * ss[w];
+      const float f = ex2(sw[w] - mw);
+      o0 += f * sv[w][2 * threadIdx.x];
+      o1 += f * sv[w][2 * threadIdx.x + 1];
+    }
+    const float inv = total == 0.0f ? 0.0f : ex2(mw - mx) / total;
+    reinterpret_cast<uint32_t*>(a.out + (int64_t)row * D)[threadIdx.x] = bf2(o0 * inv, o1 * inv);
+    if (a.lse && threadIdx.x == 0) a.lse[row] = lse_of(mx, total);
+  };
+  if constexpr (RPB == 1) {
+    const int parts = RowSum<D>::count(a, blockIdx.x, own, c_at);
+    if (!(a.direct && own == 1)) together(blockIdx.x, parts);
+  } else {
+    const uint32_t row = blockIdx.x * RPB + warp;
+    bool split = false;
+    if (row < a.n_rows) {
+      const int parts = RowSum<D>::count(a, row, own, c_at);
+      split = parts > kJoinAlone;
+      if (!split && !(a.direct && own == 1)) {
+        RowSum<D> r;
+        r.add(a, row, own, c_at, parts, 0, 1);
+        const float mx = base_of(r.mu);
+        const float inv = r.sum == 0.0f ? 0.0f : ex2(base_of(r.wu) - mx) / r.sum;
+        uint32_t* o = reinterpret_cast<uint32_t*>(a.out + (int64_t)row * D) + lane * (V / 2);
+        if constexpr (V == 4)
+          *reinterpret_cast<uint2*>(o) = make_uint2(bf2(r.v[0] * inv, r.v[1] * inv),
+                                                    bf2(r.v[2] * inv, r.v[3] * inv));
+        else
+          *o = bf2(r.v[0] * inv, r.v[1] * inv);
+        if (a.lse && lane == 0) a.lse[row] = lse_of(mx, r.sum);
+      }
+    }
+    if (__syncthreads_or(split)) {
+      for (int w = 0; w < RPB; ++w) {
+        const uint32_t other = blockIdx.x * RPB + w;
+        if (other >= a.n_rows) break;
+        const int parts = RowSum<D>::count(a, other, own, c_at);
+        if (parts > kJoinAlone) {
+          __syncthreads();  // the row before is read
+          together(other, parts);
+        }
+      }
+    }
   }
-  const float inv = total == 0.0f ? 0.0f : ex2(mw - mx) / total;
-  reinterpret_cast<uint32_t*>(out + (int64_t)row * D)[threadIdx.x] = bf2(o0 * inv, o1 * inv);
-  if (lse && threadIdx.x == 0)
-    lse[row] = total == 0.0f ? -INFINITY : (mx + __log2f(total)) * 0.69314718055994531f;
 }
 
 // How a call is cut: column tiles of 8 query rows per CTA, CTAs for the
@@ -1151,11 +1214,16 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
     if (r != MXB_OK) return r;
   }
   if (p.join) {
-    MXB_CUDA_TRY(launch_pdl(
-        dim == 128 ? pattn::paged_join_kernel<128> : pattn::paged_join_kernel<64>,
-        dim3((unsigned)a.n_rows), pattn::kThreads, 0, st, own, cta, pre, a.plan,
-        p.ctas_own > 0 ? lengths : nullptr, width * page, p.splits_pre, a.n_rows, (int)T, heads,
-        group, p.tiles_own, 8 * p.nt_own, a.direct, a.out, lse));
+    pattn::JoinArgs j = {own, cta, pre, a.plan, p.ctas_own > 0 ? lengths : nullptr, width * page,
+                         a.n_rows, p.splits_pre, (int)T, heads, group, p.tiles_own, 8 * p.nt_own,
+                         a.direct, a.out, lse};
+    const bool many = a.n_rows >= pattn::kJoinManyRows;
+    auto kern = dim == 128 ? (many ? pattn::paged_join_kernel<128, pattn::kWarps>
+                                   : pattn::paged_join_kernel<128, 1>)
+                           : (many ? pattn::paged_join_kernel<64, pattn::kWarps>
+                                   : pattn::paged_join_kernel<64, 1>);
+    MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)(many ? cdiv(a.n_rows, pattn::kWarps) : a.n_rows)),
+                            pattn::kThreads, 0, st, j));
     MXB_LAUNCH_CHECK();
   }
   return MXB_OK;
