@@ -188,6 +188,13 @@ __device__ __forceinline__ float lg2(float x) {
 // 2^(x - ref) of a running maximum; nothing seen yet gives 0
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
 
+// What turns a weighted sum relative to 2^mw into the output: 2^(mw - m) / sum.
+// No weight seen (no keys, or value scales of zero): the sum is 0 already, and
+// without a reference the power could be infinite.
+__device__ __forceinline__ float norm_of(float m, float mw, float sum) {
+  return mw == -INFINITY ? 0.0f : ex2(mw - base_of(m)) / sum;
+}
+
 // Two codes as 16-bit floats.  K: int8 bytes 0 and 2 of w -> fp16 1152 + code
 // ((code + 128) in the mantissa of 1024); int4 low nibbles of both halves ->
 // bf16 136 + code ((code + 8) in the mantissa of 128).  V: exact fp16 codes;
@@ -779,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
       const int t = rr / a.G, hh = cu / a.row_tiles;
       const int64_t id = ((int64_t)bb * a.T + t) * ((int64_t)a.H * a.G) + (int64_t)hh * a.G + (rr - t * a.G);
       if (direct) {
-        const float inv = sum == 0.0f ? 0.0f : ex2(wu - mu) / sum;
+        const float inv = norm_of(mx, mw, sum);
         *reinterpret_cast<uint2*>(a.out + id * D + d) =
             make_uint2(bf2(v.x * inv, v.y * inv), bf2(v.z * inv, v.w * inv));
         if (a.lse && d == 0)
@@ -929,6 +936,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const JoinArgs a) 
       mx = fmaxf(mx, sm[w]);
       mw = fmaxf(mw, sw[w]);
     }
+    const float mt = mx, wt = mw;
     mx = base_of(mx);
     mw = base_of(mw);
     float total = 0.0f, o0 = 0.0f, o1 = 0.0f;
@@ -939,7 +947,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const JoinArgs a) 
       o0 += f * sv[w][2 * threadIdx.x];
       o1 += f * sv[w][2 * threadIdx.x + 1];
     }
-    const float inv = total == 0.0f ? 0.0f : ex2(mw - mx) / total;
+    const float inv = norm_of(mt, wt, total);
     reinterpret_cast<uint32_t*>(a.out + (int64_t)row * D)[threadIdx.x] = bf2(o0 * inv, o1 * inv);
     if (a.lse && threadIdx.x == 0) a.lse[row] = lse_of(mx, total);
   };
@@ -955,15 +963,14 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const JoinArgs a) 
       if (!split && !(a.direct && own == 1)) {
         RowSum<D> r;
         r.add(a, row, own, c_at, parts, 0, 1);
-        const float mx = base_of(r.mu);
-        const float inv = r.sum == 0.0f ? 0.0f : ex2(base_of(r.wu) - mx) / r.sum;
+        const float inv = norm_of(r.mu, r.wu, r.sum);
         uint32_t* o = reinterpret_cast<uint32_t*>(a.out + (int64_t)row * D) + lane * (V / 2);
         if constexpr (V == 4)
           *reinterpret_cast<uint2*>(o) = make_uint2(bf2(r.v[0] * inv, r.v[1] * inv),
                                                     bf2(r.v[2] * inv, r.v[3] * inv));
         else
           *o = bf2(r.v[0] * inv, r.v[1] * inv);
-        if (a.lse && lane == 0) a.lse[row] = lse_of(mx, r.sum);
+        if (a.lse && lane == 0) a.lse[row] = lse_of(base_of(r.mu), r.sum);
       }
     }
     if (__syncthreads_or(split)) {

@@ -335,6 +335,24 @@ def test_attention_of_short_sequences_beside_a_long_one(dtype, T, group, prefix)
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths,width,prefix", [([70, 3], 2, 0), ([300, 1], 60, 0), ([70, 3], 2, 100),
+                                                  ([70] * 130, 2, 0), ([70] * 130, 2, 100)])
+def test_attention_of_zero_values_under_low_scores(lengths, width, prefix):
+    """Value scales of zero leave no weight in range, wherever the scores lie."""
+    c = pool(64, 2, 128, "int8d", 64, 5)
+    c.v_scales.zero_()
+    c.k_codes.fill_(100)
+    c.k_scales.fill_(1.0)
+    q = torch.full((len(lengths), 1, 8, 128), -1.0, device="cuda").bfloat16()
+    table = torch.arange(width, device="cuda", dtype=torch.int32).repeat(len(lengths), 1)
+    n = torch.tensor(lengths, device="cuda")
+    out, lse = mxb.paged_attention(q, c, table, n, prefix_table=table[0], prefix_len=prefix, return_lse=True)
+    assert not bool(out.any())
+    want = torch.log(n + float(prefix)) - 100 * math.sqrt(128)
+    assert torch.allclose(lse, want[:, None, None].expand_as(lse).float(), rtol=1e-5, atol=0)
+
+
+@pytest.mark.gpu
 def test_attention_scores_that_grow_and_values_of_any_scale():
     """Keys whose scores rise along the sequence move the running maximum again
     and again; value scales over six decades stay exact beside one another."""
