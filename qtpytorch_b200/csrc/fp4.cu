@@ -90,6 +90,24 @@ __device__ __forceinline__ void ld32b(const void* p, uint32_t (&r)[8]) {
                : "l"(p));
 }
 
+// i / d by a product with 2^(31 + s) / d rounded up, exact for i < 2^31 (the
+// rounding adds less than 2^s >= d to it).  A division costs some twenty
+// instructions beside about 200 for the rest of 16 elements.
+struct Div {
+  uint32_t d, m, s;  // m = 0: divide
+  __device__ __forceinline__ uint32_t operator()(uint32_t i) const { return m ? __umulhi(i, m) >> s : i / d; }
+};
+Div div_by(uint32_t d, uint64_t top) {
+  Div r = {d, 0, 0};
+  if (d < 2 || top > (uint64_t)1 << 31) return r;
+  uint32_t l = 1;
+  while (l < 31 && ((uint64_t)1 << l) < d) ++l;
+  if (((uint64_t)1 << l) < d) return r;
+  r.m = (uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d);
+  r.s = l - 1;
+  return r;
+}
+
 // Up to 16 elements of a row from column c0 on; zero past K.  vec: rows are
 // 32-byte aligned.
 template <typename InT>
@@ -126,7 +144,7 @@ __device__ __forceinline__ void load16(const InT* __restrict__ row, int64_t c0, 
 constexpr int kAmaxBlocks = 6 * kSMs;
 template <typename InT>
 __global__ void __launch_bounds__(kThreads) fp4_amax_kernel(const InT* __restrict__ x, int64_t K,
-                                                            int64_t ldx, uint32_t gpr,
+                                                            int64_t ldx, Div gpr,
                                                             uint32_t items, bool vec,
                                                             float* __restrict__ part) {
   pdl_trigger();
@@ -138,7 +156,7 @@ __global__ void __launch_bounds__(kThreads) fp4_amax_kernel(const InT* __restric
 #pragma unroll
     for (int h = 0; h < 2; ++h) {  // two in flight
       const uint64_t j = i + h * step < items ? i + h * step : i;
-      const uint32_t r = (uint32_t)j / gpr, c = (uint32_t)j - r * gpr;
+      const uint32_t r = gpr((uint32_t)j), c = (uint32_t)j - r * gpr.d;
       load16(x + (int64_t)r * ldx, (int64_t)c * kE, K, vec, v[h]);
     }
 #pragma unroll
@@ -196,7 +214,7 @@ __device__ __forceinline__ float cluster_amax(const InT* __restrict__ x, uint32_
 // from the end of the tensor, whose rows the maximum pass left in L2.
 template <typename InT, int FMT>
 __global__ void __launch_bounds__(kThreads)
-    fp4_quant_kernel(const InT* __restrict__ x, uint32_t rows, int64_t K, int64_t ldx, uint32_t gpr,
+    fp4_quant_kernel(const InT* __restrict__ x, uint32_t rows, int64_t K, int64_t ldx, Div gpr,
                      uint32_t items, uint32_t pad_words, uint32_t groups, bool vec,
                      const float* __restrict__ part, int parts, float* __restrict__ gscale,
                      uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
@@ -223,9 +241,10 @@ __global__ void __launch_bounds__(kThreads)
   };
   float next[kE];
   auto fetch = [&](uint32_t blk0) {  // the values of a later item
-    const uint64_t i = blk0 < blocks ? item_of(blk0) : items;
+    if (blk0 >= blocks) return;
+    const uint64_t i = item_of(blk0);
     if (i < items) {
-      const uint32_t r = (uint32_t)i / gpr, c = (uint32_t)i - r * gpr;
+      const uint32_t r = gpr((uint32_t)i), c = (uint32_t)i - r * gpr.d;
       load16(x + (int64_t)r * ldx, (int64_t)c * kE, K, vec, next);
     } else {
 #pragma unroll
@@ -241,7 +260,7 @@ __global__ void __launch_bounds__(kThreads)
       const uint32_t r = rows + w / groups;
       *reinterpret_cast<uint32_t*>(scales + sf_offset(r, w % groups, groups)) = 0u;
     }
-    const uint32_t r = mine ? (uint32_t)i / gpr : 0u, c = mine ? (uint32_t)i - r * gpr : 0u;
+    const uint32_t r = mine ? gpr((uint32_t)i) : 0u, c = mine ? (uint32_t)i - r * gpr.d : 0u;
     float v[kE];
 #pragma unroll
     for (int j = 0; j < kE; ++j) v[j] = next[j];
@@ -315,7 +334,7 @@ __device__ __forceinline__ void st32b(void* p, const uint32_t (&r)[8]) {
 template <typename OutT, int FMT>
 __global__ void __launch_bounds__(kThreads)
     fp4_dequant_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                       const float* __restrict__ gscale, int64_t K, uint32_t cpr, uint32_t items,
+                       const float* __restrict__ gscale, int64_t K, Div cpr, uint32_t items,
                        uint32_t groups, bool vec, OutT* __restrict__ out) {
   constexpr int kU = 2;
   constexpr int kPerBlk = FMT == MXB_FP4_NV ? 1 : 2;  // items per scale
@@ -332,7 +351,7 @@ __global__ void __launch_bounds__(kThreads)
     w[u] = make_uint2(0u, 0u);
     sb[u] = rr[u] = cc[u] = 0u;
     if (i < items) {
-      const uint32_t r = (uint32_t)i / cpr, c = (uint32_t)i - r * cpr;
+      const uint32_t r = cpr((uint32_t)i), c = (uint32_t)i - r * cpr.d;
       w[u] = __ldg(reinterpret_cast<const uint2*>(codes + (size_t)r * rb + (size_t)c * 8));
       const uint32_t blk = c / kPerBlk;
       sb[u] = __ldg(scales + sf_offset(r, blk >> 2, groups) + (blk & 3));
@@ -396,7 +415,7 @@ int quantize_t(const InT* x, int64_t rows, int64_t K, int64_t ldx, int fmt, floa
     const int64_t blocks = cdiv(aitems, kThreads);
     parts = (int)(blocks < kAmaxBlocks ? blocks : kAmaxBlocks);
     MXB_CUDA_TRY(launch_pdl(fp4_amax_kernel<InT>, dim3((unsigned)parts), kThreads, 0, st, x, K, ldx,
-                            (uint32_t)agpr, (uint32_t)aitems, vec, part));
+                            div_by((uint32_t)agpr, aitems), (uint32_t)aitems, vec, part));
     MXB_LAUNCH_CHECK();
   }
   auto kern = fmt == MXB_FP4_NV ? fp4_quant_kernel<InT, MXB_FP4_NV> : fp4_quant_kernel<InT, MXB_FP4_MX>;
@@ -420,7 +439,7 @@ int quantize_t(const InT* x, int64_t rows, int64_t K, int64_t ldx, int fmt, floa
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = small ? 2 : 1;
-  MXB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, x, (uint32_t)rows, K, ldx, (uint32_t)gpr, (uint32_t)items,
+  MXB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, x, (uint32_t)rows, K, ldx, div_by((uint32_t)gpr, items), (uint32_t)items,
                                   (uint32_t)pad, (uint32_t)groups, vec,
                                   (const float*)(derive && !small ? part : nullptr), parts, g, codes,
                                   scales));
@@ -439,7 +458,7 @@ int dequantize_t(const uint8_t* codes, const uint8_t* scales, const float* g, in
   auto kern = fmt == MXB_FP4_NV ? fp4_dequant_kernel<OutT, MXB_FP4_NV>
                                 : fp4_dequant_kernel<OutT, MXB_FP4_MX>;
   MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)grid), kThreads, 0, st, codes, scales, g, K,
-                          (uint32_t)cpr, (uint32_t)items, (uint32_t)groups, vec, out));
+                          div_by((uint32_t)cpr, items), (uint32_t)items, (uint32_t)groups, vec, out));
   MXB_LAUNCH_CHECK();
   return MXB_OK;
 }
