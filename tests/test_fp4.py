@@ -191,6 +191,24 @@ def test_quantize_codes_scales_values(fmt, dtype, rows, K):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("rows,K", [(700, 1001), (700, 1002), (700, 1004), (700, 1000), (2, 1), (1100, 3)])
+def test_rows_of_every_alignment(fmt, rows, K):
+    x = special(rows, K, rows + K)
+    x[rows - 1, K - 1] = 9.0  # the last value is the largest of nvfp4's blocks
+    if rows > 3:
+        x[3] = 1.0
+    for s in (x.cuda(), torch.cat((x, x[:, :1]), 1).cuda()[:, :K]):  # rows with a gap as well
+        t = mxb.fp4_tensor.quantize(s, fmt)
+        code, byte, g = ref_quantize(x.numpy(), fmt)
+        assert np.array_equal(unpacked(t)[0], code)
+        assert fmt == "mxfp4" or t.global_scale.item() == g
+        v = ref_values(code, byte, fmt, g, K)
+        assert np.array_equal(t.dequantize().cpu().numpy(), v)
+        assert torch.equal(t.dequantize(torch.bfloat16).cpu(), torch.from_numpy(v).bfloat16())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
 def test_quantize_infinities_and_nan_stay_in_their_block(fmt):
     x = torch.randn(4, 96, generator=torch.Generator().manual_seed(3))
     x[1, 40], x[2, 3], x[3, 95] = float("inf"), float("nan"), float("-inf")
