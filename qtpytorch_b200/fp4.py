@@ -59,7 +59,11 @@ class fp4_tensor:
     row-major, byte ((r % 32) * 4 + r // 32) * 4 + c of a tile, zero past the
     matrix.  ``global_scale``: fp32 [1] on the device (nvfp4) or None."""
 
-    __slots__ = ("fmt", "shape", "device", "_parts", "_ptrs")
+    # _parts: (codes, scales, global_scale), or (buffer, rows, bytes of codes, offset
+    # and bytes of scales, offset of the factor or the factor) as quantize made it.
+    # Device and addresses are read off the tensors at each call, so that a copied,
+    # unpickled or remapped object works on its own memory.
+    __slots__ = ("fmt", "shape", "_parts")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str, shape,
                  global_scale: Optional[torch.Tensor] = None):
@@ -83,9 +87,8 @@ class fp4_tensor:
         if codes.device != scales.device or (global_scale is not None
                                              and global_scale.device != codes.device):
             raise ValueError("fp4_tensor: codes, scales and global_scale are on different devices")
-        self.fmt, self.shape, self.device = fmt, shape, codes.device
+        self.fmt, self.shape = fmt, shape
         self._parts = (codes, scales, global_scale)
-        self._ptrs = (codes.data_ptr(), scales.data_ptr(), L.ptr(global_scale))
 
     @classmethod
     def quantize(cls, x: torch.Tensor, fmt: str = "mxfp4",
@@ -135,10 +138,22 @@ class fp4_tensor:
         elif derive:
             buf[at_g:at_g + 4].view(torch.float32).fill_(1.0)
         self = cls.__new__(cls)
-        self.fmt, self.shape, self.device = fmt, shape, dev
+        self.fmt, self.shape = fmt, shape
         self._parts = (buf, rows, cb, at_s, sb, at_g if derive else global_scale)
-        self._ptrs = (base, base + at_s, gp)
         return self
+
+    @property
+    def device(self) -> torch.device:
+        return self._parts[0].device
+
+    def _ptrs(self):
+        """Addresses of codes, scales and factor (0: none)."""
+        parts = self._parts
+        if len(parts) == 3:
+            return parts[0].data_ptr(), parts[1].data_ptr(), L.ptr(parts[2])
+        buf, _, _, at_s, _, g = parts
+        base = buf.data_ptr()
+        return base, base + at_s, base + g if isinstance(g, int) else L.ptr(g)
 
     def _views(self):
         if len(self._parts) != 3:
@@ -170,7 +185,7 @@ class fp4_tensor:
         _require_cuda(dev, "fp4_tensor.dequantize")
         rows, K = shape[:-1].numel(), shape[-1]
         out = torch.empty(shape, dtype=dtype, device=dev)
-        rc = L.call("mxb_fp4_dequantize", dev, *self._ptrs, rows, K, FORMATS[self.fmt],
+        rc = L.call("mxb_fp4_dequantize", dev, *self._ptrs(), rows, K, FORMATS[self.fmt],
                     out.data_ptr(), io)
         if rc:
             L.check(rc, f"mxb_fp4_dequantize({self.fmt}, {rows}x{K})")
@@ -216,7 +231,7 @@ def fp4_matmul(a: fp4_tensor, b: fp4_tensor, bias: Optional[torch.Tensor] = None
     if K == 0:  # an empty sum
         out.zero_()
         return out if bias is None else out.add_(bias)
-    rc = L.call("mxb_fp4_matmul", dev, *a._ptrs, *b._ptrs, M, K, N, FORMATS[a.fmt], L.ptr(bias),
+    rc = L.call("mxb_fp4_matmul", dev, *a._ptrs(), *b._ptrs(), M, K, N, FORMATS[a.fmt], L.ptr(bias),
                 out.data_ptr(), _IO[out_dtype])
     if rc:
         L.check(rc, f"mxb_fp4_matmul({M}x{K}x{N}, {a.fmt})")

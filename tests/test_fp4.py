@@ -5,7 +5,10 @@ the bound of fp32 accumulation against 64 bits; refusals.
 The reference has no counterpart (its float4 grid, mxtorch.py:1465-1528, is
 another format).
 """
+import copy
 import ctypes
+import io
+import pickle
 
 import numpy as np
 import pytest
@@ -147,6 +150,41 @@ def test_refusals():
         mxb.fp4_matmul(t, t, out_dtype=torch.float16)
     with pytest.raises(L.MxbError):
         mxb.fp4_matmul(t, t)
+
+
+def one_buffer(fmt, rows=3, K=40):
+    """An fp4_tensor as ``quantize`` leaves it (one allocation), on the host."""
+    cb, sb = rows * fp4.code_row_bytes(K), fp4.scale_bytes(rows, K, fmt)
+    at_s = -(-cb // 256) * 256
+    nv = fmt == "nvfp4"
+    t = mxb.fp4_tensor.__new__(mxb.fp4_tensor)
+    t.fmt, t.shape = fmt, torch.Size((rows, K))
+    t._parts = (torch.arange(at_s + sb + 16 * nv, dtype=torch.int64).to(torch.uint8), rows, cb, at_s, sb,
+                at_s + sb if nv else None)
+    return t
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("viewed", [False, True])
+def test_copies_own_their_addresses(fmt, viewed):
+    """A copied, pickled or saved tensor hands the kernels its own memory, on the
+    device that this memory is on."""
+    t = one_buffer(fmt)
+    buf = io.BytesIO()
+    torch.save(t, buf)
+    buf.seek(0)
+    if viewed:
+        t.codes
+    for u in (copy.deepcopy(t), pickle.loads(pickle.dumps(t)), torch.load(buf, weights_only=False)):
+        g = u.global_scale
+        assert u._ptrs() == (u.codes.data_ptr(), u.scales.data_ptr(), 0 if g is None else g.data_ptr())
+        assert not set(u._ptrs()[:2]) & set(t._ptrs()[:2]) and u.device == u.codes.device
+        assert torch.equal(u.codes, t.codes) and torch.equal(u.scales, t.scales) and u.shape == t.shape
+    same = copy.copy(t)
+    assert same._ptrs() == t._ptrs() == (t.codes.data_ptr(), t.scales.data_ptr(),
+                                         0 if fmt == "mxfp4" else t.global_scale.data_ptr())
+    buf.seek(0)
+    assert torch.load(buf, map_location="meta", weights_only=False).device.type == "meta"
 
 
 # ── quantize ─────────────────────────────────────────────────────────────────
