@@ -142,6 +142,16 @@ class fp4_tensor:
         self._parts = (buf, rows, cb, at_s, sb, at_g if derive else global_scale)
         return self
 
+    def __copy__(self) -> "fp4_tensor":
+        other = type(self).__new__(type(self))
+        other.fmt, other.shape, other._parts = self.fmt, self.shape, self._parts
+        return other
+
+    def __reduce__(self):
+        # the factor in a storage of its own: torch.save takes no storage under two types
+        codes, scales, g = self._views()
+        return type(self), (codes, scales, self.fmt, tuple(self.shape), None if g is None else g.clone())
+
     @property
     def device(self) -> torch.device:
         return self._parts[0].device
@@ -249,7 +259,9 @@ class fp4_linear(nn.Module):
         self.fmt, self.out_dtype = weight.fmt, out_dtype
         self.register_buffer("weight_codes", weight.codes)
         self.register_buffer("weight_scales", weight.scales)
-        self.register_buffer("weight_global_scale", weight.global_scale)
+        # in a storage of its own: torch.save takes no storage under two types
+        g = weight.global_scale
+        self.register_buffer("weight_global_scale", None if g is None else g.clone())
         self.register_buffer("bias", None if bias is None else bias.detach().float())
 
     @classmethod

@@ -187,6 +187,27 @@ def test_copies_own_their_addresses(fmt, viewed):
     assert torch.load(buf, map_location="meta", weights_only=False).device.type == "meta"
 
 
+def saved(x):
+    buf = io.BytesIO()
+    torch.save(x, buf)
+    buf.seek(0)
+    return torch.load(buf, weights_only=False)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_saved_after_its_parts_were_read(fmt):
+    """The parts of one allocation go through torch.save: as a tensor, as a
+    module's state and as a module."""
+    t = one_buffer(fmt)
+    t.codes
+    m = mxb.fp4_linear(t)
+    sd, u, n = saved(m.state_dict()), saved(t), saved(m)
+    for w in (u, n.weight, mxb.fp4_tensor(sd["weight_codes"], sd["weight_scales"], fmt, t.shape,
+                                          sd.get("weight_global_scale"))):
+        assert torch.equal(w.codes, t.codes) and torch.equal(w.scales, t.scales)
+        assert fmt == "mxfp4" or w.global_scale.view(torch.int32).equal(t.global_scale.view(torch.int32))
+
+
 # ── quantize ─────────────────────────────────────────────────────────────────
 def special(rows, K, seed):
     """Normal values, with exact ties, zeros, a zero block, tiny and huge blocks."""
