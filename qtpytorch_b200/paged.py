@@ -76,11 +76,22 @@ class paged_kv_cache:
             raise ValueError(f"paged_kv_cache: page_size must be a power of two from 16 to 1024, not {page}")
         if n_pages < 1 or heads < 1 or n_pages * heads * page >= 2 ** 31:
             raise ValueError("paged_kv_cache: needs pages and heads, fewer than 2^31 head rows")
-        self.k_codes, self.k_scales, self.v_codes, self.v_scales = kc, ks, vc, vs
+        self._buffers = (kc, ks, vc, vs)
         self.dtype, self.n_pages, self.n_heads = dt, n_pages, heads
         self.page_size, self.head_dim = page, dim
-        self.device = kc.device
-        self._pool = (kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr())
+
+    # The buffers are checked once, so they are not replaced; device and
+    # addresses are read off them at each call, so that a copied, unpickled or
+    # remapped cache works on its own memory.
+    k_codes = property(lambda self: self._buffers[0])
+    k_scales = property(lambda self: self._buffers[1])
+    v_codes = property(lambda self: self._buffers[2])
+    v_scales = property(lambda self: self._buffers[3])
+    device = property(lambda self: self._buffers[0].device)
+
+    def _pool(self):
+        kc, ks, vc, vs = self._buffers
+        return kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()
 
     def _cuda(self, what: str) -> torch.device:
         L.require_cuda(self.k_codes, what)
@@ -107,7 +118,7 @@ class paged_kv_cache:
             slots = slots.to(torch.int64).contiguous()
         rc = L.call("mxb_kv_write", dev, k.data_ptr(), v.data_ptr(), _IO[k.dtype], k.shape[0], H, D,
                     k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(),
-                    self.n_pages, self.page_size, self.dtype.bits, *self._pool)
+                    self.n_pages, self.page_size, self.dtype.bits, *self._pool())
         if rc:
             L.check(rc, f"mxb_kv_write({self.dtype.name}, T={k.shape[0]})")
 
@@ -123,7 +134,7 @@ class paged_kv_cache:
             raise ValueError("read: max_len must not be negative")
         B = table.shape[0]
         k, v = torch.empty((2, B, max_len, self.n_heads, self.head_dim), dtype=dtype, device=dev).unbind()
-        rc = L.call("mxb_kv_read", dev, *self._pool, self.n_pages, self.n_heads, self.page_size,
+        rc = L.call("mxb_kv_read", dev, *self._pool(), self.n_pages, self.n_heads, self.page_size,
                     self.head_dim, self.dtype.bits, table.data_ptr(), table.shape[1],
                     lengths.data_ptr(), B, max_len, k.data_ptr(), v.data_ptr(), _IO[dtype])
         if rc:
@@ -202,7 +213,7 @@ def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
                  cache.page_size, table.shape[1], prefix_len)
     ws = L.workspace(wsb, dev)
     rc = L.call("mxb_paged_attention", dev, q.data_ptr(), B, T, H, Hq // H, D,
-                *cache._pool, cache.n_pages, cache.page_size, cache.dtype.bits,
+                *cache._pool(), cache.n_pages, cache.page_size, cache.dtype.bits,
                 table.data_ptr(), table.shape[1], lengths.data_ptr(),
                 prefix_table.data_ptr() if prefix_len else 0, width, prefix_len,
                 1.0 / math.sqrt(D) if scale is None else float(scale), out.data_ptr(), L.ptr(lse),

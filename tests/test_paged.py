@@ -5,9 +5,12 @@ that hold NaN, strides, offsets past 32 bits; refusals.
 The cache's codes and scales are those of ``mx_tensor.quantize`` with block =
 head_dim (mxtorch.py:1426-1463); attention has no counterpart in the reference.
 """
+import copy
 import ctypes
+import io
 import math
 import os
+import pickle
 import sys
 
 import numpy as np
@@ -79,6 +82,28 @@ def test_refusals():
         c.read(torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), 4)
     with pytest.raises(L.MxbError):
         mxb.paged_attention(torch.zeros(1, 1, 2, 64), c, torch.zeros(1, 1), torch.zeros(1))
+
+
+def test_copies_own_their_addresses():
+    """A copied, pickled or saved cache hands the kernels its own memory, on the
+    device that this memory is on."""
+    c = mxb.paged_kv_cache(4, 2, 64, "int4d", 16, device="cpu")
+    c.k_codes.random_(0, 256)
+    buf = io.BytesIO()
+    torch.save(c, buf)
+    buf.seek(0)
+
+    def addresses(x):
+        return tuple(t.data_ptr() for t in (x.k_codes, x.k_scales, x.v_codes, x.v_scales))
+
+    for d in (copy.deepcopy(c), pickle.loads(pickle.dumps(c)), torch.load(buf, weights_only=False)):
+        assert d._pool() == addresses(d) and not set(d._pool()) & set(c._pool())
+        assert torch.equal(d.k_codes, c.k_codes) and d.page_size == 16 and d.dtype.bits == 4
+    assert c._pool() == addresses(c) == copy.copy(c)._pool()
+    buf.seek(0)
+    assert torch.load(buf, map_location="meta", weights_only=False).device.type == "meta"
+    with pytest.raises(AttributeError):
+        c.k_codes = c.k_codes[:1]  # a smaller pool behind the geometry that was checked
 
 
 @pytest.mark.gpu
