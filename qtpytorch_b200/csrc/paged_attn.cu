@@ -800,6 +800,9 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
       }
     }
     if (!more) break;
+    // where the join buffer lies over the rings, its ordinary stores come before
+    // the copies (async proxy) of the next unit to the same bytes
+    if (!Ge::kApart) fence_proxy_async_shared();
     __syncthreads();  // the join buffer is read
     if (!Ge::kApart) fill();
   }

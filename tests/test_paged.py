@@ -472,6 +472,27 @@ def test_attention_repeats_on_any_stream_and_in_a_graph():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,group,T", [
+    ("int8d", 128, 4, 1), ("int8d", 128, 8, 2), ("int8d", 64, 8, 3), ("int4d", 128, 8, 3), ("int4d", 128, 8, 4)])
+def test_attention_of_several_units_in_a_row_repeats(dtype, dim, group, T):
+    """A CTA takes unit after unit, and the next unit's keys are copied over the
+    buffer that the last one's rows were joined in."""
+    lengths = [(29 * i) % 150 for i in range(150)]
+    width = -(-4200 // 32)  # longer than one unit a CTA is used for
+    c = pool(600, 4, dim, dtype, 32, 11)
+    table = torch.randint(0, 600, (len(lengths), width), generator=torch.Generator().manual_seed(5),
+                          dtype=torch.int32).cuda()
+    q = torch.randn(len(lengths), T, 4 * group, dim, generator=torch.Generator().manual_seed(6)).cuda().bfloat16()
+    n = torch.tensor(lengths, device="cuda")
+    out, lse = mxb.paged_attention(q, c, table, n, return_lse=True)
+    check_attention(out, lse, q, c, table, lengths, None, 0)
+    for _ in range(20):
+        again, _ = mxb.paged_attention(q, c, table, n, return_lse=True)
+        assert torch.equal(again, out)
+    assert L.load().mxb_device_error(1) == 0
+
+
+@pytest.mark.gpu
 def test_attention_bad_tables_are_recorded():
     c = pool(4, 1, 64, "int8d", 16, 1)
     q = torch.randn(1, 1, 2, 64, device="cuda").bfloat16()
