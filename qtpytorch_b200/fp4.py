@@ -273,6 +273,16 @@ class fp4_linear(nn.Module):
         bias = None if linear.bias is None else linear.bias.data.to(w.device)
         return cls(fp4_tensor.quantize(w, fmt), bias, out_dtype)
 
+    def _apply(self, fn, *args, **kwargs):
+        # casts of the whole model (.bfloat16(), .half(), .to(dtype)) move these two but
+        # leave them fp32: the factor belongs to the codes bit for bit
+        kept = {n: self._buffers[n] for n in ("weight_global_scale", "bias")}
+        super()._apply(fn, *args, **kwargs)
+        for n, t in kept.items():
+            if t is not None and self._buffers[n].dtype != torch.float32:
+                self._buffers[n] = t.to(self._buffers[n].device)
+        return self
+
     @property
     def weight(self) -> fp4_tensor:
         return fp4_tensor(self.weight_codes, self.weight_scales, self.fmt,

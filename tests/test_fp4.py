@@ -208,6 +208,23 @@ def test_saved_after_its_parts_were_read(fmt):
         assert fmt == "mxfp4" or w.global_scale.view(torch.int32).equal(t.global_scale.view(torch.int32))
 
 
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("cast", [lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.double(),
+                                  lambda m: m.to(torch.bfloat16), lambda m: m.to("cpu", torch.half)])
+def test_linear_module_casts_leave_the_weight_alone(fmt, cast):
+    t = one_buffer(fmt, 5, 64)
+    bias = torch.randn(5, generator=torch.Generator().manual_seed(0))
+    if fmt == "nvfp4":
+        t = mxb.fp4_tensor(t.codes, t.scales, fmt, t.shape, torch.tensor([0.1234567]))
+    m = cast(torch.nn.Sequential(torch.nn.Linear(64, 64), mxb.fp4_linear(t, bias)))
+    w = m[1].weight  # raises where the factor's type changed
+    assert m[0].weight.dtype != torch.float32
+    assert torch.equal(w.codes, t.codes) and torch.equal(w.scales, t.scales)
+    assert fmt == "mxfp4" or torch.equal(w.global_scale, t.global_scale)
+    assert m[1].bias.dtype == torch.float32 and torch.equal(m[1].bias, bias)
+    assert m.to("meta")[1].weight.device.type == "meta" and m[1].bias.dtype == torch.float32
+
+
 # ── quantize ─────────────────────────────────────────────────────────────────
 def special(rows, K, seed):
     """Normal values, with exact ties, zeros, a zero block, tiny and huge blocks."""
