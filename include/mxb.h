@@ -474,7 +474,7 @@ size_t mxb_paged_attention_workspace_size(int64_t B, int64_t T, int heads, int g
  *           zero for a row without keys
  *   lse     [B][T][heads * group] fp32 log of the sum of exponentials (-inf
  *           for a row without keys), or NULL
- * A page number outside the pool reads page 0 and a length past the table is
+ * A page number outside the pool holds no keys and a length past the table is
  * cut, both recorded (mxb_device_error: 8).
  */
 int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim,

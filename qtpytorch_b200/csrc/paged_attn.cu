@@ -373,15 +373,17 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
   // page numbers are fetched one tile before the copies that need them
   auto page_of = [&](int tile) -> int {
     const int pos = tile * kTile + (lane << a.box_shift);
-    if (lane >= boxes || tile >= t_hi || pos >= len) return -1;
-    int p = __ldg(table + (pos >> a.page_shift));
-    if (p < 0 || p >= a.n_pages) {
-      if (a.err) atomicCAS(a.err, 0, kErrIndex);
-      p = 0;
-    }
-    return p;
+    return lane < boxes && tile < t_hi && pos < len ? __ldg(table + (pos >> a.page_shift)) : 0;
   };
+  // Keys behind a number outside the pool are not copied and hidden from every
+  // row: once the warp has met one, each tile looks its numbers up again (below).
+  bool bad_pages = false;
   auto issue = [&](int tile, int h, int s, int p) {
+    const bool used = lane < boxes && tile * kTile + (lane << a.box_shift) < len;
+    const bool bad = used && (uint32_t)p >= (uint32_t)a.n_pages;  // n_pages < 2^31
+    if (bad && a.err) atomicCAS(a.err, 0, kErrIndex);
+    bad_pages = __any_sync(0xffffffffu, bad) || bad_pages;
+    if (!used || bad) p = -1;
     uint64_t* bar = &full[warp][s];
     if (lane < boxes) {
       if (p >= 0) {
@@ -614,7 +616,17 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
       // One column tile after the other, to keep few values alive; the two
       // columns of an accumulator pair go through packed operations.
       const int key0 = tile * kTile + g;
-      const bool ragged = (tile + 1) * kTile > lim_min;  // some key is hidden from some row
+      bool ragged = (tile + 1) * kTile > lim_min;  // some key is hidden from some row
+      uint32_t hide = 0;  // 16-key halves of the tile behind bad page numbers
+      if (bad_pages) {
+        ragged = true;
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          const int key = tile * kTile + 16 * i;
+          const int p = key < len ? __ldg(table + (key >> a.page_shift)) : 0;
+          hide |= ((uint32_t)p >= (uint32_t)a.n_pages ? 1u : 0u) << i;
+        }
+      }
       uint32_t pb[2][NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -630,8 +642,9 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float2 v = unpack2(v2[i]), w = unpack2(w2[i]);
-            if (key0 + 8 * i >= limit[n][0]) v.x = w.x = -INFINITY;  // whatever its scales hold
-            if (key0 + 8 * i >= limit[n][1]) v.y = w.y = -INFINITY;
+            const int key = (hide >> (i >> 1)) & 1u ? INT32_MAX : key0 + 8 * i;
+            if (key >= limit[n][0]) v.x = w.x = -INFINITY;  // whatever its scales hold
+            if (key >= limit[n][1]) v.y = w.y = -INFINITY;
             v2[i] = pack2(v.x, v.y);
             w2[i] = pack2(w.x, w.y);
           }

@@ -73,6 +73,7 @@ struct Bars {
   uint64_t scready[kSlots];
   uint64_t qready;
   uint32_t tmem_base;
+  uint32_t gone[kStages];  // bit i: keys 16 i .. of the tile lie behind a number outside the pool
 };
 static_assert(sizeof(Bars) <= 512, "barrier block overflows its slot");
 
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
   Bars* bars = reinterpret_cast<Bars*>(smem + C::oBars);
   float* sc_slots = reinterpret_cast<float*>(smem + C::oSc);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int boxes = KT / box;
+  const int boxes = KT / box, box_shift = 31 - __clz(box);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -220,11 +221,14 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
         p = __ldg(a.table + (pos >> a.page_shift));
         if (p < 0 || p >= a.n_pages) {
           if (a.err) atomicCAS(a.err, 0, kErrIndex);
-          p = 0;
+          p = -2;
         }
       }
+      const int p16 = __shfl_sync(0xffffffffu, p, lane >> (box_shift - 4));
+      const uint32_t gone = __ballot_sync(0xffffffffu, lane < KT / 16 && p16 == -2);
       if (round > 0 && !mbar_wait_warp_to(&bars->raw_empty[s], (round - 1) & 1, kErrTimeoutEmpty, a.err))
         break;
+      if (lane == 0) bars->gone[s] = gone;  // before its arrival
       if (lane < boxes) {
         uint64_t* bar = &bars->raw_full[s];
         if (p >= 0) {
@@ -301,8 +305,13 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
       {
         // scales: every warp finds the tile's largest value scale for itself
         const int valid = a.len - (t_lo + i) * KT;
-        const float v0 = lane < valid ? rsc[KT + lane] : 0.0f;
-        const float v1 = lane + 32 < valid ? rsc[KT + lane + 32] : 0.0f;
+        const uint32_t gone = bars->gone[s];
+        float v0 = lane < valid ? rsc[KT + lane] : 0.0f;
+        float v1 = lane + 32 < valid ? rsc[KT + lane + 32] : 0.0f;
+        if (gone) {  // nothing was copied for these keys
+          if (gone >> (lane >> 4) & 1u) v0 = 0.0f;
+          if (gone >> (2 + (lane >> 4)) & 1u) v1 = 0.0f;
+        }
         float mx = fmaxf(v0, v1);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -317,7 +326,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
           sl[j] = j < valid ? rsc[j] * a.scale_log2 : 0.0f;
           sl[KT + j] = (warp == 2 ? v0 : v1) * (kRoom / c);
         } else if (warp == 4 && lane == 0) {
-          sl[2 * KT] = c;
+          *reinterpret_cast<float2*>(sl + 2 * KT) = make_float2(c, __uint_as_float(gone));
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->scready[slot]);
@@ -416,6 +425,13 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
         }
       }
       const int valid = a.len - (t_lo + t) * KT;
+      const float2 cg = *reinterpret_cast<const float2*>(sc_slots + slot * (2 * KT + 4) + 2 * KT);
+      const uint32_t gone = __float_as_uint(cg.y);
+      if (gone) {
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+          if (gone >> (j >> 4) & 1u) v[j] = -INFINITY;
+      }
       if (valid < KT) {
 #pragma unroll
         for (int j = 0; j < KT; ++j)
@@ -425,7 +441,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
 #pragma unroll
       for (int j = 4; j < KT; ++j) m4[j & 3] = fmaxf(m4[j & 3], v[j]);
       const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * rowf;
-      const float cn = sc_slots[slot * (2 * KT + 4) + 2 * KT];
+      const float cn = cg.x;
       bool waited = t == 0;
       if (__any_sync(0xffffffffu, mx > m_top || cn != c)) {
         const float m0 = m_top == -INFINITY ? -INFINITY : mu;

@@ -176,7 +176,8 @@ def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
     lengths[b] - (T - 1 - t).  ``prefix_table`` [pages] and ``prefix_len`` name
     keys that every query sees in front of its own; they are read once for the
     whole batch.  ``scale`` defaults to 1 / sqrt(head_dim).  A row without keys
-    gives zeros.  Returns out (q's shape, bf16), with ``return_lse`` also the fp32
+    gives zeros; a page number outside the pool holds no keys (recorded in the
+    library's device error word).  Returns out (q's shape, bf16), with ``return_lse`` also the fp32
     log-sum-exp [B, T, Hq] of the scaled scores."""
     dev = cache._cuda("paged_attention")
     H, D = cache.n_heads, cache.head_dim

@@ -508,6 +508,38 @@ def test_attention_bad_tables_are_recorded():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,page,group,B,spare", [
+    ("int8d", 128, 16, 4, 3, 0), ("int4d", 64, 64, 8, 3, 0),                 # a unit a CTA
+    ("int8d", 64, 32, 4, 3, 300), ("int4d", 128, 128, 8, 3, 60),             # the shared list
+    ("int8d", 128, 16, 8, 40, 0), ("int4d", 64, 32, 8, 40, 0), ("int4d", 128, 128, 8, 40, 0)])  # many rows
+def test_attention_sees_no_keys_behind_bad_pages(dtype, dim, page, group, B, spare):
+    """A page number outside the pool holds no keys, as in ``read``: the call gives
+    what it gives without those pages, and page 0 is no stand-in."""
+    c = pool(16, 2, dim, dtype, page, 12)
+    c.k_scales[0] *= 20
+    c.v_scales[0] *= 100
+    rest = [0] * spare
+    bad = torch.tensor([[4, 10 ** 6, 5, -7, 6, 7, 9] + rest] * B, device="cuda", dtype=torch.int32)
+    good = torch.tensor([[4, 5, 6, 7, 9] + rest] * B, device="cuda", dtype=torch.int32)
+    q = torch.randn(B, 1, 2 * group, dim, generator=torch.Generator().manual_seed(1)).cuda().bfloat16()
+    n = [5 * page + 3] * B
+    L.load().mxb_device_error(1)
+    for own in (False, True):
+        for pre in ((False, True) if own else (True,)):
+            length = torch.tensor(n if own else [0] * B, device="cuda")
+            out, lse = mxb.paged_attention(q, c, bad, length, prefix_table=bad[0], prefix_len=n[0] * pre,
+                                           return_lse=True)
+            assert L.load().mxb_device_error(1) == 8
+            less = n[0] - 2 * page
+            check_attention(out, lse, q, c, good, [less * own] * B, good[0], less * pre)
+    none = torch.full_like(bad, 16)
+    out, lse = mxb.paged_attention(q, c, none, torch.tensor(n, device="cuda"), prefix_table=none[0],
+                                   prefix_len=n[0], return_lse=True)
+    assert not out.any() and bool((lse == float("-inf")).all())
+    assert L.load().mxb_device_error(1) == 8
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """A pool of 5.4 GB of codes each for K and V: the last page works like the first."""
     pages, heads, dim, page = 41000, 8, 128, 128
