@@ -16,10 +16,14 @@
 //                 weights back to TMEM over S.
 // Scores: Q is fp16 under a power of two per row that puts its largest value
 // into [2^14, 2^15), the codes are exact.  Weights: p_j = exp2(s_j - m) times
-// sv_j / c, c a power of two of at least the largest value scale so far; with
-// 2^6 of room above and m following the maximum within 2^8, fp16 keeps 11 bits
-// of every weight down to 2^-20 of the largest possible one.  m, sums and
-// outputs are fp32; O is rescaled in TMEM only when m or c moves.
+// 2^6 sv_j / c, c a power of two of at least the largest value scale so far, and m
+// following the maximum within 2^8.  While the value scales span less than 2^-11
+// of c, a row's largest weight is at least 2^-5, so fp16 keeps 11 bits of those
+// down to 2^-9 of it and is off by 2^-20 of it below.  From the first tile with a
+// wider span on, c is each row's own and follows its largest weight, as that
+// may belong to a key whose value scale is far under another's (a wide tile
+// costs one more multiplication and comparison a score).  m, sums and outputs
+// are fp32; O is rescaled in TMEM only when m or c moves.
 // Pairs of codes unpack out of order; Q's columns are stored in the same
 // order and O's columns are put back when they are written.
 //
@@ -47,6 +51,7 @@ constexpr int kStages = 3;
 constexpr int kSlots = 4;  // scale slots: softmax may lag the unpacking by two tiles
 constexpr int kConvWarps = 4;
 constexpr float kRoom = 64.0f;  // 2^6
+constexpr float kWide = 0x1p-11f;  // of c: scales below make a tile wide
 
 template <int BITS, int D, int MT>
 struct Cfg {
@@ -158,6 +163,181 @@ __device__ __forceinline__ void unpack_tile(const uint8_t* raw, uint8_t* plane, 
       *reinterpret_cast<uint4*>(plane + (ch >> 3) * kAtom + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = o[k];
     }
   }
+}
+
+// A row of the softmax: reference and sum; lc, log2 of the c that its O stands
+// under; top_w, log2 of the largest weight stored (kept for wide tiles).
+struct Row {
+  float mu = 0.0f, m_top = -INFINITY, l = 0.0f, lc = 0.0f, top_w = -5.0f;
+  bool ok = true;
+};
+struct RowTiles {
+  Bars* bars;
+  const float* sc_slots;
+  uint32_t tmem;  // S of this warp's rows; O follows after 128 columns
+  int x, lane, keys;  // row group; keys of the run
+  float rowf;
+  int* err;
+};
+
+// One tile of 64 keys; false where a wait gave up, or at the first wide tile (W:
+// this one may be wide).
+template <int D, bool W>
+__device__ __forceinline__ bool softmax_tile(Row& r, const RowTiles& g, int t) {
+  const int b = t & 1, slot = t % kSlots;
+  r.ok = mbar_wait_warp_to(&g.bars->scready[slot], (t / kSlots) & 1, kErrTimeoutFull, g.err) &&
+       mbar_wait_warp_to(&g.bars->sready[g.x][b], (t >> 1) & 1, kErrTimeoutTmemFull, g.err);
+  if (!r.ok) return false;
+  const float4 of_tile = *reinterpret_cast<const float4*>(g.sc_slots + slot * (2 * KT + 4) + 2 * KT);
+  const float lcn = of_tile.x;
+  const uint32_t gone = __float_as_uint(of_tile.y);
+  if (!W && __float_as_uint(of_tile.z) != 0u) return false;
+  tc_fence_after();
+  float v[KT];
+  {
+    uint32_t r0v[32], r1v[32];
+    tmem_ld32(g.tmem + b * 64, r0v);
+    tmem_ld32(g.tmem + b * 64 + 32, r1v);
+    tmem_wait_ld();
+    tmem_landed(r0v);
+    tmem_landed(r1v);
+    const float4* ks = reinterpret_cast<const float4*>(g.sc_slots + slot * (2 * KT + 4));
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 k0 = ks[j / 4], k1 = ks[8 + j / 4];
+      v[j] = __uint_as_float(r0v[j]) * k0.x;
+      v[j + 1] = __uint_as_float(r0v[j + 1]) * k0.y;
+      v[j + 2] = __uint_as_float(r0v[j + 2]) * k0.z;
+      v[j + 3] = __uint_as_float(r0v[j + 3]) * k0.w;
+      v[32 + j] = __uint_as_float(r1v[j]) * k1.x;
+      v[33 + j] = __uint_as_float(r1v[j + 1]) * k1.y;
+      v[34 + j] = __uint_as_float(r1v[j + 2]) * k1.z;
+      v[35 + j] = __uint_as_float(r1v[j + 3]) * k1.w;
+    }
+  }
+  const int valid = g.keys - t * KT;
+  if (gone) {
+#pragma unroll
+    for (int j = 0; j < KT; ++j)
+      if (gone >> (j >> 4) & 1u) v[j] = -INFINITY;
+  }
+  if (valid < KT) {
+#pragma unroll
+    for (int j = 0; j < KT; ++j)
+      if (j >= valid) v[j] = -INFINITY;
+  }
+  float m4[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int j = 4; j < KT; ++j) m4[j & 3] = fmaxf(m4[j & 3], v[j]);
+  const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * g.rowf;
+  const float4* vs = reinterpret_cast<const float4*>(g.sc_slots + slot * (2 * KT + 4) + KT);
+  bool waited = t == 0;
+  float alpha = 1.0f, dm = 0.0f;
+  if (t == 0) {
+    r.lc = lcn;
+    r.top_w = -INFINITY;
+  }
+  bool rescale = mx > r.m_top || (!W && lcn != r.lc);
+  if (__any_sync(0xffffffffu, rescale)) {
+    const float m0 = r.m_top == -INFINITY ? -INFINITY : r.mu;
+    const float m1 = fmaxf(m0, mx);
+    r.mu = m1 == -INFINITY ? 0.0f : m1;
+    dm = m0 - r.mu;
+    alpha = ex2(dm);
+    r.l *= alpha;
+    r.m_top = m1 + 8.0f;
+    if (!W) {
+      alpha *= ex2(r.lc - lcn);
+      r.lc = lcn;
+    }
+    rescale = true;
+  }
+  uint32_t pk[32];
+  float s0 = 0.0f, s1 = 0.0f;
+  if (W) {
+    // the weights first, then a c for this row that puts its largest so far
+    // between 2^-2 and 2^12
+    float u4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < KT; j += 4) {
+      const float4 w = vs[j / 4];
+      const float p0 = ex2(__fmaf_rn(v[j], g.rowf, -r.mu)), p1 = ex2(__fmaf_rn(v[j + 1], g.rowf, -r.mu));
+      const float p2 = ex2(__fmaf_rn(v[j + 2], g.rowf, -r.mu)), p3 = ex2(__fmaf_rn(v[j + 3], g.rowf, -r.mu));
+      s0 += p0 + p2;
+      s1 += p1 + p3;
+      v[j] = p0 * w.x;
+      v[j + 1] = p1 * w.y;
+      v[j + 2] = p2 * w.z;
+      v[j + 3] = p3 * w.w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) u4[k] = fmaxf(u4[k], v[j + k]);
+    }
+    const float u = fmaxf(fmaxf(u4[0], u4[1]), fmaxf(u4[2], u4[3]));
+    r.top_w = fminf(fmaxf(r.top_w + dm, log2f(u) + (lcn - r.lc)), 200.0f);
+    const bool off = r.top_w > 12.0f || (r.top_w < -2.0f && r.top_w > -INFINITY) || lcn - r.lc > 120.0f;
+    if (__any_sync(0xffffffffu, off)) {
+      if (off) {
+        // no further below the tile's c than 2^120: fp32 holds little under that
+        const float up = fminf(6.0f - floorf(r.top_w), 120.0f - (lcn - r.lc));
+        r.lc -= up;
+        r.top_w += up;
+        alpha *= ex2(up);
+      }
+      rescale = true;
+    }
+    const float up = ex2(lcn - r.lc);
+#pragma unroll
+    for (int j = 0; j < KT; j += 2) pk[j / 2] = hf2(v[j] * up, v[j + 1] * up);
+  }
+  if (rescale && t > 0) {
+    // O of the tiles before has to be complete; the next product waits
+    // for this tile's weights
+    r.ok = mbar_wait_warp_to(&g.bars->pvdone[g.x], (t - 1) & 1, kErrTimeoutTmemEmpty, g.err);
+    if (!r.ok) return false;
+    waited = true;
+    tc_fence_after();
+#pragma unroll 1
+    for (int d = 0; d < D; d += 32) {
+      uint32_t o[32];
+      tmem_ld32(g.tmem + 128 + d, o);
+      tmem_wait_ld();
+      tmem_landed(o);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+      tmem_st32(g.tmem + 128 + d, o);
+    }
+  }
+  if (!W) {
+#pragma unroll
+    for (int j = 0; j < KT; j += 4) {
+      const float4 w = vs[j / 4];
+      const float p0 = ex2(__fmaf_rn(v[j], g.rowf, -r.mu)), p1 = ex2(__fmaf_rn(v[j + 1], g.rowf, -r.mu));
+      const float p2 = ex2(__fmaf_rn(v[j + 2], g.rowf, -r.mu)), p3 = ex2(__fmaf_rn(v[j + 3], g.rowf, -r.mu));
+      s0 += p0 + p2;
+      s1 += p1 + p3;
+      pk[j / 2] = hf2(p0 * w.x, p1 * w.y);
+      pk[j / 2 + 1] = hf2(p2 * w.z, p3 * w.w);
+    }
+  }
+  r.l += s0 + s1;
+  // every phase of pvdone is waited for in turn: a parity tells only the
+  // last completed phase from the one before it
+  if (!waited) {
+    r.ok = mbar_wait_warp_to(&g.bars->pvdone[g.x], (t - 1) & 1, kErrTimeoutTmemEmpty, g.err);
+    if (!r.ok) return false;
+  }
+  tmem_st32(g.tmem + b * 64, pk);
+  tmem_wait_st();
+  tc_fence_before();
+  __syncwarp();
+  if (g.lane == 0) mbar_arrive(&g.bars->pready[g.x][b]);
+  return true;
+}
+// The wide tiles, apart: in line they cost a call whose tiles are all narrow 2 us of 69.
+template <int D>
+__device__ __noinline__ Row wide_tiles(Row r, const RowTiles w, int t, int n) {
+  while (t < n && softmax_tile<D, true>(r, w, t)) ++t;
+  return r;
 }
 
 template <int BITS, int D, int MT>
@@ -296,6 +476,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
   } else if (warp < 2 + kConvWarps) {
     const int t = threadIdx.x - 64;
     float c = 0.0f;  // power of two above every value scale so far (0: none)
+    uint32_t least = 0x7F800000u;  // bits of the smallest so far
     for (int i = 0; i < n; ++i) {
       const int s = i % kStages, b = i & 1, slot = i % kSlots;
       if (!mbar_wait_warp_to(&bars->raw_full[s], (i / kStages) & 1, kErrTimeoutFull, a.err)) break;
@@ -312,21 +493,25 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
           if (gone >> (lane >> 4) & 1u) v0 = 0.0f;
           if (gone >> (2 + (lane >> 4)) & 1u) v1 = 0.0f;
         }
-        float mx = fmaxf(v0, v1);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        // bits of non-negative floats rise with them (no NaN passes the fmaxf)
+        const float mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(v0, v1), 0.0f))));
         if (mx > c || c == 0.0f) {
           // four times the next power of two, between 2^-100 and 2^100
           const int ex = min(max((int)(__float_as_uint(mx) >> 23) + 3, 27), 227);
           c = __uint_as_float((uint32_t)ex << 23);
         }
+        least = min(least, __reduce_min_sync(0xffffffffu, min(lane < valid ? __float_as_uint(v0) : least,
+                                                              lane + 32 < valid ? __float_as_uint(v1) : least)));
         float* sl = sc_slots + slot * (2 * KT + 4);
         if (warp < 4) {  // the first two of these warps: 32 keys each
           const int j = (warp - 2) * 32 + lane;
           sl[j] = j < valid ? rsc[j] * a.scale_log2 : 0.0f;
           sl[KT + j] = (warp == 2 ? v0 : v1) * (kRoom / c);
         } else if (warp == 4 && lane == 0) {
-          *reinterpret_cast<float2*>(sl + 2 * KT) = make_float2(c, __uint_as_float(gone));
+          const bool wide = __uint_as_float(least) < c * kWide;
+          *reinterpret_cast<float4*>(sl + 2 * KT) =
+              make_float4((float)((int)(__float_as_uint(c) >> 23) - 127), __uint_as_float(gone),
+                          __uint_as_float(wide), 0.0f);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->scready[slot]);
@@ -394,130 +579,32 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->qready);
     }
-    float mu = 0.0f, m_top = -INFINITY, l = 0.0f, c = 1.0f;
-    bool ok = true;
-    for (int t = 0; t < n; ++t) {
-      const int b = t & 1, slot = t % kSlots;
-      ok = mbar_wait_warp_to(&bars->scready[slot], (t / kSlots) & 1, kErrTimeoutFull, a.err) &&
-           mbar_wait_warp_to(&bars->sready[x][b], (t >> 1) & 1, kErrTimeoutTmemFull, a.err);
-      if (!ok) break;
-      tc_fence_after();
-      float v[KT];
-      {
-        uint32_t r0v[32], r1v[32];
-        tmem_ld32(t_s(x, b) + lane_sel, r0v);
-        tmem_ld32(t_s(x, b) + lane_sel + 32, r1v);
-        tmem_wait_ld();
-        tmem_landed(r0v);
-        tmem_landed(r1v);
-        const float4* ks = reinterpret_cast<const float4*>(sc_slots + slot * (2 * KT + 4));
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 k0 = ks[j / 4], k1 = ks[8 + j / 4];
-          v[j] = __uint_as_float(r0v[j]) * k0.x;
-          v[j + 1] = __uint_as_float(r0v[j + 1]) * k0.y;
-          v[j + 2] = __uint_as_float(r0v[j + 2]) * k0.z;
-          v[j + 3] = __uint_as_float(r0v[j + 3]) * k0.w;
-          v[32 + j] = __uint_as_float(r1v[j]) * k1.x;
-          v[33 + j] = __uint_as_float(r1v[j + 1]) * k1.y;
-          v[34 + j] = __uint_as_float(r1v[j + 2]) * k1.z;
-          v[35 + j] = __uint_as_float(r1v[j + 3]) * k1.w;
-        }
-      }
-      const int valid = a.len - (t_lo + t) * KT;
-      const float2 cg = *reinterpret_cast<const float2*>(sc_slots + slot * (2 * KT + 4) + 2 * KT);
-      const uint32_t gone = __float_as_uint(cg.y);
-      if (gone) {
-#pragma unroll
-        for (int j = 0; j < KT; ++j)
-          if (gone >> (j >> 4) & 1u) v[j] = -INFINITY;
-      }
-      if (valid < KT) {
-#pragma unroll
-        for (int j = 0; j < KT; ++j)
-          if (j >= valid) v[j] = -INFINITY;
-      }
-      float m4[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-      for (int j = 4; j < KT; ++j) m4[j & 3] = fmaxf(m4[j & 3], v[j]);
-      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * rowf;
-      const float cn = cg.x;
-      bool waited = t == 0;
-      if (__any_sync(0xffffffffu, mx > m_top || cn != c)) {
-        const float m0 = m_top == -INFINITY ? -INFINITY : mu;
-        const float m1 = fmaxf(m0, mx);
-        mu = m1 == -INFINITY ? 0.0f : m1;
-        const float am = ex2(m0 - mu);
-        l *= am;
-        if (t > 0) {
-          // O of the tiles before has to be complete; the next product waits
-          // for this tile's weights
-          ok = mbar_wait_warp_to(&bars->pvdone[x], (t - 1) & 1, kErrTimeoutTmemEmpty, a.err);
-          if (!ok) break;
-          waited = true;
-          tc_fence_after();
-          const float alpha = am * (c / cn);
-#pragma unroll 1
-          for (int d = 0; d < D; d += 32) {
-            uint32_t r[32];
-            tmem_ld32(t_o(x) + lane_sel + d, r);
-            tmem_wait_ld();
-            tmem_landed(r);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-            tmem_st32(t_o(x) + lane_sel + d, r);
-          }
-        }
-        m_top = m1 + 8.0f;
-        c = cn;
-      }
-      const float4* vs = reinterpret_cast<const float4*>(sc_slots + slot * (2 * KT + 4) + KT);
-      uint32_t pk[32];
-      float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-      for (int j = 0; j < KT; j += 4) {
-        const float4 w = vs[j / 4];
-        const float p0 = ex2(__fmaf_rn(v[j], rowf, -mu)), p1 = ex2(__fmaf_rn(v[j + 1], rowf, -mu));
-        const float p2 = ex2(__fmaf_rn(v[j + 2], rowf, -mu)), p3 = ex2(__fmaf_rn(v[j + 3], rowf, -mu));
-        s0 += p0 + p2;
-        s1 += p1 + p3;
-        pk[j / 2] = hf2(p0 * w.x, p1 * w.y);
-        pk[j / 2 + 1] = hf2(p2 * w.z, p3 * w.w);
-      }
-      l += s0 + s1;
-      // every phase of pvdone is waited for in turn: a parity tells only the
-      // last completed phase from the one before it
-      if (!waited) {
-        ok = mbar_wait_warp_to(&bars->pvdone[x], (t - 1) & 1, kErrTimeoutTmemEmpty, a.err);
-        if (!ok) break;
-      }
-      tmem_st32(t_s(x, b) + lane_sel, pk);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->pready[x][b]);
-    }
+    Row r;
+    const RowTiles w = {bars, sc_slots, t_s(x, 0) + lane_sel, x, lane, a.len - t_lo * KT, rowf, a.err};
+    int t = 0;
+    while (t < n && softmax_tile<D, false>(r, w, t)) ++t;
+    if (t < n && r.ok) r = wide_tiles<D>(r, w, t, n);  // the scales' range only grows
     // ── this split's part ──
-    if (ok && n > 0) ok = mbar_wait_warp_to(&bars->pvdone[x], (n - 1) & 1, kErrTimeoutDone, a.err);
+    if (r.ok && n > 0) mbar_wait_warp_to(&bars->pvdone[x], (n - 1) & 1, kErrTimeoutDone, a.err);
     tc_fence_after();
     const int64_t pr = (int64_t)blockIdx.x * a.n_rows + id;
 #pragma unroll 1
     for (int d = 0; d < D; d += 32) {
-      uint32_t r[32];
+      uint32_t v[32];
       if (n > 0) {
-        tmem_ld32(t_o(x) + lane_sel + d, r);
+        tmem_ld32(t_o(x) + lane_sel + d, v);
         tmem_wait_ld();
-        tmem_landed(r);
+        tmem_landed(v);
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) r[i] = 0u;
+        for (int i = 0; i < 32; ++i) v[i] = 0u;
       }
       if (live) {
 #pragma unroll
         for (int g8 = 0; g8 < 32; g8 += 8) {
           float o[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o[order<BITS>(i)] = __uint_as_float(r[g8 + i]);
+          for (int i = 0; i < 8; ++i) o[order<BITS>(i)] = __uint_as_float(v[g8 + i]);
           // a whole 32-byte sector a lane
           asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(
                            a.o + pr * D + d + g8),
@@ -528,11 +615,10 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
       }
     }
     if (live) {
-      // O = 2^m' sum: m' = m + log2(c / room), c a power of two
-      const float lc = (float)((int)(__float_as_uint(c) >> 23) - 127) - 6.0f;
+      // O = 2^m' sum: m' = m + log2(c / room)
       reinterpret_cast<float4*>(a.ml)[pr] =
-          m_top == -INFINITY ? make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f)
-                             : make_float4(mu, l, mu + lc, 0.0f);
+          r.m_top == -INFINITY ? make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f)
+                             : make_float4(r.mu, r.l, r.mu + (r.lc - 6.0f), 0.0f);
     }
   }
   tc_fence_before();

@@ -540,6 +540,39 @@ def test_attention_sees_no_keys_behind_bad_pages(dtype, dim, page, group, B, spa
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["int8d", "int4d"])
+@pytest.mark.parametrize("B", [2, 12, 24])  # groups of 32 rows; 128-row tiles, one and two
+@pytest.mark.parametrize("exponent", [-10, -20, -24, -40, -60])
+@pytest.mark.parametrize("loud", [[3], [700], [1499], [64, 900]])
+def test_attention_of_quiet_values_beside_loud_ones(dtype, B, exponent, loud):
+    """Rows that rest on keys whose value scale lies far under another's, which
+    they hardly see: the weights are held relative to the row's largest, so each
+    is off by 2^-11 of itself or 2^-24 of that."""
+    c = pool(24, 1, 128, dtype, 64, 13)
+    top = 127 if dtype == "int8d" else 7
+    c.v_scales.mul_(2.0 ** exponent)
+    for j in loud:
+        c.k_codes[j // 64, 0, j % 64] = 0x81 if dtype == "int8d" else 0x99  # -127, -7 and -7
+        c.k_scales[j // 64, 0, j % 64] = 6.0 / top
+        c.v_scales[j // 64, 0, j % 64] = 1.0
+    g = torch.Generator("cuda").manual_seed(3)
+    q = (1 + 0.5 * torch.randn(B, 1, 8, 128, generator=g, device="cuda")).bfloat16()
+    pre = torch.arange(24, device="cuda", dtype=torch.int32)
+    own, n, prefix = pre[None, :1].repeat(B, 1), [0] * B, 1500
+    out, _ = mxb.paged_attention(q, c, own, torch.tensor(n, device="cuda"), prefix_table=pre,
+                                 prefix_len=prefix, return_lse=True)
+    out64, _, mag = attend64(q, c, own, n, pre, prefix, 128 ** -0.5)
+    k, v = (history(c, w, pre, prefix)[0] for w in "kv")
+    p = torch.softmax(torch.einsum("bgd,ld->bgl", q[:, 0].double(), k) * 128 ** -0.5, -1)
+    largest = (p * c.v_scales[:, 0].flatten()[:prefix].double()).amax(-1)[:, None, :, None]
+    off = 1152 + 127 if dtype == "int8d" else 136 + 8
+    e_s = ((128 / 16 + 4) * 2.0 ** -23 * off * q.double().abs().sum(-1) * c.k_scales.max().double()
+           * 128 ** -0.5 * 1.4427 + 2.0 ** -22)[..., None]
+    tol = (2.0 ** -11 + 4 * e_s + 2.0 ** -20) * mag + 2.0 ** -8 * out64.abs() + prefix * 2.0 ** -24 * 128 * largest
+    assert bool(((out.double() - out64).abs() <= tol).all())
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """A pool of 5.4 GB of codes each for K and V: the last page works like the first."""
     pages, heads, dim, page = 41000, 8, 128, 128
