@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
     if (live) {
       // O = 2^m' sum: m' = m + log2(c / room)
       reinterpret_cast<float4*>(a.ml)[pr] =
-          r.m_top == -INFINITY ? make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f)
+          r.m_top == -INFINITY ? make_float4(-INFINITY, r.l, -INFINITY, 0.0f)  // l: 0, or of NaN scores
                              : make_float4(r.mu, r.l, r.mu + (r.lc - 6.0f), 0.0f);
     }
   }

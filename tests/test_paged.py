@@ -573,6 +573,25 @@ def test_attention_of_quiet_values_beside_loud_ones(dtype, B, exponent, loud):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["int8d", "int4d"])
+@pytest.mark.parametrize("B", [1, 12, 40])
+def test_attention_nan_query_has_a_nan_sum(dtype, B):
+    """A NaN query's log-sum-exp is NaN, behind a prefix alone as with keys of its
+    own; the other rows are untouched."""
+    c = pool(4, 1, 64, dtype, 64, 14)
+    q = torch.randn(B, 1, 8, 64, generator=torch.Generator().manual_seed(2)).cuda().bfloat16()
+    q[0, 0, 3, 5] = float("nan")
+    pre = torch.arange(4, device="cuda", dtype=torch.int32)
+    for n in (0, 20):
+        out, lse = mxb.paged_attention(q, c, pre[None, :1].repeat(B, 1), torch.full((B,), n, device="cuda"),
+                                       prefix_table=pre, prefix_len=200, return_lse=True)
+        want = torch.zeros(B, 1, 8, dtype=torch.bool, device="cuda")
+        want[0, 0, 3] = True
+        assert torch.equal(lse.isnan(), want) and torch.equal(out.isnan().all(-1), want)
+        assert torch.equal(out.isnan().any(-1), want)
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """A pool of 5.4 GB of codes each for K and V: the last page works like the first."""
     pages, heads, dim, page = 41000, 8, 128, 128
