@@ -284,12 +284,13 @@ __global__ void __launch_bounds__(kThreads)
       const float s = __fmul_rn(e4m3_value(sb), g);
       if (s >= 7.9e-31f && s <= 1.2e30f) {
         // x / s by Markstein's corrected product (r correctly rounded, the
-        // residual exact in an FMA): three operations instead of a division
+        // residual exact in an FMA): three operations instead of a division.  The
+        // residual is taken as q0 s - x: for x = -0 that is +0, and -0 stays -0.
         const float rs = __frcp_rn(s);
 #pragma unroll
         for (int j = 0; j < kE; ++j) {
           const float q0 = __fmul_rn(v[j], rs);
-          q[j] = __fmaf_rn(__fmaf_rn(-q0, s, v[j]), rs, q0);
+          q[j] = __fmaf_rn(-__fmaf_rn(q0, s, -v[j]), rs, q0);
         }
       } else {
 #pragma unroll

@@ -315,6 +315,17 @@ def test_quantize_factor_rules():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_keeps_the_sign_of_zero(fmt, dtype):
+    x = torch.randn(40, 100, generator=torch.Generator().manual_seed(6)).to(dtype)
+    x[:, ::3], x[:, 1::6] = -0.0, 0.0
+    t = mxb.fp4_tensor.quantize(x.cuda(), fmt)
+    code, _, _ = ref_quantize(x.float().numpy(), fmt)
+    assert np.array_equal(unpacked(t)[0], code)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
 def test_quantize_strides_types_and_empty(fmt):
     base = torch.randn(9, 3, 80, generator=torch.Generator().manual_seed(2)).cuda()
     want = mxb.fp4_tensor.quantize(base[:, 1].contiguous(), fmt)
