@@ -282,11 +282,12 @@ __global__ void __launch_bounds__(kThreads)
     } else {
       sb = e4m3_of(fminf(__fdiv_rn(a, __fmul_rn(6.0f, g)), 448.0f));
       const float s = __fmul_rn(e4m3_value(sb), g);
-      if (s >= 7.9e-31f && s <= 1.2e30f) {
+      const float rs = __frcp_rn(s);
+      // (under a given factor far too small a quotient may pass fp32's range)
+      if (s >= 7.9e-31f && s <= 1.2e30f && __fmul_rn(a, rs) <= 3.4028235e38f) {
         // x / s by Markstein's corrected product (r correctly rounded, the
         // residual exact in an FMA): three operations instead of a division.  The
         // residual is taken as q0 s - x: for x = -0 that is +0, and -0 stays -0.
-        const float rs = __frcp_rn(s);
 #pragma unroll
         for (int j = 0; j < kE; ++j) {
           const float q0 = __fmul_rn(v[j], rs);

@@ -325,6 +325,19 @@ def test_quantize_keeps_the_sign_of_zero(fmt, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("g", [1e-20, 1e-25, 1e-30, 2e-33])
+def test_quantize_under_a_factor_far_too_small_saturates(g):
+    """Quotients past fp32 go to 6 with their sign, like smaller ones."""
+    x = torch.randn(20, 96, generator=torch.Generator().manual_seed(7))
+    x *= 10.0 ** torch.arange(-20, 40, 3)[:, None].float().clamp(max=37)
+    t = mxb.fp4_tensor.quantize(x.cuda(), "nvfp4", torch.tensor([g], device="cuda"))
+    with np.errstate(over="ignore"):
+        code, byte, _ = ref_quantize(x.numpy(), "nvfp4", F32(g))
+    assert np.array_equal(unpacked(t)[0], code)
+    assert np.array_equal(t.block_scales().cpu().numpy(), byte)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
 def test_quantize_strides_types_and_empty(fmt):
     base = torch.randn(9, 3, 80, generator=torch.Generator().manual_seed(2)).cuda()
