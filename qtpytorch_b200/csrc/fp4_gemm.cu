@@ -300,8 +300,23 @@ __global__ void __launch_bounds__(kThreads, 2)
   const bool epi = warp >= 2 && warp < 2 + kEpiWarps;
   const int q = warp & 3, half = (warp - 2) >> 2;  // TMEM lane quarter, column half
   constexpr int kPer = NT >= 64 ? 32 : NT / 2;     // columns per tcgen05.ld
-  float factor = 1.0f;
-  if (FMT == MXB_FP4_NV) factor = __fmul_rn(*a.fg, *a.tg);
+  // the factors' product, and a power of two for where it leaves the range that
+  // keeps it and its products with the sums normal (a sum of zero times an
+  // infinite factor would be NaN, a subnormal one has few bits)
+  float factor = 1.0f, post = 1.0f;
+  if (FMT == MXB_FP4_NV) {
+    const float ga = *a.fg, gb = *a.tg;
+    factor = __fmul_rn(ga, gb);
+    if (!(factor >= 0x1p-90f && factor <= 0x1p90f)) {
+      const bool low = factor < 1.0f;
+      factor = low ? __fmul_rn(__fmul_rn(fminf(ga, gb), 0x1p120f), fmaxf(ga, gb))
+                   : __fmul_rn(__fmul_rn(fmaxf(ga, gb), 0x1p-120f), fminf(ga, gb));
+      post = low ? 0x1p-120f : 0x1p120f;
+    }
+  }
+  auto scaled = [&](float sum) {
+    return FMT == MXB_FP4_NV ? __fmul_rn(__fmul_rn(sum, factor), post) : sum;
+  };
   OutT* out = static_cast<OutT*>(a.out);
   if (a.splits == 1) {
     if (epi && mbar_wait_warp_to(&bars->acc, 0, kErrTimeoutDone, a.err)) {
@@ -322,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int j = 0; j < kPer; ++j)
             if (m0 + c0 + j < a.M)
-              store1(o + (size_t)j * a.N, __fadd_rn(__fmul_rn(__uint_as_float(r[j]), factor), bv));
+              store1(o + (size_t)j * a.N, __fadd_rn(scaled(__uint_as_float(r[j])), bv));
         }
       }
     }
@@ -361,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (n0 + f + j < a.N)
-          store1(o + j, __fadd_rn(__fmul_rn(e[j], factor), a.bias ? a.bias[n0 + f + j] : 0.0f));
+          store1(o + j, __fadd_rn(scaled(e[j]), a.bias ? a.bias[n0 + f + j] : 0.0f));
     }
     cluster_sync();  // the partial tiles are read: the CTAs may go
   }

@@ -407,6 +407,25 @@ def test_product_nan_stays_in_its_row_and_column():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 200])
+@pytest.mark.parametrize("sx,sw", [(1e-18, 1e-18), (3e-19, 1e-17), (1e-30, 1e-6), (1e25, 1e25), (1e30, 1e15), (1e36, 1e-36)])
+def test_product_of_factors_past_the_range(m, sx, sw):
+    """Two nvfp4 factors whose product leaves fp32's normal range: the result is
+    as near as any other where it lies in that range, and zeros stay zeros."""
+    g = torch.Generator("cuda").manual_seed(1)
+    x = torch.rand(m, 64, generator=g, device="cuda").add_(0.5).mul_(sx)
+    w = torch.rand(130, 64, generator=g, device="cuda").add_(0.5).mul_(sw)
+    x[1], w[129] = 0.0, 0.0
+    a, b = mxb.fp4_tensor.quantize(x, "nvfp4"), mxb.fp4_tensor.quantize(w, "nvfp4")
+    y = mxb.fp4_matmul(a, b, out_dtype=torch.float32)
+    y64 = a.dequantize().double() @ b.dequantize().double().t()
+    fits = y64 < 3e38
+    # one rounding an addition and each of the factors' products, all terms positive
+    assert bool(((y.double() - y64).abs() <= (64 + 6) * 2.0 ** -23 * y64)[fits].all())
+    assert bool(y[~fits].isinf().all()) and not y[1].any() and not y[:, 129].any()
+
+
+@pytest.mark.gpu
 def test_product_repeats_bit_for_bit_on_any_stream_and_in_a_graph():
     a, b = product_case(20, 4096, 512, "nvfp4", 9)  # split over K
     y = mxb.fp4_matmul(a, b)
