@@ -446,6 +446,10 @@ int mxb_kv_write(const void* k, const void* v, int x_dtype, int64_t T, int heads
                  int64_t v_head_stride, const int64_t* slots, int64_t n_pages, int page, int bits,
                  void* k_codes, float* k_scales, void* v_codes, float* v_scales, void* stream);
 
+/* dst[i] = src[i] saturated to 32 bits: page tables and lengths kept as int64,
+ * whose values outside every pool stay outside. */
+int mxb_narrow_i64(const int64_t* src, int64_t n, int* dst, void* stream);
+
 /*
  * Read histories back: out [B][max_len][heads][dim] (out_dtype MXB_F32 /
  * MXB_BF16) of K and V, position p of sequence b from page

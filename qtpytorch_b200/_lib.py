@@ -74,6 +74,7 @@ PROTOTYPES = {
                                        _int, _vp, _vp]),
     "mxb_kv_write": (_int, [_vp, _vp, _int, _i64, _int, _int, _i64, _i64, _i64, _i64, _vp, _i64, _int,
                             _int, _vp, _vp, _vp, _vp, _vp]),
+    "mxb_narrow_i64": (_int, [_vp, _i64, _vp, _vp]),
     "mxb_kv_read": (_int, [_vp, _vp, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _i64, _vp, _i64,
                            _i64, _vp, _vp, _int, _vp]),
     "mxb_paged_attention_workspace_size": (_sz, [_i64, _i64, _int, _int, _int, _int, _int, _i64,

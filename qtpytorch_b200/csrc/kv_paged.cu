@@ -200,6 +200,14 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+__global__ void __launch_bounds__(kThreads)
+    narrow_i64_kernel(const int64_t* __restrict__ src, int64_t n, int* __restrict__ dst) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x;
+  if (i < n) dst[i] = (int)max(min(src[i], (int64_t)INT32_MAX), (int64_t)INT32_MIN);
+}
+
 int shift_of(int page) { return 31 - __builtin_clz((unsigned)page); }
 
 struct WriteArgs {
@@ -286,6 +294,16 @@ int kv_pool_check(int64_t n_pages, int heads, int page, int dim, int bits, const
 }  // namespace mxb
 
 extern "C" {
+
+int mxb_narrow_i64(const int64_t* src, int64_t n, int* dst, void* stream) {
+  if (n < 0 || n > ((int64_t)INT32_MAX - 1) * kThreads) return MXB_E_SHAPE;
+  if (n == 0) return MXB_OK;
+  if (!src || !dst) return MXB_E_ARG;
+  MXB_CUDA_TRY(launch_pdl(narrow_i64_kernel, dim3((unsigned)cdiv(n, kThreads)), kThreads, 0,
+                          static_cast<cudaStream_t>(stream), src, n, dst));
+  MXB_LAUNCH_CHECK();
+  return MXB_OK;
+}
 
 int mxb_kv_write(const void* k, const void* v, int x_dtype, int64_t T, int heads, int dim,
                  int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,

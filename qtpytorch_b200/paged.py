@@ -151,6 +151,22 @@ class paged_kv_cache:
                 f"page={self.page_size}, dtype={self.dtype.name})")
 
 
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous int32 on the device; 64-bit values saturate, so that what lies
+    outside every pool or table stays outside."""
+    if not t.is_contiguous():
+        t = t.contiguous()
+    if t.dtype == torch.int32:
+        return t
+    if t.dtype != torch.int64:
+        return t.to(torch.int32)
+    out = torch.empty_like(t, dtype=torch.int32)
+    rc = L.call("mxb_narrow_i64", t.device, t.data_ptr(), t.numel(), out.data_ptr())
+    if rc:
+        L.check(rc, f"mxb_narrow_i64({t.numel()})")
+    return out
+
+
 def _tables(table: torch.Tensor, lengths: torch.Tensor, dev, what: str):
     if table.dim() != 2 or lengths.shape != table.shape[:1]:
         raise ValueError(f"{what}: table must be [B, width] and lengths [B]")
@@ -158,11 +174,7 @@ def _tables(table: torch.Tensor, lengths: torch.Tensor, dev, what: str):
         raise ValueError(f"{what}: table and lengths must be on {dev}")
     if table.is_floating_point() or lengths.is_floating_point():
         raise ValueError(f"{what}: table and lengths hold integers")
-    if table.dtype != torch.int32 or not table.is_contiguous():
-        table = table.to(torch.int32).contiguous()
-    if lengths.dtype != torch.int32 or not lengths.is_contiguous():
-        lengths = lengths.to(torch.int32).contiguous()
-    return table, lengths
+    return _int32(table), _int32(lengths)
 
 
 def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
@@ -204,7 +216,7 @@ def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
         if prefix_len > width * cache.page_size:
             raise ValueError(f"paged_attention: prefix_len {prefix_len} needs more than the "
                              f"{width} pages of prefix_table")
-        prefix_table = prefix_table.to(torch.int32).contiguous()
+        prefix_table = _int32(prefix_table)
     q = q.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()

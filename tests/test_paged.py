@@ -592,6 +592,34 @@ def test_attention_nan_query_has_a_nan_sum(dtype, B):
 
 
 @pytest.mark.gpu
+def test_64_bit_tables_and_lengths_do_not_wrap():
+    """Page numbers and lengths past 32 bits are outside the pool and the table, not
+    their low halves."""
+    c = pool(4, 2, 64, "int8d", 16, 15)
+    q = torch.randn(1, 1, 4, 64, generator=torch.Generator().manual_seed(0)).cuda().bfloat16()
+    L.load().mxb_device_error(1)
+    wide = torch.tensor([[1, 2 ** 32 + 2, -2 ** 32 + 3, 2]], device="cuda")
+    n = torch.tensor([60], device="cuda")
+    k, _ = c.read(wide, n, 64, torch.float32)
+    assert L.load().mxb_device_error(1) == 8
+    assert k[0, :16].any() and not k[0, 16:48].any() and k[0, 48:60].any()
+    far = torch.tensor([2 ** 32 + 3], device="cuda")
+    good = torch.tensor([[1, 2, 3, 2]], device="cuda")
+    a = mxb.paged_attention(q, c, good, far)
+    assert L.load().mxb_device_error(1) == 8
+    assert torch.equal(a, mxb.paged_attention(q, c, good, torch.tensor([64], device="cuda")))
+    none = mxb.paged_attention(q, c, good, torch.tensor([-2 ** 32 + 3], device="cuda"))
+    assert not none.any() and L.load().mxb_device_error(1) == 0
+    for rep in (1, 10):  # both prefix kernels
+        qq = q.repeat(rep, 1, 4, 1)
+        short = torch.tensor([[1, 2]] * rep, device="cuda")
+        zero = torch.zeros(rep, dtype=torch.int32, device="cuda")
+        out, lse = mxb.paged_attention(qq, c, short, zero, prefix_table=wide[0], prefix_len=60, return_lse=True)
+        assert L.load().mxb_device_error(1) == 8
+        check_attention(out, lse, qq, c, short, [0] * rep, short[0], 28)
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """A pool of 5.4 GB of codes each for K and V: the last page works like the first."""
     pages, heads, dim, page = 41000, 8, 128, 128
