@@ -166,13 +166,14 @@ class fp4_tensor:
         return base, base + at_s, base + g if isinstance(g, int) else L.ptr(g)
 
     def _views(self):
-        if len(self._parts) != 3:
-            buf, rows, cb, at_s, sb, g = self._parts
+        parts = self._parts  # read once: another thread may replace it
+        if len(parts) != 3:
+            buf, rows, cb, at_s, sb, g = parts
             if isinstance(g, int):
                 g = buf[g:g + 4].view(torch.float32)
-            self._parts = (buf[:cb].view(rows, -1) if cb else buf[:0].view(rows, 0),
-                           buf[at_s:at_s + sb], g)
-        return self._parts
+            parts = self._parts = (buf[:cb].view(rows, -1) if cb else buf[:0].view(rows, 0),
+                                   buf[at_s:at_s + sb], g)
+        return parts
 
     @property
     def codes(self) -> torch.Tensor:

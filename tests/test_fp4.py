@@ -187,6 +187,22 @@ def test_copies_own_their_addresses(fmt, viewed):
     assert torch.load(buf, map_location="meta", weights_only=False).device.type == "meta"
 
 
+def test_parts_asked_for_by_two_threads():
+    """Another thread makes the views between this one's look at the parts and its
+    use of them."""
+    t = one_buffer("nvfp4")
+    made = one_buffer("nvfp4")._views()
+
+    class Meanwhile(tuple):
+        def __len__(self):
+            n = super().__len__()
+            t._parts = made
+            return n
+
+    t._parts = Meanwhile(t._parts)
+    assert torch.equal(t.codes, made[0]) and torch.equal(t.scales, made[1])
+
+
 def saved(x):
     buf = io.BytesIO()
     torch.save(x, buf)
