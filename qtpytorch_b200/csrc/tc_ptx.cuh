@@ -253,14 +253,6 @@ __device__ __forceinline__ void mma_fp4(uint32_t d_tmem, uint64_t adesc, uint64_
   }
 }
 
-// 512 bytes of shared memory (32 rows x 16 bytes, unswizzled) -> 4 TMEM
-// columns, lanes 0..31, repeated in the other three lane quarters.  Ordered
-// before MMAs that the same thread issues later.
-__device__ __forceinline__ void tmem_cp_32x128(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
-               : "memory");
-}
-
 // Arrive on `bar` when all previously issued MMAs of this thread complete.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile(
@@ -339,13 +331,6 @@ __device__ __forceinline__ uint64_t desc_kmajor_sw128(uint32_t saddr) {
 __device__ __forceinline__ uint64_t desc_mnmajor_sw128(uint32_t saddr, uint32_t mn_atom_stride) {
   return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)((mn_atom_stride >> 4) & 0x3FFF) << 16) |
          ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
-// Unswizzled rows of 16 bytes, 8-row core matrices 128 bytes apart (scale
-// factor blocks for tcgen05.cp).
-__device__ __forceinline__ uint64_t desc_rows16(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(128 >> 4) << 32) |
-         ((uint64_t)1 << 46);
 }
 
 // Instruction descriptor of the block-scaled 4-bit kinds, dense, K = 64, both
