@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp == 0) {
     if (lane == 0) {
-      for (int i = 0; i < nk; ++i) {
+      int i = 0;
+      for (; i < nk; ++i) {
         const int s = i % S, round = i / S, ks = k_lo + i;
         if (round > 0 && !mbar_wait_to(&bars->empty[s], (round - 1) & 1, kErrTimeoutEmpty, a.err))
           break;
@@ -202,18 +203,20 @@ __global__ void __launch_bounds__(kThreads, 2)
         tma_load_2d(sF + s * kTileF, &tmap_f, &bars->full[s], ks * (BK / 2), n0);
         tma_load_2d(sT + s * kTileT, &tmap_t, &bars->full[s], ks * (BK / 2), m0);
       }
+      // the last copies land before the CTA may end, also where a wait gave up
+      for (int j = max(i - S, 0); j < i; ++j)
+        mbar_wait_to(&bars->full[j % S], (j / S) & 1, kErrTimeoutFull, a.err);
     }
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t i0 = make_idesc_fp4(FMT == MXB_FP4_MX, BM, NT, 0);
       constexpr uint32_t i2 = make_idesc_fp4(FMT == MXB_FP4_MX, BM, NT, 2);
-      bool ok = true;
       for (int i = 0; i < nk; ++i) {
         const int s = i % S, round = i / S, ks = k_lo + i;
         const uint32_t sf0 = tbase + kAcc + (i & 1) * kSfCols;
-        ok = mbar_wait_to(&bars->sf_ready[i & 1], (i >> 1) & 1, kErrTimeoutTmemFull, a.err) &&
-             mbar_wait_to(&bars->full[s], round & 1, kErrTimeoutFull, a.err);
-        if (!ok) break;
+        if (!mbar_wait_to(&bars->sf_ready[i & 1], (i >> 1) & 1, kErrTimeoutTmemFull, a.err) ||
+            !mbar_wait_to(&bars->full[s], round & 1, kErrTimeoutFull, a.err))
+          break;
         tc_fence_after();
         const uint32_t pf = smem_u32(sF + s * kTileF), pt = smem_u32(sT + s * kTileT);
         const int ng = min(G, a.kgroups - ks * G);
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         mma_commit(&bars->empty[s]);
         mma_commit(&bars->sf_free[i & 1]);
       }
-      if (ok) mma_commit(&bars->acc);
+      mma_commit(&bars->acc);  // of all that were issued, also where a wait gave up
     }
   } else if (warp >= 2 + kEpiWarps) {
     // Scales: every warp fills the lane quarter of TMEM that it may write (each

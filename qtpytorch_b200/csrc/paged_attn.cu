@@ -410,6 +410,7 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
     }
     cp_async_arrive(bar);
   };
+  bool ok = true;  // no wait of this warp gave up
   int next_page = -1;
   int stage = 0;  // ring position of the warp's next tile, and its parity
   uint32_t round = 0;
@@ -420,14 +421,13 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
     for (int i = 0; i < kStages; ++i) pg[i] = page_of(t_lo + warp + i * kWarps);
 #pragma unroll
     for (int i = 0; i < kStages; ++i)
-      if (t_lo + warp + i * kWarps < t_hi)
+      if (ok && t_lo + warp + i * kWarps < t_hi)
         issue(t_lo + warp + i * kWarps, u / a.row_tiles,
               stage + i < kStages ? stage + i : stage + i - kStages, pg[i]);
     next_page = page_of(t_lo + warp + kStages * kWarps);
   };
   fill();
 
-  bool ok = true;
   while (true) {
     const int h = u / a.row_tiles, r0 = (u - h * a.row_tiles) * R;
     const bool first = t_lo == 0, last = t_hi == n_tiles;
@@ -563,9 +563,22 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
       }
     }
 
-    for (int tile = t_lo + warp; tile < t_hi; tile += kWarps) {
+    for (int tile = t_lo + warp; ok && tile < t_hi; tile += kWarps) {
       const int s = stage;
-      ok = ok && mbar_wait_warp_to(&full[warp][s], round, kErrTimeoutFull, a.err);
+      ok = mbar_wait_warp_to(&full[warp][s], round, kErrTimeoutFull, a.err);
+      if (!ok) {
+        // the warp's copies in flight, this one among them, before the CTA may
+        // end; from here on it only keeps the others' barriers company
+#pragma unroll 1
+        for (int i = 0; i < kStages && tile + i * kWarps < t_hi; ++i) {
+          mbar_wait_warp_to(&full[warp][stage], round, kErrTimeoutFull, a.err);
+          if (++stage == kStages) {
+            stage = 0;
+            round ^= 1u;
+          }
+        }
+        break;
+      }
       if (++stage == kStages) {
         stage = 0;
         round ^= 1u;

@@ -77,6 +77,7 @@ struct Bars {
   uint64_t sready[2][2], pready[2][2], pvdone[2];
   uint64_t scready[kSlots];
   uint64_t qready;
+  uint64_t drained;  // every product issued is complete
   uint32_t tmem_base;
   uint32_t gone[kStages];  // bit i: keys 16 i .. of the tile lie behind a number outside the pool
 };
@@ -371,6 +372,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
     }
     for (int s = 0; s < kSlots; ++s) mbar_init(&bars->scready[s], kConvWarps);
     mbar_init(&bars->qready, 4 * MT);
+    mbar_init(&bars->drained, 1);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -393,7 +395,8 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
 
   if (warp == 0) {
     const int page_mask = (1 << a.page_shift) - 1;
-    for (int i = 0; i < n; ++i) {
+    int i = 0;
+    for (; i < n; ++i) {
       const int s = i % kStages, round = i / kStages;
       const int pos = (t_lo + i) * KT + lane * box;
       int p = -1;
@@ -426,6 +429,9 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
         }
       }
     }
+    // the last copies land before the CTA may end, also where a wait gave up
+    for (int j = max(i - kStages, 0); j < i; ++j)
+      mbar_wait_warp_to(&bars->raw_full[j % kStages], (j / kStages) & 1, kErrTimeoutFull, a.err);
   } else if (warp == 1) {
     if (lane == 0 && n > 0) {
       constexpr uint32_t id_s = make_idesc(/*F32*/ 1, /*F16*/ 0, 0, 0, 128, KT);
@@ -472,6 +478,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
         }
         if (ok) mma_commit(&bars->vfree[b]);
       }
+      mma_commit(&bars->drained);
     }
   } else if (warp < 2 + kConvWarps) {
     const int t = threadIdx.x - 64;
@@ -624,8 +631,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, MT>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
-    // every product issued is complete once the last commits are (they were
-    // waited for by the softmax warps)
+    if (n > 0) mbar_wait_warp_to(&bars->drained, 0, kErrTimeoutDone, a.err);
     tc_fence_after();
     tmem_dealloc(tbase, C::kCols);
   }
