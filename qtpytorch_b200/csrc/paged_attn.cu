@@ -1156,7 +1156,9 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) % 16) return MXB_E_ALIGN;
   const pattn::Plan p =
       pattn::make_plan(B, T, heads, group, dim, bits, width * page, prefix_len);
+  const int64_t pre_rows = B * T * group;
   if ((int64_t)p.tiles_own * heads > 65535 || (int64_t)p.tiles_pre * heads > 65535 ||
+      (p.splits_pre > 0 && p.nt_pre == 0 && cdiv(pre_rows, prefix_rows_per_cta(pre_rows)) > 65535) ||
       B * heads * p.tiles_own > INT32_MAX || B * T * heads * group > INT32_MAX ||
       (int64_t)heads * p.tiles_own * (width * page / pattn::kTile + 1) > INT32_MAX)
     return MXB_E_SHAPE;

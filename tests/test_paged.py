@@ -61,6 +61,17 @@ def test_argument_errors_need_no_gpu():
     assert attend(B=0) == 0 and attend(T=0) == 0
 
 
+def test_more_prefix_rows_than_a_grid_holds_are_refused():
+    lib, p = L.load(), ctypes.c_void_p(32)
+
+    def attend(B, prefix):
+        return lib.mxb_paged_attention(p, B, 1, 2, 1024, 128, p, p, p, p, 4, 16, 8, p, 3, p, p, 1, prefix, 0.1, p,
+                                       None, None, 0, None)
+
+    assert attend(65535, 16) == -1            # 262140 groups of 256 rows a KV head
+    assert attend(16383, 16) == -7            # 65532: the workspace is looked at next
+
+
 def test_refusals():
     with pytest.raises(NotImplementedError):
         mxb.paged_kv_cache(4, 2, 128, "int2d", device="cpu")
