@@ -442,6 +442,19 @@ def test_product_of_factors_past_the_range(m, sx, sw):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [9, 40, 300])
+def test_nvfp4_product_nan_stays_in_its_row_and_column(m):
+    g = torch.Generator("cuda").manual_seed(m)
+    x, w = torch.randn(m, 200, generator=g, device="cuda"), torch.randn(300, 200, generator=g, device="cuda")
+    x[5, 3], w[290, 199] = float("nan"), float("-inf")
+    one = torch.ones(1, device="cuda")  # a given factor: one from the data would be 1 here too
+    y = mxb.fp4_matmul(mxb.fp4_tensor.quantize(x, "nvfp4", one / 100), mxb.fp4_tensor.quantize(w, "nvfp4"))
+    want = torch.zeros(m, 300, dtype=torch.bool, device="cuda")
+    want[5], want[:, 290] = True, True
+    assert torch.equal(y.isnan(), want)
+
+
+@pytest.mark.gpu
 def test_product_repeats_bit_for_bit_on_any_stream_and_in_a_graph():
     a, b = product_case(20, 4096, 512, "nvfp4", 9)  # split over K
     y = mxb.fp4_matmul(a, b)

@@ -355,6 +355,17 @@ def test_attention_with_a_shared_prefix(dtype, dim, page, heads, group, T, lengt
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["int8d", "int4d"])
+@pytest.mark.parametrize("dim,page,heads,group,T,lengths,prefix", [
+    (128, 16, 2, 4, 16, [16, 40, 7, 0], 0), (64, 32, 1, 8, 70, [70, 200, 71, 3], 0),   # a unit a CTA
+    (128, 64, 1, 5, 33, [33, 4500, 100], 0), (64, 64, 2, 1, 129, [5000, 129], 0),       # the shared list
+    (128, 32, 2, 2, 40, [40, 90], 500), (64, 16, 1, 3, 7, [9, 7], 200)])                # behind a prefix
+def test_attention_of_a_chunk_of_a_prompt(dtype, dim, page, heads, group, T, lengths, prefix):
+    """Many query tokens a sequence: several row tiles, each row with a limit of its own."""
+    run_attention(dtype, dim, page, heads, group, T, lengths, prefix)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["int8d", "int4d"])
 def test_attention_long_skewed_batch(dtype):
     run_attention(dtype, 128, 64, 2, 4, 1, [20000, 3, 0, 700, 129], 0)
     run_attention(dtype, 64, 16, 1, 8, 3, [9000, 1, 0, 77], 3000, outlier=True)
