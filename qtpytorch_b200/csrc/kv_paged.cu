@@ -333,7 +333,7 @@ int mxb_kv_read(const void* k_codes, const float* k_scales, const void* v_codes,
   if (B < 0 || B > 65535 || max_len < 0 || max_len > INT32_MAX || width < 0 || width > INT32_MAX)
     return MXB_E_SHAPE;
   if (B == 0 || max_len == 0) return MXB_OK;
-  if (!table || !lengths || !k_out || !v_out) return MXB_E_ARG;
+  if ((width > 0 && !table) || !lengths || !k_out || !v_out) return MXB_E_ARG;
   if (((uintptr_t)k_out | (uintptr_t)v_out) % 16) return MXB_E_ALIGN;
   ReadArgs a = {static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(v_codes),
                 k_scales, v_scales, table, (int)width, lengths, B, n_pages, heads, page, max_len};

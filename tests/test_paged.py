@@ -263,6 +263,19 @@ def test_read_bad_pages_read_as_zero():
     assert not k[0, 16:].any() and not k[1, :16].any() and not k[1, 32:].any()
 
 
+@pytest.mark.gpu
+def test_read_through_tables_without_pages():
+    """A batch whose sequences have no pages yet reads as zeros, as attention takes it."""
+    c = pool(2, 2, 64, "int4d", 16, 5)
+    L.load().mxb_device_error(1)
+    for table in (torch.zeros(3, 0, dtype=torch.int32, device="cuda"), torch.zeros(3, 0, device="cuda").long()):
+        for x in c.read(table, torch.zeros(3, dtype=torch.int32, device="cuda"), 4):
+            assert x.shape == (3, 4, 2, 64) and not x.any()
+        assert L.load().mxb_device_error(1) == 0
+        c.read(table, torch.ones(3, dtype=torch.int32, device="cuda"), 4)
+        assert L.load().mxb_device_error(1) == 8
+
+
 # ── attention ────────────────────────────────────────────────────────────────
 def attend64(q, c, table, lengths, prefix, prefix_len, scale):
     """(out, lse) in 64 bits, with sum_j p_j |v_j| for the tolerance."""
