@@ -609,6 +609,34 @@ def test_attention_of_quiet_values_beside_loud_ones(dtype, B, exponent, loud):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["int8d", "int4d"])
+@pytest.mark.parametrize("B,own", [(2, False), (12, False), (24, True)])
+@pytest.mark.parametrize("span", [5, 14, 30])
+def test_attention_of_value_scales_of_any_size(dtype, B, own, span):
+    """Value scales over 2^-span, in no order: every weight is off by 2^-11 of itself
+    or 2^-20 of the row's largest (the floor of tiles of a narrow span)."""
+    c = pool(30, 1, 64, dtype, 64, 16)
+    g = torch.Generator("cuda").manual_seed(span)
+    c.v_scales.copy_(2.0 ** (torch.rand(30, 1, 64, generator=g, device="cuda") * -span))
+    q = (3 * torch.randn(B, 1, 8, 64, generator=g, device="cuda")).bfloat16()
+    pages = torch.arange(30, device="cuda", dtype=torch.int32)
+    table, n, prefix = pages[None, 24:].repeat(B, 1), [300 * own] * B, 1500
+    out = mxb.paged_attention(q, c, table, torch.tensor(n, device="cuda"), prefix_table=pages[:24],
+                              prefix_len=prefix)
+    out64, _, mag = attend64(q, c, table, n, pages[:24], prefix, 0.125)
+    k, s = history(c, "k", pages, 1920)[0], c.v_scales[:, 0].flatten().double()
+    live = torch.arange(1920, device="cuda")
+    live = (live < prefix) | ((live >= 24 * 64) & (live < 24 * 64 + n[0]))
+    p = torch.softmax((torch.einsum("bgd,ld->bgl", q[:, 0].double(), k) * 0.125).masked_fill(~live, float("-inf")), -1)
+    largest = (p * s).amax(-1)[:, None, :, None]
+    off, top = (1152 + 127, 127) if dtype == "int8d" else (136 + 8, 8)
+    e_s = ((64 / 16 + 4) * 2.0 ** -23 * off * q.double().abs().sum(-1) * c.k_scales.max().double()
+           * 0.125 * 1.4427 + 2.0 ** -22)[..., None]
+    tol = (2.0 ** -11 + 4 * e_s + 2.0 ** -20) * mag + 2.0 ** -8 * out64.abs() + 2.0 ** -20 * top * largest * int(live.sum())
+    assert bool(((out.double() - out64).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["int8d", "int4d"])
 @pytest.mark.parametrize("B", [1, 12, 40])
 def test_attention_nan_query_has_a_nan_sum(dtype, B):
     """A NaN query's log-sum-exp is NaN, behind a prefix alone as with keys of its
