@@ -389,7 +389,7 @@ int mxb_linear_wonly_noalloc(const void* x, int x_dtype, int64_t M, int64_t K,
 size_t mxb_fp4_code_bytes(int64_t rows, int64_t K);
 size_t mxb_fp4_scale_bytes(int64_t rows, int64_t K, int fmt);
 
-/* Workspace bytes for mxb_fp4_quantize (0 unless derive is set). */
+/* Workspace bytes for mxb_fp4_quantize (0 unless derive is set; 4-byte aligned). */
 size_t mxb_fp4_quantize_workspace_size(int64_t rows, int64_t K, int fmt, int derive);
 
 /*
@@ -462,7 +462,7 @@ int mxb_kv_read(const void* k_codes, const float* k_scales, const void* v_codes,
                 const int* table, int64_t width, const int* lengths, int64_t B, int64_t max_len,
                 void* k_out, void* v_out, int out_dtype, void* stream);
 
-/* Workspace bytes for mxb_paged_attention. */
+/* Workspace bytes for mxb_paged_attention (32-byte aligned). */
 size_t mxb_paged_attention_workspace_size(int64_t B, int64_t T, int heads, int group, int dim,
                                           int bits, int page, int64_t width, int64_t prefix_len);
 

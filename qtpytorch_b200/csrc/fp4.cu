@@ -529,7 +529,9 @@ int mxb_fp4_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int64_
   if (rows < 0 || K < 0 || (rows > 1 && ldx < K)) return MXB_E_SHAPE;
   if (rows == 0 || K == 0) return MXB_OK;
   if (!x || !codes || !scales || (fmt == MXB_FP4_NV) != (global_scale != nullptr)) return MXB_E_ARG;
-  if ((uintptr_t)codes % 16 || (uintptr_t)scales % 16) return MXB_E_ALIGN;
+  if ((uintptr_t)codes % 16 || (uintptr_t)scales % 16 || (uintptr_t)workspace % 4 ||
+      (uintptr_t)x % (x_dtype == MXB_BF16 ? 2 : 4))
+    return MXB_E_ALIGN;
   const bool d = fmt == MXB_FP4_NV && derive != 0;
   if (d && (!workspace || workspace_bytes < mxb_fp4_quantize_workspace_size(rows, K, fmt, 1)))
     return MXB_E_WORKSPACE;
@@ -550,7 +552,8 @@ int mxb_fp4_dequantize(const void* codes, const void* scales, const float* globa
   if (rows == 0 || K == 0) return MXB_OK;
   if (!codes || !scales || !out || (fmt == MXB_FP4_NV) != (global_scale != nullptr))
     return MXB_E_ARG;
-  if ((uintptr_t)codes % 16 || (uintptr_t)scales % 16) return MXB_E_ALIGN;
+  if ((uintptr_t)codes % 16 || (uintptr_t)scales % 16 || (uintptr_t)out % (out_dtype == MXB_BF16 ? 2 : 4))
+    return MXB_E_ALIGN;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   const uint8_t* s = static_cast<const uint8_t*>(scales);

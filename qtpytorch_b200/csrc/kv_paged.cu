@@ -315,6 +315,7 @@ int mxb_kv_write(const void* k, const void* v, int x_dtype, int64_t T, int heads
   if (T < 0) return MXB_E_SHAPE;
   if (T == 0) return MXB_OK;
   if (!k || !v || !slots) return MXB_E_ARG;
+  if (((uintptr_t)k | (uintptr_t)v) % (x_dtype == MXB_BF16 ? 2 : 4)) return MXB_E_ALIGN;
   WriteArgs a = {T, heads, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots,
                  n_pages * page, page, static_cast<uint8_t*>(k_codes),
                  static_cast<uint8_t*>(v_codes), k_scales, v_scales};

@@ -1153,7 +1153,8 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
   if (B == 0 || T == 0) return MXB_OK;
   if (!q || !out || !lengths || (width > 0 && !table) || (prefix_len > 0 && !prefix_table))
     return MXB_E_ARG;
-  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) % 16) return MXB_E_ALIGN;
+  // parts are stored 32 bytes at a time
+  if (((uintptr_t)q | (uintptr_t)out) % 16 || (uintptr_t)workspace % 32) return MXB_E_ALIGN;
   const pattn::Plan p =
       pattn::make_plan(B, T, heads, group, dim, bits, width * page, prefix_len);
   const int64_t pre_rows = B * T * group;

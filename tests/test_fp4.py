@@ -121,6 +121,16 @@ def test_argument_errors_need_no_gpu():
     assert m(p, p, None, p, p, None, 0, 64, 4, 0, None, p, 1, None) == 0
 
 
+def test_misaligned_pointers_are_refused():
+    lib, p, g, odd = L.load(), ctypes.c_void_p(32), ctypes.c_void_p(16), ctypes.c_void_p(33)
+    n = lib.mxb_fp4_quantize_workspace_size(4, 64, 1, 1)
+    for dt in (0, 1):
+        assert lib.mxb_fp4_quantize(odd, dt, 4, 64, 64, 0, None, 0, p, p, None, 0, None) == -3
+        assert lib.mxb_fp4_dequantize(p, p, None, 4, 64, 0, odd, dt, None) == -3
+    assert lib.mxb_fp4_quantize(p, 0, 4, 64, 64, 1, g, 1, p, p, odd, n - 1, None) == -3
+    assert lib.mxb_fp4_quantize(p, 0, 4, 64, 64, 1, g, 1, p, p, p, n - 1, None) == -7
+
+
 def test_refusals():
     with pytest.raises(L.MxbError):
         mxb.fp4_tensor.quantize(torch.zeros(4, 64))

@@ -61,6 +61,23 @@ def test_argument_errors_need_no_gpu():
     assert attend(B=0) == 0 and attend(T=0) == 0
 
 
+def test_misaligned_pointers_are_refused():
+    lib, p = L.load(), ctypes.c_void_p(32)
+    need = lib.mxb_paged_attention_workspace_size(2, 1, 2, 4, 128, 8, 16, 1000, 0)
+
+    def attend(ws):
+        return lib.mxb_paged_attention(p, 2, 1, 2, 4, 128, p, p, p, p, 4, 16, 8, p, 1000, p, None, 0, 0, 0.1, p,
+                                       None, ctypes.c_void_p(ws), need - 1, None)
+
+    assert attend(48) == -3 and attend(64) == -7  # parts are stored 32 bytes at a time
+
+    def write(k, v, dt):
+        return lib.mxb_kv_write(ctypes.c_void_p(k), ctypes.c_void_p(v), dt, 2, 2, 128, 256, 128, 256, 128, p, 4, 16,
+                                8, p, p, p, p, None)
+
+    assert write(34, 32, 0) == -3 and write(32, 33, 1) == -3
+
+
 def test_more_prefix_rows_than_a_grid_holds_are_refused():
     lib, p = L.load(), ctypes.c_void_p(32)
 
