@@ -17,11 +17,11 @@
 // Scores: Q is fp16 under a power of two per row that puts its largest value
 // into [2^14, 2^15), the codes are exact.  Weights: p_j = exp2(s_j - m) times
 // 2^6 sv_j / c, c a power of two of at least the largest value scale so far, and m
-// following the maximum within 2^8.  While the value scales span less than 2^-11
-// of c, a row's largest weight is at least 2^-5, so fp16 keeps 11 bits of those
-// down to 2^-9 of it and is off by 2^-20 of it below.  From the first tile with a
-// wider span on, c is each row's own and follows its largest weight, as that
-// may belong to a key whose value scale is far under another's (a wide tile
+// following the maximum within 2^8.  While the value scales span less than 2^-14
+// of c, a row's largest weight is at least 2^-8, so fp16 keeps 11 bits of those
+// down to 2^-6 of it and is off by at most 2^-17 of it below.  From the first tile
+// with a wider span on, c is each row's own and follows its largest weight, as
+// that may belong to a key whose value scale is far under another's (a wide tile
 // costs one more multiplication and comparison a score).  m, sums and outputs
 // are fp32; O is rescaled in TMEM only when m or c moves.
 // Pairs of codes unpack out of order; Q's columns are stored in the same
@@ -51,7 +51,11 @@ constexpr int kStages = 3;
 constexpr int kSlots = 4;  // scale slots: softmax may lag the unpacking by two tiles
 constexpr int kConvWarps = 4;
 constexpr float kRoom = 64.0f;  // 2^6
-constexpr float kWide = 0x1p-11f;  // of c: scales below make a tile wide
+// Value scales below this part of c make a tile wide: of the largest, 2^-11 or 2^-12.
+// 64 x 8 rows of 8 heads over 8192 keys take 45 us while all tiles are narrow, 60
+// when all are wide, 70 with both (ncu), so a span that a cache has in earnest is
+// left narrow.
+constexpr float kWide = 0x1p-14f;
 
 template <int BITS, int D, int MT>
 struct Cfg {
@@ -167,9 +171,10 @@ __device__ __forceinline__ void unpack_tile(const uint8_t* raw, uint8_t* plane, 
 }
 
 // A row of the softmax: reference and sum; lc, log2 of the c that its O stands
-// under; top_w, log2 of the largest weight stored (kept for wide tiles).
+// under; top_w, log2 of the largest weight stored, or less (kept for wide tiles;
+// -8 is what narrow ones reach).
 struct Row {
-  float mu = 0.0f, m_top = -INFINITY, l = 0.0f, lc = 0.0f, top_w = -5.0f;
+  float mu = 0.0f, m_top = -INFINITY, l = 0.0f, lc = 0.0f, top_w = -8.0f;
   bool ok = true;
 };
 struct RowTiles {

@@ -630,7 +630,8 @@ def test_attention_of_quiet_values_beside_loud_ones(dtype, B, exponent, loud):
 @pytest.mark.parametrize("span", [5, 14, 30])
 def test_attention_of_value_scales_of_any_size(dtype, B, own, span):
     """Value scales over 2^-span, in no order: every weight is off by 2^-11 of itself
-    or 2^-20 of the row's largest (the floor of tiles of a narrow span)."""
+    or, below fp16's normal range, by 2^-17 of the row's largest at most, either way;
+    over the keys that is held to 2^-20 each."""
     c = pool(30, 1, 64, dtype, 64, 16)
     g = torch.Generator("cuda").manual_seed(span)
     c.v_scales.copy_(2.0 ** (torch.rand(30, 1, 64, generator=g, device="cuda") * -span))
