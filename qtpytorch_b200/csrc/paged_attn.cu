@@ -37,9 +37,9 @@
 // Rows with a single part are written directly.
 //
 // 2 x 131072 keys and less, 4 rows of each of 8 heads of 128 dims in int8 (346 MB):
-// 71 us = 4.9 TB/s, 62 without any arithmetic.  24 rows of 64 dims in int4 take
-// about 1080 instructions a tile for 2 KB of codes and are bound by their latency
-// (0.43 issued a cycle with 8 warps an SM): 50 us for 48 x up to 6000 keys.
+// 69 - 72 us = 4.8 - 5.0 TB/s, 62 without any arithmetic.  24 rows of 64 dims in int4
+// take about 1000 instructions a tile for 2 KB of codes and are bound by their latency
+// (0.47 issued a cycle with 12 warps an SM): 50 us for 48 x up to 6000 keys.
 #include "mxb_common.cuh"
 #include "mxb_internal.h"
 

@@ -95,7 +95,7 @@ class fp4_tensor:
                  global_scale: Optional[torch.Tensor] = None) -> "fp4_tensor":
         """Quantize along the last dim (fp32 and bf16 as they are, other types
         through fp32).  ``global_scale`` (nvfp4): a positive fp32 factor to
-        use, e.g. a calibrated one; by default from the data."""
+        use, e.g. a calibrated one; by default from the data.  No gradient."""
         f = _fmt(fmt)
         L.require_cuda(x, "fp4_tensor.quantize")
         if x.dim() < 1:
@@ -219,7 +219,7 @@ class fp4_tensor:
 def fp4_matmul(a: fp4_tensor, b: fp4_tensor, bias: Optional[torch.Tensor] = None,
                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """a [..., K] @ b [N, K]^T (+ bias [N]) of two matrices of one format, fp32
-    accumulation, rounded once to ``out_dtype`` (bf16 or fp32)."""
+    accumulation, rounded once to ``out_dtype`` (bf16 or fp32).  No gradient."""
     if not isinstance(a, fp4_tensor) or not isinstance(b, fp4_tensor):
         raise TypeError("fp4_matmul takes two fp4_tensors")
     if a.fmt != b.fmt:
@@ -251,7 +251,8 @@ def fp4_matmul(a: fp4_tensor, b: fp4_tensor, bias: Optional[torch.Tensor] = None
 
 class fp4_linear(nn.Module):
     """nn.Linear with a microscaled 4-bit weight; the activations are quantized
-    to the same format on every call.  Inference only (no gradient)."""
+    to the same format on every call.  Inference only (no gradient).  Dtype casts
+    of a model leave the codes, the factor and the fp32 bias as they are."""
 
     def __init__(self, weight: fp4_tensor, bias: Optional[torch.Tensor] = None,
                  out_dtype: torch.dtype = torch.bfloat16):

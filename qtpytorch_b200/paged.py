@@ -190,7 +190,7 @@ def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
     whole batch.  ``scale`` defaults to 1 / sqrt(head_dim).  A row without keys
     gives zeros; a page number outside the pool holds no keys (recorded in the
     library's device error word).  Returns out (q's shape, bf16), with ``return_lse`` also the fp32
-    log-sum-exp [B, T, Hq] of the scaled scores."""
+    log-sum-exp [B, T, Hq] of the scaled scores.  No gradient."""
     dev = cache._cuda("paged_attention")
     H, D = cache.n_heads, cache.head_dim
     if q.dim() != 4 or q.shape[3] != D or q.shape[2] % H or q.shape[2] == 0:
