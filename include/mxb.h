@@ -489,6 +489,78 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
                         float scale, void* out, float* lse, void* workspace,
                         size_t workspace_bytes, void* stream);
 
+/* Workspace bytes for mxb_tree_attention (32-byte aligned). */
+size_t mxb_tree_attention_workspace_size(int64_t B, int64_t T, int heads, int group, int dim, int bits,
+                                         int page, int64_t width, int64_t prefix_len);
+
+/*
+ * mxb_paged_attention of T drafted tokens a sequence that form a tree: query t
+ * sees the keys j < lengths[b] - T and, of the T newest, key i where byte
+ * tree_mask[b * tree_batch_stride + t * tree_token_stride + i] is not 0 (a batch
+ * stride of 0: one mask for all).  A sequence shorter than T holds the last of
+ * the T only.
+ */
+int mxb_tree_attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim, const void* k_codes,
+                       const float* k_scales, const void* v_codes, const float* v_scales, int64_t n_pages,
+                       int page, int bits, const int* table, int64_t width, const int* lengths,
+                       const int* prefix_table, int64_t prefix_width, int64_t prefix_len,
+                       const uint8_t* tree_mask, int64_t tree_batch_stride, int64_t tree_token_stride,
+                       float scale, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/*
+ * mxb_kv_write with the keys rotated by their positions, and queries rotated
+ * beside them.  Pair i < rot / 2 of a head row, elements (i, i + rot / 2) or, if
+ * `interleaved`, (2 i, 2 i + 1), turns by positions[a * axis_stride + t] *
+ * inv_freq[i]; dims from rot (a multiple of 8) on stay.  One axis: a = 0; up to
+ * four: sections[0] pairs turn by axis 0, the next sections[1] by axis 1, ...
+ * (host memory, their sum rot / 2).
+ *   q      [T][q_heads][dim] under its strides, or q_heads 0; q_out contiguous,
+ *          of the input's type, written for skipped tokens too
+ *   k, v   as for mxb_kv_write; a key's codes and scale are those of the
+ *          rotation in 64 bits rounded to fp32
+ */
+int mxb_kv_append(const void* q, const void* k, const void* v, int x_dtype, int64_t T, int q_heads, int heads,
+                  int dim, int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                  int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                  const int64_t* positions, int axes, int64_t axis_stride, const float* inv_freq, int rot,
+                  const int* sections, int interleaved, const int64_t* slots, int64_t n_pages, int page,
+                  int bits, void* k_codes, float* k_scales, void* v_codes, float* v_scales, void* q_out,
+                  void* stream);
+
+/* ── int8 rows: norm and product ── */
+
+/*
+ * Root-mean-square norm of rows into int8 codes: h = x (+ residual), y = h * weight
+ * / sqrt(mean(h^2) + eps), scale = max(amax|y|, 1e-12) / 127, code = y / scale
+ * rounded to the nearest, ties to even, as exact arithmetic gives it (a row with an
+ * infinity or NaN: codes 0, scale NaN).
+ *   x, residual  [rows][d] of x_dtype, rows x_stride / residual_stride apart;
+ *                residual may be NULL
+ *   weight       [d] of w_dtype (MXB_F32 / MXB_BF16)
+ *   codes        int8 [rows][d], scales fp32 [rows]
+ *   sum          [rows][d] of x_dtype, h rounded, or NULL
+ */
+int mxb_rms_norm_quantize(const void* x, const void* residual, int x_dtype, int64_t rows, int64_t d,
+                          int64_t x_stride, int64_t residual_stride, const void* weight, int w_dtype,
+                          double eps, void* codes, float* scales, void* sum, void* stream);
+
+/* Workspace bytes for mxb_int8_matmul (16-byte aligned): 0 where K is a multiple
+ * of 16 and both operands start at multiples of 16 bytes (`aligned`). */
+size_t mxb_int8_matmul_workspace_size(int64_t M, int64_t K, int64_t N, int aligned);
+
+/*
+ * C[m][n] = fl(fl(P sa[m]) sb[n]) (+ bias[n]), P the exact integer product of int8
+ * codes a [M][K] and b [N][K], K at most 131071.
+ *   a_scales, b_scales  fp32, one a row (step 1) or one for all (step 0)
+ *   bias                fp32 [N] or NULL
+ *   out                 [M][N] MXB_F32 or MXB_BF16
+ */
+int mxb_int8_matmul(const void* a_codes, const float* a_scales, int a_scale_step, const void* b_codes,
+                    const float* b_scales, int b_scale_step, int64_t M, int64_t K, int64_t N,
+                    const float* bias, void* out, int out_dtype, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

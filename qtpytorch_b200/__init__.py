@@ -6,7 +6,8 @@ The reference's hot-path API (DHDev0/qtpytorch ``mxtorch``) on CUDA kernels:
 ``fused_int8_linear``, ``mx_dynamic_linear``, ``fused_linear_relu``,
 ``fused_silu_and_mul``, ``kv_cache_quantizer``, ``save_quantized``, ``load_quantized``;
 beyond it: ``fp4_tensor``, ``fp4_matmul``, ``fp4_linear`` (microscaled 4-bit
-floating point), ``paged_kv_cache``, ``paged_attention``.
+floating point), ``rms_norm_quantize``, ``int8_matmul``, ``int8_linear`` (int8 with a
+scale a row), ``paged_kv_cache``, ``paged_attention``.
 """
 from .dtypes import (  # noqa: F401
     _DTYPE_REGISTRY,
@@ -20,6 +21,7 @@ from .dynamic import dynamic_quantize, fused_int8_linear, mx_dynamic_linear  # n
 from .fp4 import fp4_linear, fp4_matmul, fp4_tensor  # noqa: F401
 from .fused import fused_linear_relu, fused_silu_and_mul  # noqa: F401
 from .hadamard import sign_vector  # noqa: F401
+from .int8 import int8_linear, int8_matmul, rms_norm_quantize  # noqa: F401
 from .kv_cache import kv_cache_quantizer  # noqa: F401
 from .linear import mx_linear, to_mx  # noqa: F401
 from .paged import paged_attention, paged_kv_cache  # noqa: F401

@@ -82,6 +82,18 @@ PROTOTYPES = {
     "mxb_paged_attention": (_int, [_vp, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _vp, _i64, _int,
                                    _int, _vp, _i64, _vp, _vp, _i64, _i64, C.c_float, _vp, _vp, _vp,
                                    _sz, _vp]),
+    "mxb_tree_attention_workspace_size": (_sz, [_i64, _i64, _int, _int, _int, _int, _int, _i64, _i64]),
+    "mxb_tree_attention": (_int, [_vp, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _vp, _i64, _int,
+                                  _int, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, C.c_float, _vp,
+                                  _vp, _vp, _sz, _vp]),
+    "mxb_kv_append": (_int, [_vp, _vp, _vp, _int, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64,
+                             _vp, _int, _i64, _vp, _int, _vp, _int, _vp, _i64, _int, _int, _vp, _vp, _vp, _vp,
+                             _vp, _vp]),
+    "mxb_rms_norm_quantize": (_int, [_vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _int, C.c_double, _vp, _vp,
+                                     _vp, _vp]),
+    "mxb_int8_matmul_workspace_size": (_sz, [_i64, _i64, _i64, _int]),
+    "mxb_int8_matmul": (_int, [_vp, _vp, _int, _vp, _vp, _int, _i64, _i64, _i64, _vp, _vp, _int, _vp, _sz,
+                               _vp]),
     "mxb_fp4_code_bytes": (_sz, [_i64, _i64]),
     "mxb_fp4_scale_bytes": (_sz, [_i64, _i64, _int]),
     "mxb_fp4_quantize_workspace_size": (_sz, [_i64, _i64, _int, _int]),

@@ -1,0 +1,377 @@
+// Product of two int8 matrices with one scale a token and one a feature:
+//
+//   C[m, n] = sa[m] sb[n] sum_k a[m, k] b[n, k] (+ bias[n])
+//
+// The sum is the tensor core's exact int32 (kind::i8), so neither the split of K
+// nor the tiles change a result; the epilogue rounds fl(fl(P sa) sb), the order of
+// the framework's other integer products, then adds the bias and rounds to the
+// output's type.
+#include "mxb_common.cuh"
+#include "mxb_internal.h"
+
+#include <cuda.h>
+
+#define MXB_ERROR_WORD_BY_POINTER
+#include "tc_ptx.cuh"
+
+using namespace mxb;
+
+namespace mxb {
+namespace i8g {
+
+constexpr int BK = 128;  // K values (bytes) a stage: a 128-byte swizzled row
+// |a b| <= 2^14: sums of up to this many of them fit an int32
+constexpr int64_t kMaxK = 131071;
+
+struct Args {
+  const float* sf;  // feature scales, sf_step apart (0: one for all)
+  const float* st;  // token scales
+  const float* bias;
+  void* out;
+  int* err;
+  int M, N;  // tokens, features
+  int ksteps;
+  int splits;
+  int sf_step, st_step;
+};
+
+template <typename OutT>
+__device__ __forceinline__ void store1(OutT* p, float v) {
+  if constexpr (sizeof(OutT) == 2) *p = __float2bfloat16_rn(v);
+  else *p = v;
+}
+// The value of a sum P under its two scales: 0 + x turns -0 into +0, as an
+// accumulator that starts from 0 does.
+__device__ __forceinline__ float scaled(int p, float st, float sf, float bias) {
+  return __fadd_rn(__fmul_rn(__fmul_rn((float)p, st), sf), bias);
+}
+
+// ── few tokens or few tiles ─────────────────────────────────────────────────
+// The 128 rows of an MMA are features, its NT columns tokens: one token costs an
+// MMA of N = 16, and a warp of the epilogue holds 32 adjacent features of a token,
+// which leave as one run.  One CTA owns a 128 x NT tile or, with split K, one of
+// `splits` ranges of it; those CTAs form a cluster and add their partial tiles
+// over distributed shared memory.
+//   warp 0     TMA producer;  warp 1  TMEM allocation and MMAs;
+//   warps 2-9  epilogue
+constexpr int BM = 128;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kMaxSplit = 8;  // portable cluster size
+constexpr int kTileF = BM * BK;
+constexpr int kBarBytes = 256;
+
+template <int NT>
+constexpr int stages() { return NT >= 128 ? 3 : NT == 64 ? 4 : 5; }
+template <int NT>
+constexpr int stage_bytes() { return kTileF + NT * BK; }
+template <int NT>
+constexpr int acc_cols() { return NT < 32 ? 32 : NT; }
+template <int NT>
+constexpr size_t smem_bytes() { return 1024 + (size_t)stages<NT>() * stage_bytes<NT>() + kBarBytes; }
+
+struct Bars {
+  uint64_t full[5], empty[5];
+  uint64_t acc;
+  uint32_t tmem_base;
+};
+static_assert(sizeof(Bars) <= kBarBytes, "barrier block overflows its slot");
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+__device__ __forceinline__ int4 ld_cluster_i4(uint32_t saddr, uint32_t rank) {
+  uint32_t a;
+  int4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a));
+  return v;
+}
+
+template <int NT, typename OutT>
+__global__ void __launch_bounds__(kThreads, 2)
+    int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_f,
+                     const __grid_constant__ CUtensorMap tmap_t, const Args a) {
+  constexpr int S = stages<NT>(), kTileT = NT * BK, kAcc = acc_cols<NT>();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  // [S feature tiles][S token tiles][barriers]
+  uint8_t* sF = smem;
+  uint8_t* sT = sF + S * kTileF;
+  Bars* bars = reinterpret_cast<Bars*>(sT + S * kTileT);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = a.splits > 1 ? (int)(blockIdx.x % a.splits) : 0;
+  const int n0 = (int)(blockIdx.x / a.splits) * BM;  // first feature
+  const int m0 = (int)blockIdx.y * NT;               // first token
+  const int per = (a.ksteps + a.splits - 1) / a.splits;
+  const int k_lo = min(split * per, a.ksteps), k_hi = min(k_lo + per, a.ksteps);
+  const int nk = k_hi - k_lo;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    mbar_init(&bars->acc, 1);
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tmap_f);
+    prefetch_tmap(&tmap_t);
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_base, kAcc);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = bars->tmem_base;
+  pdl_trigger();
+  pdl_wait();  // the setup above overlaps the end of the kernel before
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int i = 0;
+      for (; i < nk; ++i) {
+        const int s = i % S, round = i / S, ks = k_lo + i;
+        if (round > 0 && !mbar_wait_to(&bars->empty[s], (round - 1) & 1, kErrTimeoutEmpty, a.err))
+          break;
+        mbar_expect_tx(&bars->full[s], kTileF + kTileT);
+        tma_load_2d(sF + s * kTileF, &tmap_f, &bars->full[s], ks * BK, n0);
+        tma_load_2d(sT + s * kTileT, &tmap_t, &bars->full[s], ks * BK, m0);
+      }
+      // the last copies land before the CTA may end, also where a wait gave up
+      for (int j = max(i - S, 0); j < i; ++j)
+        mbar_wait_to(&bars->full[j % S], (j / S) & 1, kErrTimeoutFull, a.err);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t id = make_idesc(/*S32*/ 2, /*signed*/ 1, 0, 0, BM, NT);
+      for (int i = 0; i < nk; ++i) {
+        const int s = i % S, round = i / S;
+        if (!mbar_wait_to(&bars->full[s], round & 1, kErrTimeoutFull, a.err)) break;
+        tc_fence_after();
+        const uint32_t pf = smem_u32(sF + s * kTileF), pt = smem_u32(sT + s * kTileT);
+#pragma unroll
+        for (int kk = 0; kk < BK / 32; ++kk)
+          mma_i8(tbase, desc_kmajor_sw128(pf + kk * 32), desc_kmajor_sw128(pt + kk * 32), id,
+                 (i > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(&bars->empty[s]);
+      }
+      mma_commit(&bars->acc);  // of all that were issued, also where a wait gave up
+    }
+  }
+  __syncwarp();  // warps 0 and 1 ran on one lane
+
+  // ── epilogue ──
+  const bool epi = warp >= 2;
+  const int q = warp & 3, half = (warp - 2) >> 2;  // TMEM lane quarter, column half
+  constexpr int kPer = NT >= 64 ? 32 : NT / 2;     // columns per tcgen05.ld
+  OutT* out = static_cast<OutT*>(a.out);
+  if (a.splits == 1) {
+    if (epi && mbar_wait_warp_to(&bars->acc, 0, kErrTimeoutDone, a.err)) {
+      tc_fence_after();
+      const int n = n0 + q * 32 + lane;
+      const float sf = n < a.N ? a.sf[(int64_t)n * a.sf_step] : 0.0f;
+      const float bv = a.bias && n < a.N ? a.bias[n] : 0.0f;
+#pragma unroll
+      for (int cb = 0; cb < (NT >= 64 ? NT / 64 : 1); ++cb) {
+        const int c0 = half * (NT / 2) + cb * kPer;
+        if (m0 + c0 >= a.M) break;
+        uint32_t r[32];
+        tmem_ld32(tbase + ((uint32_t)(q * 32) << 16) + c0, r);
+        tmem_wait_ld();
+        tmem_landed(r);
+        if (n < a.N) {
+          OutT* o = out + (size_t)(m0 + c0) * a.N + n;
+          const float* st = a.st + (int64_t)(m0 + c0) * a.st_step;
+#pragma unroll
+          for (int j = 0; j < kPer; ++j)
+            if (m0 + c0 + j < a.M)
+              store1(o + (size_t)j * a.N, scaled((int)r[j], __ldg(st + j * a.st_step), sf, bv));
+        }
+      }
+    }
+  } else {
+    // partial tile -> the idle stage buffers, [token][feature]
+    int* part = reinterpret_cast<int*>(smem);
+    if (epi && nk > 0 && mbar_wait_warp_to(&bars->acc, 0, kErrTimeoutDone, a.err)) {
+      tc_fence_after();
+#pragma unroll
+      for (int cb = 0; cb < (NT >= 64 ? NT / 64 : 1); ++cb) {
+        const int c0 = half * (NT / 2) + cb * kPer;
+        if (m0 + c0 >= a.M) break;
+        uint32_t r[32];
+        tmem_ld32(tbase + ((uint32_t)(q * 32) << 16) + c0, r);
+        tmem_wait_ld();
+        tmem_landed(r);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) part[(c0 + j) * BM + q * 32 + lane] = (int)r[j];
+      }
+    }
+    cluster_sync();
+    // each rank adds its share of the tokens, four features a thread
+    const int toks = min(NT, a.M - m0);
+    const int ranks = min(a.splits, (a.ksteps + per - 1) / per);  // ranks with K values
+    const uint32_t base = smem_u32(part);
+    for (int u = split * kThreads + threadIdx.x; u < toks * (BM / 4); u += a.splits * kThreads) {
+      const int t = u / (BM / 4), f = (u % (BM / 4)) * 4;
+      int e[4] = {0, 0, 0, 0};
+      for (int r = 0; r < ranks; ++r) {
+        const int4 w = ld_cluster_i4(base + (uint32_t)(t * BM + f) * 4u, (uint32_t)r);
+        e[0] += w.x; e[1] += w.y; e[2] += w.z; e[3] += w.w;
+      }
+      const float st = a.st[(int64_t)(m0 + t) * a.st_step];
+      OutT* o = out + (size_t)(m0 + t) * a.N + n0 + f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n0 + f + j < a.N)
+          store1(o + j, scaled(e[j], st, a.sf[(int64_t)(n0 + f + j) * a.sf_step],
+                               a.bias ? a.bias[n0 + f + j] : 0.0f));
+    }
+    cluster_sync();  // the partial tiles are read: the CTAs may go
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (nk > 0) mbar_wait_to(&bars->acc, 0, kErrTimeoutDone, a.err);
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tbase, kAcc);
+  }
+}
+
+template <int NT, typename OutT>
+int launch(const CUtensorMap& tf, const CUtensorMap& tt, const Args& a, cudaStream_t st) {
+  auto kern = int8_gemm_kernel<NT, OutT>;
+  constexpr size_t smem = smem_bytes<NT>();
+  MXB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(cdiv(a.N, BM) * a.splits), (unsigned)cdiv(a.M, NT));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)a.splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  MXB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tf, tt, a));
+  MXB_LAUNCH_CHECK();
+  return MXB_OK;
+}
+
+// Rows of K bytes -> rows of Kp, zero from K on.
+__global__ void __launch_bounds__(256)
+    pad_rows_kernel(const uint8_t* __restrict__ a, int64_t ra, const uint8_t* __restrict__ b, int64_t rb, int K,
+                    int Kp, uint8_t* __restrict__ out) {
+  pdl_trigger();
+  pdl_wait();
+  const int chunks = Kp / 16;
+  const int64_t n = (ra + rb) * chunks;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int64_t row = i / chunks;
+    const int k0 = (int)(i - row * chunks) * 16;
+    const uint8_t* src = row < ra ? a + row * K : b + (row - ra) * K;
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (k0 + j < K) w[j >> 2] |= (uint32_t)__ldg(src + k0 + j) << (8 * (j & 3));
+    reinterpret_cast<uint4*>(out)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <typename OutT>
+int dispatch(const void* fcodes, const void* tcodes, int64_t ldk, Args& a, cudaStream_t st) {
+  const int64_t ft = cdiv(a.N, BM);
+  CUtensorMap tf, tt;
+  const int nt = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+  const int64_t tiles = ft * cdiv(a.M, nt);
+  int64_t splits = (nt >= 128 ? kSMs : 2 * kSMs) / tiles;
+  if (splits > a.ksteps / 2) splits = a.ksteps / 2;
+  if (splits > kMaxSplit) splits = kMaxSplit;
+  while (splits * splits > 2 * (int64_t)a.ksteps) --splits;
+  a.splits = (int)(splits < 1 ? 1 : splits);
+  if (!encode_tmap_2d(&tf, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, fcodes, (uint64_t)ldk, (uint64_t)a.N, BK, BM,
+                      CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !encode_tmap_2d(&tt, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, tcodes, (uint64_t)ldk, (uint64_t)a.M, BK, nt,
+                      CU_TENSOR_MAP_SWIZZLE_128B))
+    return MXB_E_CUDA;
+  switch (nt) {
+    case 16: return launch<16, OutT>(tf, tt, a, st);
+    case 32: return launch<32, OutT>(tf, tt, a, st);
+    case 64: return launch<64, OutT>(tf, tt, a, st);
+    default: return launch<128, OutT>(tf, tt, a, st);
+  }
+}
+
+int64_t padded(int64_t K) { return (K + 15) / 16 * 16; }
+
+}  // namespace i8g
+}  // namespace mxb
+
+extern "C" {
+
+size_t mxb_int8_matmul_workspace_size(int64_t M, int64_t K, int64_t N, int aligned) {
+  if (M <= 0 || K <= 0 || N <= 0 || (K % 16 == 0 && aligned)) return 0;
+  return (size_t)(M + N) * (size_t)i8g::padded(K);
+}
+
+int mxb_int8_matmul(const void* a_codes, const float* a_scales, int a_scale_step, const void* b_codes,
+                    const float* b_scales, int b_scale_step, int64_t M, int64_t K, int64_t N,
+                    const float* bias, void* out, int out_dtype, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  if (out_dtype != MXB_F32 && out_dtype != MXB_BF16) return MXB_E_DTYPE;
+  if (M < 0 || N < 0 || K <= 0 || K > i8g::kMaxK) return MXB_E_SHAPE;
+  if (M > 65535 * 128 || N >= (int64_t)1 << 30) return MXB_E_SHAPE;
+  if ((a_scale_step != 0 && a_scale_step != 1) || (b_scale_step != 0 && b_scale_step != 1)) return MXB_E_ARG;
+  if (M == 0 || N == 0) return MXB_OK;
+  if (!a_codes || !a_scales || !b_codes || !b_scales || !out) return MXB_E_ARG;
+  if (((uintptr_t)a_scales | (uintptr_t)b_scales | (uintptr_t)bias) % 4 ||
+      (uintptr_t)out % (out_dtype == MXB_BF16 ? 2 : 4) || (uintptr_t)workspace % 16)
+    return MXB_E_ALIGN;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  i8g::Args a = {};
+  a.sf = b_scales;
+  a.st = a_scales;
+  a.sf_step = b_scale_step;
+  a.st_step = a_scale_step;
+  a.bias = bias;
+  a.out = out;
+  a.err = device_error_ptr();
+  a.M = (int)M;
+  a.N = (int)N;
+  a.ksteps = (int)cdiv(K, i8g::BK);
+  const void *tc = a_codes, *fc = b_codes;
+  int64_t ldk = K;
+  // TMA wants rows that start at multiples of 16 bytes
+  if (K % 16 || ((uintptr_t)a_codes | (uintptr_t)b_codes) % 16) {
+    ldk = i8g::padded(K);
+    const size_t need = mxb_int8_matmul_workspace_size(M, K, N, 0);
+    if (need > 0) {
+      if (!workspace || workspace_bytes < need) return MXB_E_WORKSPACE;
+      const int64_t blocks = cdiv((M + N) * (ldk / 16), 256);
+      MXB_CUDA_TRY(launch_pdl(i8g::pad_rows_kernel, dim3((unsigned)(blocks < 16 * kSMs ? blocks : 16 * kSMs)),
+                              256, 0, st, static_cast<const uint8_t*>(a_codes), M,
+                              static_cast<const uint8_t*>(b_codes), N, (int)K, (int)ldk,
+                              static_cast<uint8_t*>(workspace)));
+      MXB_LAUNCH_CHECK();
+      tc = workspace;
+      fc = static_cast<uint8_t*>(workspace) + M * ldk;
+    }
+  }
+  return out_dtype == MXB_BF16 ? i8g::dispatch<__nv_bfloat16>(fc, tc, ldk, a, st)
+                               : i8g::dispatch<float>(fc, tc, ldk, a, st);
+}
+
+}  // extern "C"

@@ -129,6 +129,205 @@ __global__ void __launch_bounds__(kThreads)
   put_row<BITS, D>(y, b, r, part, vc, vs);
 }
 
+// ── append: keys and queries rotated on the way ─────────────────────────────
+// Pair i of a head row, (i, i + rot / 2) or with ILV (2 i, 2 i + 1), turns by
+// position * inv_freq[i].  A block takes TB tokens: it finds their cosines and
+// sines once, in 64 bits as float pairs hi + lo, and turns every head of q and k
+// with the fp32 halves.
+//
+// A key's codes and scale are those of the quantizer fed the rotation in 64 bits
+// rounded to fp32, bit for bit.  The fp32 rotation is off by at most
+// 4 * 2^-24 of the row's largest value, so only the values within 2^-20 of the
+// largest and those whose quotient comes within m 2^-20 of a border between two
+// codes are turned again in 64 bits.
+struct Rotary {
+  const int64_t* pos;  // [axes][axis_stride]
+  int64_t axis_stride;
+  const float* inv_freq;
+  int pairs;      // rot / 2
+  int end[3];     // first pair of axes 1 to 3
+};
+
+struct AppendRows {
+  const void *q, *k, *v;
+  int64_t T;
+  int Hq, H;  // Hq 0: no queries
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+  bool vec;
+};
+
+// Four consecutive values.
+__device__ __forceinline__ void load4v(const float* p, bool vec, float (&v)[4]) {
+  if (vec) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = p[i];
+  }
+}
+__device__ __forceinline__ void load4v(const __nv_bfloat16* p, bool vec, float (&v)[4]) {
+  if (vec) {
+    const uint2 r = __ldg(reinterpret_cast<const uint2*>(p));
+    v[0] = __uint_as_float(r.x << 16);
+    v[1] = __uint_as_float(r.x & 0xffff0000u);
+    v[2] = __uint_as_float(r.y << 16);
+    v[3] = __uint_as_float(r.y & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __bfloat162float(p[i]);
+  }
+}
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// cos and sin of an angle in 64 bits, however large: in turns, as a product and its
+// rounding error, so that the whole turns leave exactly.
+__device__ __forceinline__ void turn64(double angle, double& c, double& s) {
+  constexpr double kHi = 0.15915494309189535, kLo = -9.839338337591243e-18;  // 1 / (2 pi)
+  const double t = __dmul_rn(angle, kHi), lo = fma(angle, kLo, fma(angle, kHi, -t));
+  sincospi(2.0 * ((t - rint(t)) + lo), &s, &c);
+}
+
+constexpr int kAppendTokens = 4;  // at most, a block
+
+template <typename InT, int BITS, int D, bool ILV>
+__global__ void __launch_bounds__(kThreads)
+    kv_append_kernel(const AppendRows a, const Rotary ro, int TB, const int64_t* __restrict__ slots,
+                     int64_t n_slots, int page_shift, InT* __restrict__ q_out, uint8_t* __restrict__ kc,
+                     float* __restrict__ ks, uint8_t* __restrict__ vc, float* __restrict__ vs,
+                     int* __restrict__ err) {
+  constexpr int L = D / 8, kRows = kThreads / L;
+  constexpr float m = BITS == 8 ? 127.0f : 7.0f;
+  __shared__ float4 hi[kAppendTokens][D / 4];  // (cos, sin) of two pairs
+  __shared__ float4 lo[kAppendTokens][D / 4];
+  pdl_trigger();
+  pdl_wait();
+  const int64_t t0 = (int64_t)blockIdx.x * TB;
+  const int tokens = (int)min((int64_t)TB, a.T - t0);
+  for (int i = threadIdx.x; i < tokens * ro.pairs; i += kThreads) {
+    const int t = i / ro.pairs, p = i - t * ro.pairs;
+    const int axis = (p >= ro.end[0]) + (p >= ro.end[1]) + (p >= ro.end[2]);
+    double c, s;
+    turn64(__dmul_rn((double)ro.pos[axis * ro.axis_stride + t0 + t], (double)__ldg(ro.inv_freq + p)), c, s);
+    const float ch = (float)c, sh = (float)s;
+    reinterpret_cast<float2*>(hi[t])[p] = make_float2(ch, sh);
+    reinterpret_cast<float2*>(lo[t])[p] = make_float2((float)(c - (double)ch), (float)(s - (double)sh));
+  }
+  __syncthreads();
+  const int part = threadIdx.x % L, R = a.Hq + a.H;
+  // this lane's two runs of four values, and whether they turn
+  const bool turns = part < ro.pairs / 4;
+  const int oa = ILV || !turns ? part * 8 : part * 4, ob = ILV || !turns ? oa + 4 : ro.pairs + part * 4;
+  const int q_rows = tokens * a.Hq, units = tokens * R;
+  // q rows of all tokens, then the keys with the values beside them
+  for (int u0 = threadIdx.x / 32 * (32 / L); u0 < units; u0 += kRows) {
+    const int u = u0 + (threadIdx.x % 32) / L;
+    const bool live = u < units, is_q = u < q_rows;
+    const int row = live ? (is_q ? u : u - q_rows) : 0, per = is_q || !live ? a.Hq : a.H;
+    const int t = per ? row / per : 0, h = row - t * per;
+    float x[8], y[8], w[8];
+    float (&xa)[4] = *reinterpret_cast<float (*)[4]>(x), (&xb)[4] = *reinterpret_cast<float (*)[4]>(x + 4);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = w[j] = 0.0f;
+    int64_t slot = -1;
+    if (live) {
+      const InT* p = is_q ? static_cast<const InT*>(a.q) + (t0 + t) * a.q_ts + h * a.q_hs
+                          : static_cast<const InT*>(a.k) + (t0 + t) * a.k_ts + h * a.k_hs;
+      load4v(p + oa, a.vec, xa);
+      load4v(p + ob, a.vec, xb);
+      if (!is_q) {
+        slot = slots[t0 + t];
+        load8v(static_cast<const InT*>(a.v) + (t0 + t) * a.v_ts + h * a.v_hs + part * 8, a.vec, w);
+      }
+    }
+    // pair j of this lane: values (j, j + 4), or (2 j, 2 j + 1)
+    auto first = [](int j) { return ILV ? 2 * j : j; };
+    auto second = [](int j) { return ILV ? 2 * j + 1 : j + 4; };
+    float cs[8];  // cosine and sine of the four pairs
+    if (turns) {
+      const float4 c0 = hi[t][part * 2], c1 = hi[t][part * 2 + 1];
+      cs[0] = c0.x; cs[1] = c0.y; cs[2] = c0.z; cs[3] = c0.w;
+      cs[4] = c1.x; cs[5] = c1.y; cs[6] = c1.z; cs[7] = c1.w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float v0 = x[first(j)], v1 = x[second(j)], c = cs[2 * j], s = cs[2 * j + 1];
+        y[first(j)] = fmaf(v0, c, -__fmul_rn(v1, s));
+        y[second(j)] = fmaf(v0, s, __fmul_rn(v1, c));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = x[j];
+    }
+    if (live && is_q) {
+      InT* o = q_out + ((t0 + t) * a.Hq + h) * D;
+      store4(o + oa, *reinterpret_cast<float (*)[4]>(y));
+      store4(o + ob, *reinterpret_cast<float (*)[4]>(y + 4));
+    }
+    if (!__any_sync(0xffffffffu, live && !is_q)) continue;
+    // value j turned in 64 bits, rounded to fp32
+    auto again = [&](int j) -> float {
+      const int i = ILV ? j >> 1 : j & 3;
+      const float2 l = reinterpret_cast<const float2*>(lo[t])[part * 4 + i];
+      const double c = (double)cs[2 * i] + (double)l.x, s = (double)cs[2 * i + 1] + (double)l.y;
+      const double v0 = (double)x[first(i)], v1 = (double)x[second(i)];
+      return (float)(j == first(i) ? v0 * c - v1 * s : v0 * s + v1 * c);
+    };
+    float top = 0.0f, top_v = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      top = amax_step(top, y[j]);
+      top_v = amax_step(top_v, w[j]);
+    }
+#pragma unroll
+    for (int o = L >> 1; o > 0; o >>= 1) {
+      top = nan_max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      top_v = nan_max(top_v, __shfl_xor_sync(0xffffffffu, top_v, o));
+    }
+    if (ro.pairs > 0) {
+      const float near_top = top * (1.0f - 0x1p-20f);
+      float best = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (!(fabsf(y[j]) < near_top)) best = amax_step(best, turns ? again(j) : y[j]);
+#pragma unroll
+      for (int o = L >> 1; o > 0; o >>= 1) best = nan_max(best, __shfl_xor_sync(0xffffffffu, best, o));
+      top = best;
+    }
+    if (!live || is_q || slot < 0) continue;
+    if (slot >= n_slots) {
+      if (part == 0 && err) atomicCAS(err, 0, kErrIndexCode);
+      continue;
+    }
+    const int64_t r = (((slot >> page_shift) * a.H + h) << page_shift) + (slot & ((1 << page_shift) - 1));
+    put_row<BITS, D>(w, top_v, r, part, vc, vs);
+    const float si = __fmul_rn(__frcp_rn(nan_max(top, 1e-12f)), m);
+    const bool ok = si > 0.0f && si <= 3.4028235e38f;  // no infinity or NaN in the row
+    uint32_t c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float v = __fmul_rn(y[j], si);
+      if (turns && fabsf(v - rintf(v)) > 0.5f - m * 0x1p-20f) v = __fmul_rn(again(j), si);
+      c[j] = ok ? __float_as_uint(__fadd_rn(v, 12582912.0f)) & (BITS == 8 ? 255u : 15u) : 0u;
+    }
+    uint8_t* dst = kc + r * (D * BITS / 8);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint8_t* d = dst + (i ? ob : oa) * BITS / 8;
+      const uint32_t b = c[4 * i] | c[4 * i + 1] << BITS | c[4 * i + 2] << (2 * BITS) | c[4 * i + 3] << (3 * BITS);
+      if (BITS == 8) *reinterpret_cast<uint32_t*>(d) = b;
+      else *reinterpret_cast<uint16_t*>(d) = (uint16_t)b;
+    }
+    if (part == 0) ks[r] = __frcp_rn(si);
+  }
+}
+
 // blockIdx.y: sequence, blockIdx.z: 0 the keys, 1 the values.  A thread makes
 // 16 bytes of output; kU of them in flight.
 template <typename OutT, int BITS, int D>
@@ -236,6 +435,37 @@ int write_t(const void* k, const void* v, const WriteArgs& a, cudaStream_t st) {
   return MXB_OK;
 }
 
+struct AppendArgs {
+  AppendRows rows;
+  Rotary ro;
+  bool interleaved;
+  const int64_t* slots;
+  int64_t n_slots;
+  int page;
+  void* q_out;
+  uint8_t *kc, *vc;
+  float *ks, *vs;
+};
+
+template <typename InT, int BITS, int D>
+int append_t(const AppendArgs& a, cudaStream_t st) {
+  AppendRows r = a.rows;
+  const int64_t per = 16 / sizeof(InT);
+  r.vec = ((uintptr_t)r.q | (uintptr_t)r.k | (uintptr_t)r.v) % 16 == 0 && (r.Hq == 0 || (r.q_ts % per == 0 && r.q_hs % per == 0)) &&
+          r.k_ts % per == 0 && r.k_hs % per == 0 && r.v_ts % per == 0 && r.v_hs % per == 0;
+  // a block's tokens share nothing but its threads: one each until the SMs are full
+  const int64_t tb = cdiv(r.T, 4 * kSMs);
+  const int TB = (int)(tb < kAppendTokens ? tb : kAppendTokens);
+  const dim3 grid((unsigned)cdiv(r.T, TB));
+  auto go = [&](auto kern) -> int {
+    MXB_CUDA_TRY(launch_pdl(kern, grid, kThreads, 0, st, r, a.ro, TB, a.slots, a.n_slots, shift_of(a.page),
+                            static_cast<InT*>(a.q_out), a.kc, a.ks, a.vc, a.vs, device_error_ptr()));
+    MXB_LAUNCH_CHECK();
+    return MXB_OK;
+  };
+  return a.interleaved ? go(kv_append_kernel<InT, BITS, D, true>) : go(kv_append_kernel<InT, BITS, D, false>);
+}
+
 struct ReadArgs {
   const uint8_t *kc, *vc;
   const float *ks, *vs;
@@ -268,6 +498,11 @@ template <typename T, int BITS, int D>
 struct Write {
   template <typename... A>
   static int run(A&&... a) { return write_t<T, BITS, D>(a...); }
+};
+template <typename T, int BITS, int D>
+struct Append {
+  template <typename... A>
+  static int run(A&&... a) { return append_t<T, BITS, D>(a...); }
 };
 template <typename T, int BITS, int D>
 struct Read {
@@ -322,6 +557,44 @@ int mxb_kv_write(const void* k, const void* v, int x_dtype, int64_t T, int heads
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return x_dtype == MXB_BF16 ? by_format<__nv_bfloat16, Write>(bits, dim, k, v, a, st)
                              : by_format<float, Write>(bits, dim, k, v, a, st);
+}
+
+int mxb_kv_append(const void* q, const void* k, const void* v, int x_dtype, int64_t T, int q_heads, int heads,
+                  int dim, int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                  int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                  const int64_t* positions, int axes, int64_t axis_stride, const float* inv_freq, int rot,
+                  const int* sections, int interleaved, const int64_t* slots, int64_t n_pages, int page,
+                  int bits, void* k_codes, float* k_scales, void* v_codes, float* v_scales, void* q_out,
+                  void* stream) {
+  if (x_dtype != MXB_F32 && x_dtype != MXB_BF16) return MXB_E_DTYPE;
+  const int rc = kv_pool_check(n_pages, heads, page, dim, bits, k_codes, k_scales, v_codes, v_scales);
+  if (rc != MXB_OK) return rc;
+  if (T < 0 || q_heads < 0 || q_heads > 65535 || rot < 0 || rot > dim || rot % 8 || axes < 1 || axes > 4)
+    return MXB_E_SHAPE;
+  if ((int64_t)kAppendTokens * (q_heads + heads) > INT32_MAX || T > ((int64_t)1 << 31)) return MXB_E_SHAPE;
+  if (axes > 1 && !sections) return MXB_E_ARG;
+  Rotary ro = {positions, axis_stride, inv_freq, rot / 2, {INT32_MAX, INT32_MAX, INT32_MAX}};
+  int64_t at = 0;
+  for (int i = 0; i < axes && axes > 1; ++i) {
+    if (sections[i] < 0) return MXB_E_SHAPE;
+    if (i > 0) ro.end[i - 1] = (int)at;
+    at += sections[i];
+  }
+  if (axes > 1 && at != rot / 2) return MXB_E_SHAPE;
+  if (T == 0) return MXB_OK;
+  if (!k || !v || !slots || (q_heads > 0 && (!q || !q_out)) || (rot > 0 && (!positions || !inv_freq)))
+    return MXB_E_ARG;
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % (x_dtype == MXB_BF16 ? 2 : 4) ||
+      (q_heads > 0 && (uintptr_t)q_out % 16) || ((uintptr_t)positions | (uintptr_t)slots) % 8 ||
+      (uintptr_t)inv_freq % 4)
+    return MXB_E_ALIGN;
+  AppendArgs a = {{q_heads > 0 ? q : nullptr, k, v, T, q_heads, heads, q_token_stride, q_head_stride, k_token_stride,
+                   k_head_stride, v_token_stride, v_head_stride, false},
+                  ro, interleaved != 0, slots, n_pages * page, page, q_out, static_cast<uint8_t*>(k_codes),
+                  static_cast<uint8_t*>(v_codes), k_scales, v_scales};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return x_dtype == MXB_BF16 ? by_format<__nv_bfloat16, Append>(bits, dim, a, st)
+                             : by_format<float, Append>(bits, dim, a, st);
 }
 
 int mxb_kv_read(const void* k_codes, const float* k_scales, const void* v_codes,

@@ -120,6 +120,10 @@ struct Args {
   __nv_bfloat16* out;
   float* lse;
   int* err;
+  // TREE: query t sees newest key i of its sequence where tree[b tree_b + t tree_t + i]
+  // is not 0
+  const uint8_t* tree;
+  int64_t tree_b, tree_t;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
@@ -248,7 +252,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& before, int64_
   return total;
 }
 
-template <int BITS, int D, int NT>
+template <int BITS, int D, int NT, bool TREE>
 __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
     paged_attn_kernel(const __grid_constant__ CUtensorMap tmap_k,
                       const __grid_constant__ CUtensorMap tmap_v, const Args a) {
@@ -527,10 +531,10 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
         cfac[n][e] = __shfl_sync(0xffffffffu, fac, (2 * c + e) * 4);
         const int rr = r0 + 8 * n + 2 * c + e;
         limit[n][e] = len;
-        if (own && rr < a.rows) limit[n][e] = len - (a.T - 1 - rr / a.G);
+        if (own && rr < a.rows) limit[n][e] = TREE ? len - a.T : len - (a.T - 1 - rr / a.G);
       }
     }
-    const int lim_min = own ? len - (a.T - 1) : len;
+    const int lim_min = own ? len - (TREE ? a.T : a.T - 1) : len;
     if constexpr (kQs) {
       if (warp == 0) {
 #pragma unroll
@@ -656,8 +660,19 @@ __global__ void __launch_bounds__(kThreads, Geo<BITS, D, NT>::kCtas)
           for (int i = 0; i < 4; ++i) {
             float2 v = unpack2(v2[i]), w = unpack2(w2[i]);
             const int key = (hide >> (i >> 1)) & 1u ? INT32_MAX : key0 + 8 * i;
-            if (key >= limit[n][0]) v.x = w.x = -INFINITY;  // whatever its scales hold
-            if (key >= limit[n][1]) v.y = w.y = -INFINITY;
+            if constexpr (TREE) {
+              // from limit on the T newest keys, as far as the row's mask names them
+              if (key >= limit[n][0]) {
+                const int rr = r0 + 8 * n + 2 * c, at = key - limit[n][0];
+                const uint8_t* mask = a.tree + b * a.tree_b + at;
+                if (key >= len || rr >= a.rows || !__ldg(mask + rr / a.G * a.tree_t)) v.x = w.x = -INFINITY;
+                if (key >= len || rr + 1 >= a.rows || !__ldg(mask + (rr + 1) / a.G * a.tree_t))
+                  v.y = w.y = -INFINITY;
+              }
+            } else {
+              if (key >= limit[n][0]) v.x = w.x = -INFINITY;  // whatever its scales hold
+              if (key >= limit[n][1]) v.y = w.y = -INFINITY;
+            }
             v2[i] = pack2(v.x, v.y);
             w2[i] = pack2(w.x, w.y);
           }
@@ -1090,9 +1105,9 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, in
   return p;
 }
 
-template <int BITS, int D, int NT>
+template <int BITS, int D, int NT, bool TREE>
 int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, dim3 grid, cudaStream_t st) {
-  auto kern = paged_attn_kernel<BITS, D, NT>;
+  auto kern = paged_attn_kernel<BITS, D, NT, TREE>;
   constexpr size_t smem = Geo<BITS, D, NT>::kSmem;
   MXB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   MXB_CUDA_TRY(launch_pdl(kern, grid, kThreads, smem, st, tk, tv, a));
@@ -1100,24 +1115,25 @@ int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, dim3 gri
   return MXB_OK;
 }
 
-template <int BITS, int D>
+template <int BITS, int D, bool TREE>
 int launch_nt(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int nt, dim3 grid,
               cudaStream_t st) {
   switch (nt) {
-    case 1: return launch<BITS, D, 1>(tk, tv, a, grid, st);
-    case 2: return launch<BITS, D, 2>(tk, tv, a, grid, st);
-    case 3: return launch<BITS, D, 3>(tk, tv, a, grid, st);
-    default: return launch<BITS, D, 4>(tk, tv, a, grid, st);
+    case 1: return launch<BITS, D, 1, TREE>(tk, tv, a, grid, st);
+    case 2: return launch<BITS, D, 2, TREE>(tk, tv, a, grid, st);
+    case 3: return launch<BITS, D, 3, TREE>(tk, tv, a, grid, st);
+    default: return launch<BITS, D, 4, TREE>(tk, tv, a, grid, st);
   }
 }
 
+template <bool TREE>
 int launch_any(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int bits, int dim,
                int nt, dim3 grid, cudaStream_t st) {
   if (bits == 8)
-    return dim == 128 ? launch_nt<8, 128>(tk, tv, a, nt, grid, st)
-                      : launch_nt<8, 64>(tk, tv, a, nt, grid, st);
-  return dim == 128 ? launch_nt<4, 128>(tk, tv, a, nt, grid, st)
-                    : launch_nt<4, 64>(tk, tv, a, nt, grid, st);
+    return dim == 128 ? launch_nt<8, 128, TREE>(tk, tv, a, nt, grid, st)
+                      : launch_nt<8, 64, TREE>(tk, tv, a, nt, grid, st);
+  return dim == 128 ? launch_nt<4, 128, TREE>(tk, tv, a, nt, grid, st)
+                    : launch_nt<4, 64, TREE>(tk, tv, a, nt, grid, st);
 }
 
 Part part_at(void* ws, size_t off, size_t rows, int dim) {
@@ -1125,24 +1141,12 @@ Part part_at(void* ws, size_t off, size_t rows, int dim) {
   return {reinterpret_cast<float*>(p), reinterpret_cast<float4*>(p + rows * dim * 4)};
 }
 
-}  // namespace pattn
-}  // namespace mxb
-
-extern "C" {
-
-size_t mxb_paged_attention_workspace_size(int64_t B, int64_t T, int heads, int group, int dim,
-                                          int bits, int page, int64_t width, int64_t prefix_len) {
-  if (B <= 0 || T <= 0 || heads <= 0 || group <= 0 || dim <= 0 || page <= 0 || bits <= 0) return 0;
-  return pattn::make_plan(B, T, heads, group, dim, bits, width * page, prefix_len).bytes;
-}
-
-int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim,
-                        const void* k_codes, const float* k_scales, const void* v_codes,
-                        const float* v_scales, int64_t n_pages, int page, int bits,
-                        const int* table, int64_t width, const int* lengths,
-                        const int* prefix_table, int64_t prefix_width, int64_t prefix_len,
-                        float scale, void* out, float* lse, void* workspace,
-                        size_t workspace_bytes, void* stream) {
+// A call; tree null: the causal order of the newest tokens.
+int attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim, const void* k_codes,
+              const float* k_scales, const void* v_codes, const float* v_scales, int64_t n_pages, int page,
+              int bits, const int* table, int64_t width, const int* lengths, const int* prefix_table,
+              int64_t prefix_width, int64_t prefix_len, const uint8_t* tree, int64_t tree_b, int64_t tree_t,
+              float scale, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
   const int rc = kv_pool_check(n_pages, heads, page, dim, bits, k_codes, k_scales, v_codes, v_scales);
   if (rc != MXB_OK) return rc;
   if (B < 0 || B > 65535 || T < 0 || T > 65535 || group <= 0 || group > 1024 || width < 0 ||
@@ -1155,19 +1159,19 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
     return MXB_E_ARG;
   // parts are stored 32 bytes at a time
   if (((uintptr_t)q | (uintptr_t)out) % 16 || (uintptr_t)workspace % 32) return MXB_E_ALIGN;
-  const pattn::Plan p =
-      pattn::make_plan(B, T, heads, group, dim, bits, width * page, prefix_len);
+  const Plan p =
+      make_plan(B, T, heads, group, dim, bits, width * page, prefix_len);
   const int64_t pre_rows = B * T * group;
   if ((int64_t)p.tiles_own * heads > 65535 || (int64_t)p.tiles_pre * heads > 65535 ||
       (p.splits_pre > 0 && p.nt_pre == 0 && cdiv(pre_rows, prefix_rows_per_cta(pre_rows)) > 65535) ||
       B * heads * p.tiles_own > INT32_MAX || B * T * heads * group > INT32_MAX ||
-      (int64_t)heads * p.tiles_own * (width * page / pattn::kTile + 1) > INT32_MAX)
+      (int64_t)heads * p.tiles_own * (width * page / kTile + 1) > INT32_MAX)
     return MXB_E_SHAPE;
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return MXB_E_WORKSPACE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 
   CUtensorMap tk, tv;
-  const int box = page < pattn::kTile ? page : pattn::kTile;
+  const int box = page < kTile ? page : kTile;
   const uint64_t rb = (uint64_t)dim * bits / 8, lines = (uint64_t)n_pages * heads * page * rb / 128;
   const uint32_t box_lines = (uint32_t)(box * rb / 128);
   if (!encode_tmap_2d(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, k_codes, 128, lines, 128, box_lines,
@@ -1176,7 +1180,7 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
                       CU_TENSOR_MAP_SWIZZLE_128B))
     return MXB_E_CUDA;
 
-  pattn::Args a = {};
+  Args a = {};
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.ks = k_scales;
   a.vs = v_scales;
@@ -1192,9 +1196,12 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
   a.out = static_cast<__nv_bfloat16*>(out);
   a.lse = lse;
   a.err = device_error_ptr();
-  pattn::Part pre = {}, own = {}, cta = {};
+  a.tree = tree;
+  a.tree_b = tree_b;
+  a.tree_t = tree_t;
+  Part pre = {}, own = {}, cta = {};
   if (p.splits_pre > 0) {
-    pre = pattn::part_at(workspace, p.o_pre, (size_t)p.splits_pre * a.n_rows, dim);
+    pre = part_at(workspace, p.o_pre, (size_t)p.splits_pre * a.n_rows, dim);
     a.table = prefix_table;
     a.width = (int)prefix_width;
     a.prefix_len = (int)prefix_len;
@@ -1228,7 +1235,7 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
       x.err = a.err;
       r = prefix_attention(x, st);
     } else {
-      r = pattn::launch_any(tk, tv, a, bits, dim, p.nt_pre,
+      r = launch_any<false>(tk, tv, a, bits, dim, p.nt_pre,
                             dim3((unsigned)p.splits_pre, (unsigned)(p.tiles_pre * heads)), st);
     }
     if (r != MXB_OK) return r;
@@ -1241,31 +1248,74 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
   a.whole = p.whole;
   a.direct = p.splits_pre == 0;
   if (p.ctas_own > 0) {
-    if (p.join) own = pattn::part_at(workspace, p.o_main, (size_t)a.n_rows, dim);
+    if (p.join) own = part_at(workspace, p.o_main, (size_t)a.n_rows, dim);
     if (!p.whole) {
-      cta = pattn::part_at(workspace, p.o_cta, (size_t)p.ctas_own * 8 * p.nt_own, dim);
+      cta = part_at(workspace, p.o_cta, (size_t)p.ctas_own * 8 * p.nt_own, dim);
       a.plan = reinterpret_cast<int64_t*>(static_cast<char*>(workspace) + p.o_plan);
     }
     a.main = own;
     a.cta = cta;
-    const int r =
-        pattn::launch_any(tk, tv, a, bits, dim, p.nt_own, dim3((unsigned)p.ctas_own), st);
+    const dim3 grid((unsigned)p.ctas_own);
+    const int r = tree ? launch_any<true>(tk, tv, a, bits, dim, p.nt_own, grid, st)
+                       : launch_any<false>(tk, tv, a, bits, dim, p.nt_own, grid, st);
     if (r != MXB_OK) return r;
   }
   if (p.join) {
-    pattn::JoinArgs j = {own, cta, pre, a.plan, p.ctas_own > 0 ? lengths : nullptr, width * page,
+    JoinArgs j = {own, cta, pre, a.plan, p.ctas_own > 0 ? lengths : nullptr, width * page,
                          a.n_rows, p.splits_pre, (int)T, heads, group, p.tiles_own, 8 * p.nt_own,
                          a.direct, a.out, lse};
-    const bool many = a.n_rows >= pattn::kJoinManyRows;
-    auto kern = dim == 128 ? (many ? pattn::paged_join_kernel<128, pattn::kWarps>
-                                   : pattn::paged_join_kernel<128, 1>)
-                           : (many ? pattn::paged_join_kernel<64, pattn::kWarps>
-                                   : pattn::paged_join_kernel<64, 1>);
-    MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)(many ? cdiv(a.n_rows, pattn::kWarps) : a.n_rows)),
-                            pattn::kThreads, 0, st, j));
+    const bool many = a.n_rows >= kJoinManyRows;
+    auto kern = dim == 128 ? (many ? paged_join_kernel<128, kWarps>
+                                   : paged_join_kernel<128, 1>)
+                           : (many ? paged_join_kernel<64, kWarps>
+                                   : paged_join_kernel<64, 1>);
+    MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)(many ? cdiv(a.n_rows, kWarps) : a.n_rows)),
+                            kThreads, 0, st, j));
     MXB_LAUNCH_CHECK();
   }
   return MXB_OK;
+}
+
+}  // namespace pattn
+}  // namespace mxb
+
+extern "C" {
+
+size_t mxb_paged_attention_workspace_size(int64_t B, int64_t T, int heads, int group, int dim,
+                                          int bits, int page, int64_t width, int64_t prefix_len) {
+  if (B <= 0 || T <= 0 || heads <= 0 || group <= 0 || dim <= 0 || page <= 0 || bits <= 0) return 0;
+  return pattn::make_plan(B, T, heads, group, dim, bits, width * page, prefix_len).bytes;
+}
+
+int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim,
+                        const void* k_codes, const float* k_scales, const void* v_codes,
+                        const float* v_scales, int64_t n_pages, int page, int bits,
+                        const int* table, int64_t width, const int* lengths,
+                        const int* prefix_table, int64_t prefix_width, int64_t prefix_len,
+                        float scale, void* out, float* lse, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  return pattn::attention(q, B, T, heads, group, dim, k_codes, k_scales, v_codes, v_scales, n_pages, page, bits,
+                          table, width, lengths, prefix_table, prefix_width, prefix_len, nullptr, 0, 0, scale,
+                          out, lse, workspace, workspace_bytes, stream);
+}
+
+size_t mxb_tree_attention_workspace_size(int64_t B, int64_t T, int heads, int group, int dim, int bits,
+                                         int page, int64_t width, int64_t prefix_len) {
+  return mxb_paged_attention_workspace_size(B, T, heads, group, dim, bits, page, width, prefix_len);
+}
+
+int mxb_tree_attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim, const void* k_codes,
+                       const float* k_scales, const void* v_codes, const float* v_scales, int64_t n_pages,
+                       int page, int bits, const int* table, int64_t width, const int* lengths,
+                       const int* prefix_table, int64_t prefix_width, int64_t prefix_len,
+                       const uint8_t* tree_mask, int64_t tree_batch_stride, int64_t tree_token_stride,
+                       float scale, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  if (B > 0 && T > 0 && !tree_mask) return MXB_E_ARG;
+  return pattn::attention(q, B, T, heads, group, dim, k_codes, k_scales, v_codes, v_scales, n_pages, page, bits,
+                          table, width, lengths, prefix_table, prefix_width, prefix_len, tree_mask,
+                          tree_batch_stride, tree_token_stride, scale, out, lse, workspace, workspace_bytes,
+                          stream);
 }
 
 }  // extern "C"

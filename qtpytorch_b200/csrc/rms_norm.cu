@@ -1,0 +1,336 @@
+// Root-mean-square norm of rows, with the residual's addition in front and int8
+// codes with one scale a row behind:
+//
+//   h = x + r,  y = h w / sqrt(mean(h^2) + eps),
+//   s = max(amax|y|, 1e-12) / 127,  code = rint(y / s)   (ties to even)
+//
+// The quotient is 127 u / amax|u| of u = h w: the root cancels, so a row's sum
+// of squares and its largest u are found in the same pass and the codes need one
+// reduction, not two.
+//
+// The codes are the ones of exact arithmetic.  The fp32 quotient is off by less
+// than 127 * 2^-22 (h, u and the factor 127 / amax are rounded once each, as is
+// their product); where it comes within twice that of a border between two codes
+// it is found again in 64 bits from x, r and w, whose sums and products 64 bits
+// hold.  That meets 1 value in 8000.  The largest u is found in 64 bits too, among
+// those within 2^-22 of the fp32 one.  Rows that hold infinities or NaN, or whose
+// values leave the range in which all this holds, take a slow path in 64 bits.
+//
+// One pass over HBM: a row stays in the registers of its block, 8 NC values a
+// thread.
+#include "mxb_common.cuh"
+#include "mxb_internal.h"
+
+using namespace mxb;
+
+namespace {
+
+constexpr int kWarpRows = 8;     // rows a block where a row is a warp's
+constexpr int kMaxRow = 32768;   // 1024 threads of 32 values
+
+// 8 consecutive values at p + i (VEC: 16-byte aligned; i + 8 <= d).
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+  const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+  const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&t);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <typename InT, typename WT>
+struct Row {
+  const InT* x;
+  const InT* r;  // null: none
+  const WT* w;
+  int d;
+  __device__ __forceinline__ double h64(int i) const {
+    double h = (double)load_as_f32(x, i);
+    if (r) h += (double)load_as_f32(r, i);
+    return h;
+  }
+  __device__ __forceinline__ float h32(int i) const {
+    float h = load_as_f32(x, i);
+    if (r) h = __fadd_rn(h, load_as_f32(r, i));
+    return h;
+  }
+  __device__ __noinline__ double u64(int i) const { return h64(i) * (double)load_as_f32(w, i); }
+};
+
+struct Shared {
+  float ssq[32], top[32];
+  double dsq[32], dtop[32];
+  unsigned long long most;  // bits of the largest |u| in 64 bits
+};
+
+// The slow path: everything in 64 bits, the row read again.  t of n threads;
+// the reductions are the warp's, then (n > 32) the block's.
+template <typename InT, typename WT>
+__device__ __noinline__ void row_in_64_bits(const Row<InT, WT>& row, double eps, int t, int n, Shared* sm,
+                                            int8_t* code, float* scale, InT* h_out) {
+  double ssq = 0.0, top = 0.0;
+  bool bad = false;  // an infinity or NaN
+  for (int i = t; i < row.d; i += n) {
+    const double h = row.h64(i), u = fabs(row.u64(i));
+    if (h_out) store1(h_out + i, row.h32(i));
+    bad |= !(u <= 1.7976931348623157e308) || !(fabs(h) <= 1.7976931348623157e308);
+    ssq += h * h;
+    top = fmax(top, u);
+  }
+  if (bad) ssq = __longlong_as_double(0x7ff8000000000000ll);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
+    top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  if (n > 32) {
+    if ((t & 31) == 0) {
+      sm->dsq[t >> 5] = ssq;
+      sm->dtop[t >> 5] = top;
+    }
+    __syncthreads();
+    ssq = top = 0.0;
+    for (int i = 0; i < n >> 5; ++i) {
+      ssq += sm->dsq[i];
+      top = fmax(top, sm->dtop[i]);
+    }
+  }
+  const double root = sqrt(ssq / row.d + eps);
+  // no root (eps 0 and a row of zeros) leaves 0 / 0
+  const bool ok = root > 0.0 && root <= 1.7976931348623157e308;
+  const double den = fmax(top, 1e-12 * root);
+  for (int i = t; i < row.d; i += n)
+    code[i] = ok ? (int8_t)__double2int_rn(__ddiv_rn(127.0 * row.u64(i), den)) : (int8_t)0;
+  if (t == 0) *scale = ok ? (float)(den / root / 127.0) : __int_as_float(0x7fc00000);
+}
+
+// WARP: a warp a row, kWarpRows of them a block; otherwise a block of up to MAX
+// threads a row.
+template <typename InT, typename WT, int NC, int MAX, bool VEC, bool WARP>
+__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : MAX)
+    rms_norm_kernel(const InT* __restrict__ x, const InT* __restrict__ r, int64_t rows, int d, int64_t ldx,
+                    int64_t ldr, const WT* __restrict__ w, double eps, float inv_d, int8_t* __restrict__ codes,
+                    float* __restrict__ scales, InT* __restrict__ h_out) {
+  __shared__ Shared sm;
+  const int t = WARP ? threadIdx.x & 31 : threadIdx.x, n = WARP ? 32 : blockDim.x;
+  const int64_t at = WARP ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+  pdl_trigger();
+  if (!WARP && t == 0) sm.most = 0;
+  pdl_wait();
+  if (WARP && at >= rows) return;
+  const Row<InT, WT> row = {x + at * ldx, r ? r + at * ldr : nullptr, w, d};
+  int8_t* code = codes + at * d;
+  InT* ho = h_out ? h_out + at * d : nullptr;
+  if (d > kMaxRow) {  // longer than the registers
+    row_in_64_bits(row, eps, t, n, &sm, code, scales + at, ho);
+    return;
+  }
+  // value j of chunk c
+  auto index = [&](int c, int j) { return VEC ? (c * n + t) * 8 + j : (c * 8 + j) * n + t; };
+  float u[NC][8];
+  float ssq = 0.0f, top = 0.0f;
+  if constexpr (VEC) {
+    float xv[NC][8], rv[NC][8];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (index(c, 0) < d) {
+        load8(row.x + index(c, 0), xv[c]);
+        if (r) load8(row.r + index(c, 0), rv[c]);
+        load8(w + index(c, 0), u[c]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (index(c, 0) < d) {
+        if (r) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) xv[c][j] = __fadd_rn(xv[c][j], rv[c][j]);
+        }
+        if (ho) store8(ho + index(c, 0), xv[c]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          ssq = fmaf(xv[c][j], xv[c][j], ssq);
+          u[c][j] = __fmul_rn(xv[c][j], u[c][j]);
+          top = amax_step(top, u[c][j]);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = index(c, j);
+        u[c][j] = 0.0f;
+        if (i < d) {
+          const float h = row.h32(i);
+          if (ho) store1(ho + i, h);
+          ssq = fmaf(h, h, ssq);
+          u[c][j] = __fmul_rn(h, load_as_f32(w, i));
+          top = amax_step(top, u[c][j]);
+        }
+      }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
+    top = nan_max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  if constexpr (!WARP) {
+    if ((t & 31) == 0) {
+      sm.ssq[t >> 5] = ssq;
+      sm.top[t >> 5] = top;
+    }
+    __syncthreads();
+    const int lane = t & 31, warps = n >> 5;
+    ssq = lane < warps ? sm.ssq[lane] : 0.0f;
+    top = lane < warps ? sm.top[lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
+      top = nan_max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+  }
+  // squares and products in the range in which fp32 holds them to 2^-24, the
+  // largest y above what the scale's lower bound asks for
+  const float root32 = sqrtf(fmaf(ssq, inv_d, (float)eps));
+  const bool fast = ssq >= 1e-30f && ssq <= 1e37f && top >= 1e-30f && top <= 1e37f && top >= 1.01e-12f * root32;
+  if (!fast) {  // the same for the whole row
+    row_in_64_bits<InT, WT>(row, eps, t, n, &sm, code, scales + at, nullptr);
+    return;
+  }
+  // ── the largest |u| in 64 bits, of those that fp32 cannot tell from it ──
+  const float near_top = top * (1.0f - 0x1p-21f);
+  double most = 0.0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (index(c, VEC ? 0 : j) < d && fabsf(u[c][j]) >= near_top) most = fmax(most, fabs(row.u64(index(c, j))));
+  if constexpr (WARP) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, o));
+  } else {
+    // bits of non-negative numbers rise with them
+    if (most > 0.0) atomicMax(&sm.most, (unsigned long long)__double_as_longlong(most));
+    __syncthreads();
+    most = __longlong_as_double((long long)sm.most);
+  }
+  const float factor = __fdiv_rn(127.0f, (float)most);
+  constexpr float kNear = 0.5f - 127.0f * 0x1p-21f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (VEC && index(c, 0) >= d) break;
+    int q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = __fmul_rn(u[c][j], factor), k = rintf(v);
+      q[j] = (int)k;
+      if (fabsf(v - k) > kNear && (VEC || index(c, j) < d))
+        q[j] = __double2int_rn(__ddiv_rn(127.0 * row.u64(index(c, j)), most));
+    }
+    if constexpr (VEC) {
+      uint32_t p[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        p[i] = (q[4 * i] & 255) | (q[4 * i + 1] & 255) << 8 | (q[4 * i + 2] & 255) << 16 |
+               (uint32_t)q[4 * i + 3] << 24;
+      *reinterpret_cast<uint2*>(code + index(c, 0)) = make_uint2(p[0], p[1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (index(c, j) < d) code[index(c, j)] = (int8_t)q[j];
+    }
+  }
+  if (t == 0) scales[at] = (float)(most / sqrt((double)ssq / d + eps) / 127.0);
+}
+
+struct NormArgs {
+  const void *x, *r, *w;
+  int64_t rows, d, ldx, ldr;
+  double eps;
+  int8_t* codes;
+  float* scales;
+  void* h;
+};
+
+template <typename InT, typename WT, int NC, int MAX, bool VEC, bool WARP>
+int launch(const NormArgs& a, int threads, cudaStream_t st) {
+  const int64_t blocks = WARP ? cdiv(a.rows, kWarpRows) : a.rows;
+  MXB_CUDA_TRY(launch_pdl(rms_norm_kernel<InT, WT, NC, MAX, VEC, WARP>, dim3((unsigned)blocks),
+                          WARP ? 32 * kWarpRows : threads, 0, st, static_cast<const InT*>(a.x),
+                          static_cast<const InT*>(a.r), a.rows, (int)a.d, a.ldx, a.ldr,
+                          static_cast<const WT*>(a.w), a.eps, (float)(1.0 / (double)a.d), a.codes, a.scales,
+                          static_cast<InT*>(a.h)));
+  MXB_LAUNCH_CHECK();
+  return MXB_OK;
+}
+
+template <typename InT, typename WT, bool VEC>
+int by_size(const NormArgs& a, cudaStream_t st) {
+  // threads of a row with 8 nc values each
+  auto threads = [&](int nc) { return (int)cdiv(cdiv(a.d, 8 * nc), 32) * 32; };
+  if (a.d > kMaxRow) return launch<InT, WT, 1, 1024, VEC, false>(a, 1024, st);
+  if (a.d <= 1024 && a.rows > kSMs) {
+    return a.d <= 256   ? launch<InT, WT, 1, 32, VEC, true>(a, 32, st)
+           : a.d <= 512 ? launch<InT, WT, 2, 32, VEC, true>(a, 32, st)
+                        : launch<InT, WT, 4, 32, VEC, true>(a, 32, st);
+  }
+  // few rows: as many threads as a row has use for
+  if (a.rows <= 2 * kSMs && threads(1) <= 1024) return launch<InT, WT, 1, 1024, VEC, false>(a, threads(1), st);
+  if (threads(4) <= 512) return launch<InT, WT, 4, 512, VEC, false>(a, threads(4), st);
+  return launch<InT, WT, 4, 1024, VEC, false>(a, threads(4), st);
+}
+
+template <typename InT>
+int by_type(const NormArgs& a, int w_dtype, cudaStream_t st) {
+  constexpr int64_t per = 16 / sizeof(InT);
+  const bool vec = a.d % 8 == 0 && a.ldx % per == 0 && (!a.r || a.ldr % per == 0) &&
+                   ((uintptr_t)a.x | (uintptr_t)a.r | (uintptr_t)a.w | (uintptr_t)a.h | (uintptr_t)a.codes) % 16 == 0;
+  if (w_dtype == MXB_BF16)
+    return vec ? by_size<InT, __nv_bfloat16, true>(a, st) : by_size<InT, __nv_bfloat16, false>(a, st);
+  return vec ? by_size<InT, float, true>(a, st) : by_size<InT, float, false>(a, st);
+}
+
+}  // namespace
+
+extern "C" int mxb_rms_norm_quantize(const void* x, const void* residual, int x_dtype, int64_t rows, int64_t d,
+                                     int64_t x_stride, int64_t residual_stride, const void* weight, int w_dtype,
+                                     double eps, void* codes, float* scales, void* sum, void* stream) {
+  if ((x_dtype != MXB_F32 && x_dtype != MXB_BF16) || (w_dtype != MXB_F32 && w_dtype != MXB_BF16))
+    return MXB_E_DTYPE;
+  if (rows < 0 || rows > INT32_MAX || d <= 0 || d > (int64_t)1 << 30) return MXB_E_SHAPE;
+  if (!(eps >= 0.0 && eps <= 1e30)) return MXB_E_ARG;
+  if (rows == 0) return MXB_OK;
+  if (!x || !weight || !codes || !scales) return MXB_E_ARG;
+  const uintptr_t xa = x_dtype == MXB_BF16 ? 2 : 4, wa = w_dtype == MXB_BF16 ? 2 : 4;
+  if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)sum) % xa || (uintptr_t)weight % wa ||
+      (uintptr_t)scales % 4)
+    return MXB_E_ALIGN;
+  const NormArgs a = {x, residual, weight, rows, d, x_stride, residual_stride, eps, static_cast<int8_t*>(codes),
+                      scales, sum};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return x_dtype == MXB_BF16 ? by_type<__nv_bfloat16>(a, w_dtype, st) : by_type<float>(a, w_dtype, st);
+}

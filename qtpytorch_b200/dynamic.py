@@ -10,7 +10,8 @@ Mirrors of mxtorch's ``dynamic_quantize`` (mxtorch.py:2665-2712),
   integer GEMM (tcgen05 ``kind::i8`` where the shape allows), which returns
   the fp32 sum over K-blocks of sx * sw * (integer dot product); the
   reference's CPU branch is F.linear of the dequantized operands, so the
-  result agrees to fp32 rounding.  A per-token x (one scale per row) meets
+  result agrees to fp32 rounding (one scale a row of both: the product of
+  ``int8_matmul``, which does not cut the sum).  A per-token x (one scale per row) meets
   the weight's K-blocks by repeating its scale per block.
 - ``mx_dynamic_linear``: the reference quantizes the activations but its
   output uses the fp32 activations and the dequantized weight (8960-8967),
@@ -26,7 +27,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import ops
+from . import int8, ops
 from .dtypes import get_mx_dtype, mx_dtype
 from .tensor import mx_tensor
 
@@ -101,8 +102,14 @@ def fused_int8_linear(x: mx_tensor, weight: mx_tensor, bias: Optional[torch.Tens
     if direct:
         sx = _kblock_scales(x, M, K, kb)
         sw = _kblock_scales(weight, N, K, kb)
-        _, _, out = ops.qgemm(x._mx_packed, sx, weight._mx_packed, sw, M, K, N, xd.bits, kb,
-                              32, b_kmajor=True)
+        if xd.bits == 8 and kb == K and K <= int8.MAX_K and x.device == weight.device:
+            # one scale a token and a channel: the same sums and roundings, not cut into K-blocks
+            out = torch.empty(M, N, dtype=torch.float32, device=x._mx_packed.device)
+            int8._product((x._mx_packed.contiguous(), sx, 1), (weight._mx_packed.contiguous(), sw, 1), M, K, N,
+                          None, out)
+        else:
+            _, _, out = ops.qgemm(x._mx_packed, sx, weight._mx_packed, sw, M, K, N, xd.bits, kb,
+                                  32, b_kmajor=True)
     elif ops.kernel_dtype_ok(wd) and weight._mx_n == N * K:
         # the dequantized x against the packed weight, read K-major as stored
         out = _kmajor_linear(x.dequantize().reshape(M, K), weight, K, N)

@@ -8,6 +8,8 @@ to any slot of a pool of pages, and attention reads the packed codes:
     cache.write(k, v, slots)                       # k, v [T, 8, 128]
     out = paged_attention(q, cache, table, lengths)  # q [B, T, Hq, 128] bf16
     out = paged_attention(q, cache, table, lengths, prefix_table=pages, prefix_len=5000)
+    q = cache.append(k, v, slots, positions, inv_freq, q=q)  # rotated on the way
+    out = paged_attention(q, cache, table, lengths, tree_mask=mask)  # a tree of drafts
 
 A token's slot is page number * page_size + offset; ``table`` [B, width] holds
 the page numbers of each sequence, ``lengths`` [B] its tokens.  A head row's codes
@@ -15,8 +17,10 @@ and scale are those of ``mx_tensor.quantize(row, dtype, head_dim)``.
 """
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
-from typing import Optional, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -122,6 +126,73 @@ class paged_kv_cache:
         if rc:
             L.check(rc, f"mxb_kv_write({self.dtype.name}, T={k.shape[0]})")
 
+    def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
+               inv_freq: torch.Tensor, q: Optional[torch.Tensor] = None,
+               sections: Optional[Sequence[int]] = None, interleaved: bool = False) -> Optional[torch.Tensor]:
+        """``write`` of keys rotated by their positions; ``q`` [T, heads of queries,
+        head_dim] is rotated beside them and returned (contiguous, in its type).
+
+        Pair i of a head row turns by ``positions[t] * inv_freq[i]`` (inv_freq fp32
+        [pairs], pairs a multiple of 4, at most head_dim / 2): elements (i, i +
+        pairs), or (2 i, 2 i + 1) where ``interleaved``; the others stay.  With
+        ``sections`` (pairs of each axis, up to four, in order) positions are
+        [axes, T], one row an axis.  Angles are found in 64 bits; a key's codes and
+        scale are those of its rotation in 64 bits rounded to fp32.  The queries of
+        skipped tokens are rotated too.  No gradient."""
+        dev = self._cuda("paged_kv_cache.append")
+        H, D = self.n_heads, self.head_dim
+        if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (H, D) or slots.shape != k.shape[:1]:
+            raise ValueError(f"append: k and v must be [T, {H}, {D}] and slots [T]; got "
+                             f"{tuple(k.shape)}, {tuple(v.shape)}, {tuple(slots.shape)}")
+        T = k.shape[0]
+        if q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != D):
+            raise ValueError(f"append: q must be [{T}, heads, {D}], got {tuple(q.shape)}")
+        pairs = inv_freq.shape[0] if inv_freq.dim() == 1 else -1
+        if pairs < 0 or pairs % 4 or pairs > D // 2 or not inv_freq.is_floating_point():
+            raise ValueError(f"append: inv_freq must hold a multiple of 4 of at most {D // 2} frequencies, "
+                             f"got {inv_freq.dtype} {tuple(inv_freq.shape)}")
+        axes, c_sections = 1, None
+        if sections is not None:
+            sections = tuple(int(x) for x in sections)
+            axes = len(sections)
+            if not 1 <= axes <= 4 or min(sections) < 0 or sum(sections) != pairs:
+                raise ValueError(f"append: sections must be one to four counts that add up to {pairs} pairs, "
+                                 f"not {sections}")
+            c_sections = _ints(sections)
+        want = (T,) if sections is None else (axes, T)
+        if positions.shape != want or positions.is_floating_point() or slots.is_floating_point():
+            raise ValueError(f"append: positions must be integers {list(want)}, got {positions.dtype} "
+                             f"{tuple(positions.shape)}")
+        for t in (k, v, slots, positions, inv_freq) if q is None else (k, v, slots, positions, inv_freq, q):
+            if t.device != dev:
+                raise ValueError(f"append: tensors must be on {dev}")
+        q_type = None if q is None else q.dtype
+        if k.dtype not in _IO or k.dtype != v.dtype or (q is not None and q_type != k.dtype):
+            k, v, q = k.float(), v.float(), None if q is None else q.float()
+        if k.stride(2) != 1:
+            k = k.contiguous()
+        if v.stride(2) != 1:
+            v = v.contiguous()
+        if q is not None and q.stride(2) != 1:
+            q = q.contiguous()
+        if slots.dtype != torch.int64 or not slots.is_contiguous():
+            slots = slots.to(torch.int64).contiguous()
+        if positions.dtype != torch.int64 or (T > 1 and positions.stride(-1) != 1):
+            positions = positions.to(torch.int64).contiguous()
+        if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+            inv_freq = inv_freq.float().contiguous()
+        out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=dev)
+        Hq = 0 if q is None else q.shape[1]
+        rc = L.call("mxb_kv_append", dev, L.ptr(q), k.data_ptr(), v.data_ptr(), _IO[k.dtype], T, Hq, H, D,
+                    0 if q is None else q.stride(0), 0 if q is None else q.stride(1), k.stride(0), k.stride(1),
+                    v.stride(0), v.stride(1), positions.data_ptr(), axes,
+                    positions.stride(0) if axes > 1 else 0, inv_freq.data_ptr(), 2 * pairs, c_sections,
+                    int(interleaved), slots.data_ptr(), self.n_pages, self.page_size, self.dtype.bits,
+                    *self._pool(), L.ptr(out))
+        if rc:
+            L.check(rc, f"mxb_kv_append({self.dtype.name}, T={T}, heads={Hq}+{H})")
+        return out if out is None or out.dtype == q_type else out.to(q_type)
+
     def read(self, table: torch.Tensor, lengths: torch.Tensor, max_len: int,
              dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
         """(k, v) [B, max_len, n_heads, head_dim] of the sequences' histories,
@@ -149,6 +220,11 @@ class paged_kv_cache:
     def __repr__(self):
         return (f"paged_kv_cache(pages={self.n_pages}, heads={self.n_heads}, dim={self.head_dim}, "
                 f"page={self.page_size}, dtype={self.dtype.name})")
+
+
+@functools.lru_cache(maxsize=256)
+def _ints(values: Tuple[int, ...]):
+    return (ctypes.c_int * len(values))(*values)
 
 
 def _int32(t: torch.Tensor) -> torch.Tensor:
@@ -179,7 +255,8 @@ def _tables(table: torch.Tensor, lengths: torch.Tensor, dev, what: str):
 
 def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
                     lengths: torch.Tensor, prefix_table: Optional[torch.Tensor] = None,
-                    prefix_len: int = 0, scale: Optional[float] = None, return_lse: bool = False):
+                    prefix_len: int = 0, scale: Optional[float] = None, return_lse: bool = False,
+                    tree_mask: Optional[torch.Tensor] = None):
     """softmax(scale * q k^T) v over a paged quantized cache.
 
     q [B, T, Hq, head_dim] bf16, Hq a multiple of the cache's heads (query head i
@@ -187,7 +264,9 @@ def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
     its T newest tokens included: query t sees the keys before
     lengths[b] - (T - 1 - t).  ``prefix_table`` [pages] and ``prefix_len`` name
     keys that every query sees in front of its own; they are read once for the
-    whole batch.  ``scale`` defaults to 1 / sqrt(head_dim).  A row without keys
+    whole batch.  ``tree_mask`` [T, T] or [B, T, T] bool: the T newest tokens are a
+    tree of drafts; query t sees all keys before them and of them those that row t
+    names (its own among them, if it is to be seen).  ``scale`` defaults to 1 / sqrt(head_dim).  A row without keys
     gives zeros; a page number outside the pool holds no keys (recorded in the
     library's device error word).  Returns out (q's shape, bf16), with ``return_lse`` also the fp32
     log-sum-exp [B, T, Hq] of the scaled scores.  No gradient."""
@@ -217,20 +296,31 @@ def paged_attention(q: torch.Tensor, cache: paged_kv_cache, table: torch.Tensor,
             raise ValueError(f"paged_attention: prefix_len {prefix_len} needs more than the "
                              f"{width} pages of prefix_table")
         prefix_table = _int32(prefix_table)
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.bool or tree_mask.shape not in ((T, T), (B, T, T)):
+            raise ValueError(f"paged_attention: tree_mask must be bool [{T}, {T}] or [{B}, {T}, {T}], got "
+                             f"{tree_mask.dtype} {tuple(tree_mask.shape)}")
+        if tree_mask.device != dev:
+            raise ValueError(f"paged_attention: tree_mask must be on {dev}")
+        if tree_mask.stride(-1) != 1:
+            tree_mask = tree_mask.contiguous()
     q = q.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
     out = torch.empty_like(q)
     lse = torch.empty(B, T, Hq, dtype=torch.float32, device=dev) if return_lse else None
-    wsb = L.size("mxb_paged_attention_workspace_size", B, T, H, Hq // H, D, cache.dtype.bits,
-                 cache.page_size, table.shape[1], prefix_len)
+    op = "mxb_paged_attention" if tree_mask is None else "mxb_tree_attention"
+    tree = () if tree_mask is None else (tree_mask.data_ptr(), tree_mask.stride(0) if tree_mask.dim() == 3 else 0,
+                                         tree_mask.stride(-2))
+    wsb = L.size(op + "_workspace_size", B, T, H, Hq // H, D, cache.dtype.bits, cache.page_size,
+                 table.shape[1], prefix_len)
     ws = L.workspace(wsb, dev)
-    rc = L.call("mxb_paged_attention", dev, q.data_ptr(), B, T, H, Hq // H, D,
+    rc = L.call(op, dev, q.data_ptr(), B, T, H, Hq // H, D,
                 *cache._pool(), cache.n_pages, cache.page_size, cache.dtype.bits,
                 table.data_ptr(), table.shape[1], lengths.data_ptr(),
-                prefix_table.data_ptr() if prefix_len else 0, width, prefix_len,
+                prefix_table.data_ptr() if prefix_len else 0, width, prefix_len, *tree,
                 1.0 / math.sqrt(D) if scale is None else float(scale), out.data_ptr(), L.ptr(lse),
                 L.ptr(ws), wsb)
     if rc:
-        L.check(rc, f"mxb_paged_attention(B={B}, T={T}, heads={H}x{Hq // H}, dim={D})")
+        L.check(rc, f"{op}(B={B}, T={T}, heads={H}x{Hq // H}, dim={D})")
     return (out, lse) if return_lse else out

@@ -1,0 +1,356 @@
+"""int8 with a scale a row: norm into codes, product, linear; against 64 bits.
+
+The norm's codes and the product's integer sums are exact, so both are compared
+for equality; the reference's counterpart of the product is ``fused_int8_linear``
+(mxtorch.py:3910-3960)."""
+import copy
+import ctypes
+import io
+
+import pytest
+import torch
+
+import qtpytorch_b200 as mxb
+from qtpytorch_b200 import _lib as L
+
+P = ctypes.c_void_p(32)
+
+
+# ── host ─────────────────────────────────────────────────────────────────────
+def test_argument_errors_need_no_gpu():
+    lib = L.load()
+
+    def norm(x=P, r=None, dt=1, rows=2, d=64, w=P, wt=1, eps=1e-6, codes=P, scales=P, h=None):
+        return lib.mxb_rms_norm_quantize(x, r, dt, rows, d, 64, 64, w, wt, eps, codes, scales, h, None)
+
+    assert norm(dt=2) == -2 and norm(wt=5) == -2
+    assert norm(rows=-1) == -1 and norm(d=0) == -1 and norm(d=(1 << 30) + 1) == -1 and norm(rows=1 << 31) == -1
+    assert norm(eps=-1.0) == -6 and norm(eps=float("nan")) == -6 and norm(eps=float("inf")) == -6
+    assert norm(x=None) == -6 and norm(w=None) == -6 and norm(codes=None) == -6 and norm(scales=None) == -6
+    odd = ctypes.c_void_p(33)
+    assert norm(x=odd) == -3 and norm(r=odd) == -3 and norm(h=odd) == -3 and norm(w=odd) == -3
+    assert norm(scales=ctypes.c_void_p(34)) == -3 and norm(dt=0, x=ctypes.c_void_p(34)) == -3
+    assert norm(rows=0) == 0
+
+    def product(a=P, sa=P, sta=1, b=P, sb=P, stb=1, M=2, K=64, N=3, bias=None, out=P, od=1, ws=None, n=0):
+        return lib.mxb_int8_matmul(a, sa, sta, b, sb, stb, M, K, N, bias, out, od, ws, n, None)
+
+    assert product(od=2) == -2
+    assert product(M=-1) == -1 and product(N=-1) == -1 and product(K=0) == -1 and product(K=131072) == -1
+    assert product(M=65535 * 128 + 1) == -1 and product(N=1 << 30) == -1
+    assert product(sta=2) == -6 and product(stb=-1) == -6
+    assert product(a=None) == -6 and product(sb=None) == -6 and product(out=None) == -6
+    assert product(out=odd) == -3 and product(sa=ctypes.c_void_p(34)) == -3 and product(bias=ctypes.c_void_p(34)) == -3
+    assert product(M=0) == 0 and product(N=0) == 0
+    size = lib.mxb_int8_matmul_workspace_size
+    assert size(2, 64, 3, 1) == 0 and size(2, 64, 3, 0) == 5 * 64 and size(2, 65, 3, 1) == 5 * 80
+    assert product(K=65) == -7 and product(K=65, ws=P, n=399) == -7 and product(a=odd) == -7
+    assert product(K=65, ws=ctypes.c_void_p(40), n=400) == -3
+
+
+def fake(rows, k, block=None, scales=None, dtype="int8d"):
+    block = k if block is None else block
+    n = -(-rows * k // block) if scales is None else scales
+    return mxb.mx_tensor(torch.zeros(rows * k, dtype=torch.int8), torch.ones(n), mxb.get_mx_dtype(dtype), (rows, k),
+                         rows * k, block)
+
+
+def test_refusals():
+    x, w = torch.zeros(2, 8), torch.ones(8)
+    with pytest.raises(L.MxbError):
+        mxb.rms_norm_quantize(x, w)  # on the CPU
+    with pytest.raises(L.MxbError):
+        mxb.int8_matmul(fake(2, 8), fake(3, 8))
+    with pytest.raises(TypeError):
+        mxb.int8_matmul(x, fake(3, 8))
+    for a, b, kw in ((fake(2, 8), fake(3, 9), {}), (fake(2, 8), fake(3, 8), dict(out_dtype=torch.float16)),
+                     (fake(2, 8, 4), fake(3, 8), {}), (fake(2, 8), fake(3, 8, 4), {})):
+        with pytest.raises(ValueError):
+            mxb.int8_matmul(a, b, **kw)
+    with pytest.raises(NotImplementedError):
+        mxb.int8_matmul(fake(2, 8, dtype="int4d"), fake(3, 8))
+    with pytest.raises(NotImplementedError):
+        mxb.int8_matmul(fake(2, 8, dtype="int8dh"), fake(3, 8))
+    big = 131072
+    with pytest.raises(NotImplementedError):
+        mxb.int8_matmul(fake(1, big), fake(1, big))
+    with pytest.raises(TypeError):
+        mxb.int8_linear(torch.zeros(3, 8))
+
+
+def test_linear_module_casts_and_copies():
+    lin = mxb.int8_linear(fake(3, 8), torch.ones(3))
+    for m in (copy.deepcopy(lin).bfloat16(), copy.deepcopy(lin).half(), copy.deepcopy(lin).to(torch.float64)):
+        assert m.weight_codes.dtype == torch.int8
+        assert m.weight_scales.dtype == torch.float32 and m.bias.dtype == torch.float32
+    buf = io.BytesIO()
+    torch.save(lin.state_dict(), buf)
+    buf.seek(0)
+    other = mxb.int8_linear(fake(3, 8), torch.zeros(3))
+    other.load_state_dict(torch.load(buf))
+    assert torch.equal(other.bias, lin.bias) and other.weight.shape == (3, 8)
+    one = mxb.int8_linear(fake(3, 8, block=24))  # one scale for the whole weight
+    assert one.weight_scales.shape == (3,)
+    with pytest.raises(ValueError):
+        lin(fake(2, 9))
+
+
+# ── norm ─────────────────────────────────────────────────────────────────────
+def norm64(x, w, r, eps):
+    h = x.double() if r is None else x.double() + r.double()
+    rms = torch.sqrt((h * h).mean(-1, keepdim=True) + eps)
+    u = h * w.double()
+    den = torch.maximum(u.abs().amax(-1, keepdim=True), 1e-12 * rms)
+    return torch.round(127 * u / den), (den / rms / 127)[..., 0]
+
+
+def check_norm(x, w, r=None, eps=1e-6):
+    got = mxb.rms_norm_quantize(x, w, residual=r, eps=eps)
+    if r is not None:
+        got, h = got
+        assert h.dtype == x.dtype and torch.equal(h, (x.float() + r.float()).to(x.dtype))
+    code, scale = norm64(x, w, r, eps)
+    assert got.shape == x.shape and got.mx_block == x.shape[-1] and got.mx_dtype.name == "int8d"
+    codes = got.packed.view(x.shape)
+    bad = codes.double() != code
+    assert not bool(bad.any()), (int(bad.sum()), bad.nonzero()[:3].tolist())
+    # the sum of squares: at most 32 fused steps a thread and 10 of the tree, each
+    # 2^-24, halved by the root; 2^-24 for the scale itself
+    d = (got.mx_scales.view(scale.shape).double() - scale).abs()
+    assert bool((d <= 2.0 ** -19 * scale).all())
+
+
+def rows(seed, *shape, loud=True):
+    g = torch.Generator("cuda").manual_seed(seed)
+    x = torch.randn(*shape, generator=g, device="cuda")
+    if loud:
+        x *= 1 + 20 * (torch.rand(shape[-1], generator=g, device="cuda") < 0.02)
+    return x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,d", [(1, 1), (3, 7), (200, 8), (5, 64), (300, 100), (149, 256), (700, 512), (150, 1000),
+                                 (2, 1024), (400, 1024), (33, 1999), (8, 4096), (500, 4096), (320, 8192), (3, 11008),
+                                 (300, 11008), (297, 16384), (2, 16384), (299, 20000), (1, 20001), (300, 32768),
+                                 (2, 32769)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm(dtype, n, d, residual):
+    x = rows(d, n, d).to(dtype)
+    r = rows(d + 1, n, d).mul_(3).to(dtype) if residual else None
+    w = (1 + 0.2 * rows(d + 2, d, loud=False)).to(dtype)
+    check_norm(x, w, r)
+
+
+@pytest.mark.gpu
+def test_norm_many_values_next_to_borders():
+    """Values k + 1/2 +- a few 2^-24 of a code, where fp32 alone rounds either way."""
+    g = torch.Generator("cuda").manual_seed(0)
+    k = torch.randint(-127, 127, (300, 4096), generator=g, device="cuda").double() + 0.5
+    k = k * (1 + torch.randint(-4, 5, k.shape, generator=g, device="cuda") * 2.0 ** -24)
+    k[:, 17] = 127.0
+    w = 0.5 + torch.rand(4096, generator=g, device="cuda")
+    check_norm((k / w.double()).float(), w)
+    check_norm((k / w.double()).float(), w, rows(3, 300, 4096).mul_(1e-6))
+    check_norm(k.float(), torch.ones(4096, device="cuda").bfloat16())  # ties among them
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(64, 24), (4, 3, 40)])
+def test_norm_strides_types_and_alignment(shape):
+    d = shape[-1]
+    w = 1 + 0.2 * rows(1, d, loud=False)
+    wide = rows(2, *shape[:-1], 3 * d)
+    x, r = wide[..., d:2 * d], wide[..., 2 * d:]
+    check_norm(x, w, r)
+    check_norm(wide.bfloat16()[..., 1:d + 1], w.bfloat16(), wide.bfloat16()[..., 7:d + 7])  # unaligned
+    check_norm(x, w.bfloat16())
+    check_norm(wide.bfloat16()[..., :d], w)
+    check_norm(x.transpose(0, -1).contiguous().transpose(0, -1), w)  # last dim strided
+    check_norm(x[:1].expand(5, *shape[1:]), w)                       # rows that share memory
+    h = x.half()
+    a, b = mxb.rms_norm_quantize(h, w), mxb.rms_norm_quantize(h.float(), w)
+    assert torch.equal(a.packed, b.packed) and torch.equal(a.mx_scales, b.mx_scales)
+    a, s = mxb.rms_norm_quantize(h, w, residual=r)  # mixed types go through fp32
+    b, t = mxb.rms_norm_quantize(h.float(), w, residual=r)
+    assert torch.equal(a.packed, b.packed) and s.dtype == torch.float16 and torch.equal(s, t.half())
+    a = mxb.rms_norm_quantize(x, w.double())
+    assert torch.equal(a.packed, mxb.rms_norm_quantize(x, w).packed)
+    e = mxb.rms_norm_quantize(x[..., :0, :] if len(shape) == 3 else x[:0], w)
+    assert e.numel() == 0 and e.mx_scales.numel() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d", [(3, 200), (400, 200), (2, 4096), (2, 40000)])
+def test_norm_rows_outside_the_usual_range(n, d):
+    w = torch.ones(d, device="cuda")
+    base = rows(5, n, d)
+    for size in (0.0, 1e-25, 1e-17, 1e-12, 1e15, 1e25, 1e36):
+        check_norm(base * size, w)
+        check_norm(base * size, w, eps=0.0) if size else None
+    check_norm(base, w * 1e-20)     # under the scale's lower bound
+    check_norm(base * 1e30, w * 1e30)  # products past fp32
+    z = mxb.rms_norm_quantize(base * 0, w)
+    assert not z.packed.any() and torch.equal(z.mx_scales, torch.full((n,), 1e-12 / 127, device="cuda"))
+    x = base.clone()
+    x[0, 3], x[1, d - 1] = float("nan"), float("-inf")
+    z = mxb.rms_norm_quantize(x, w)
+    assert z.mx_scales[:2].isnan().all() and not z.packed.view(n, d)[:2].any()
+    if n > 2:
+        assert z.mx_scales[2:].isfinite().all() and z.packed.view(n, d)[2:].any()
+    assert mxb.rms_norm_quantize(base * 0, w, eps=0.0).mx_scales.isnan().all()  # 0 / 0
+
+
+@pytest.mark.gpu
+def test_norm_refusals_on_the_device():
+    x, w = torch.zeros(2, 8, device="cuda"), torch.ones(8, device="cuda")
+    for a in ((x, w[:7]), (x, w.cpu()), (x[0, 0], w), (x.int(), w), (x, w.int()), (x[:, :0], w[:0])):
+        with pytest.raises(ValueError):
+            mxb.rms_norm_quantize(*a)
+    for kw in (dict(residual=x[:1]), dict(residual=x.cpu()), dict(residual=x.int()), dict(eps=-1e-6),
+               dict(eps=float("nan"))):
+        with pytest.raises(ValueError):
+            mxb.rms_norm_quantize(x, w, **kw)
+
+
+# ── product ──────────────────────────────────────────────────────────────────
+def operand(n, k, seed, block=None, full=False):
+    g = torch.Generator("cuda").manual_seed(seed)
+    codes = torch.randint(-128 if full else -127, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    count = n if block is None else 1
+    scales = torch.rand(count, generator=g, device="cuda") * 0.02 + 1e-3
+    return mxb.mx_tensor(codes.view(-1), scales, mxb.int8d, (n, k), n * k, k if block is None else max(n * k, 1))
+
+
+def product_ref(a, b, bias, dtype):
+    """The integer sum exactly, then the documented roundings."""
+    (M, K), N = a.shape, b.shape[0]
+    p = torch.mm(a.packed.view(M, K).double(), b.packed.view(N, K).double().t())
+    y = p.float() * a.mx_scales.view(-1, 1) * b.mx_scales.view(1, -1)
+    return (y if bias is None else y + bias).to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k,n", [
+    (1, 1, 1), (2, 15, 5), (1, 16, 8), (3, 31, 127), (16, 128, 128), (17, 129, 130), (33, 257, 64), (1, 4096, 1000),
+    (64, 1000, 96), (65, 640, 200), (5, 11008, 300), (128, 512, 256), (129, 130, 1), (200, 2048, 1000),
+    (300, 4096, 130), (1000, 333, 257), (513, 1024, 640), (1, 2048, 11008), (2300, 64, 64), (700, 1600, 1928),
+    (2048, 1024, 2048), (1111, 4096, 3000)])
+def test_product(out, m, k, n):
+    a, b = operand(m, k, m + k), operand(n, k, n, full=True)
+    bias = torch.randn(n, generator=torch.Generator("cuda").manual_seed(1), device="cuda") if (m + n) % 2 else None
+    y = mxb.int8_matmul(a, b, bias=bias, out_dtype=out)
+    assert y.shape == (m, n) and torch.equal(y, product_ref(a, b, bias, out))
+    assert L.load().mxb_device_error(1) == 0
+
+
+@pytest.mark.gpu
+def test_product_largest_sums():
+    k = 131071
+    a = mxb.mx_tensor(torch.full((2 * k,), -128, dtype=torch.int8, device="cuda"), torch.ones(2, device="cuda"),
+                      mxb.int8d, (2, k), 2 * k, k)
+    y = mxb.int8_matmul(a, a, out_dtype=torch.float32)
+    assert torch.equal(y, torch.full((2, 2), float(2 ** 14 * k), device="cuda"))
+
+
+@pytest.mark.gpu
+def test_product_scales_layouts_and_empty():
+    m, k, n = 40, 272, 100
+    for ba, bb in ((None, 1), (1, None), (1, 1)):
+        a, b = operand(m, k, 1, ba), operand(n, k, 2, bb)
+        assert torch.equal(mxb.int8_matmul(a, b), product_ref(a, b, None, torch.bfloat16))
+    a, b = operand(m, k, 1), operand(n, k, 2)
+    want = mxb.int8_matmul(a, b)
+    lead = mxb.mx_tensor(a.packed, a.mx_scales, mxb.int8d, (4, 10, k), m * k, k)
+    assert torch.equal(mxb.int8_matmul(lead, b), want.view(4, 10, n))
+    row = mxb.mx_tensor(a.packed[:k], a.mx_scales[:1], mxb.int8d, (k,), k, k)
+    assert torch.equal(mxb.int8_matmul(row, b), want[0])
+    for at in (1, 4, 8):  # codes that do not start at a multiple of 16 bytes
+        moved = torch.empty(m * k + at, dtype=torch.int8, device="cuda")[at:].copy_(a.packed)
+        am = mxb.mx_tensor(moved, a.mx_scales, mxb.int8d, (m, k), m * k, k)
+        assert torch.equal(mxb.int8_matmul(am, b), want)
+    bias = torch.arange(n, device="cuda").bfloat16()
+    assert torch.equal(mxb.int8_matmul(a, b, bias=bias), product_ref(a, b, bias.float(), torch.bfloat16))
+    assert mxb.int8_matmul(operand(0, k, 1), b).shape == (0, n) and mxb.int8_matmul(a, operand(0, k, 1)).shape == (m, 0)
+    z = mxb.int8_matmul(operand(3, 0, 1, 1), operand(n, 0, 1, 1), bias=bias)
+    assert torch.equal(z, bias.expand(3, n))
+    for bad in (bias[:-1], bias.cpu()):
+        with pytest.raises(ValueError):
+            mxb.int8_matmul(a, b, bias=bad)
+
+
+@pytest.mark.gpu
+def test_product_odd_scales():
+    """Scales that are infinite, NaN, zero or negative act on their rows alone."""
+    a, b = operand(6, 64, 3), operand(130, 64, 4)
+    for i, s in enumerate((float("inf"), float("nan"), 0.0, -1.0, 1e-40)):
+        a.mx_scales[i] = s
+        b.mx_scales[20 * i] = s
+    y, want = mxb.int8_matmul(a, b, out_dtype=torch.float32), product_ref(a, b, None, torch.float32) + 0.0
+    assert torch.equal(y.nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(y.isnan(), want.isnan())
+
+
+@pytest.mark.gpu
+def test_product_repeats_on_any_stream_and_in_a_graph():
+    a, b = operand(70, 4096, 1), operand(1000, 4096, 2)
+    c, e = operand(600, 1003, 3), operand(700, 1003, 4)
+    want, want2 = product_ref(a, b, None, torch.bfloat16), product_ref(c, e, None, torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ys = [mxb.int8_matmul(a, b) for _ in range(20)]
+        zs = [mxb.int8_matmul(c, e) for _ in range(20)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in ys) and all(torch.equal(z, want2) for z in zs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, z = mxb.int8_matmul(a, b), mxb.int8_matmul(c, e)
+    for _ in range(3):
+        y.zero_()
+        z.zero_()
+        graph.replay()
+        assert torch.equal(y, want) and torch.equal(z, want2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(5, 300, 70), (64, 1024, 512), (200, 2000, 130)])
+def test_fused_int8_linear_of_row_scales(m, k, n):
+    """The framework's fp32 linear of the same operands is this product."""
+    x, w = rows(1, m, k), rows(2, n, k) * 0.02
+    qx, qw = mxb.dynamic_quantize(x, "int8d", "per_token"), mxb.dynamic_quantize(w, "int8d", "per_token")
+    bias = rows(3, n, loud=False)
+    assert torch.equal(mxb.fused_int8_linear(qx, qw, bias), product_ref(qx, qw, bias, torch.float32))
+
+
+@pytest.mark.gpu
+def test_linear_module():
+    lin = torch.nn.Linear(320, 200, device="cuda")
+    layer = mxb.int8_linear.from_linear(lin)
+    x = rows(4, 3, 7, 320).bfloat16()
+    q = mxb.dynamic_quantize(x, "int8d", "per_token")
+    y = layer(x)
+    assert y.shape == (3, 7, 200) and y.dtype == torch.bfloat16 and torch.equal(y, layer(q))
+    flat = mxb.mx_tensor(q.packed, q.mx_scales, mxb.int8d, (21, 320), 21 * 320, 320)
+    assert torch.equal(y.view(21, 200), product_ref(flat, layer.weight, lin.bias.detach(), torch.bfloat16))
+    want = lin(x.float())
+    # each operand is off by half a code of its row's largest value
+    ax, aw = x.float().abs(), lin.weight.abs()
+    tol = (ax.amax(-1, keepdim=True) / 254 * aw.sum(1) + ax.sum(-1, keepdim=True) * aw.amax(1) / 254
+           + 320 * ax.amax(-1, keepdim=True) * aw.amax(1) / 254 ** 2)
+    assert bool(((y.float() - want).abs() <= 1.01 * tol + 2.0 ** -8 * want.abs() + 1e-5).all())
+
+
+@pytest.mark.gpu
+def test_norm_into_linear():
+    """A layer's norm, its product and the residual that goes on."""
+    x, h, w = (rows(i, 40, 512).bfloat16() for i in range(3))
+    weight = 1 + 0.1 * rows(5, 512, loud=False).bfloat16()
+    layer = mxb.int8_linear(mxb.dynamic_quantize(w, "int8d", "per_token"))
+    a, h2 = mxb.rms_norm_quantize(x, weight, residual=h)
+    code, scale = norm64(x, weight, h, 1e-6)
+    y = layer(a)
+    ref = torch.mm(code, layer.weight_codes.double().t()) * scale[:, None] * layer.weight_scales.double()
+    # the scale is off by 2^-19, the roundings of the product are three of 2^-24 and one of 2^-8
+    assert bool(((y.double() - ref).abs() <= (2.0 ** -8 + 2.0 ** -18) * ref.abs()).all())
+    assert torch.equal(h2, x + h)
