@@ -40,6 +40,34 @@ int prefix_rows_per_cta(int64_t rows);
 constexpr int kPrefixKeys = 64;
 int prefix_attention(const PrefixArgs& a, cudaStream_t st);
 
+// tree_attn.cu: tcgen05 attention of many query rows a sequence (a tree of the T
+// newest tokens) over the sequence's own keys.  Parts as paged_attn.cu makes them:
+// by output row (main), by CTA (cta), o [..][dim] relative to 2^m', ml (m, l, m', 0).
+struct TreeArgs {
+  const void* q;  // bf16 [B][T][H * G][dim]
+  int B, T, H, G, dim, bits;
+  const void *k_codes, *v_codes;
+  const float *k_scales, *v_scales;
+  int64_t n_pages;
+  int page_shift;
+  const int* table;  // [B][width]
+  int width;
+  const int* lengths;
+  const uint8_t* tree;  // query t sees newest key i where tree[b tree_b + t tree_t + i] is not 0
+  int64_t tree_b, tree_t;
+  int rows, row_tiles;  // T * G, and CTAs' shares of them
+  float scale_log2;
+  float *main_o, *main_ml, *cta_o, *cta_ml;
+  int64_t* plan;  // [0] tiles per CTA, [1 + b] first tile of sequence b
+  bool direct;    // rows with one part go straight to out
+  void* out;
+  float* lse;
+  int* err;
+};
+constexpr int kTreeKeys = 128;  // keys per tile
+int tree_rows_per_cta(int64_t rows);
+int tree_attention(const TreeArgs& a, int ctas, cudaStream_t st);
+
 // gemm_cuda_core.cu
 int qgemm_generic(const void* a, const float* sa, bool sa_ok, const void* b, const float* sb,
                   bool sb_ok, int64_t M, int64_t K, int64_t N, int bits, int block, float* C,

@@ -856,6 +856,7 @@ struct JoinArgs {
   const int* lengths;   // null: no keys of its own
   int64_t cap, n_rows;
   int pre_parts, T, H, G, row_tiles, R;
+  int tile;  // keys of a tile of the plan
   bool direct;  // rows with one part of their own are written already
   __nv_bfloat16* out;
   float* lse;
@@ -875,7 +876,7 @@ struct RowSum {
     own = 0;
     c_at = 0;
     if (a.lengths) {
-      const int64_t n = (min((int64_t)max(__ldg(a.lengths + b), 0), a.cap) + kTile - 1) / kTile;
+      const int n = (int)((min((int64_t)max(__ldg(a.lengths + b), 0), a.cap) + a.tile - 1) / a.tile);
       if (n > 0) {
         own = 1;
         if (a.plan) {
@@ -1036,6 +1037,8 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const JoinArgs a) 
 struct Plan {
   int nt_own, tiles_own, ctas_own;        // ctas_own 0: no own keys possible
   bool whole;                             // a unit per CTA
+  int rows_own, tile_own;                 // query rows a CTA and keys a tile, of the own keys
+  bool tensor;                            // own keys on tree_attn.cu
   bool join;                              // rows may have several parts
   int nt_pre, tiles_pre, splits_pre;      // splits_pre 0: no prefix; nt_pre 0: prefix_attn.cu
   size_t o_plan, o_main, o_cta, o_pre, bytes;  // workspace offsets
@@ -1043,13 +1046,19 @@ struct Plan {
 
 int nt_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4; }
 
+// Rows of a tree a KV head from which its own keys go to the tcgen05 kernel.
+constexpr int64_t kTreeRows = 33;
+
 Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, int64_t max_keys,
-               int64_t prefix) {
+               int64_t prefix, bool tree) {
   Plan p = {};
   const int64_t n_rows = B * T * H * G;
   const int rb = dim * bits / 8;
   p.nt_own = nt_of(T * G);
-  p.tiles_own = (int)cdiv(T * G, 8 * p.nt_own);
+  p.tensor = tree && max_keys > 0 && T * G >= kTreeRows;
+  p.rows_own = p.tensor ? tree_rows_per_cta(T * G) : 8 * p.nt_own;
+  p.tile_own = p.tensor ? kTreeKeys : kTile;
+  p.tiles_own = (int)cdiv(T * G, p.rows_own);
   const int64_t units = B * H * p.tiles_own;
   // Short units: one CTA each, and the hardware shares them out.  The list's
   // even runs cost a plan, a second unit's start in most CTAs (5 us) and a
@@ -1060,8 +1069,11 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, in
   // 31), 16 x 4096 45 / 37, 4 x 2048 18.5 / 15.8, 1 x 1024 11.6 / 13.0.
   const int64_t slots = kSMs * ctas(p.nt_own, rb, dim);
   const int64_t whole_keys = units >= slots ? 4096 : units >= kSMs * 3 / 4 ? 2048 : 1024;
-  p.whole = max_keys <= whole_keys && (max_keys > 0 || prefix == 0);
-  if (p.whole) {
+  p.whole = !p.tensor && max_keys <= whole_keys && (max_keys > 0 || prefix == 0);
+  if (p.tensor) {
+    const int64_t most = units * cdiv(max_keys, kTreeKeys);
+    p.ctas_own = (int)(most < kSMs ? most : kSMs);
+  } else if (p.whole) {
     p.ctas_own = (int)units;
   } else if (max_keys > 0) {
     const int64_t most = units * cdiv(max_keys, kTile * kWarps);
@@ -1098,7 +1110,7 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, in
   if (p.join) {
     p.o_plan = take(p.whole ? 0 : (size_t)(B + 1) * 8);
     p.o_main = take(p.ctas_own ? (size_t)n_rows * row : 0);
-    p.o_cta = take(p.whole ? 0 : (size_t)p.ctas_own * 8 * p.nt_own * row);
+    p.o_cta = take(p.whole ? 0 : (size_t)p.ctas_own * p.rows_own * row);
     p.o_pre = take((size_t)p.splits_pre * n_rows * row);
   }
   p.bytes = at;
@@ -1160,12 +1172,12 @@ int attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim
   // parts are stored 32 bytes at a time
   if (((uintptr_t)q | (uintptr_t)out) % 16 || (uintptr_t)workspace % 32) return MXB_E_ALIGN;
   const Plan p =
-      make_plan(B, T, heads, group, dim, bits, width * page, prefix_len);
+      make_plan(B, T, heads, group, dim, bits, width * page, prefix_len, tree != nullptr);
   const int64_t pre_rows = B * T * group;
   if ((int64_t)p.tiles_own * heads > 65535 || (int64_t)p.tiles_pre * heads > 65535 ||
       (p.splits_pre > 0 && p.nt_pre == 0 && cdiv(pre_rows, prefix_rows_per_cta(pre_rows)) > 65535) ||
       B * heads * p.tiles_own > INT32_MAX || B * T * heads * group > INT32_MAX ||
-      (int64_t)heads * p.tiles_own * (width * page / kTile + 1) > INT32_MAX)
+      (int64_t)heads * p.tiles_own * (width * page / p.tile_own + 1) > INT32_MAX)
     return MXB_E_SHAPE;
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return MXB_E_WORKSPACE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -1250,19 +1262,28 @@ int attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim
   if (p.ctas_own > 0) {
     if (p.join) own = part_at(workspace, p.o_main, (size_t)a.n_rows, dim);
     if (!p.whole) {
-      cta = part_at(workspace, p.o_cta, (size_t)p.ctas_own * 8 * p.nt_own, dim);
+      cta = part_at(workspace, p.o_cta, (size_t)p.ctas_own * p.rows_own, dim);
       a.plan = reinterpret_cast<int64_t*>(static_cast<char*>(workspace) + p.o_plan);
     }
     a.main = own;
     a.cta = cta;
     const dim3 grid((unsigned)p.ctas_own);
-    const int r = tree ? launch_any<true>(tk, tv, a, bits, dim, p.nt_own, grid, st)
-                       : launch_any<false>(tk, tv, a, bits, dim, p.nt_own, grid, st);
+    int r;
+    if (p.tensor) {
+      const TreeArgs x = {q, a.B, a.T, a.H, a.G, dim, bits, k_codes, v_codes, k_scales, v_scales, n_pages,
+                          a.page_shift, table, a.width, lengths, tree, tree_b, tree_t, a.rows, a.row_tiles,
+                          a.scale_log2, own.o, reinterpret_cast<float*>(own.ml), cta.o,
+                          reinterpret_cast<float*>(cta.ml), a.plan, a.direct, out, lse, a.err};
+      r = tree_attention(x, p.ctas_own, st);
+    } else {
+      r = tree ? launch_any<true>(tk, tv, a, bits, dim, p.nt_own, grid, st)
+               : launch_any<false>(tk, tv, a, bits, dim, p.nt_own, grid, st);
+    }
     if (r != MXB_OK) return r;
   }
   if (p.join) {
     JoinArgs j = {own, cta, pre, a.plan, p.ctas_own > 0 ? lengths : nullptr, width * page,
-                         a.n_rows, p.splits_pre, (int)T, heads, group, p.tiles_own, 8 * p.nt_own,
+                         a.n_rows, p.splits_pre, (int)T, heads, group, p.tiles_own, p.rows_own, p.tile_own,
                          a.direct, a.out, lse};
     const bool many = a.n_rows >= kJoinManyRows;
     auto kern = dim == 128 ? (many ? paged_join_kernel<128, kWarps>
@@ -1284,7 +1305,7 @@ extern "C" {
 size_t mxb_paged_attention_workspace_size(int64_t B, int64_t T, int heads, int group, int dim,
                                           int bits, int page, int64_t width, int64_t prefix_len) {
   if (B <= 0 || T <= 0 || heads <= 0 || group <= 0 || dim <= 0 || page <= 0 || bits <= 0) return 0;
-  return pattn::make_plan(B, T, heads, group, dim, bits, width * page, prefix_len).bytes;
+  return pattn::make_plan(B, T, heads, group, dim, bits, width * page, prefix_len, false).bytes;
 }
 
 int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim,
@@ -1301,7 +1322,8 @@ int mxb_paged_attention(const void* q, int64_t B, int64_t T, int heads, int grou
 
 size_t mxb_tree_attention_workspace_size(int64_t B, int64_t T, int heads, int group, int dim, int bits,
                                          int page, int64_t width, int64_t prefix_len) {
-  return mxb_paged_attention_workspace_size(B, T, heads, group, dim, bits, page, width, prefix_len);
+  if (B <= 0 || T <= 0 || heads <= 0 || group <= 0 || dim <= 0 || page <= 0 || bits <= 0) return 0;
+  return pattn::make_plan(B, T, heads, group, dim, bits, width * page, prefix_len, true).bytes;
 }
 
 int mxb_tree_attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim, const void* k_codes,
