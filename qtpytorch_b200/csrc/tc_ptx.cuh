@@ -111,6 +111,32 @@ __device__ __forceinline__ bool mbar_wait_warp_to(uint64_t* bar, uint32_t parity
   return __all_sync(0xffffffffu, ok);
 }
 
+// The same bounded wait for kernels whose many warps wait beside others that compute:
+// a failed try_wait comes back after up to half a millisecond instead of some 100
+// cycles, so that a waiting warp takes no issue slots from its neighbours.
+__device__ __forceinline__ bool mbar_sleep_to(uint64_t* bar, uint32_t parity, int err_code, int* err) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(500000u)
+        : "memory");
+    if (ok) return true;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) break;
+  }
+  if (err) atomicCAS(err, 0, err_code);
+  return false;
+}
+__device__ __forceinline__ bool mbar_sleep_warp_to(uint64_t* bar, uint32_t parity, int err_code, int* err) {
+  const bool ok = mbar_sleep_to(bar, parity, err_code, err);
+  return __all_sync(0xffffffffu, ok);
+}
+
 #ifndef MXB_ERROR_WORD_BY_POINTER
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int err_code) {
   return mbar_wait_to(bar, parity, err_code, &g_mxb_device_error);

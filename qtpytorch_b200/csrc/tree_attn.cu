@@ -7,20 +7,21 @@
 // CTA owns 128 rows or 256 and walks tiles of 128 keys:
 //   warp 0        MMA issue and TMEM allocation;
 //   warp 1        TMA producer: raw codes and scales, a ring of steps of 64 keys of K
-//                 or V (2 and 3 idle);
-//   warps 4-11    softmax: S from TMEM, running maximum, sum, weights (fp16) back to
+//                 or V;
+//   warps 2-17    softmax: S from TMEM, running maximum, sum, weights (fp16) back to
 //                 TMEM over S;
-//   warps 12-15   unpack codes to exact fp16 in shared memory (one layout for K and
+//   warps 18-21   unpack codes to exact fp16 in shared memory (one layout for K and
 //                 V: K-major for the first product, MN-major for the second), and
 //                 lay out a tile's scales.
 // Two streams of softmax warps take turns on the tensor cores, one multiplying
 // while the other exponentiates: with 256 rows the two halves of the rows, with 128
 // the even and the odd tiles of the same rows, joined at the end of a unit.
 //
-// A softmax warp reads S of its 32 rows in the fragment layout of 16 x 8 pieces: a
-// lane holds 4 rows and a quarter of the keys, so that the keys' scales cost a
-// quarter of the shared memory reads that a thread a row makes (with those the reads
-// of scales took 3000 cycles a tile, more than both products).
+// A softmax warp has 16 rows, in the fragment layout of 16 x 8 pieces: a lane holds 2
+// rows and a quarter of the keys.  Four such warps a scheduler hide one another's
+// latencies (with 32 rows a warp, a thread a row or not, a warp issued an instruction
+// every 8 cycles and a tile took 9000), and the keys' scales cost a quarter of the
+// shared memory reads that a thread a row makes.
 //
 // Scores: Q is fp16 under a power of two per row that puts its largest value into
 // [2^14, 2^15), the codes are exact.  Weights: p_j = exp2(s_j - m) times 2^6 sv_j /
@@ -45,7 +46,8 @@ namespace mxb {
 namespace tree {
 
 constexpr int KT = kTreeKeys;  // 128
-constexpr int kThreads = 512;
+constexpr int kSoftWarps = 16, kFirstSoft = 2, kFirstUnpack = kFirstSoft + kSoftWarps;
+constexpr int kThreads = 32 * (kFirstUnpack + 4);
 constexpr int kSlots = 4;      // scale slots: a tile's is written after S of the tile two before
 constexpr int kSlotF = 2 * KT + 8;  // key scales, value scales, header
 constexpr float kRoom = 64.0f;      // 2^6
@@ -58,10 +60,11 @@ struct Cfg {
   static constexpr int kPlane = kAtom * (D / 64);  // 32 or 16 KB
   static constexpr int kQAtom = 128 * 128;
   static constexpr int kQ = kQAtom * (D / 64);
-  static constexpr int kXPitch = 33;               // floats of a row in the exchange of two streams
+  // exchange of two streams, 32 columns at a time: 16 values a thread, and (m, l, m') of its 2 rows
+  static constexpr int kX = 32 * (kSoftWarps / 2) * 16 * 4, kXml = 32 * (kSoftWarps / 2) * 32;
   static constexpr size_t oK = (size_t)MT * kQ, oV = oK + 2 * kPlane, oSc = oV + 2 * kPlane;
   static constexpr size_t oX = oSc + (size_t)kSlots * kSlotF * 4;
-  static constexpr size_t oBars = oX + (MT == 1 ? 128 * (kXPitch * 4 + 16) : 0);
+  static constexpr size_t oBars = oX + (MT == 1 ? kX + kXml : 0);
   // ring of raw codes, 64 keys of K (with both scales of those) or of V a step
   static constexpr int kStep = 64 * RB, kSlot = kStep + 512;
   static constexpr size_t oRaw = oBars + 768;
@@ -78,12 +81,12 @@ struct Bars {
   uint64_t raw_full[kMaxRing], raw_empty[kMaxRing];
   uint64_t qready, xfull, xfree;
   uint64_t drained;  // every product issued is complete
-  int64_t scan[16];
+  int64_t scan[24];
   uint32_t tmem_base;
   int b, off;
   uint32_t gone[kMaxRing];  // bit i: keys 16 i .. of the step lie behind a number outside the pool
 };
-static_assert(sizeof(Bars) <= 768, "barrier block overflows its slot");
+static_assert(sizeof(Bars) <= 768 && kThreads / 32 <= 24, "barrier block overflows its slot");
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -174,6 +177,14 @@ __device__ __forceinline__ void tmem_st_16x32h(uint32_t taddr, const uint32_t (&
                "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
+__device__ __forceinline__ void tmem_st_16x32(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 // After tmem_wait_ld: no use of the registers before it.
 __device__ __forceinline__ void landed16(uint32_t (&r)[16]) {
   asm volatile(""
@@ -181,6 +192,12 @@ __device__ __forceinline__ void landed16(uint32_t (&r)[16]) {
                  "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                :
                : "memory");
+}
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[16]) {
+  __syncwarp();
+  tmem_ld_16x32(taddr, r);
+  tmem_wait_ld();
+  landed16(r);
 }
 
 template <int BITS, int D>
@@ -229,7 +246,17 @@ struct Place {
   }
 };
 
-// Sum over the block of one value a thread, and its exclusive prefix.
+// Sum over the warp, or the block, of one value a thread, and its exclusive prefix.
+__device__ __forceinline__ int64_t warp_scan(int64_t v, int64_t& before) {
+  int64_t inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, inc, o);
+    if ((threadIdx.x & 31) >= o) inc += t;
+  }
+  before = inc - v;
+  return __shfl_sync(0xffffffffu, inc, 31);
+}
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& before, int64_t* sm) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t inc = v;
@@ -250,11 +277,11 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& before, int64_
   return total;
 }
 
-// A lane's four rows of the softmax, k * 8 + lane / 4 of the warp's 32: reference and
-// sum (of the lane's own keys); lc, log2 of the c that O stands under; top_w, log2 of
-// the largest weight of wide tiles, or less.
+// A lane's two rows of the softmax, 8 k + lane / 4 of the warp's 16: reference and sum
+// (of the lane's own keys); lc, log2 of the c that O stands under; top_w, log2 of the
+// largest weight of wide tiles, or less.
 struct Rows {
-  float mu[4], m_top[4], l[4], lc[4], top_w[4];
+  float mu[2], m_top[2], l[2], lc[2], top_w[2];
 };
 struct Tile {
   const float* slot;
@@ -266,223 +293,233 @@ struct Tile {
   int64_t mask_t;
 };
 
-// Value of row `lane` of what the four rows' lanes hold.
-__device__ __forceinline__ float to_row(const float (&x)[4]) {
-  const int lane = threadIdx.x & 31, src = (lane & 7) * 4, k = lane >> 3;
-  const float a = __shfl_sync(0xffffffffu, x[0], src), b = __shfl_sync(0xffffffffu, x[1], src);
-  const float c = __shfl_sync(0xffffffffu, x[2], src), d = __shfl_sync(0xffffffffu, x[3], src);
-  return k == 0 ? a : k == 1 ? b : k == 2 ? c : d;
-}
-
-// Scores of a piece of 32 keys: v[k][i], keys 8 i + 2 (lane % 4) and the next of row
-// k; hidden ones (bit 8 i + 2 k + e) -inf.
-__device__ __forceinline__ void scores(const Tile& g, int c, uint32_t hidden, uint64_t (&v)[4][4]) {
-  uint32_t s0[16], s1[16];
-  __syncwarp();
-  tmem_ld_16x32(g.s + 32 * c, s0);
-  tmem_ld_16x32(g.s + (16u << 16) + 32 * c, s1);
-  const float* ks = g.slot + 32 * c + 2 * (threadIdx.x & 3);
-  uint64_t k2[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) k2[i] = *reinterpret_cast<const uint64_t*>(ks + 8 * i);
-  tmem_wait_ld();
-  landed16(s0);
-  landed16(s1);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      v[h][i] = fmul2(pack2(__uint_as_float(s0[4 * i + 2 * h]), __uint_as_float(s0[4 * i + 2 * h + 1])), k2[i]);
-      v[2 + h][i] = fmul2(pack2(__uint_as_float(s1[4 * i + 2 * h]), __uint_as_float(s1[4 * i + 2 * h + 1])), k2[i]);
-    }
-  if (hidden) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float2 x = unpack2(v[k][i]);
-        if (hidden >> (8 * i + 2 * k) & 1u) x.x = -INFINITY;
-        if (hidden >> (8 * i + 2 * k + 1) & 1u) x.y = -INFINITY;
-        v[k][i] = pack2(x.x, x.y);
-      }
-  }
-}
-
-// The softmax of one tile; P is in TMEM afterwards.  Loops over 32 keys are not
-// unrolled: three roles share the instruction cache, and straight code of this
-// length ran from beyond it.
+// Multiplies the D columns of O, and with them the P of `pieces` pieces of this tile,
+// of the lane's rows by 2^x, in place.
 template <int D>
-__device__ __forceinline__ void softmax_tile(Rows& r, const Tile& g, const float (&rowf)[4], const int (&tok)[4]) {
+__device__ __noinline__ void rescale(uint32_t o_at, uint32_t s_at, bool has_o, int pieces, float x0, float x1) {
+  const float by[2] = {ex2(x0), ex2(x1)};
+  tmem_wait_st();
+  if (has_o) {
+#pragma unroll 1
+    for (int d = 0; d < D; d += 32) {
+      uint32_t o[16];
+      tmem_get(o_at + d, o);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by[(i >> 1) & 1]);
+      tmem_st_16x32(o_at + d, o);
+    }
+  }
+  // 32 columns of P are two pieces; where the second is none of them it is put back as it was
+#pragma unroll 1
+  for (int c = 0; c < pieces; c += 2) {
+    uint32_t p[16];
+    tmem_get(s_at + 16 * c, p);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[i]));
+      const uint32_t y = hf2(f.x * by[(i >> 1) & 1], f.y * by[(i >> 1) & 1]);
+      if (i < 8 || c + 1 < pieces) p[i] = y;
+    }
+    tmem_st_16x32(s_at + 16 * c, p);
+  }
+  tmem_wait_st();
+}
+
+// The softmax of one tile in one pass over S; P is in TMEM afterwards.  References and
+// c move where a piece's scores or weights ask for it, and take O and the P before
+// that piece along; they are whole powers of two, so that a P that moves with them is
+// not rounded again (but where it becomes subnormal).  The loop over pieces of 32 keys
+// is not unrolled: three roles share the instruction cache, and four pieces in a row,
+// the next one's S on its way, took 304 us where the loop takes 245.
+template <int D>
+__device__ __forceinline__ void softmax_tile(Rows& r, const Tile& g, const float (&rowf)[2], const int (&tok)[2]) {
   const float* head = g.slot + 2 * KT;
   const float lcn = head[0];
   const bool wide = __float_as_uint(head[1]) != 0u;
   uint4 hidden = *reinterpret_cast<const uint4*>(head + 4);
-  if (g.key0 + KT > g.hist || (hidden.x | hidden.y | hidden.z | hidden.w)) {
-    // from keys that are hidden to which of a lane's scores are: bit 8 i + 2 k + e of a word
+  const int lane = threadIdx.x & 31;
+  if (__builtin_expect(g.key0 + KT > g.hist || (hidden.x | hidden.y | hidden.z | hidden.w), 0)) {
+    // from keys that are hidden to which of a lane's scores are: bit 4 i + 2 k + e of a
+    // word for key 8 i + 2 (lane % 4) + e of row 8 k + lane / 4
+    const uint8_t* mask[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) mask[k] = g.mask + min(tok[k], g.T - 1) * g.mask_t;
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
       const uint32_t gone = hidden.x;
       uint32_t bits = 0;
+      if (gone != 0u || g.key0 + 32 * c + 32 > g.hist) {
+        // the tree's own keys, as far as the row's mask names them: all bytes at once, those
+        // of other places are not looked at
+        uint32_t seen[4][2][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = 8 * i + 2 * (threadIdx.x & 3) + e, at = g.key0 + 32 * c + j - g.hist;
+          for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            // the tree's own keys, as far as the row's mask names them
-            const bool off = (gone >> j & 1u) ||
-                             (at >= 0 && (at >= g.T || tok[k] >= g.T || !__ldg(g.mask + tok[k] * g.mask_t + at)));
-            bits |= (off ? 1u : 0u) << (8 * i + 2 * k + e);
-          }
-        }
+            for (int e = 0; e < 2; ++e) {
+              const int at = g.key0 + 32 * c + 8 * i + 2 * (lane & 3) + e - g.hist;
+              seen[i][k][e] = __ldg(mask[k] + max(min(at, g.T - 1), 0));
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int j = 8 * i + 2 * (lane & 3) + e, at = g.key0 + 32 * c + j - g.hist;
+              const bool off = (gone >> j & 1u) || (at >= 0 && (at >= g.T || tok[k] >= g.T || seen[i][k][e] == 0u));
+              bits |= (off ? 1u : 0u) << (4 * i + 2 * k + e);
+            }
+      }
       hidden = make_uint4(hidden.y, hidden.z, hidden.w, bits);  // four turns: each word in its place
     }
     __syncwarp();
   }
-  auto hid = [&](int c) { return c == 0 ? hidden.x : c == 1 ? hidden.y : c == 2 ? hidden.z : hidden.w; };
-  // ── maximum ──
-  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    uint64_t v[4][4];
-    scores(g, c, hid(c), v);
+  if (g.first) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 x = unpack2(v[k][i]);
-        mx[k] = fmaxf(mx[k], fmaxf(x.x, x.y));
-      }
-  }
-  float alpha[4], dm[4], up[4];
-  bool moved = false;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 1));
-    mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 2)) * rowf[k];
-    if (g.first) {
+    for (int k = 0; k < 2; ++k) {
       r.mu[k] = r.l[k] = 0.0f;
       r.m_top[k] = r.top_w[k] = -INFINITY;
       r.lc[k] = lcn;
     }
-    alpha[k] = up[k] = 1.0f;
-    dm[k] = 0.0f;
-    if (mx[k] > r.m_top[k]) {
-      const float m0 = r.m_top[k] == -INFINITY ? -INFINITY : r.mu[k];
-      const float m1 = fmaxf(m0, mx[k]);
-      r.mu[k] = m1;
-      dm[k] = m0 - m1;
-      alpha[k] = ex2(dm[k]);
-      r.l[k] *= alpha[k];
-      r.m_top[k] = m1 + 8.0f;
-      moved = true;
-    }
   }
-  if (wide) {
-    // a c for each row that puts its largest weight so far between 2^-2 and 2^12
-    float u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  bool turn = !wide && lcn != r.lc[0];  // the narrow tiles' c is one for all rows
+  uint64_t sum[2] = {0, 0};
+  const float* ks = g.slot + 2 * (lane & 3);
 #pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-      uint64_t v[4][4];
-      const uint32_t h = hid(c);
-      scores(g, c, h, v);
-      const float* vs = g.slot + KT + 32 * c + 2 * (threadIdx.x & 3);
+  for (int c = 0; c < 4; ++c, ks += 32) {
+    const uint32_t h = hidden.x;
+    hidden = make_uint4(hidden.y, hidden.z, hidden.w, h);
+    uint32_t s[16];
+    uint64_t v[2][4];
+    tmem_get(g.s + 32 * c, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t k2 = *reinterpret_cast<const uint64_t*>(ks + 8 * i);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        v[k][i] = fmul2(pack2(__uint_as_float(s[4 * i + 2 * k]), __uint_as_float(s[4 * i + 2 * k + 1])), k2);
+    }
+    if (__builtin_expect(h != 0u, 0)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 x = unpack2(ffma2(v[k][i], pack2(rowf[k], rowf[k]), pack2(-r.mu[k], -r.mu[k])));
-          u[k] = fmaxf(u[k], h >> (8 * i + 2 * k) & 1u ? 0.0f : ex2(x.x) * vs[8 * i]);
-          u[k] = fmaxf(u[k], h >> (8 * i + 2 * k + 1) & 1u ? 0.0f : ex2(x.y) * vs[8 * i + 1]);
+        for (int k = 0; k < 2; ++k) {
+          float2 x = unpack2(v[k][i]);
+          if (h >> (4 * i + 2 * k) & 1u) x.x = -INFINITY;
+          if (h >> (4 * i + 2 * k + 1) & 1u) x.y = -INFINITY;
+          v[k][i] = pack2(x.x, x.y);
         }
     }
+    float mx[2], up[2] = {1.0f, 1.0f};
+    bool move = turn || wide;
+    turn = false;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      u[k] = fmaxf(u[k], __shfl_xor_sync(0xffffffffu, u[k], 1));
-      u[k] = fmaxf(u[k], __shfl_xor_sync(0xffffffffu, u[k], 2));
-      r.top_w[k] = fminf(fmaxf(r.top_w[k] + dm[k], log2f(u[k]) + (lcn - r.lc[k])), 200.0f);
-      if (r.top_w[k] > 12.0f || (r.top_w[k] < -2.0f && r.top_w[k] > -INFINITY) || lcn - r.lc[k] > 120.0f) {
-        // no further below the tile's c than 2^120: fp32 holds little under that
-        const float by = fminf(6.0f - floorf(r.top_w[k]), 120.0f - (lcn - r.lc[k]));
-        r.lc[k] -= by;
-        r.top_w[k] += by;
-        alpha[k] *= ex2(by);
-        moved = true;
-      }
-      up[k] = ex2(lcn - r.lc[k]);
+    for (int k = 0; k < 2; ++k) {
+      const float2 x0 = unpack2(v[k][0]), x1 = unpack2(v[k][1]), x2 = unpack2(v[k][2]), x3 = unpack2(v[k][3]);
+      mx[k] = fmaxf(fmaxf(fmaxf(x0.x, x0.y), fmaxf(x1.x, x1.y)), fmaxf(fmaxf(x2.x, x2.y), fmaxf(x3.x, x3.y))) * rowf[k];
+      move |= mx[k] > r.m_top[k];
     }
-  } else {
+    if (__builtin_expect(__any_sync(0xffffffffu, move), 0)) {
+      float by[2];  // log2 of what O and P are multiplied with
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (lcn != r.lc[k]) {
-        alpha[k] *= ex2(r.lc[k] - lcn);
-        r.lc[k] = lcn;
-        moved = true;
+      for (int k = 0; k < 2; ++k) {
+        mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 1));
+        mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 2));
+        by[k] = 0.0f;
+        if (mx[k] > r.m_top[k]) {
+          const float m0 = r.m_top[k] == -INFINITY ? -INFINITY : r.mu[k];
+          const float m1 = ceilf(fmaxf(m0, mx[k]));
+          by[k] = m0 - m1;
+          const float alpha = ex2(by[k]);
+          const float2 t = unpack2(sum[k]);
+          sum[k] = pack2(t.x * alpha, t.y * alpha);
+          r.l[k] *= alpha;
+          r.mu[k] = m1;
+          r.m_top[k] = m1 + 8.0f;
+        }
+        if (wide) {
+          // a c for the row that puts its largest weight so far between 2^-2 and 2^12
+          float u = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 x = unpack2(ffma2(v[k][i], pack2(rowf[k], rowf[k]), pack2(-r.mu[k], -r.mu[k])));
+            u = fmaxf(u, h >> (4 * i + 2 * k) & 1u ? 0.0f : ex2(x.x) * ks[KT + 8 * i]);
+            u = fmaxf(u, h >> (4 * i + 2 * k + 1) & 1u ? 0.0f : ex2(x.y) * ks[KT + 8 * i + 1]);
+          }
+          u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 1));
+          u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 2));
+          r.top_w[k] = fminf(fmaxf(r.top_w[k] + by[k], log2f(u) + (lcn - r.lc[k])), 200.0f);
+          if (r.top_w[k] > 12.0f || (r.top_w[k] < -2.0f && r.top_w[k] > -INFINITY) || lcn - r.lc[k] > 120.0f) {
+            // no further below the tile's c than 2^120: fp32 holds little under that
+            const float x = fminf(6.0f - floorf(r.top_w[k]), 120.0f - (lcn - r.lc[k]));
+            r.lc[k] -= x;
+            r.top_w[k] += x;
+            by[k] += x;
+          }
+          up[k] = ex2(lcn - r.lc[k]);
+        } else {
+          by[k] += r.lc[k] - lcn;
+          r.lc[k] = lcn;
+        }
       }
-  }
-  if (!g.first && __any_sync(0xffffffffu, moved)) {
-    const float by = to_row(alpha);
-#pragma unroll 1
-    for (int d = 0; d < D; d += 32) {
-      uint32_t o[32];
-      tmem_ld32(g.o + d, o);
-      tmem_wait_ld();
-      tmem_landed(o);
-#pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
-      tmem_st32(g.o + d, o);
+      if (__any_sync(0xffffffffu, by[0] != 0.0f || by[1] != 0.0f) && !(g.first && c == 0))
+        rescale<D>(g.o, g.s, !g.first, c, by[0], by[1]);
     }
-  }
-  // ── weights: 32 keys of S become 16 columns of P, over scores that are read ──
-  uint64_t sum[4], rowf2[4], mu2[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    sum[k] = pack2(0.0f, 0.0f);
-    rowf2[k] = pack2(rowf[k], rowf[k]);
-    mu2[k] = pack2(-r.mu[k], -r.mu[k]);
-  }
-#pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    uint64_t v[4][4];
-    const uint32_t h = hid(c);
-    scores(g, c, h, v);
-    const float* vs = g.slot + KT + 32 * c + 2 * (threadIdx.x & 3);
-    uint32_t pk[2][8];
+    uint32_t pk[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint64_t w = *reinterpret_cast<const uint64_t*>(vs + 8 * i);
+      const uint64_t w = *reinterpret_cast<const uint64_t*>(ks + KT + 8 * i);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 x = unpack2(ffma2(v[k][i], rowf2[k], mu2[k]));
+      for (int k = 0; k < 2; ++k) {
+        const float2 x = unpack2(ffma2(v[k][i], pack2(rowf[k], rowf[k]), pack2(-r.mu[k], -r.mu[k])));
         const uint64_t p = pack2(ex2(x.x), ex2(x.y));
         sum[k] = fadd2(sum[k], p);
         uint64_t q = fmul2(p, w);
-        if (wide) q = fmul2(q, pack2(up[k], up[k]));
+        q = fmul2(q, pack2(up[k], up[k]));
         const float2 y = unpack2(q);
-        pk[k >> 1][2 * i + (k & 1)] = hf2(y.x, y.y);
+        pk[2 * i + k] = hf2(y.x, y.y);
       }
     }
-    if (h) {  // whatever their scales hold
+    if (__builtin_expect(h != 0u, 0)) {  // whatever their scales hold
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (h >> (8 * i + 2 * k) & 1u) pk[k >> 1][2 * i + (k & 1)] &= 0xffff0000u;
-          if (h >> (8 * i + 2 * k + 1) & 1u) pk[k >> 1][2 * i + (k & 1)] &= 0x0000ffffu;
+        for (int k = 0; k < 2; ++k) {
+          if (h >> (4 * i + 2 * k) & 1u) pk[2 * i + k] &= 0xffff0000u;
+          if (h >> (4 * i + 2 * k + 1) & 1u) pk[2 * i + k] &= 0x0000ffffu;
         }
     }
     __syncwarp();
-    tmem_st_16x32h(g.s + 16 * c, pk[0]);
-    tmem_st_16x32h(g.s + (16u << 16) + 16 * c, pk[1]);
+    tmem_st_16x32h(g.s + 16 * c, pk);
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < 2; ++k) {
     const float2 x = unpack2(sum[k]);
     r.l[k] += x.x + x.y;
   }
   tmem_wait_st();
   tc_fence_before();
+}
+
+// Columns 2 c, 2 c + 1 (c = lane % 4) of eight unpacked ones -> dims 2 c, 2 c + 1.
+template <int BITS>
+__device__ __forceinline__ float2 in_order(float x, float y) {
+  const int lane = threadIdx.x & 31, c = lane & 3, base = lane & ~3;
+  if constexpr (BITS == 8) {  // neighbours swap the middle two of 0 2 1 3
+    const float z = __shfl_xor_sync(0xffffffffu, c & 1 ? x : y, 1);
+    return c & 1 ? make_float2(z, y) : make_float2(x, z);
+  } else {
+    float out[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int d = 2 * c + e, p = ((d & 3) << 1) | (d >> 2);  // the column that holds dim d
+      const float u = __shfl_sync(0xffffffffu, x, base + (p >> 1)), w = __shfl_sync(0xffffffffu, y, base + (p >> 1));
+      out[e] = p & 1 ? w : u;
+    }
+    return make_float2(out[0], out[1]);
+  }
 }
 
 template <int BITS, int D, int MT>
@@ -505,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->vready[b], 4);
       mbar_init(&bars->vfree[b], 1);
       mbar_init(&bars->sready[b], 1);
-      mbar_init(&bars->pready[b], 4);
+      mbar_init(&bars->pready[b], kSoftWarps / 2);
       mbar_init(&bars->pvdone[b], 1);
     }
     for (int s = 0; s < kSlots; ++s) mbar_init(&bars->scready[s], 4);
@@ -513,9 +550,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->raw_full[s], 64 / box);
       mbar_init(&bars->raw_empty[s], 4);
     }
-    mbar_init(&bars->qready, 4 * MT);
-    mbar_init(&bars->xfull, 4);
-    mbar_init(&bars->xfree, 4);
+    mbar_init(&bars->qready, kSoftWarps / 2 * MT);
+    mbar_init(&bars->xfull, kSoftWarps / 2);
+    mbar_init(&bars->xfree, kSoftWarps / 2);
     mbar_init(&bars->drained, 1);
     fence_barrier_init();
   }
@@ -536,459 +573,468 @@ __global__ void __launch_bounds__(kThreads, 1)
   Place at;
   bool any;
   {
-    int64_t total = 0, before;
-    for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-      const int i = b0 + threadIdx.x;
-      int64_t n = 0;
-      if (i < a.B) {
-        if (__ldg(a.lengths + i) > cap && blockIdx.x == 0 && a.err) atomicCAS(a.err, 0, kErrIndex);
-        n = (Place::len_of(a, i) + KT - 1) / KT;
-      }
-      total += block_scan(n * hr, before, bars->scan);
+    // every warp for itself where the batch is small, otherwise the block together
+    const bool alone = a.B <= 512;
+    const int width = alone ? 32 : kThreads, me = alone ? lane : threadIdx.x;
+    auto tiles_of = [&](int i) -> int64_t {
+      return i < a.B ? (int64_t)((Place::len_of(a, i) + KT - 1) / KT) * hr : 0;
+    };
+    auto scan = [&](int64_t v, int64_t& before) {
+      return alone ? warp_scan(v, before) : block_scan(v, before, bars->scan);
+    };
+    int64_t total = 0, before, base = 0;
+    for (int b0 = 0; b0 < a.B; b0 += width) {
+      const int i = b0 + me;
+      if (i < a.B && blockIdx.x == 0 && a.err && __ldg(a.lengths + i) > cap) atomicCAS(a.err, 0, kErrIndex);
+      total += scan(tiles_of(i), before);
     }
     const int64_t per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)1);
     const int64_t lo = blockIdx.x * per, hi = min(lo + per, total);
     if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = per;
-    int64_t base = 0;
-    for (int b0 = 0; b0 < a.B && (blockIdx.x == 0 || base <= lo); b0 += kThreads) {
-      const int i = b0 + threadIdx.x;
-      const int64_t n = i < a.B ? (int64_t)((Place::len_of(a, i) + KT - 1) / KT) * hr : 0;
-      const int64_t sum = block_scan(n, before, bars->scan);
+    int at_b = 0, at_off = 0;
+    for (int b0 = 0; b0 < a.B && (blockIdx.x == 0 || base <= lo); b0 += width) {
+      const int i = b0 + me;
+      const int64_t n = tiles_of(i), sum = scan(n, before);
       before += base;
       base += sum;
-      if (i < a.B && blockIdx.x == 0) a.plan[1 + i] = before;
-      if (lo < hi && lo >= before && lo < before + n) {
+      if (i < a.B && blockIdx.x == 0 && (!alone || warp == 0)) a.plan[1 + i] = before;
+      const bool here = lo < hi && lo >= before && lo < before + n;
+      if (alone) {
+        const uint32_t who = __ballot_sync(0xffffffffu, here);
+        if (who) {
+          at_b = __shfl_sync(0xffffffffu, i, __ffs(who) - 1);
+          at_off = __shfl_sync(0xffffffffu, (int)(lo - before), __ffs(who) - 1);
+        }
+      } else if (here) {
         bars->b = i;
         bars->off = (int)(lo - before);
       }
     }
-    __syncthreads();
+    if (!alone) {
+      __syncthreads();
+      at_b = bars->b;
+      at_off = bars->off;
+    }
     any = lo < hi;
     if (any) {
-      at.b = bars->b;
+      at.b = at_b;
       at.left = hi - lo;
       const int n = (Place::len_of(a, at.b) + KT - 1) / KT;
-      at.u = bars->off / n;
-      at.start(a, bars->off - at.u * n);
+      at.u = at_off / n;
+      at.start(a, at_off - at.u * n);
     }
   }
   auto t_s = [&](int g) { return tbase + (uint32_t)(g * KT); };
   auto t_o = [&](int g) { return tbase + (uint32_t)(2 * KT + g * D); };
 
-  if (warp == 0) {
-    if (lane == 0 && any) {
-      constexpr uint32_t id_s = make_idesc(/*F32*/ 1, /*F16*/ 0, 0, 0, 128, KT);
-      constexpr uint32_t id_o = make_idesc(1, 0, 0, /*B MN-major*/ 1, 128, D);
-      const uint32_t sq = smem_u32(smem), sk = smem_u32(smem + C::oK), sv = smem_u32(smem + C::oV);
-      bool ok = true;
-      int j0 = 0;                // tiles of the segments before
-      int step[2] = {0, 0};      // products P V issued a stream
-      uint32_t seg = 0;
-      // S of tile j (counted over the run) for stream g
-      auto issue_s = [&](int g, int j, bool wait, bool last) {
-        const int b = j & 1;
-        if (wait) ok = ok && mbar_wait_to(&bars->kready[b], (j >> 1) & 1, kErrTimeoutFull, a.err);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t q = sq + (MT == 2 ? g * C::kQ : 0);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          mma_f16(t_s(g), desc_kmajor_sw128(q + (kk >> 2) * C::kQAtom + (kk & 3) * 32),
-                  desc_kmajor_sw128(sk + b * C::kPlane + (kk >> 2) * C::kAtom + (kk & 3) * 32), id_s,
-                  kk > 0 ? 1u : 0u);
-        mma_commit(&bars->sready[g]);
-        if (last) mma_commit(&bars->kfree[b]);
-      };
-      auto issue_o = [&](int g, int j, bool first, bool wait, bool last) {
-        const int b = j & 1;
-        if (wait) ok = ok && mbar_wait_to(&bars->vready[b], (j >> 1) & 1, kErrTimeoutFull, a.err);
-        ok = ok && mbar_wait_to(&bars->pready[g], step[g] & 1, kErrTimeoutTmemFull, a.err);
-        if (!ok) return;
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk)
-          mma_f16_ts(t_o(g), t_s(g) + kk * 8,
-                     desc_mnmajor_sw128(sv + b * C::kPlane + kk * 16 * 128, C::kAtom), id_o,
-                     (!first || kk > 0) ? 1u : 0u);
-        mma_commit(&bars->pvdone[g]);
-        if (last) mma_commit(&bars->vfree[b]);
-      };
-      // the next S of a stream goes over its P: that product has to be complete
-      auto done_o = [&](int g) {
-        ok = ok && mbar_wait_to(&bars->pvdone[g], step[g] & 1, kErrTimeoutTmemEmpty, a.err);
-      };
-      do {
-        const int n = at.t_hi - at.t_lo;
-        ok = ok && mbar_wait_to(&bars->qready, seg & 1, kErrTimeoutFull, a.err);
-        if constexpr (MT == 2) {
-          issue_s(0, j0, true, false);
-          issue_s(1, j0, false, true);
-          for (int i = 0; i < n && ok; ++i) {
-            for (int g = 0; g < 2; ++g) {
-              issue_o(g, j0 + i, i == 0, g == 0, g == 1);
-              if (i + 1 < n) {
-                done_o(g);
-                issue_s(g, j0 + i + 1, g == 0, g == 1);
-              }
-              ++step[g];
+  if (warp < kFirstSoft) {
+    if (warp == 0) {
+      if (lane == 0 && any) {
+        constexpr uint32_t id_s = make_idesc(/*F32*/ 1, /*F16*/ 0, 0, 0, 128, KT);
+        constexpr uint32_t id_o = make_idesc(1, 0, 0, /*B MN-major*/ 1, 128, D);
+        // descriptors count in units of 16 bytes, and stay within their 14 bits
+        const uint64_t dq = desc_kmajor_sw128(smem_u32(smem)), dk = desc_kmajor_sw128(smem_u32(smem + C::oK));
+        const uint64_t dv = desc_mnmajor_sw128(smem_u32(smem + C::oV), C::kAtom);
+        bool ok = true;
+        int j0 = 0;                // tiles of the segments before
+        int step[2] = {0, 0};      // products P V issued a stream
+        uint32_t seg = 0;
+        // A stream's turn: P V of its tile io, then S of its tile is over that P.  256 rows:
+        // both streams take every tile; 128: the even and the odd ones.
+        do {
+          const int n = at.t_hi - at.t_lo;
+          ok = ok && mbar_sleep_to(&bars->qready, seg & 1, kErrTimeoutFull, a.err);
+#pragma unroll 1
+          for (int k = 0; k < (MT == 2 ? 2 * n : n) + 2 && ok; ++k) {
+            const int g = k & 1, io = MT == 2 ? (k >> 1) - 1 : k - 2, is = io + (MT == 2 ? 1 : 2);
+            if (io >= 0) {
+              const int j = j0 + io, b = j & 1;
+              if (MT == 1 || g == 0) ok = mbar_sleep_to(&bars->vready[b], (j >> 1) & 1, kErrTimeoutFull, a.err);
+              ok = ok && mbar_sleep_to(&bars->pready[g], step[g] & 1, kErrTimeoutTmemFull, a.err);
+              if (!ok) break;
+              tc_fence_after();
+              const uint64_t v = dv + (uint32_t)(b * (C::kPlane >> 4));
+#pragma unroll 2
+              for (int kk = 0; kk < KT / 16; ++kk)
+                mma_f16_ts(t_o(g), t_s(g) + kk * 8, v + kk * (16 * 128 >> 4), id_o,
+                           (is >= (MT == 2 ? 2 : 4) || kk > 0) ? 1u : 0u);
+              mma_commit(&bars->pvdone[g]);
+              if (MT == 1 || g == 1) mma_commit(&bars->vfree[b]);
             }
-          }
-        } else {
-          issue_s(0, j0, true, true);
-          if (n > 1) issue_s(1, j0 + 1, true, true);
-          for (int i = 0; i < n && ok; ++i) {
-            const int g = i & 1;
-            issue_o(g, j0 + i, i < 2, true, true);
-            if (i + 2 < n) {
-              done_o(g);
-              issue_s(g, j0 + i + 2, true, true);
+            if (is < n) {
+              const int j = j0 + is, b = j & 1;
+              // S goes over the stream's P: that product has to be complete
+              if (io >= 0) ok = mbar_sleep_to(&bars->pvdone[g], step[g] & 1, kErrTimeoutTmemEmpty, a.err);
+              if (MT == 1 || g == 0)
+                ok = ok && mbar_sleep_to(&bars->kready[b], (j >> 1) & 1, kErrTimeoutFull, a.err);
+              if (!ok) break;
+              tc_fence_after();
+              const uint64_t q = dq + (MT == 2 ? (uint32_t)(g * (C::kQ >> 4)) : 0u);
+              const uint64_t kd = dk + (uint32_t)(b * (C::kPlane >> 4));
+#pragma unroll 2
+              for (int kk = 0; kk < D / 16; ++kk)
+                mma_f16(t_s(g), q + (kk >> 2) * (C::kQAtom >> 4) + (kk & 3) * 2,
+                        kd + (kk >> 2) * (C::kAtom >> 4) + (kk & 3) * 2, id_s, kk > 0 ? 1u : 0u);
+              mma_commit(&bars->sready[g]);
+              if (MT == 1 || g == 1) mma_commit(&bars->kfree[b]);
             }
-            ++step[g];
+            if (io >= 0) ++step[g];
           }
-        }
-        j0 += n;
-        ++seg;
-      } while (ok && at.next_segment(a));
-      mma_commit(&bars->drained);
-    }
-  } else if (warp == 1) {
-    // ── raw codes and scales: K 0 - 63, K 64 - 127, V 0 - 63, V 64 - 127 of a tile ──
-    const int page_mask = (1 << a.page_shift) - 1, per = box >> 4;  // groups of 16 keys a copy
-    // lane i < 8: first head row of keys 16 i .. of a tile; -1 where there are none, -2
-    // behind a number outside the pool
-    auto rows_of = [&](const Place& p) -> int {
-      const int pos = p.t * KT + lane * 16;
-      int row = -1;
-      if (lane < 8 && pos < p.len) {
-        const int pg = __ldg(a.table + (int64_t)p.b * a.width + (pos >> a.page_shift));
-        if ((uint32_t)pg < (uint32_t)a.n_pages) {  // n_pages < 2^31
-          row = ((pg * a.H + p.u / a.row_tiles) << a.page_shift) + (pos & page_mask);
-        } else {
-          if (a.err) atomicCAS(a.err, 0, kErrIndex);
-          row = -2;
-        }
+          j0 += n;
+          ++seg;
+        } while (ok && at.next_segment(a));
+        mma_commit(&bars->drained);
       }
-      return row;
-    };
-    int step = 0;
+    } else if (warp == 1) {
+      // ── raw codes and scales: K 0 - 63, K 64 - 127, V 0 - 63, V 64 - 127 of a tile ──
+      const int page_mask = (1 << a.page_shift) - 1, per = box >> 4;  // groups of 16 keys a copy
+      // lane i < 8: first head row of keys 16 i .. of a tile; -1 where there are none, -2
+      // behind a number outside the pool
+      auto rows_of = [&](const Place& p) -> int {
+        const int pos = p.t * KT + lane * 16;
+        int row = -1;
+        if (lane < 8 && pos < p.len) {
+          const int pg = __ldg(a.table + (int64_t)p.b * a.width + (pos >> a.page_shift));
+          if ((uint32_t)pg < (uint32_t)a.n_pages) {  // n_pages < 2^31
+            row = ((pg * a.H + p.u / a.row_tiles) << a.page_shift) + (pos & page_mask);
+          } else {
+            if (a.err) atomicCAS(a.err, 0, kErrIndex);
+            row = -2;
+          }
+        }
+        return row;
+      };
+      int step = 0;
+      if (any) {
+        int rows = rows_of(at);
+        bool more = true, ok = true;
+        while (more && ok) {
+          Place next = at;
+          more = next.next_tile(a);
+          const int next_rows = more ? rows_of(next) : -1;
+          for (int q = 0; q < 4; ++q, ++step) {
+            const int s = step % C::kRing;
+            ok = step < C::kRing ||
+                 mbar_sleep_warp_to(&bars->raw_empty[s], (step / C::kRing - 1) & 1, kErrTimeoutEmpty, a.err);
+            if (!ok) break;
+            const int row = __shfl_sync(0xffffffffu, rows, (q & 1) * 4 + (lane & 3));
+            const uint32_t gone = __ballot_sync(0xffffffffu, lane < 4 && row == -2);
+            if (lane == 0) bars->gone[s] = gone;  // before its arrival
+            if (lane < 4 && lane % per == 0) {
+              uint64_t* bar = &bars->raw_full[s];
+              if (row >= 0) {
+                uint8_t* dst = smem + C::oRaw + (size_t)s * C::kSlot;
+                mbar_expect_tx(bar, (uint32_t)box * (C::RB + (q < 2 ? 8 : 0)));
+                tma_load_2d(dst + lane * 16 * C::RB, q < 2 ? &tmap_k : &tmap_v, bar, 0,
+                            (int)((int64_t)row * C::RB / 128));  // lines of 128 bytes
+                if (q < 2) {
+                  float* sc = reinterpret_cast<float*>(dst + C::kStep) + lane * 16;
+                  bulk_load_g2s(sc, a.k_scales + row, (uint32_t)box * 4, bar);
+                  bulk_load_g2s(sc + 64, a.v_scales + row, (uint32_t)box * 4, bar);
+                }
+              } else {
+                mbar_arrive(bar);
+              }
+            }
+          }
+          at = next;
+          rows = next_rows;
+        }
+        // the last copies land before the CTA may end, also where a wait gave up
+        for (int j = max(step - C::kRing, 0); j < step; ++j)
+          mbar_sleep_warp_to(&bars->raw_full[j % C::kRing], (j / C::kRing) & 1, kErrTimeoutFull, a.err);
+      }
+    }
+  } else if (warp >= kFirstUnpack) {
     if (any) {
-      int rows = rows_of(at);
+      // ── unpack ──
+      const int t = threadIdx.x - 32 * kFirstUnpack, w = warp - kFirstUnpack;
+      int step = 0;
       bool more = true, ok = true;
-      while (more && ok) {
-        Place next = at;
-        more = next.next_tile(a);
-        const int next_rows = more ? rows_of(next) : -1;
+      float c = 0.0f;                // power of two above every value scale so far (0: none)
+      uint32_t least = 0x7F800000u;  // bits of the smallest so far
+      bool fresh = true;             // a segment's first tile
+      for (int j = 0; more && ok; ++j) {
+        const int b = j & 1, valid = at.len - at.t * KT;  // keys of the tile, from 128 on all
+        if (fresh) {
+          c = 0.0f;
+          least = 0x7F800000u;
+        }
+        float ks = 0.0f, vs = 0.0f, top = 0.0f;  // of this warp's 32 keys; every warp looks at all value scales
+        uint32_t small = least;
+        uint4 gone = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
         for (int q = 0; q < 4; ++q, ++step) {
           const int s = step % C::kRing;
-          ok = step < C::kRing ||
-               mbar_wait_warp_to(&bars->raw_empty[s], (step / C::kRing - 1) & 1, kErrTimeoutEmpty, a.err);
+          ok = mbar_sleep_warp_to(&bars->raw_full[s], (step / C::kRing) & 1, kErrTimeoutFull, a.err);
+          if (ok && j >= 2 && !(q & 1))
+            ok = mbar_sleep_warp_to(q == 0 ? &bars->kfree[b] : &bars->vfree[b], ((j >> 1) - 1) & 1, kErrTimeoutEmpty, a.err);
           if (!ok) break;
-          const int row = __shfl_sync(0xffffffffu, rows, (q & 1) * 4 + (lane & 3));
-          const uint32_t gone = __ballot_sync(0xffffffffu, lane < 4 && row == -2);
-          if (lane == 0) bars->gone[s] = gone;  // before its arrival
-          if (lane < 4 && lane % per == 0) {
-            uint64_t* bar = &bars->raw_full[s];
-            if (row >= 0) {
-              uint8_t* dst = smem + C::oRaw + (size_t)s * C::kSlot;
-              mbar_expect_tx(bar, (uint32_t)box * (C::RB + (q < 2 ? 8 : 0)));
-              tma_load_2d(dst + lane * 16 * C::RB, q < 2 ? &tmap_k : &tmap_v, bar, 0,
-                          (int)((int64_t)row * C::RB / 128));  // lines of 128 bytes
-              if (q < 2) {
-                float* sc = reinterpret_cast<float*>(dst + C::kStep) + lane * 16;
-                bulk_load_g2s(sc, a.k_scales + row, (uint32_t)box * 4, bar);
-                bulk_load_g2s(sc + 64, a.v_scales + row, (uint32_t)box * 4, bar);
+          const uint8_t* src = smem + C::oRaw + (size_t)s * C::kSlot;
+          if (q < 2) {
+            const float* sc = reinterpret_cast<const float*>(src + C::kStep);
+            const uint32_t bad = bars->gone[s];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int key = x * 32 + lane;
+              const bool some = q * 64 + key < valid && !(bad >> (key >> 4) & 1u);
+              const float v = some ? sc[64 + key] : 0.0f;  // nothing was copied for the others
+              top = fmaxf(top, v);
+              if (some) small = min(small, __float_as_uint(v));
+              const uint32_t off = __ballot_sync(0xffffffffu, !some);
+              if (q == 0) (x == 0 ? gone.x : gone.y) = off;
+              else (x == 0 ? gone.z : gone.w) = off;
+              if (w == q * 2 + x) {
+                ks = some ? sc[key] : 0.0f;
+                vs = v;
               }
-            } else {
-              mbar_arrive(bar);
             }
           }
-        }
-        at = next;
-        rows = next_rows;
-      }
-      // the last copies land before the CTA may end, also where a wait gave up
-      for (int j = max(step - C::kRing, 0); j < step; ++j)
-        mbar_wait_warp_to(&bars->raw_full[j % C::kRing], (j / C::kRing) & 1, kErrTimeoutFull, a.err);
-    }
-  } else if (warp >= 12 && any) {
-    // ── unpack ──
-    const int t = threadIdx.x - 384, w = warp - 12;
-    int step = 0;
-    bool more = true, ok = true;
-    float c = 0.0f;                // power of two above every value scale so far (0: none)
-    uint32_t least = 0x7F800000u;  // bits of the smallest so far
-    bool fresh = true;             // a segment's first tile
-    for (int j = 0; more && ok; ++j) {
-      const int b = j & 1, valid = at.len - at.t * KT;  // keys of the tile, from 128 on all
-      if (fresh) {
-        c = 0.0f;
-        least = 0x7F800000u;
-      }
-      float ks = 0.0f, vs = 0.0f, top = 0.0f;  // of this warp's 32 keys; every warp looks at all value scales
-      uint32_t small = least;
-      uint4 gone = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 1
-      for (int q = 0; q < 4; ++q, ++step) {
-        const int s = step % C::kRing;
-        ok = mbar_wait_warp_to(&bars->raw_full[s], (step / C::kRing) & 1, kErrTimeoutFull, a.err);
-        if (ok && j >= 2 && !(q & 1))
-          ok = mbar_wait_warp_to(q == 0 ? &bars->kfree[b] : &bars->vfree[b], ((j >> 1) - 1) & 1, kErrTimeoutEmpty, a.err);
-        if (!ok) break;
-        const uint8_t* src = smem + C::oRaw + (size_t)s * C::kSlot;
-        if (q < 2) {
-          const float* sc = reinterpret_cast<const float*>(src + C::kStep);
-          const uint32_t bad = bars->gone[s];
+          uint8_t* plane = smem + (q < 2 ? C::oK : C::oV) + b * C::kPlane;
+          uint4 raw[C::kPieces];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int key = x * 32 + lane;
-            const bool some = q * 64 + key < valid && !(bad >> (key >> 4) & 1u);
-            const float v = some ? sc[64 + key] : 0.0f;  // nothing was copied for the others
-            top = fmaxf(top, v);
-            if (some) small = min(small, __float_as_uint(v));
-            const uint32_t off = __ballot_sync(0xffffffffu, !some);
-            if (q == 0) (x == 0 ? gone.x : gone.y) = off;
-            else (x == 0 ? gone.z : gone.w) = off;
-            if (w == q * 2 + x) {
-              ks = some ? sc[key] : 0.0f;
-              vs = v;
-            }
+          for (int i = 0; i < C::kPieces; ++i) {
+            int row, cc;
+            piece<BITS, D>(i, t, row, cc);
+            raw[i] = *reinterpret_cast<const uint4*>(src + row * C::RB + cc * 16);
           }
-        }
-        uint8_t* plane = smem + (q < 2 ? C::oK : C::oV) + b * C::kPlane;
-        uint4 raw[C::kPieces];
 #pragma unroll
-        for (int i = 0; i < C::kPieces; ++i) {
-          int row, cc;
-          piece<BITS, D>(i, t, row, cc);
-          raw[i] = *reinterpret_cast<const uint4*>(src + row * C::RB + cc * 16);
-        }
-#pragma unroll
-        for (int i = 0; i < C::kPieces; ++i) {
-          int row, cc;
-          piece<BITS, D>(i, t, row, cc);
-          put_piece<BITS, D>(raw[i], plane, (q & 1) * 64 + row, cc);
-        }
-        if (q & 1) fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars->raw_empty[s]);
-          if (q & 1) mbar_arrive(q == 1 ? &bars->kready[b] : &bars->vready[b]);
-        }
-        if (q == 1) {
-          // bits of non-negative floats rise with them (no NaN passes the fmaxf)
-          const float mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(top, 0.0f))));
-          if (mx > c || c == 0.0f) {
-            // four times the next power of two, between 2^-100 and 2^100
-            const int ex = min(max((int)(__float_as_uint(mx) >> 23) + 3, 27), 227);
-            c = __uint_as_float((uint32_t)ex << 23);
+          for (int i = 0; i < C::kPieces; ++i) {
+            int row, cc;
+            piece<BITS, D>(i, t, row, cc);
+            put_piece<BITS, D>(raw[i], plane, (q & 1) * 64 + row, cc);
           }
-          least = __reduce_min_sync(0xffffffffu, small);
-          float* sl = slots + (j & 3) * kSlotF;
-          sl[t] = ks * a.scale_log2;
-          sl[KT + t] = vs * (kRoom / c);
-          if (t == 0) {
-            const bool wide = __uint_as_float(least) < c * kWide;
-            sl[2 * KT] = (float)((int)(__float_as_uint(c) >> 23) - 127);
-            sl[2 * KT + 1] = __uint_as_float(wide ? 1u : 0u);
-            *reinterpret_cast<uint4*>(sl + 2 * KT + 4) = gone;
-          }
+          if (q & 1) fence_proxy_async_shared();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->scready[j & 3]);
-        }
-      }
-      const int u0 = at.u, b0 = at.b;
-      more = at.next_tile(a);
-      fresh = at.u != u0 || at.b != b0;
-    }
-  } else if (warp >= 4 && any) {
-    // ── softmax ──
-    const int g = (warp >> 2) - 1, q4 = warp & 3, lr = q4 * 32 + lane;
-    const uint32_t lane_sel = (uint32_t)(q4 * 32) << 16;
-    float* xbuf = reinterpret_cast<float*>(smem + C::oX);
-    float4* xml = reinterpret_cast<float4*>(smem + C::oX + 128 * C::kXPitch * 4);
-    bool ok = true;
-    int j0 = 0, step = 0, xs = 0;
-    do {
-      const int n = at.t_hi - at.t_lo;
-      const int h = at.u / a.row_tiles, r0 = (at.u - h * a.row_tiles) * R;
-      const int row = r0 + (MT == 2 ? g * 128 : 0) + lr, tok = row / a.G;
-      const bool live = row < a.rows;
-      const int64_t id = live ? ((int64_t)at.b * a.T + tok) * ((int64_t)a.H * a.G) + (int64_t)h * a.G + (row - tok * a.G) : 0;
-      // ── Q row: bf16 -> fp16 under a power of two, columns in unpack order ──
-      float rowf;
-      {
-        const uint4* qp = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + id * D);
-        float top = 0.0f;
-#pragma unroll 4
-        for (int ch = 0; ch < D / 8; ++ch) {
-          const uint4 x = __ldg(qp + ch);
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)),
-                                   fabsf(__uint_as_float(w[i] & 0xffff0000u))));
-        }
-        const int ex = (int)(__float_as_uint(top) >> 23);
-        const int up = !live || ex == 0 || ex == 255 ? 127 : min(127 + 14 + 127 - ex, 227);
-        const float f = live ? __uint_as_float((uint32_t)up << 23) : 0.0f;
-        rowf = __uint_as_float((uint32_t)(254 - up) << 23);
-        if (MT == 2 || g == 0) {
-          uint8_t* dst = smem + (MT == 2 ? (size_t)g * C::kQ : 0);
-#pragma unroll 4
-          for (int ch = 0; ch < D / 8; ++ch) {
-            const uint4 x = __ldg(qp + ch);  // again, from L1: 16 pieces in registers would spill
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              v[2 * i] = live ? __uint_as_float(w[i] << 16) * f : 0.0f;
-              v[2 * i + 1] = live ? __uint_as_float(w[i] & 0xffff0000u) * f : 0.0f;
-            }
-            const uint4 o = make_uint4(hf2(v[order<BITS>(0)], v[order<BITS>(1)]),
-                                       hf2(v[order<BITS>(2)], v[order<BITS>(3)]),
-                                       hf2(v[order<BITS>(4)], v[order<BITS>(5)]),
-                                       hf2(v[order<BITS>(6)], v[order<BITS>(7)]));
-            *reinterpret_cast<uint4*>(dst + (ch >> 3) * C::kQAtom + lr * 128 + (((ch & 7) ^ (lr & 7)) << 4)) = o;
+          if (lane == 0) {
+            mbar_arrive(&bars->raw_empty[s]);
+            if (q & 1) mbar_arrive(q == 1 ? &bars->kready[b] : &bars->vready[b]);
           }
-          fence_proxy_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->qready);
+          if (q == 1) {
+            // bits of non-negative floats rise with them (no NaN passes the fmaxf)
+            const float mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(top, 0.0f))));
+            if (mx > c || c == 0.0f) {
+              // four times the next power of two, between 2^-100 and 2^100
+              const int ex = min(max((int)(__float_as_uint(mx) >> 23) + 3, 27), 227);
+              c = __uint_as_float((uint32_t)ex << 23);
+            }
+            least = __reduce_min_sync(0xffffffffu, small);
+            float* sl = slots + (j & 3) * kSlotF;
+            sl[t] = ks * a.scale_log2;
+            sl[KT + t] = vs * (kRoom / c);
+            if (t == 0) {
+              const bool wide = __uint_as_float(least) < c * kWide;
+              sl[2 * KT] = (float)((int)(__float_as_uint(c) >> 23) - 127);
+              sl[2 * KT + 1] = __uint_as_float(wide ? 1u : 0u);
+              *reinterpret_cast<uint4*>(sl + 2 * KT + 4) = gone;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->scready[j & 3]);
+          }
         }
+        const int u0 = at.u, b0 = at.b;
+        more = at.next_tile(a);
+        fresh = at.u != u0 || at.b != b0;
       }
-      float rowf4[4];
-      int tok4[4];
+    }
+  } else {
+    if (any) {
+      // ── softmax ──
+      constexpr int kGroup = kSoftWarps / 2;
+      const int g = (warp - kFirstSoft) / kGroup, w16 = (warp - kFirstSoft) % kGroup;  // stream, warp of it
+      const int lane0 = (warp & 3) * 32 + (w16 >> 2) * 16;  // its first TMEM lane, and row
+      const uint32_t lane_sel = (uint32_t)lane0 << 16;
+      const int xt = w16 * 32 + lane;
+      float* xbuf = reinterpret_cast<float*>(smem + C::oX) + xt;
+      float4* xml = reinterpret_cast<float4*>(smem + C::oX + C::kX) + xt;
+      bool ok = true;
+      int j0 = 0, step = 0, xs = 0;
+      do {
+        const int n = at.t_hi - at.t_lo;
+        const int h = at.u / a.row_tiles, r0 = (at.u - h * a.row_tiles) * R + (MT == 2 ? g * 128 : 0) + lane0;
+        auto row_id = [&](int row) -> int64_t {  // row of the unit -> row of the output
+          const int t = row / a.G;
+          return ((int64_t)at.b * a.T + t) * ((int64_t)a.H * a.G) + (int64_t)h * a.G + (row - t * a.G);
+        };
+        // ── Q rows, two lanes each: bf16 -> fp16 under a power of two, columns in unpack order ──
+        float rowf[2];
+        {
+          constexpr int N = D / 16;  // 16-byte pieces a lane, every other of its row
+          const int row = r0 + (lane >> 1);
+          const bool live = row < a.rows;
+          const uint4* qp = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) +
+                                                           (live ? row_id(row) : 0) * D) + (lane & 1);
+          uint4 raw[N];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        rowf4[k] = __shfl_sync(0xffffffffu, rowf, k * 8 + (lane >> 2));
-        tok4[k] = __shfl_sync(0xffffffffu, tok, k * 8 + (lane >> 2));
-      }
-      Rows r4 = {};
-      Tile tile;
-      tile.s = t_s(g) + lane_sel;
-      tile.o = t_o(g) + lane_sel;
-      tile.hist = at.len - a.T;
-      tile.T = a.T;
-      tile.mask = a.tree + (int64_t)at.b * a.tree_b;
-      tile.mask_t = a.tree_t;
-      const int i0 = MT == 2 ? 0 : g, di = MT == 2 ? 1 : 2;
-      for (int i = i0; i < n && ok; i += di, ++step) {
-        const int j = j0 + i;
-        ok = mbar_wait_warp_to(&bars->scready[j & 3], (j >> 2) & 1, kErrTimeoutFull, a.err) &&
-             mbar_wait_warp_to(&bars->sready[g], step & 1, kErrTimeoutTmemFull, a.err);
+          for (int i = 0; i < N; ++i) raw[i] = __ldg(qp + 2 * i);
+          float top = 0.0f;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x[j] << 16)), fabsf(__uint_as_float(x[j] & 0xffff0000u))));
+          }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          const int ex = (int)(__float_as_uint(top) >> 23);
+          const int up = !live || ex == 0 || ex == 255 ? 127 : min(127 + 14 + 127 - ex, 227);
+          const float f = live ? __uint_as_float((uint32_t)up << 23) : 0.0f;
+          const float inv = __uint_as_float((uint32_t)(254 - up) << 23);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) rowf[k] = __shfl_sync(0xffffffffu, inv, (8 * k + (lane >> 2)) * 2);
+          if (MT == 2 || g == 0) {
+            const int lr = lane0 + (lane >> 1);
+            uint8_t* dst = smem + (MT == 2 ? (size_t)g * C::kQ : 0) + lr * 128;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+              float v[8];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                v[2 * j] = live ? __uint_as_float(x[j] << 16) * f : 0.0f;
+                v[2 * j + 1] = live ? __uint_as_float(x[j] & 0xffff0000u) * f : 0.0f;
+              }
+              const uint4 o = make_uint4(hf2(v[order<BITS>(0)], v[order<BITS>(1)]),
+                                         hf2(v[order<BITS>(2)], v[order<BITS>(3)]),
+                                         hf2(v[order<BITS>(4)], v[order<BITS>(5)]),
+                                         hf2(v[order<BITS>(6)], v[order<BITS>(7)]));
+              const int ch = 2 * i + (lane & 1);
+              *reinterpret_cast<uint4*>(dst + (ch >> 3) * C::kQAtom + (((ch & 7) ^ (lr & 7)) << 4)) = o;
+            }
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->qready);
+          }
+        }
+        int tok[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) tok[k] = (r0 + 8 * k + (lane >> 2)) / a.G;
+        Rows r = {};
+        Tile tile;
+        tile.s = t_s(g) + lane_sel;
+        tile.o = t_o(g) + lane_sel;
+        tile.hist = at.len - a.T;
+        tile.T = a.T;
+        tile.mask = a.tree + (int64_t)at.b * a.tree_b;
+        tile.mask_t = a.tree_t;
+        const int i0 = MT == 2 ? 0 : g, di = MT == 2 ? 1 : 2;
+        for (int i = i0; i < n && ok; i += di, ++step) {
+          const int j = j0 + i;
+          ok = mbar_sleep_warp_to(&bars->scready[j & 3], (j >> 2) & 1, kErrTimeoutFull, a.err) &&
+               mbar_sleep_warp_to(&bars->sready[g], step & 1, kErrTimeoutTmemFull, a.err);
+          if (!ok) break;
+          tc_fence_after();
+          tile.slot = slots + (j & 3) * kSlotF;
+          tile.first = i < di;
+          tile.key0 = (at.t_lo + i) * KT;
+          softmax_tile<D>(r, tile, rowf, tok);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->pready[g]);
+        }
+        const bool some = i0 < n;  // this stream had tiles
+        if (some && ok) ok = mbar_sleep_warp_to(&bars->pvdone[g], (step - 1) & 1, kErrTimeoutDone, a.err);
         if (!ok) break;
         tc_fence_after();
-        tile.slot = slots + (j & 3) * kSlotF;
-        tile.first = i < di;
-        tile.key0 = (at.t_lo + i) * KT;
-        softmax_tile<D>(r4, tile, rowf4, tok4);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->pready[g]);
-      }
-      const bool some = i0 < n;  // this stream had tiles
-      if (some && ok) ok = mbar_wait_warp_to(&bars->pvdone[g], (step - 1) & 1, kErrTimeoutDone, a.err);
-      if (!ok) break;
-      tc_fence_after();
-      // ── the segment's part: O = 2^m' sum, m' = m + log2(c / room) ──
+        // ── the segment's part: O = 2^m' sum, m' = m + log2(c / room) ──
+        float4 ml[2];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        r4.l[k] += __shfl_xor_sync(0xffffffffu, r4.l[k], 1);
-        r4.l[k] += __shfl_xor_sync(0xffffffffu, r4.l[k], 2);
-        if (!some) r4.m_top[k] = -INFINITY;
-      }
-      const float l = to_row(r4.l), mu = to_row(r4.mu), lc = to_row(r4.lc);
-      const bool none = to_row(r4.m_top) == -INFINITY;  // l: 0, or of NaN scores
-      float4 ml = none ? make_float4(-INFINITY, l, -INFINITY, 0.0f) : make_float4(mu, l, mu + (lc - 6.0f), 0.0f);
-      float f0 = 1.0f, f1 = 0.0f;
-      if (MT == 1 && n > 1) {
-        // the odd tiles' stream hands its rows to the even tiles', 32 dims at a time
-        if (g == 1) {
-          if (xs > 0) ok = mbar_wait_warp_to(&bars->xfree, (xs - 1) & 1, kErrTimeoutEmpty, a.err);
-          xml[lr] = ml;
+        for (int k = 0; k < 2; ++k) {
+          float l = r.l[k];
+          l += __shfl_xor_sync(0xffffffffu, l, 1);
+          l += __shfl_xor_sync(0xffffffffu, l, 2);
+          const bool none = !some || r.m_top[k] == -INFINITY;  // l: 0, or of NaN scores
+          ml[k] = none ? make_float4(-INFINITY, l, -INFINITY, 0.0f)
+                       : make_float4(r.mu[k], l, r.mu[k] + (r.lc[k] - 6.0f), 0.0f);
         }
-      }
-      const bool first = at.t_lo == 0, direct = a.direct && first && at.t_hi == at.n_tiles;
-      float* po = nullptr;
-      float inv = 0.0f;
+        const bool both = MT == 1 && n > 1;
+        if (MT == 1 && g == 1 && !both) {  // a single tile: nothing to hand over
+          j0 += n;
+          continue;
+        }
+        float f0[2] = {1.0f, 1.0f}, f1[2] = {0.0f, 0.0f}, inv[2] = {0.0f, 0.0f};
+        const bool first = at.t_lo == 0, direct = a.direct && first && at.t_hi == at.n_tiles;
+        int64_t id[2], part[2];
 #pragma unroll 1
-      for (int d = 0; d < D; d += 32) {
-        uint32_t v[32];
-        __syncwarp();
-        if (some) {
-          tmem_ld32(t_o(g) + lane_sel + d, v);
-          tmem_wait_ld();
-          tmem_landed(v);
-        }
-        if (MT == 1 && n > 1) {
-          if (g == 1) {
-            if (d > 0) ok = ok && mbar_wait_warp_to(&bars->xfree, (xs - 1) & 1, kErrTimeoutEmpty, a.err);
+        for (int d = 0; d < D; d += 32) {
+          uint32_t v[16];
+          tmem_get(t_o(g) + lane_sel + d, v);
+          if (both) {
+            // the odd tiles' stream hands its rows to the even tiles', 32 columns at a time
+            if (g == 1) {
+              if (xs > 0) ok = mbar_sleep_warp_to(&bars->xfree, (xs - 1) & 1, kErrTimeoutEmpty, a.err);
+              if (!ok) break;
+              if (d == 0) {
+                xml[0] = ml[0];
+                xml[32 * kGroup] = ml[1];
+              }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) xbuf[i * 32 * kGroup] = __uint_as_float(v[i]);
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bars->xfull);
+              ++xs;
+              continue;
+            }
+            ok = mbar_sleep_warp_to(&bars->xfull, xs & 1, kErrTimeoutFull, a.err);
             if (!ok) break;
+            if (d == 0) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) xbuf[lr * C::kXPitch + i] = __uint_as_float(v[i]);
+              for (int k = 0; k < 2; ++k) {
+                const float4 x = ml[k], y = xml[k * 32 * kGroup];
+                const float mx = fmaxf(x.x, y.x), mw = fmaxf(x.z, y.z);
+                const float mb = mx == -INFINITY ? 0.0f : mx, wb = mw == -INFINITY ? 0.0f : mw;
+                f0[k] = ex2(x.z - wb);
+                f1[k] = ex2(y.z - wb);
+                // the sum of NaN scores alone stands beside no maximum
+                ml[k] = make_float4(mx, mx == -INFINITY ? x.y + y.y : ex2(x.x - mb) * x.y + ex2(y.x - mb) * y.y, mw,
+                                    0.0f);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              v[i] = __float_as_uint(f0[(i >> 1) & 1] * __uint_as_float(v[i]) +
+                                     f1[(i >> 1) & 1] * xbuf[i * 32 * kGroup]);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->xfull);
+            if (lane == 0) mbar_arrive(&bars->xfree);
             ++xs;
-            continue;
           }
-          ok = mbar_wait_warp_to(&bars->xfull, xs & 1, kErrTimeoutFull, a.err);
-          if (!ok) break;
           if (d == 0) {
-            const float4 other = xml[lr];
-            const float mx = fmaxf(ml.x, other.x), mw = fmaxf(ml.z, other.z);
-            const float mb = mx == -INFINITY ? 0.0f : mx, wb = mw == -INFINITY ? 0.0f : mw;
-            f0 = ex2(ml.z - wb);
-            f1 = ex2(other.z - wb);
-            ml = make_float4(mx, ex2(ml.x - mb) * ml.y + ex2(other.x - mb) * other.y, mw, 0.0f);
-            // the sum of NaN scores alone stands beside no maximum
-            if (mx == -INFINITY) ml.y = l + other.y;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int row = r0 + 8 * k + (lane >> 2);
+              id[k] = row < a.rows ? row_id(row) : -1;
+              part[k] = first ? id[k] : (int64_t)blockIdx.x * R + row - (at.u - h * a.row_tiles) * R;
+              const float mb = ml[k].x == -INFINITY ? 0.0f : ml[k].x, l = ml[k].y;
+              inv[k] = l != l ? l : ml[k].z == -INFINITY ? 0.0f : ex2(ml[k].z - mb) / l;  // NaN scores: NaN
+              if (id[k] >= 0 && (lane & 3) == 0) {
+                if (!direct) reinterpret_cast<float4*>(first ? a.main_ml : a.cta_ml)[part[k]] = ml[k];
+                else if (a.lse) a.lse[id[k]] = l == 0.0f ? -INFINITY : (mb + __log2f(l)) * 0.69314718055994531f;
+              }
+            }
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            v[i] = __float_as_uint(f0 * __uint_as_float(v[i]) + f1 * xbuf[lr * C::kXPitch + i]);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->xfree);
-          ++xs;
-        } else if (MT == 1 && g == 1) {
-          break;  // a single tile: nothing to hand over
-        }
-        if (!live) continue;
-        if (d == 0) {
-          const int64_t pr = first ? id : (int64_t)blockIdx.x * R + (row - r0);
-          po = (first ? a.main_o : a.cta_o) + pr * D;
-          if (direct) {
-            const float mb = ml.x == -INFINITY ? 0.0f : ml.x;
-            inv = ml.z == -INFINITY ? 0.0f : ex2(ml.z - mb) / ml.y;
-            if (ml.y != ml.y) inv = ml.y;  // NaN scores
-            if (a.lse) a.lse[id] = ml.y == 0.0f ? -INFINITY : (mb + __log2f(ml.y)) * 0.69314718055994531f;
-          } else {
-            reinterpret_cast<float4*>(first ? a.main_ml : a.cta_ml)[pr] = ml;
-          }
-        }
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int g8 = 0; g8 < 32; g8 += 8) {
-          float o[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[order<BITS>(i)] = __uint_as_float(v[g8 + i]);
-          if (direct) {
-            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + id * D + d + g8) =
-                make_uint4(bf2(o[0] * inv, o[1] * inv), bf2(o[2] * inv, o[3] * inv), bf2(o[4] * inv, o[5] * inv),
-                           bf2(o[6] * inv, o[7] * inv));
-          } else {
-            // a whole 32-byte sector a lane
-            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(po + d + g8),
-                         "f"(o[0]), "f"(o[1]), "f"(o[2]), "f"(o[3]), "f"(o[4]), "f"(o[5]), "f"(o[6]), "f"(o[7])
-                         : "memory");
-          }
+            for (int k = 0; k < 2; ++k) {
+              const float2 o = in_order<BITS>(__uint_as_float(v[4 * i + 2 * k]), __uint_as_float(v[4 * i + 2 * k + 1]));
+              const int col = d + 8 * i + 2 * (lane & 3);
+              if (id[k] < 0) continue;
+              if (direct)
+                *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + id[k] * D + col) =
+                    bf2(o.x * inv[k], o.y * inv[k]);
+              else
+                *reinterpret_cast<float2*>((first ? a.main_o : a.cta_o) + part[k] * D + col) = o;
+            }
         }
-      }
-      __syncwarp();
-      tc_fence_before();
-      j0 += n;
-    } while (ok && at.next_segment(a));
+        __syncwarp();
+        tc_fence_before();
+        j0 += n;
+      } while (ok && at.next_segment(a));
+    }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
-    if (any) mbar_wait_warp_to(&bars->drained, 0, kErrTimeoutDone, a.err);
+    if (any) mbar_sleep_warp_to(&bars->drained, 0, kErrTimeoutDone, a.err);
     tc_fence_after();
     tmem_dealloc(tbase, 512);
   }
