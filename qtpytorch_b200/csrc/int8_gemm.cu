@@ -271,6 +271,284 @@ int launch(const CUtensorMap& tf, const CUtensorMap& tt, const Args& a, cudaStre
   return MXB_OK;
 }
 
+// ── many tokens ─────────────────────────────────────────────────────────────
+// A pair of CTAs (cta_group::2) owns a tile of 256 tokens x BN features: each loads
+// its 128 tokens and half of the features, and the pair's MMAs (M = 256) read both
+// halves, so that an SM draws 64 bytes a cycle of operands at the full rate where one
+// CTA's 128 x 128 tile draws 128.  Pairs walk the list of tiles; the accumulators are
+// double (2 x BN columns of TMEM), so that the epilogue of a tile runs beside the
+// products of the next.
+//   warp 0      TMA producer (either CTA; both count on the leader's barriers);
+//   warp 1      MMAs (the leader's);  warps 2, 3  TMEM allocation, idle;
+//   warps 4-11  epilogue: a thread a token and half of the columns; 32 tokens x 128
+//               bytes leave as one TMA store from shared memory.
+namespace wide {
+
+constexpr int kEpi = 8;
+constexpr int kThreads = 128 + 32 * kEpi;
+constexpr int kA = 128 * BK;            // a CTA's tokens of a stage
+constexpr int kOut = 32 * 128;          // a warp's piece of the output
+template <int BN>
+struct Cfg {
+  static constexpr int kB = BN / 2 * BK;  // and features
+  static constexpr int kStage = kA + kB;
+  static constexpr int S = BN == 256 ? 6 : 8;
+  static constexpr size_t oOut = (size_t)S * kStage, oBars = oOut + kEpi * kOut;
+  static constexpr size_t kSmem = 1024 + oBars + 512;
+};
+
+struct Bars {
+  uint64_t full[8], empty[8];
+  uint64_t acc[2], acc_free[2];
+  uint32_t tmem_base;
+};
+static_assert(sizeof(Bars) <= 512, "barrier block overflows its slot");
+
+struct Tiles {
+  int m, n, total;  // tiles along the tokens and the features
+};
+
+__device__ __forceinline__ uint32_t rank_of() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The address of a shared variable in the pair's leader.
+__device__ __forceinline__ uint32_t in_leader(const void* p) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(0));
+  return a;
+}
+// A TMA load into this CTA whose bytes count on the leader's barrier (no multicast).
+__device__ __forceinline__ void load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on `bar` of both CTAs when all MMAs issued so far are complete.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Tile i: runs of 8 tiles along the tokens, so that the pairs at work share both
+// operands in L2.
+__device__ __forceinline__ void tile_at(const Tiles& t, int i, int& m, int& n) {
+  const int band = 8 * t.n, b = i / band, rows = min(8, t.m - 8 * b), r = i - b * band;
+  n = r / rows;
+  m = 8 * b + (r - n * rows);
+}
+
+template <int BN, typename OutT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    int8_wide_kernel(const __grid_constant__ CUtensorMap tmap_f, const __grid_constant__ CUtensorMap tmap_t,
+                     const __grid_constant__ CUtensorMap tmap_o, const Args a, const Tiles tiles) {
+  using C = Cfg<BN>;
+  constexpr int S = C::S;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  Bars* bars = reinterpret_cast<Bars*>(smem + C::oBars);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = rank_of();
+  const int first = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars->acc[b], 1);
+      mbar_init(&bars->acc_free[b], 2 * kEpi);
+    }
+    fence_barrier_init();
+    prefetch_tmap(&tmap_f);
+    prefetch_tmap(&tmap_t);
+    prefetch_tmap(&tmap_o);
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&bars->tmem_base)),
+                 "r"(2 * BN)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are set up
+  tc_fence_after();
+  const uint32_t tbase = bars->tmem_base;
+  pdl_trigger();
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0, round = 0, issued = 0;
+      bool ok = true;
+      for (int i = first; i < tiles.total && ok; i += pairs) {
+        int m, n;
+        tile_at(tiles, i, m, n);
+        const int y_t = m * 256 + (int)rank * 128, y_f = n * BN + (int)rank * (BN / 2);
+        for (int k = 0; k < a.ksteps; ++k) {
+          if (round > 0 && !mbar_wait_to(&bars->empty[s], (round - 1) & 1, kErrTimeoutEmpty, a.err)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_expect_tx(&bars->full[s], 2 * C::kStage);
+          const uint32_t bar = in_leader(&bars->full[s]);
+          uint8_t* dst = smem + s * C::kStage;
+          load_pair(dst, &tmap_t, bar, k * BK, y_t);
+          load_pair(dst + kA, &tmap_f, bar, k * BK, y_f);
+          ++issued;
+          if (++s == S) {
+            s = 0;
+            ++round;
+          }
+        }
+      }
+      // the pair's last copies land before it may end (the leader counts both CTAs'), also
+      // where a wait gave up
+      if (rank == 0)
+        for (int j = max(issued - S, 0); j < issued; ++j)
+          mbar_wait_to(&bars->full[j % S], (j / S) & 1, kErrTimeoutFull, a.err);
+    }
+  } else if (warp == 1 && rank == 0) {
+    if (lane == 0) {
+      constexpr uint32_t id = make_idesc(/*S32*/ 2, /*signed*/ 1, 0, 0, 256, BN);
+      const uint64_t da = desc_kmajor_sw128(smem_u32(smem)), db = desc_kmajor_sw128(smem_u32(smem + kA));
+      int s = 0, round = 0, t = 0;
+      bool ok = true;
+      for (int i = first; i < tiles.total && ok; i += pairs, ++t) {
+        const int b = t & 1;
+        if (t >= 2) ok = mbar_wait_to(&bars->acc_free[b], ((t >> 1) - 1) & 1, kErrTimeoutTmemEmpty, a.err);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t acc = tbase + b * BN;
+        for (int k = 0; k < a.ksteps; ++k) {
+          if (!mbar_wait_to(&bars->full[s], round & 1, kErrTimeoutFull, a.err)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t off = (uint32_t)(s * C::kStage) >> 4;
+#pragma unroll
+          for (int kk = 0; kk < BK / 32; ++kk)
+            mma_pair(acc, da + off + kk * 2, db + off + kk * 2, id, (k > 0 || kk > 0) ? 1u : 0u);
+          commit_pair(&bars->empty[s]);
+          if (++s == S) {
+            s = 0;
+            ++round;
+          }
+        }
+        commit_pair(&bars->acc[b]);  // of all that were issued, also where a wait gave up
+      }
+    }
+  } else if (warp >= 4) {
+    // ── epilogue ──
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    uint8_t* stage = smem + C::oOut + (warp - 4) * kOut;
+    constexpr int kCols = 128 / sizeof(OutT);  // a piece's columns: 64 or 32
+    int t = 0;
+    for (int i = first; i < tiles.total; i += pairs, ++t) {
+      int m, n;
+      tile_at(tiles, i, m, n);
+      const int b = t & 1, row0 = m * 256 + (int)rank * 128 + q * 32;
+      if (!mbar_wait_warp_to(&bars->acc[b], (t >> 1) & 1, kErrTimeoutDone, a.err)) break;
+      tc_fence_after();
+      const float st = row0 + lane < a.M ? __ldg(a.st + (int64_t)(row0 + lane) * a.st_step) : 0.0f;
+      const uint32_t acc = tbase + b * BN + ((uint32_t)(q * 32) << 16) + half * (BN / 2);
+      const int c0 = n * BN + half * (BN / 2);
+#pragma unroll 1
+      for (int p = 0; p < BN / 2; p += kCols) {
+        // the piece before has been read
+        if (lane == 0) bulk_wait_read();
+        __syncwarp();
+#pragma unroll
+        for (int x = 0; x < kCols; x += 32) {
+          uint32_t r[32];
+          tmem_ld32(acc + p + x, r);
+          tmem_wait_ld();
+          tmem_landed(r);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const int col = c0 + p + x + j;
+            float4 sf = make_float4(0.0f, 0.0f, 0.0f, 0.0f), bv = sf;
+            if (col < a.N) {  // N is a multiple of 4
+              if (a.sf_step) sf = __ldg(reinterpret_cast<const float4*>(a.sf + col));
+              else sf.x = sf.y = sf.z = sf.w = __ldg(a.sf);
+              if (a.bias) bv = __ldg(reinterpret_cast<const float4*>(a.bias + col));
+            }
+            const float v0 = scaled((int)r[j], st, sf.x, bv.x), v1 = scaled((int)r[j + 1], st, sf.y, bv.y);
+            const float v2 = scaled((int)r[j + 2], st, sf.z, bv.z), v3 = scaled((int)r[j + 3], st, sf.w, bv.w);
+            if constexpr (sizeof(OutT) == 4) {
+              *reinterpret_cast<float4*>(stage + lane * 128 + (((j / 4) ^ (lane & 7)) << 4)) =
+                  make_float4(v0, v1, v2, v3);
+            } else {
+              const __nv_bfloat162 lo = __floats2bfloat162_rn(v0, v1), hi = __floats2bfloat162_rn(v2, v3);
+              // 16-byte chunk (x + j) / 8 of the row, its half j / 4 % 2
+              *reinterpret_cast<uint2*>(stage + lane * 128 + ((((x + j) / 8) ^ (lane & 7)) << 4) + (j & 4) * 2) =
+                  make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            }
+          }
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0 && row0 < a.M && c0 + p < a.N) {
+          tma_store_2d(&tmap_o, stage, c0 + p, row0);
+          bulk_commit();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_remote(in_leader(&bars->acc_free[b]));
+    }
+    if (lane == 0) bulk_wait_read();
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no CTA ends while its pair may still read or signal it
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(2 * BN));
+  }
+}
+
+template <int BN, typename OutT>
+int launch(const CUtensorMap& tf, const CUtensorMap& tt, const CUtensorMap& to, const Args& a, cudaStream_t st) {
+  using C = Cfg<BN>;
+  static_assert(C::kSmem <= 227 * 1024, "shared memory");
+  auto kern = int8_wide_kernel<BN, OutT>;
+  MXB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem));
+  Tiles t;
+  t.m = (int)cdiv(a.M, 256);
+  t.n = (int)cdiv(a.N, BN);
+  t.total = t.m * t.n;
+  const int pairs = t.total < kSMs / 2 ? t.total : kSMs / 2;
+  MXB_CUDA_TRY(launch_pdl(kern, dim3((unsigned)(2 * pairs)), kThreads, C::kSmem, st, tf, tt, to, a, t));
+  MXB_LAUNCH_CHECK();
+  return MXB_OK;
+}
+
+}  // namespace wide
+
 // Rows of K bytes -> rows of Kp, zero from K on.
 __global__ void __launch_bounds__(256)
     pad_rows_kernel(const uint8_t* __restrict__ a, int64_t ra, const uint8_t* __restrict__ b, int64_t rb, int K,
@@ -291,10 +569,35 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Features of a pair's tile, 0: the kernel for few tokens.
+int wide_features(int64_t M, int64_t N) {
+  if (M <= 128) return 0;
+  const int64_t m = cdiv(M, 256);
+  if (m * cdiv(N, 256) >= kSMs / 2) return 256;
+  return m * cdiv(N, 128) >= kSMs / 4 ? 128 : 0;
+}
+
 template <typename OutT>
 int dispatch(const void* fcodes, const void* tcodes, int64_t ldk, Args& a, cudaStream_t st) {
   const int64_t ft = cdiv(a.N, BM);
   CUtensorMap tf, tt;
+  // whole TMA lines of the output, 16-byte groups of scales and bias
+  const bool lines = a.N % (16 / (int)sizeof(OutT)) == 0 && (uintptr_t)a.out % 16 == 0 &&
+                     ((uintptr_t)a.sf | (uintptr_t)a.bias) % 16 == 0;
+  const int bn = wide_features(a.M, a.N);
+  if (lines && bn) {
+    CUtensorMap to;
+    const bool half = sizeof(OutT) == 2;
+    if (!encode_tmap_2d(&tf, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, fcodes, (uint64_t)ldk, (uint64_t)a.N, BK, bn / 2,
+                        CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !encode_tmap_2d(&tt, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, tcodes, (uint64_t)ldk, (uint64_t)a.M, BK, 128,
+                        CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !encode_tmap_2d(&to, half ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                        sizeof(OutT), a.out, (uint64_t)a.N, (uint64_t)a.M, 128 / sizeof(OutT), 32,
+                        CU_TENSOR_MAP_SWIZZLE_128B))
+      return MXB_E_CUDA;
+    return bn == 256 ? wide::launch<256, OutT>(tf, tt, to, a, st) : wide::launch<128, OutT>(tf, tt, to, a, st);
+  }
   const int nt = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
   const int64_t tiles = ft * cdiv(a.M, nt);
   int64_t splits = (nt >= 128 ? kSMs : 2 * kSMs) / tiles;
