@@ -156,28 +156,38 @@ struct AppendRows {
   bool vec;
 };
 
-// Four consecutive values.
-__device__ __forceinline__ void load4v(const float* p, bool vec, float (&v)[4]) {
-  if (vec) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = p[i];
+// Four values as they lie in memory, for loads in flight.
+template <typename T>
+struct Raw4;
+template <>
+struct Raw4<float> {
+  float4 r;
+  __device__ __forceinline__ void load(const float* p, bool vec) {
+    if (vec) r = __ldg(reinterpret_cast<const float4*>(p));
+    else r = make_float4(p[0], p[1], p[2], p[3]);
   }
-}
-__device__ __forceinline__ void load4v(const __nv_bfloat16* p, bool vec, float (&v)[4]) {
-  if (vec) {
-    const uint2 r = __ldg(reinterpret_cast<const uint2*>(p));
+  __device__ __forceinline__ void get(float (&v)[4]) const {
+    v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
+  }
+};
+template <>
+struct Raw4<__nv_bfloat16> {
+  uint2 r;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, bool vec) {
+    if (vec) {
+      r = __ldg(reinterpret_cast<const uint2*>(p));
+    } else {
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+      r = make_uint2(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[4]) const {
     v[0] = __uint_as_float(r.x << 16);
     v[1] = __uint_as_float(r.x & 0xffff0000u);
     v[2] = __uint_as_float(r.y << 16);
     v[3] = __uint_as_float(r.y & 0xffff0000u);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __bfloat162float(p[i]);
   }
-}
+};
 __device__ __forceinline__ void store4(float* p, const float (&v)[4]) {
   *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
@@ -211,6 +221,28 @@ __global__ void __launch_bounds__(kThreads)
   pdl_wait();
   const int64_t t0 = (int64_t)blockIdx.x * TB;
   const int tokens = (int)min((int64_t)TB, a.T - t0);
+  const int part = threadIdx.x % L, q_rows = tokens * a.Hq, kv_rows = tokens * a.H;
+  // this lane's two runs of four values, and whether they turn
+  const bool turns = part < ro.pairs / 4;
+  const int oa = ILV || !turns ? part * 8 : part * 4, ob = ILV || !turns ? oa + 4 : ro.pairs + part * 4;
+  // rows of queries, kU of them in flight; the first while the angles are found
+  constexpr int kU = 4;
+  const InT* q = static_cast<const InT*>(a.q);
+  Raw4<InT> qa[kU], qb[kU];
+  auto load_q = [&](int u0) {
+#pragma unroll
+    for (int i = 0; i < kU; ++i) {
+      const int u = u0 + i * kRows;
+      if (u < q_rows) {
+        const int t = u / a.Hq, h = u - t * a.Hq;
+        const InT* p = q + (t0 + t) * a.q_ts + h * a.q_hs;
+        qa[i].load(p + oa, a.vec);
+        qb[i].load(p + ob, a.vec);
+      }
+    }
+  };
+  int u0 = threadIdx.x / L;
+  load_q(u0);
   for (int i = threadIdx.x; i < tokens * ro.pairs; i += kThreads) {
     const int t = i / ro.pairs, p = i - t * ro.pairs;
     const int axis = (p >= ro.end[0]) + (p >= ro.end[1]) + (p >= ro.end[2]);
@@ -221,36 +253,10 @@ __global__ void __launch_bounds__(kThreads)
     reinterpret_cast<float2*>(lo[t])[p] = make_float2((float)(c - (double)ch), (float)(s - (double)sh));
   }
   __syncthreads();
-  const int part = threadIdx.x % L, R = a.Hq + a.H;
-  // this lane's two runs of four values, and whether they turn
-  const bool turns = part < ro.pairs / 4;
-  const int oa = ILV || !turns ? part * 8 : part * 4, ob = ILV || !turns ? oa + 4 : ro.pairs + part * 4;
-  const int q_rows = tokens * a.Hq, units = tokens * R;
-  // q rows of all tokens, then the keys with the values beside them
-  for (int u0 = threadIdx.x / 32 * (32 / L); u0 < units; u0 += kRows) {
-    const int u = u0 + (threadIdx.x % 32) / L;
-    const bool live = u < units, is_q = u < q_rows;
-    const int row = live ? (is_q ? u : u - q_rows) : 0, per = is_q || !live ? a.Hq : a.H;
-    const int t = per ? row / per : 0, h = row - t * per;
-    float x[8], y[8], w[8];
-    float (&xa)[4] = *reinterpret_cast<float (*)[4]>(x), (&xb)[4] = *reinterpret_cast<float (*)[4]>(x + 4);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = w[j] = 0.0f;
-    int64_t slot = -1;
-    if (live) {
-      const InT* p = is_q ? static_cast<const InT*>(a.q) + (t0 + t) * a.q_ts + h * a.q_hs
-                          : static_cast<const InT*>(a.k) + (t0 + t) * a.k_ts + h * a.k_hs;
-      load4v(p + oa, a.vec, xa);
-      load4v(p + ob, a.vec, xb);
-      if (!is_q) {
-        slot = slots[t0 + t];
-        load8v(static_cast<const InT*>(a.v) + (t0 + t) * a.v_ts + h * a.v_hs + part * 8, a.vec, w);
-      }
-    }
-    // pair j of this lane: values (j, j + 4), or (2 j, 2 j + 1)
-    auto first = [](int j) { return ILV ? 2 * j : j; };
-    auto second = [](int j) { return ILV ? 2 * j + 1 : j + 4; };
-    float cs[8];  // cosine and sine of the four pairs
+  // pair j of this lane: values (j, j + 4), or (2 j, 2 j + 1)
+  auto first = [](int j) { return ILV ? 2 * j : j; };
+  auto second = [](int j) { return ILV ? 2 * j + 1 : j + 4; };
+  auto turn = [&](int t, const float (&x)[8], float (&y)[8], float (&cs)[8]) {
     if (turns) {
       const float4 c0 = hi[t][part * 2], c1 = hi[t][part * 2 + 1];
       cs[0] = c0.x; cs[1] = c0.y; cs[2] = c0.z; cs[3] = c0.w;
@@ -265,12 +271,47 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = x[j];
     }
-    if (live && is_q) {
-      InT* o = q_out + ((t0 + t) * a.Hq + h) * D;
-      store4(o + oa, *reinterpret_cast<float (*)[4]>(y));
-      store4(o + ob, *reinterpret_cast<float (*)[4]>(y + 4));
+  };
+  auto get8 = [](const Raw4<InT>& r0, const Raw4<InT>& r1, float (&x)[8]) {
+    r0.get(*reinterpret_cast<float (*)[4]>(x));
+    r1.get(*reinterpret_cast<float (*)[4]>(x + 4));
+  };
+  while (u0 < q_rows) {
+#pragma unroll
+    for (int i = 0; i < kU; ++i) {
+      const int u = u0 + i * kRows;
+      if (u < q_rows) {
+        const int t = u / a.Hq;
+        float x[8], y[8], cs[8];
+        get8(qa[i], qb[i], x);
+        turn(t, x, y, cs);
+        InT* o = q_out + (t0 * a.Hq + u) * D;  // u counts a token's heads in their order
+        store4(o + oa, *reinterpret_cast<float (*)[4]>(y));
+        store4(o + ob, *reinterpret_cast<float (*)[4]>(y + 4));
+      }
     }
-    if (!__any_sync(0xffffffffu, live && !is_q)) continue;
+    u0 += kU * kRows;
+    load_q(u0);
+  }
+  // keys, with the values beside them; a warp goes through its loop as one
+  for (int u1 = threadIdx.x / 32 * (32 / L); u1 < kv_rows; u1 += kRows) {
+    const int u = u1 + (threadIdx.x % 32) / L;
+    const bool live = u < kv_rows;
+    const int t = live ? u / a.H : 0, h = live ? u - t * a.H : 0;
+    float x[8], y[8], w[8], cs[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = w[j] = 0.0f;
+    int64_t slot = -1;
+    if (live) {
+      const InT* p = static_cast<const InT*>(a.k) + (t0 + t) * a.k_ts + h * a.k_hs;
+      Raw4<InT> r0, r1;
+      r0.load(p + oa, a.vec);
+      r1.load(p + ob, a.vec);
+      slot = slots[t0 + t];
+      load8v(static_cast<const InT*>(a.v) + (t0 + t) * a.v_ts + h * a.v_hs + part * 8, a.vec, w);
+      get8(r0, r1, x);
+    }
+    turn(t, x, y, cs);
     // value j turned in 64 bits, rounded to fp32
     auto again = [&](int j) -> float {
       const int i = ILV ? j >> 1 : j & 3;
@@ -300,7 +341,7 @@ __global__ void __launch_bounds__(kThreads)
       for (int o = L >> 1; o > 0; o >>= 1) best = nan_max(best, __shfl_xor_sync(0xffffffffu, best, o));
       top = best;
     }
-    if (!live || is_q || slot < 0) continue;
+    if (!live || slot < 0) continue;
     if (slot >= n_slots) {
       if (part == 0 && err) atomicCAS(err, 0, kErrIndexCode);
       continue;

@@ -28,22 +28,34 @@ namespace {
 constexpr int kWarpRows = 8;     // rows a block where a row is a warp's
 constexpr int kMaxRow = 32768;   // 1024 threads of 32 values
 
-// 8 consecutive values at p + i (VEC: 16-byte aligned; i + 8 <= d).
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-  const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+// 8 consecutive values as they lie in memory (16-byte aligned).
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = __ldg(reinterpret_cast<const float4*>(p));
+    b = __ldg(reinterpret_cast<const float4*>(p) + 1);
   }
-}
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+};
+template <>
+struct Raw8<__nv_bfloat16> {
+  uint4 r;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { r = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -76,7 +88,7 @@ struct Row {
     if (r) h = __fadd_rn(h, load_as_f32(r, i));
     return h;
   }
-  __device__ __noinline__ double u64(int i) const { return h64(i) * (double)load_as_f32(w, i); }
+  __device__ __forceinline__ double u64(int i) const { return h64(i) * (double)load_as_f32(w, i); }
 };
 
 struct Shared {
@@ -127,9 +139,9 @@ __device__ __noinline__ void row_in_64_bits(const Row<InT, WT>& row, double eps,
 }
 
 // WARP: a warp a row, kWarpRows of them a block; otherwise a block of up to MAX
-// threads a row.
-template <typename InT, typename WT, int NC, int MAX, bool VEC, bool WARP>
-__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : MAX)
+// threads a row, MIN of them on an SM.
+template <typename InT, typename WT, int NC, int MAX, int MIN, bool VEC, bool WARP>
+__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : MAX, MIN)
     rms_norm_kernel(const InT* __restrict__ x, const InT* __restrict__ r, int64_t rows, int d, int64_t ldx,
                     int64_t ldr, const WT* __restrict__ w, double eps, float inv_d, int8_t* __restrict__ codes,
                     float* __restrict__ scales, InT* __restrict__ h_out) {
@@ -152,45 +164,57 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : MAX)
   float u[NC][8];
   float ssq = 0.0f, top = 0.0f;
   if constexpr (VEC) {
-    float xv[NC][8], rv[NC][8];
+    // x and r of the whole row on their way at once; as many registers as u takes after
+    Raw8<InT> xr[NC], rr[NC];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
+    for (int c = 0; c < NC; ++c)
       if (index(c, 0) < d) {
-        load8(row.x + index(c, 0), xv[c]);
-        if (r) load8(row.r + index(c, 0), rv[c]);
-        load8(w + index(c, 0), u[c]);
+        xr[c].load(row.x + index(c, 0));
+        if (r) rr[c].load(row.r + index(c, 0));
       }
-    }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       if (index(c, 0) < d) {
+        Raw8<WT> wr;
+        wr.load(w + index(c, 0));
+        float h[8], v[8];
+        xr[c].get(h);
         if (r) {
+          rr[c].get(v);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) xv[c][j] = __fadd_rn(xv[c][j], rv[c][j]);
+          for (int j = 0; j < 8; ++j) h[j] = __fadd_rn(h[j], v[j]);
         }
-        if (ho) store8(ho + index(c, 0), xv[c]);
+        if (ho) store8(ho + index(c, 0), h);
+        wr.get(v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          ssq = fmaf(xv[c][j], xv[c][j], ssq);
-          u[c][j] = __fmul_rn(xv[c][j], u[c][j]);
+          ssq = fmaf(h[j], h[j], ssq);
+          u[c][j] = __fmul_rn(h[j], v[j]);
           top = amax_step(top, u[c][j]);
         }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[c][j] = 0.0f;
       }
     }
   } else {
+    float h[NC][8];
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int i = index(c, j);
-        u[c][j] = 0.0f;
-        if (i < d) {
-          const float h = row.h32(i);
-          if (ho) store1(ho + i, h);
-          ssq = fmaf(h, h, ssq);
-          u[c][j] = __fmul_rn(h, load_as_f32(w, i));
-          top = amax_step(top, u[c][j]);
-        }
+        h[c][j] = i < d ? row.h32(i) : 0.0f;
+        u[c][j] = i < d ? load_as_f32(w, i) : 0.0f;
+      }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (ho && index(c, j) < d) store1(ho + index(c, j), h[c][j]);
+        ssq = fmaf(h[c][j], h[c][j], ssq);
+        u[c][j] = index(c, j) < d ? __fmul_rn(h[c][j], u[c][j]) : 0.0f;
+        top = amax_step(top, u[c][j]);
       }
   }
 #pragma unroll
@@ -221,14 +245,20 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : MAX)
     row_in_64_bits<InT, WT>(row, eps, t, n, &sm, code, scales + at, nullptr);
     return;
   }
+  // Elements that need 64 bits: a bit each, so that there is one place that reads them again.
+  auto of_bit = [&](uint32_t bits) {
+    const int b = __ffs(bits) - 1;
+    return index(b >> 3, b & 7);
+  };
   // ── the largest |u| in 64 bits, of those that fp32 cannot tell from it ──
   const float near_top = top * (1.0f - 0x1p-21f);
   double most = 0.0;
+  uint32_t bits = 0;
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (index(c, VEC ? 0 : j) < d && fabsf(u[c][j]) >= near_top) most = fmax(most, fabs(row.u64(index(c, j))));
+    for (int j = 0; j < 8; ++j) bits |= fabsf(u[c][j]) >= near_top ? 1u << (8 * c + j) : 0u;
+  for (; bits; bits &= bits - 1) most = fmax(most, fabs(row.u64(of_bit(bits))));
   if constexpr (WARP) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -239,30 +269,33 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : MAX)
     most = __longlong_as_double((long long)sm.most);
   }
   const float factor = __fdiv_rn(127.0f, (float)most);
-  constexpr float kNear = 0.5f - 127.0f * 0x1p-21f;
+  constexpr float kNear = 0.5f - 127.0f * 0x1p-21f, kRound = 12582912.0f;  // 1.5 * 2^23
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    if (VEC && index(c, 0) >= d) break;
-    int q[8];
+    uint32_t q[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float v = __fmul_rn(u[c][j], factor), k = rintf(v);
-      q[j] = (int)k;
-      if (fabsf(v - k) > kNear && (VEC || index(c, j) < d))
-        q[j] = __double2int_rn(__ddiv_rn(127.0 * row.u64(index(c, j)), most));
+      const float v = __fmul_rn(u[c][j], factor), k = __fadd_rn(v, kRound);
+      q[j] = __float_as_uint(k);  // the code in the low byte
+      bits |= fabsf(v - __fadd_rn(k, -kRound)) > kNear ? 1u << (8 * c + j) : 0u;
     }
     if constexpr (VEC) {
       uint32_t p[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        p[i] = (q[4 * i] & 255) | (q[4 * i + 1] & 255) << 8 | (q[4 * i + 2] & 255) << 16 |
-               (uint32_t)q[4 * i + 3] << 24;
-      *reinterpret_cast<uint2*>(code + index(c, 0)) = make_uint2(p[0], p[1]);
+        p[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040),
+                           0x5410);
+      if (index(c, 0) < d) *reinterpret_cast<uint2*>(code + index(c, 0)) = make_uint2(p[0], p[1]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (index(c, j) < d) code[index(c, j)] = (int8_t)q[j];
     }
+  }
+  // over what this thread has just stored
+  for (; bits; bits &= bits - 1) {
+    const int i = of_bit(bits);
+    code[i] = (int8_t)__double2int_rn(__ddiv_rn(127.0 * row.u64(i), most));
   }
   if (t == 0) scales[at] = (float)(most / sqrt((double)ssq / d + eps) / 127.0);
 }
@@ -276,10 +309,10 @@ struct NormArgs {
   void* h;
 };
 
-template <typename InT, typename WT, int NC, int MAX, bool VEC, bool WARP>
+template <typename InT, typename WT, int NC, int MAX, int MIN, bool VEC, bool WARP>
 int launch(const NormArgs& a, int threads, cudaStream_t st) {
   const int64_t blocks = WARP ? cdiv(a.rows, kWarpRows) : a.rows;
-  MXB_CUDA_TRY(launch_pdl(rms_norm_kernel<InT, WT, NC, MAX, VEC, WARP>, dim3((unsigned)blocks),
+  MXB_CUDA_TRY(launch_pdl(rms_norm_kernel<InT, WT, NC, MAX, MIN, VEC, WARP>, dim3((unsigned)blocks),
                           WARP ? 32 * kWarpRows : threads, 0, st, static_cast<const InT*>(a.x),
                           static_cast<const InT*>(a.r), a.rows, (int)a.d, a.ldx, a.ldr,
                           static_cast<const WT*>(a.w), a.eps, (float)(1.0 / (double)a.d), a.codes, a.scales,
@@ -292,16 +325,20 @@ template <typename InT, typename WT, bool VEC>
 int by_size(const NormArgs& a, cudaStream_t st) {
   // threads of a row with 8 nc values each
   auto threads = [&](int nc) { return (int)cdiv(cdiv(a.d, 8 * nc), 32) * 32; };
-  if (a.d > kMaxRow) return launch<InT, WT, 1, 1024, VEC, false>(a, 1024, st);
+  if (a.d > kMaxRow) return launch<InT, WT, 1, 1024, 1, VEC, false>(a, 1024, st);
   if (a.d <= 1024 && a.rows > kSMs) {
-    return a.d <= 256   ? launch<InT, WT, 1, 32, VEC, true>(a, 32, st)
-           : a.d <= 512 ? launch<InT, WT, 2, 32, VEC, true>(a, 32, st)
-                        : launch<InT, WT, 4, 32, VEC, true>(a, 32, st);
+    return a.d <= 256   ? launch<InT, WT, 1, 32, 4, VEC, true>(a, 32, st)
+           : a.d <= 512 ? launch<InT, WT, 2, 32, 4, VEC, true>(a, 32, st)
+                        : launch<InT, WT, 4, 32, 3, VEC, true>(a, 32, st);
   }
-  // few rows: as many threads as a row has use for
-  if (a.rows <= 2 * kSMs && threads(1) <= 1024) return launch<InT, WT, 1, 1024, VEC, false>(a, threads(1), st);
-  if (threads(4) <= 512) return launch<InT, WT, 4, 512, VEC, false>(a, threads(4), st);
-  return launch<InT, WT, 4, 1024, VEC, false>(a, threads(4), st);
+  // few rows, or values loaded one by one: as many threads as a row has use for
+  if ((a.rows <= 2 * kSMs || !VEC) && threads(1) <= 1024)
+    return launch<InT, WT, 1, 1024, 1, VEC, false>(a, threads(1), st);
+  if constexpr (VEC) {
+    if (threads(4) <= 256) return launch<InT, WT, 4, 256, 3, VEC, false>(a, threads(4), st);
+  }
+  if (threads(4) <= 512) return launch<InT, WT, 4, 512, 1, VEC, false>(a, threads(4), st);
+  return launch<InT, WT, 4, 1024, 1, VEC, false>(a, threads(4), st);
 }
 
 template <typename InT>

@@ -29,7 +29,8 @@ MAX_K = 131071  # |a b| <= 2^14: sums that an int32 holds
 
 def _rows(t: torch.Tensor, d: int) -> Tuple[torch.Tensor, int]:
     """A [rows, d] view (or copy) with adjacent elements, and its row stride."""
-    t = t.reshape(-1, d)
+    if t.dim() != 2:
+        t = t.reshape(-1, d)
     ld = t.stride(0) if t.shape[0] > 1 else d
     if (d > 1 and t.stride(1) != 1) or ld < d:
         t, ld = t.contiguous(), d

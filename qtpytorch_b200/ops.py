@@ -110,20 +110,22 @@ def dequantize(packed: torch.Tensor, scales: torch.Tensor, dt, n: int, block: in
         raise NotImplementedError(f"dequantize of {dt.name} is not on the B200 path")
     L.require_cuda(packed, "dequantize")
     dev = packed.device
-    shape = tuple(shape) if shape is not None else (n,)
-    out = torch.empty(n, dtype=torch.float32, device=dev)
-    if n == 0:
-        return out.reshape(shape)
-    row_len = row_len_of(shape)
-    variant = L.VAR_H if dt.is_hadamard else L.VAR_BASE
-    signs = device_signs(row_len, dt.hadamard_seed, dev) if dt.is_hadamard else None
-    lib = L.load()
-    with torch.cuda.device(dev):
-        rc = lib.mxb_dequantize(L.ptr(packed.contiguous()), L.ptr(scales.contiguous()), n,
-                                row_len, dt.bits, _kind(dt), variant, block, L.ptr(signs),
-                                L.ptr(out), L.stream_of(dev))
-    L.check(rc, f"mxb_dequantize({dt.name}, n={n})")
-    return out.reshape(shape)
+    shape = (n,) if shape is None else shape
+    fits = math.prod(shape) == n
+    out = torch.empty(shape if fits else n, dtype=torch.float32, device=dev)
+    if n:
+        row_len = shape[-1] if len(shape) >= 2 else max(n, 1)
+        hadamard = dt.is_hadamard
+        signs = device_signs(row_len, dt.hadamard_seed, dev) if hadamard else None
+        if not packed.is_contiguous():
+            packed = packed.contiguous()
+        if not scales.is_contiguous():
+            scales = scales.contiguous()
+        rc = L.call("mxb_dequantize", dev, packed.data_ptr(), scales.data_ptr(), n, row_len, dt.bits, _kind(dt),
+                    L.VAR_H if hadamard else L.VAR_BASE, block, L.ptr(signs), out.data_ptr())
+        if rc:
+            L.check(rc, f"mxb_dequantize({dt.name}, n={n})")
+    return out if fits else out.reshape(tuple(shape))
 
 
 def hadamard_rows(y: torch.Tensor, seed: Optional[int], inverse: bool) -> torch.Tensor:

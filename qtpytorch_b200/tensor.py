@@ -32,13 +32,27 @@ from .dtypes import get_mx_dtype, mx_dtype, optimal_output_dtype
 _STRICT = os.environ.get("MX_STRICT", "0") == "1"
 
 
+_placeholders: dict = {}
+
+
+def _placeholder(device: torch.device) -> torch.Tensor:
+    """What stands behind the wrapper itself: an fp32 scalar that nothing reads or
+    writes, one a device."""
+    t = _placeholders.get(device)
+    if t is None:
+        t = torch.empty((), dtype=torch.float32, device=device)
+        # a capture's allocations belong to its graph
+        if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
+            _placeholders[device] = t
+    return t
+
+
 class mx_tensor(torch.Tensor):
     """A quantized tensor that is a torch.Tensor (mxtorch.py:6028)."""
 
     def __new__(cls, packed: torch.Tensor, scales: torch.Tensor, mx_dtype: mx_dtype,
                 orig_shape, n: int, block: int = 128, requires_grad: bool = False):
-        dummy = torch.empty((), dtype=torch.float32, device=packed.device)
-        inst = torch.Tensor._make_subclass(cls, dummy, False)
+        inst = torch.Tensor._make_subclass(cls, _placeholder(packed.device), False)
         inst._mx_packed = packed
         inst._mx_scales = scales
         inst._mx_dtype = get_mx_dtype(mx_dtype)
