@@ -515,7 +515,8 @@ int mxb_tree_attention(const void* q, int64_t B, int64_t T, int heads, int group
  * inv_freq[i]; dims from rot (a multiple of 8) on stay.  One axis: a = 0; up to
  * four: sections[0] pairs turn by axis 0, the next sections[1] by axis 1, ...
  * (host memory, their sum rot / 2).
- *   q      [T][q_heads][dim] under its strides, or q_heads 0; q_out contiguous,
+ *   q      [T][q_heads][dim] under its strides (all strides in elements, below 2^31),
+ *          or q_heads 0; q_out contiguous,
  *          of the input's type, written for skipped tokens too
  *   k, v   as for mxb_kv_write; a key's codes and scale are those of the
  *          rotation in 64 bits rounded to fp32

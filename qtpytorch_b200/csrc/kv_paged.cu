@@ -152,7 +152,7 @@ struct AppendRows {
   const void *q, *k, *v;
   int64_t T;
   int Hq, H;  // Hq 0: no queries
-  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+  int q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;  // strides below 2^31, their products are not
   bool vec;
 };
 
@@ -206,6 +206,14 @@ __device__ __forceinline__ void turn64(double angle, double& c, double& s) {
 }
 
 constexpr int kAppendTokens = 4;  // at most, a block
+// Token of row u of a block, `per` rows a token: a division costs a fifth of a row's work.
+__device__ __forceinline__ int token_of(int u, int per) {
+  static_assert(kAppendTokens == 4, "three borders");
+  return (u >= per) + (u >= 2 * per) + (u >= 3 * per);
+}
+__device__ __forceinline__ int64_t offset_of(int t, int ts, int h, int hs) {
+  return (int64_t)t * ts + (int64_t)h * hs;
+}
 
 template <typename InT, int BITS, int D, bool ILV>
 __global__ void __launch_bounds__(kThreads)
@@ -227,15 +235,17 @@ __global__ void __launch_bounds__(kThreads)
   const int oa = ILV || !turns ? part * 8 : part * 4, ob = ILV || !turns ? oa + 4 : ro.pairs + part * 4;
   // rows of queries, kU of them in flight; the first while the angles are found
   constexpr int kU = 4;
-  const InT* q = static_cast<const InT*>(a.q);
+  const InT* q = static_cast<const InT*>(a.q) + t0 * a.q_ts;
+  const InT* k = static_cast<const InT*>(a.k) + t0 * a.k_ts;
+  const InT* v = static_cast<const InT*>(a.v) + t0 * a.v_ts + part * 8;
   Raw4<InT> qa[kU], qb[kU];
   auto load_q = [&](int u0) {
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
       const int u = u0 + i * kRows;
       if (u < q_rows) {
-        const int t = u / a.Hq, h = u - t * a.Hq;
-        const InT* p = q + (t0 + t) * a.q_ts + h * a.q_hs;
+        const int t = token_of(u, a.Hq);
+        const InT* p = q + offset_of(t, a.q_ts, u - t * a.Hq, a.q_hs);
         qa[i].load(p + oa, a.vec);
         qb[i].load(p + ob, a.vec);
       }
@@ -243,6 +253,7 @@ __global__ void __launch_bounds__(kThreads)
   };
   int u0 = threadIdx.x / L;
   load_q(u0);
+  q_out += t0 * a.Hq * D;
   for (int i = threadIdx.x; i < tokens * ro.pairs; i += kThreads) {
     const int t = i / ro.pairs, p = i - t * ro.pairs;
     const int axis = (p >= ro.end[0]) + (p >= ro.end[1]) + (p >= ro.end[2]);
@@ -281,11 +292,11 @@ __global__ void __launch_bounds__(kThreads)
     for (int i = 0; i < kU; ++i) {
       const int u = u0 + i * kRows;
       if (u < q_rows) {
-        const int t = u / a.Hq;
+        const int t = token_of(u, a.Hq);
         float x[8], y[8], cs[8];
         get8(qa[i], qb[i], x);
         turn(t, x, y, cs);
-        InT* o = q_out + (t0 * a.Hq + u) * D;  // u counts a token's heads in their order
+        InT* o = q_out + u * D;  // u counts a token's heads in their order
         store4(o + oa, *reinterpret_cast<float (*)[4]>(y));
         store4(o + ob, *reinterpret_cast<float (*)[4]>(y + 4));
       }
@@ -297,18 +308,18 @@ __global__ void __launch_bounds__(kThreads)
   for (int u1 = threadIdx.x / 32 * (32 / L); u1 < kv_rows; u1 += kRows) {
     const int u = u1 + (threadIdx.x % 32) / L;
     const bool live = u < kv_rows;
-    const int t = live ? u / a.H : 0, h = live ? u - t * a.H : 0;
+    const int t = live ? token_of(u, a.H) : 0, h = live ? u - t * a.H : 0;
     float x[8], y[8], w[8], cs[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = w[j] = 0.0f;
     int64_t slot = -1;
     if (live) {
-      const InT* p = static_cast<const InT*>(a.k) + (t0 + t) * a.k_ts + h * a.k_hs;
+      const InT* p = k + offset_of(t, a.k_ts, h, a.k_hs);
       Raw4<InT> r0, r1;
       r0.load(p + oa, a.vec);
       r1.load(p + ob, a.vec);
       slot = slots[t0 + t];
-      load8v(static_cast<const InT*>(a.v) + (t0 + t) * a.v_ts + h * a.v_hs + part * 8, a.vec, w);
+      load8v(v + offset_of(t, a.v_ts, h, a.v_hs), a.vec, w);
       get8(r0, r1, x);
     }
     turn(t, x, y, cs);
@@ -612,7 +623,9 @@ int mxb_kv_append(const void* q, const void* k, const void* v, int x_dtype, int6
   if (rc != MXB_OK) return rc;
   if (T < 0 || q_heads < 0 || q_heads > 65535 || rot < 0 || rot > dim || rot % 8 || axes < 1 || axes > 4)
     return MXB_E_SHAPE;
-  if ((int64_t)kAppendTokens * (q_heads + heads) > INT32_MAX || T > ((int64_t)1 << 31)) return MXB_E_SHAPE;
+  if (T > ((int64_t)1 << 31)) return MXB_E_SHAPE;
+  for (int64_t stride : {q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride})
+    if (stride < 0 || stride > INT32_MAX) return MXB_E_SHAPE;
   if (axes > 1 && !sections) return MXB_E_ARG;
   Rotary ro = {positions, axis_stride, inv_freq, rot / 2, {INT32_MAX, INT32_MAX, INT32_MAX}};
   int64_t at = 0;
@@ -629,8 +642,8 @@ int mxb_kv_append(const void* q, const void* k, const void* v, int x_dtype, int6
       (q_heads > 0 && (uintptr_t)q_out % 16) || ((uintptr_t)positions | (uintptr_t)slots) % 8 ||
       (uintptr_t)inv_freq % 4)
     return MXB_E_ALIGN;
-  AppendArgs a = {{q_heads > 0 ? q : nullptr, k, v, T, q_heads, heads, q_token_stride, q_head_stride, k_token_stride,
-                   k_head_stride, v_token_stride, v_head_stride, false},
+  AppendArgs a = {{q_heads > 0 ? q : nullptr, k, v, T, q_heads, heads, (int)q_token_stride, (int)q_head_stride,
+                   (int)k_token_stride, (int)k_head_stride, (int)v_token_stride, (int)v_head_stride, false},
                   ro, interleaved != 0, slots, n_pages * page, page, q_out, static_cast<uint8_t*>(k_codes),
                   static_cast<uint8_t*>(v_codes), k_scales, v_scales};
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -169,12 +169,9 @@ class paged_kv_cache:
         q_type = None if q is None else q.dtype
         if k.dtype not in _IO or k.dtype != v.dtype or (q is not None and q_type != k.dtype):
             k, v, q = k.float(), v.float(), None if q is None else q.float()
-        if k.stride(2) != 1:
-            k = k.contiguous()
-        if v.stride(2) != 1:
-            v = v.contiguous()
-        if q is not None and q.stride(2) != 1:
-            q = q.contiguous()
+        k, v = _rows(k), _rows(v)
+        if q is not None:
+            q = _rows(q)
         if slots.dtype != torch.int64 or not slots.is_contiguous():
             slots = slots.to(torch.int64).contiguous()
         if positions.dtype != torch.int64 or (T > 1 and positions.stride(-1) != 1):
@@ -220,6 +217,12 @@ class paged_kv_cache:
     def __repr__(self):
         return (f"paged_kv_cache(pages={self.n_pages}, heads={self.n_heads}, dim={self.head_dim}, "
                 f"page={self.page_size}, dtype={self.dtype.name})")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[T, heads, dim] with adjacent elements and strides that 31 bits hold."""
+    a, b, c = t.stride()
+    return t if c == 1 and a < 2 ** 31 and b < 2 ** 31 else t.contiguous()
 
 
 @functools.lru_cache(maxsize=256)
