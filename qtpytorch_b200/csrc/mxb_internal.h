@@ -58,7 +58,7 @@ struct TreeArgs {
   int rows, row_tiles;  // T * G, and CTAs' shares of them
   float scale_log2;
   float *main_o, *main_ml, *cta_o, *cta_ml;
-  int64_t* plan;  // [0] tiles per CTA, [1 + b] first tile of sequence b
+  int64_t* plan;  // [0] tiles per CTA, [1 + b] first tile of sequence b; null: a unit a CTA
   bool direct;    // rows with one part go straight to out
   void* out;
   float* lse;

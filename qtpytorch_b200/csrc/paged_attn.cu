@@ -1048,6 +1048,8 @@ int nt_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3
 
 // Rows of a tree a KV head from which its own keys go to the tcgen05 kernel.
 constexpr int64_t kTreeRows = 33;
+// Keys up to which it takes a unit a CTA.
+constexpr int64_t kTreeWhole = 1024;
 
 Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, int64_t max_keys,
                int64_t prefix, bool tree) {
@@ -1069,12 +1071,12 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, in
   // 31), 16 x 4096 45 / 37, 4 x 2048 18.5 / 15.8, 1 x 1024 11.6 / 13.0.
   const int64_t slots = kSMs * ctas(p.nt_own, rb, dim);
   const int64_t whole_keys = units >= slots ? 4096 : units >= kSMs * 3 / 4 ? 2048 : 1024;
-  p.whole = !p.tensor && max_keys <= whole_keys && (max_keys > 0 || prefix == 0);
-  if (p.tensor) {
+  p.whole = max_keys <= (p.tensor ? kTreeWhole : whole_keys) && (max_keys > 0 || prefix == 0);
+  if (p.whole) {
+    p.ctas_own = (int)units;
+  } else if (p.tensor) {
     const int64_t most = units * cdiv(max_keys, kTreeKeys);
     p.ctas_own = (int)(most < kSMs ? most : kSMs);
-  } else if (p.whole) {
-    p.ctas_own = (int)units;
   } else if (max_keys > 0) {
     const int64_t most = units * cdiv(max_keys, kTile * kWarps);
     p.ctas_own = (int)(most < slots ? most : slots);

@@ -503,22 +503,27 @@ __device__ __forceinline__ void softmax_tile(Rows& r, const Tile& g, const float
   tc_fence_before();
 }
 
-// Columns 2 c, 2 c + 1 (c = lane % 4) of eight unpacked ones -> dims 2 c, 2 c + 1.
+// A row's 32 columns, 8 i + 2 c and the next in m[i] of lane c of four -> columns 8 c ..
+// of lane c, in the order of the dims.
 template <int BITS>
-__device__ __forceinline__ float2 in_order(float x, float y) {
-  const int lane = threadIdx.x & 31, c = lane & 3, base = lane & ~3;
-  if constexpr (BITS == 8) {  // neighbours swap the middle two of 0 2 1 3
-    const float z = __shfl_xor_sync(0xffffffffu, c & 1 ? x : y, 1);
-    return c & 1 ? make_float2(z, y) : make_float2(x, z);
-  } else {
-    float out[2];
+__device__ __forceinline__ void eight_columns(float2 (&m)[4], float (&o)[8]) {
+  const int c = threadIdx.x & 3;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int d = 2 * c + e, p = ((d & 3) << 1) | (d >> 2);  // the column that holds dim d
-      const float u = __shfl_sync(0xffffffffu, x, base + (p >> 1)), w = __shfl_sync(0xffffffffu, y, base + (p >> 1));
-      out[e] = p & 1 ? w : u;
-    }
-    return make_float2(out[0], out[1]);
+  for (int s = 1; s < 4; s <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!(i & s)) {
+        const bool hi = c & s;
+        float2 t = hi ? m[i] : m[i | s];
+        t.x = __shfl_xor_sync(0xffffffffu, t.x, s);
+        t.y = __shfl_xor_sync(0xffffffffu, t.y, s);
+        if (hi) m[i] = t;
+        else m[i | s] = t;
+      }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    o[order<BITS>(2 * j)] = m[j].x;
+    o[order<BITS>(2 * j + 1)] = m[j].y;
   }
 }
 
@@ -572,7 +577,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t cap = (int64_t)a.width << a.page_shift;
   Place at;
   bool any;
-  {
+  if (a.plan == nullptr) {  // a unit a CTA
+    at.b = blockIdx.x / hr;
+    at.u = blockIdx.x - at.b * hr;
+    if (at.u == 0 && threadIdx.x == 0 && a.err && __ldg(a.lengths + at.b) > cap) atomicCAS(a.err, 0, kErrIndex);
+    at.left = (Place::len_of(a, at.b) + KT - 1) / KT;
+    any = at.left > 0;
+    if (any) {
+      at.start(a, 0);
+    } else if (a.direct) {  // a sequence without keys: zeros
+      const int h = at.u / a.row_tiles, r0 = (at.u - h * a.row_tiles) * R;
+      for (int i = threadIdx.x; i < R * (D / 8); i += kThreads) {
+        const int row = r0 + i / (D / 8), tok = row / a.G;
+        if (row >= a.rows) break;
+        const int64_t id = ((int64_t)at.b * a.T + tok) * ((int64_t)a.H * a.G) + (int64_t)h * a.G + (row - tok * a.G);
+        reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + id * D)[i % (D / 8)] = make_uint4(0u, 0u, 0u, 0u);
+        if (a.lse && i % (D / 8) == 0) a.lse[id] = -INFINITY;
+      }
+    }
+  } else {
     // every warp for itself where the batch is small, otherwise the block together
     const bool alone = a.B <= 512;
     const int width = alone ? 32 : kThreads, me = alone ? lane : threadIdx.x;
@@ -1012,18 +1035,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int k = 0; k < 2; ++k) {
+            // a lane's 32 bytes, four lanes a whole line of the row (columns pair by pair
+            // took 3500 cycles more for 32 columns of a part)
+            float2 m4[4];
+            float o[8];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float2 o = in_order<BITS>(__uint_as_float(v[4 * i + 2 * k]), __uint_as_float(v[4 * i + 2 * k + 1]));
-              const int col = d + 8 * i + 2 * (lane & 3);
-              if (id[k] < 0) continue;
-              if (direct)
-                *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + id[k] * D + col) =
-                    bf2(o.x * inv[k], o.y * inv[k]);
-              else
-                *reinterpret_cast<float2*>((first ? a.main_o : a.cta_o) + part[k] * D + col) = o;
+            for (int i = 0; i < 4; ++i)
+              m4[i] = make_float2(__uint_as_float(v[4 * i + 2 * k]), __uint_as_float(v[4 * i + 2 * k + 1]));
+            eight_columns<BITS>(m4, o);
+            const int col = d + 8 * (lane & 3);
+            if (id[k] >= 0) {
+              if (direct) {
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + id[k] * D + col) =
+                    make_uint4(bf2(o[0] * inv[k], o[1] * inv[k]), bf2(o[2] * inv[k], o[3] * inv[k]),
+                               bf2(o[4] * inv[k], o[5] * inv[k]), bf2(o[6] * inv[k], o[7] * inv[k]));
+              } else {
+                asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(
+                                 (first ? a.main_o : a.cta_o) + part[k] * D + col),
+                             "f"(o[0]), "f"(o[1]), "f"(o[2]), "f"(o[3]), "f"(o[4]), "f"(o[5]), "f"(o[6]), "f"(o[7])
+                             : "memory");
+              }
             }
+            __syncwarp();
+          }
         }
         __syncwarp();
         tc_fence_before();
