@@ -1046,9 +1046,14 @@ struct Plan {
 
 int nt_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4; }
 
-// Rows of a tree a KV head from which its own keys go to the tcgen05 kernel.
-constexpr int64_t kTreeRows = 33;
-// Keys up to which it takes a unit a CTA.
+// Rows of a tree a KV head from which its own keys go to the tcgen05 kernel, which
+// costs the same for 40 rows as for 128.  Microseconds of a call, there and in groups of
+// up to 32 rows, 8 heads of 128 dims in int8: 8 sequences of up to 8000 keys, 64 rows
+// 92 / 98, 128 rows 99 / 159; 16 of up to 700, 64 rows 35 / 35, 256 rows 47 / 115; 4
+// heads of 64 dims in int4, 24 of up to 6000: 56 rows 85 / 71, 104 rows 89 / 124.
+constexpr int64_t kTreeRows = 64;
+// Keys up to which it takes a unit a CTA, where half of the SMs get one (16 x 700 keys
+// of 256 rows: 47, as a list 82; 1 x 700, 8 units: 45 and 33).
 constexpr int64_t kTreeWhole = 1024;
 
 Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, int64_t max_keys,
@@ -1071,7 +1076,8 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, in
   // 31), 16 x 4096 45 / 37, 4 x 2048 18.5 / 15.8, 1 x 1024 11.6 / 13.0.
   const int64_t slots = kSMs * ctas(p.nt_own, rb, dim);
   const int64_t whole_keys = units >= slots ? 4096 : units >= kSMs * 3 / 4 ? 2048 : 1024;
-  p.whole = max_keys <= (p.tensor ? kTreeWhole : whole_keys) && (max_keys > 0 || prefix == 0);
+  p.whole = max_keys <= (!p.tensor ? whole_keys : units >= kSMs / 2 ? kTreeWhole : 0) &&
+            (max_keys > 0 || prefix == 0);
   if (p.whole) {
     p.ctas_own = (int)units;
   } else if (p.tensor) {
