@@ -856,7 +856,7 @@ struct JoinArgs {
   const int* lengths;   // null: no keys of its own
   int64_t cap, n_rows;
   int pre_parts, T, H, G, row_tiles, R;
-  int tile;  // keys of a tile of the plan
+  int tile_shift;  // log2 of the keys of a tile of the plan
   bool direct;  // rows with one part of their own are written already
   __nv_bfloat16* out;
   float* lse;
@@ -876,7 +876,7 @@ struct RowSum {
     own = 0;
     c_at = 0;
     if (a.lengths) {
-      const int n = (int)((min((int64_t)max(__ldg(a.lengths + b), 0), a.cap) + a.tile - 1) / a.tile);
+      const int64_t n = (min((int64_t)max(__ldg(a.lengths + b), 0), a.cap) + (1 << a.tile_shift) - 1) >> a.tile_shift;
       if (n > 0) {
         own = 1;
         if (a.plan) {
@@ -1291,8 +1291,8 @@ int attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim
   }
   if (p.join) {
     JoinArgs j = {own, cta, pre, a.plan, p.ctas_own > 0 ? lengths : nullptr, width * page,
-                         a.n_rows, p.splits_pre, (int)T, heads, group, p.tiles_own, p.rows_own, p.tile_own,
-                         a.direct, a.out, lse};
+                  a.n_rows, p.splits_pre, (int)T, heads, group, p.tiles_own, p.rows_own,
+                  31 - __builtin_clz((unsigned)p.tile_own), a.direct, a.out, lse};
     const bool many = a.n_rows >= kJoinManyRows;
     auto kern = dim == 128 ? (many ? paged_join_kernel<128, kWarps>
                                    : paged_join_kernel<128, 1>)

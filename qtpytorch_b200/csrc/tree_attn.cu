@@ -6,8 +6,8 @@
 // products of matrices: 4 T G keys dim operations, and an exponential a score.  A
 // CTA owns 128 rows or 256 and walks tiles of 128 keys:
 //   warp 0        MMA issue and TMEM allocation;
-//   warp 1        TMA producer: raw codes and scales, a ring of steps of 64 keys of K
-//                 or V;
+//   warp 1        TMA producer: raw codes and scales, a ring of steps of 64 or 128 keys
+//                 of K or V;
 //   warps 2-17    softmax: S from TMEM, running maximum, sum, weights (fp16) back to
 //                 TMEM over S;
 //   warps 18-21   unpack codes to exact fp16 in shared memory (one layout for K and
@@ -65,10 +65,13 @@ struct Cfg {
   static constexpr size_t oK = (size_t)MT * kQ, oV = oK + 2 * kPlane, oSc = oV + 2 * kPlane;
   static constexpr size_t oX = oSc + (size_t)kSlots * kSlotF * 4;
   static constexpr size_t oBars = oX + (MT == 1 ? kX + kXml : 0);
-  // ring of raw codes, 64 keys of K (with both scales of those) or of V a step
-  static constexpr int kStep = 64 * RB, kSlot = kStep + 512;
+  // ring of raw codes, kKeys keys of K (with both scales of those) or of V a step: 8 KB,
+  // or a whole tile where that is less (in steps of 64 keys the barriers of int4 tiles of
+  // 64 dims took longer than their codes)
+  static constexpr int kKeys = RB == 128 ? 64 : 128, kSteps = KT / kKeys;  // steps of K, and of V, a tile
+  static constexpr int kStep = kKeys * RB, kSlot = kStep + 8 * kKeys;
   static constexpr size_t oRaw = oBars + 768;
-  static constexpr int kRing = kStep >= 8192 ? 3 : 6;
+  static constexpr int kRing = D == 128 ? 3 : 6;
   static constexpr size_t kSmem = 1024 + oRaw + (size_t)kRing * kSlot;
   static constexpr int kPieces = kStep / 16 / 128;  // 16-byte pieces of a step a thread
 };
@@ -552,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < kSlots; ++s) mbar_init(&bars->scready[s], 4);
     for (int s = 0; s < C::kRing; ++s) {
-      mbar_init(&bars->raw_full[s], 64 / box);
+      mbar_init(&bars->raw_full[s], C::kKeys / box);
       mbar_init(&bars->raw_empty[s], 4);
     }
     mbar_init(&bars->qready, kSoftWarps / 2 * MT);
@@ -709,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_commit(&bars->drained);
       }
     } else if (warp == 1) {
-      // ── raw codes and scales: K 0 - 63, K 64 - 127, V 0 - 63, V 64 - 127 of a tile ──
+      // ── raw codes and scales: a tile's keys in kSteps steps, then its values ──
       const int page_mask = (1 << a.page_shift) - 1, per = box >> 4;  // groups of 16 keys a copy
       // lane i < 8: first head row of keys 16 i .. of a tile; -1 where there are none, -2
       // behind a number outside the pool
@@ -735,25 +738,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           Place next = at;
           more = next.next_tile(a);
           const int next_rows = more ? rows_of(next) : -1;
-          for (int q = 0; q < 4; ++q, ++step) {
+          for (int q = 0; q < 2 * C::kSteps; ++q, ++step) {
+            constexpr int kGroups = C::kKeys / 16;
             const int s = step % C::kRing;
+            const bool keys = q < C::kSteps;
             ok = step < C::kRing ||
                  mbar_sleep_warp_to(&bars->raw_empty[s], (step / C::kRing - 1) & 1, kErrTimeoutEmpty, a.err);
             if (!ok) break;
-            const int row = __shfl_sync(0xffffffffu, rows, (q & 1) * 4 + (lane & 3));
-            const uint32_t gone = __ballot_sync(0xffffffffu, lane < 4 && row == -2);
+            const int row = __shfl_sync(0xffffffffu, rows, q % C::kSteps * kGroups + lane % kGroups);
+            const uint32_t gone = __ballot_sync(0xffffffffu, lane < kGroups && row == -2);
             if (lane == 0) bars->gone[s] = gone;  // before its arrival
-            if (lane < 4 && lane % per == 0) {
+            if (lane < kGroups && lane % per == 0) {
               uint64_t* bar = &bars->raw_full[s];
               if (row >= 0) {
                 uint8_t* dst = smem + C::oRaw + (size_t)s * C::kSlot;
-                mbar_expect_tx(bar, (uint32_t)box * (C::RB + (q < 2 ? 8 : 0)));
-                tma_load_2d(dst + lane * 16 * C::RB, q < 2 ? &tmap_k : &tmap_v, bar, 0,
+                mbar_expect_tx(bar, (uint32_t)box * (C::RB + (keys ? 8 : 0)));
+                tma_load_2d(dst + lane * 16 * C::RB, keys ? &tmap_k : &tmap_v, bar, 0,
                             (int)((int64_t)row * C::RB / 128));  // lines of 128 bytes
-                if (q < 2) {
+                if (keys) {
                   float* sc = reinterpret_cast<float*>(dst + C::kStep) + lane * 16;
                   bulk_load_g2s(sc, a.k_scales + row, (uint32_t)box * 4, bar);
-                  bulk_load_g2s(sc + 64, a.v_scales + row, (uint32_t)box * 4, bar);
+                  bulk_load_g2s(sc + C::kKeys, a.v_scales + row, (uint32_t)box * 4, bar);
                 }
               } else {
                 mbar_arrive(bar);
@@ -787,33 +792,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t small = least;
         uint4 gone = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q, ++step) {
-          const int s = step % C::kRing;
+        for (int q = 0; q < 2 * C::kSteps; ++q, ++step) {
+          const int s = step % C::kRing, part = q % C::kSteps;
+          const bool keys = q < C::kSteps, last = part == C::kSteps - 1;
           ok = mbar_sleep_warp_to(&bars->raw_full[s], (step / C::kRing) & 1, kErrTimeoutFull, a.err);
-          if (ok && j >= 2 && !(q & 1))
-            ok = mbar_sleep_warp_to(q == 0 ? &bars->kfree[b] : &bars->vfree[b], ((j >> 1) - 1) & 1, kErrTimeoutEmpty, a.err);
+          if (ok && j >= 2 && part == 0)
+            ok = mbar_sleep_warp_to(keys ? &bars->kfree[b] : &bars->vfree[b], ((j >> 1) - 1) & 1, kErrTimeoutEmpty, a.err);
           if (!ok) break;
           const uint8_t* src = smem + C::oRaw + (size_t)s * C::kSlot;
-          if (q < 2) {
+          if (keys) {
             const float* sc = reinterpret_cast<const float*>(src + C::kStep);
             const uint32_t bad = bars->gone[s];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int key = x * 32 + lane;
-              const bool some = q * 64 + key < valid && !(bad >> (key >> 4) & 1u);
-              const float v = some ? sc[64 + key] : 0.0f;  // nothing was copied for the others
+            for (int x = 0; x < C::kKeys / 32; ++x) {
+              const int key = x * 32 + lane, word = part * (C::kKeys / 32) + x;
+              const bool some = word * 32 + lane < valid && !(bad >> (key >> 4) & 1u);
+              const float v = some ? sc[C::kKeys + key] : 0.0f;  // nothing was copied for the others
               top = fmaxf(top, v);
               if (some) small = min(small, __float_as_uint(v));
               const uint32_t off = __ballot_sync(0xffffffffu, !some);
-              if (q == 0) (x == 0 ? gone.x : gone.y) = off;
-              else (x == 0 ? gone.z : gone.w) = off;
-              if (w == q * 2 + x) {
+              if (word == 0) gone.x = off;
+              else if (word == 1) gone.y = off;
+              else if (word == 2) gone.z = off;
+              else gone.w = off;
+              if (w == word) {
                 ks = some ? sc[key] : 0.0f;
                 vs = v;
               }
             }
           }
-          uint8_t* plane = smem + (q < 2 ? C::oK : C::oV) + b * C::kPlane;
+          uint8_t* plane = smem + (keys ? C::oK : C::oV) + b * C::kPlane;
           uint4 raw[C::kPieces];
 #pragma unroll
           for (int i = 0; i < C::kPieces; ++i) {
@@ -825,15 +833,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < C::kPieces; ++i) {
             int row, cc;
             piece<BITS, D>(i, t, row, cc);
-            put_piece<BITS, D>(raw[i], plane, (q & 1) * 64 + row, cc);
+            put_piece<BITS, D>(raw[i], plane, part * C::kKeys + row, cc);
           }
-          if (q & 1) fence_proxy_async_shared();
+          if (last) fence_proxy_async_shared();
           __syncwarp();
           if (lane == 0) {
             mbar_arrive(&bars->raw_empty[s]);
-            if (q & 1) mbar_arrive(q == 1 ? &bars->kready[b] : &bars->vready[b]);
+            if (last) mbar_arrive(keys ? &bars->kready[b] : &bars->vready[b]);
           }
-          if (q == 1) {
+          if (keys && last) {
             // bits of non-negative floats rise with them (no NaN passes the fmaxf)
             const float mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(top, 0.0f))));
             if (mx > c || c == 0.0f) {
@@ -1098,8 +1106,9 @@ int tree_rows_per_cta(int64_t rows) { return rows > 128 ? 256 : 128; }
 
 int tree_attention(const TreeArgs& a, int ctas, cudaStream_t st) {
   CUtensorMap tk, tv;
-  const int page = 1 << a.page_shift, box = page < 64 ? page : 64;
-  const uint64_t rb = (uint64_t)a.dim * a.bits / 8, lines = (uint64_t)a.n_pages * a.H * page * rb / 128;
+  const uint64_t rb = (uint64_t)a.dim * a.bits / 8;
+  const int page = 1 << a.page_shift, keys = rb == 128 ? 64 : 128, box = page < keys ? page : keys;
+  const uint64_t lines = (uint64_t)a.n_pages * a.H * page * rb / 128;
   const uint32_t box_lines = (uint32_t)(box * rb / 128);
   if (!encode_tmap_2d(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.k_codes, 128, lines, 128, box_lines,
                       CU_TENSOR_MAP_SWIZZLE_NONE) ||
