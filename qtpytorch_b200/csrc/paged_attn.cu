@@ -1049,8 +1049,10 @@ int nt_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3
 // Rows of a tree a KV head from which its own keys go to the tcgen05 kernel, which
 // costs the same for 40 rows as for 128.  Microseconds of a call, there and in groups of
 // up to 32 rows, 8 heads of 128 dims in int8: 8 sequences of up to 8000 keys, 64 rows
-// 92 / 98, 128 rows 99 / 159; 16 of up to 700, 64 rows 35 / 35, 256 rows 47 / 115; 4
-// heads of 64 dims in int4, 24 of up to 6000: 56 rows 85 / 71, 104 rows 89 / 124.
+// 91 / 98, 128 rows 98 / 159; 16 of up to 700, 64 rows 35 / 35, 256 rows 47 / 115; 4
+// heads of 64 dims in int4, 24 of up to 6000: 56 rows 72 / 71, 104 rows 76 / 124.  Where
+// every tile of keys finds an SM of its own, from 25 rows on (1 x 700 keys, 32 rows 22 /
+// 27).
 constexpr int64_t kTreeRows = 64;
 // Keys up to which it takes a unit a CTA, where half of the SMs get one (16 x 700 keys
 // of 256 rows: 47, as a list 82; 1 x 700, 8 units: 45 and 33).
@@ -1062,7 +1064,8 @@ Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t G, int dim, int bits, in
   const int64_t n_rows = B * T * H * G;
   const int rb = dim * bits / 8;
   p.nt_own = nt_of(T * G);
-  p.tensor = tree && max_keys > 0 && T * G >= kTreeRows;
+  p.tensor = tree && max_keys > 0 &&
+             (T * G >= kTreeRows || (T * G > 24 && B * H * cdiv(max_keys, kTreeKeys) <= kSMs));
   p.rows_own = p.tensor ? tree_rows_per_cta(T * G) : 8 * p.nt_own;
   p.tile_own = p.tensor ? kTreeKeys : kTile;
   p.tiles_own = (int)cdiv(T * G, p.rows_own);
