@@ -272,11 +272,11 @@ int launch(const CUtensorMap& tf, const CUtensorMap& tt, const Args& a, cudaStre
 }
 
 // ── many tokens ─────────────────────────────────────────────────────────────
-// A pair of CTAs (cta_group::2) owns a tile of 256 tokens x BN features: each loads
+// A pair of CTAs (cta_group::2) owns a tile of 256 tokens x 256 features: each loads
 // its 128 tokens and half of the features, and the pair's MMAs (M = 256) read both
 // halves, so that an SM draws 64 bytes a cycle of operands at the full rate where one
 // CTA's 128 x 128 tile draws 128.  Pairs walk the list of tiles; the accumulators are
-// double (2 x BN columns of TMEM), so that the epilogue of a tile runs beside the
+// double (2 x 256 columns of TMEM), so that the epilogue of a tile runs beside the
 // products of the next.
 //   warp 0      TMA producer (either CTA; both count on the leader's barriers);
 //   warp 1      MMAs (the leader's);  warps 2, 3  TMEM allocation, idle;
@@ -288,17 +288,17 @@ constexpr int kEpi = 8;
 constexpr int kThreads = 128 + 32 * kEpi;
 constexpr int kA = 128 * BK;            // a CTA's tokens of a stage
 constexpr int kOut = 32 * 128;          // a warp's piece of the output
-template <int BN>
+constexpr int BN = 256;                 // features of a pair
 struct Cfg {
-  static constexpr int kB = BN / 2 * BK;  // and features
+  static constexpr int kB = BN / 2 * BK;  // and features of a stage
   static constexpr int kStage = kA + kB;
-  static constexpr int S = BN == 256 ? 6 : 8;
+  static constexpr int S = 6;
   static constexpr size_t oOut = (size_t)S * kStage, oBars = oOut + kEpi * kOut;
   static constexpr size_t kSmem = 1024 + oBars + 512;
 };
 
 struct Bars {
-  uint64_t full[8], empty[8];
+  uint64_t full[Cfg::S], empty[Cfg::S];
   uint64_t acc[2], acc_free[2];
   uint32_t tmem_base;
 };
@@ -355,11 +355,11 @@ __device__ __forceinline__ void tile_at(const Tiles& t, int i, int& m, int& n) {
   m = 8 * b + (r - n * rows);
 }
 
-template <int BN, typename OutT>
+template <typename OutT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int8_wide_kernel(const __grid_constant__ CUtensorMap tmap_f, const __grid_constant__ CUtensorMap tmap_t,
                      const __grid_constant__ CUtensorMap tmap_o, const Args a, const Tiles tiles) {
-  using C = Cfg<BN>;
+  using C = Cfg;
   constexpr int S = C::S;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -531,11 +531,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int BN, typename OutT>
+template <typename OutT>
 int launch(const CUtensorMap& tf, const CUtensorMap& tt, const CUtensorMap& to, const Args& a, cudaStream_t st) {
-  using C = Cfg<BN>;
+  using C = Cfg;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
-  auto kern = int8_wide_kernel<BN, OutT>;
+  auto kern = int8_wide_kernel<OutT>;
   MXB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem));
   Tiles t;
   t.m = (int)cdiv(a.M, 256);
@@ -549,46 +549,101 @@ int launch(const CUtensorMap& tf, const CUtensorMap& tt, const CUtensorMap& to, 
 
 }  // namespace wide
 
-// Rows of K bytes -> rows of Kp, zero from K on.
+// Rows of K bytes that start anywhere -> rows of Kp, zero from K on: a warp a row, 16
+// bytes a lane from five words that lie in memory as such (64 x 8001 x 8000: 58 us byte by
+// byte).
 __global__ void __launch_bounds__(256)
     pad_rows_kernel(const uint8_t* __restrict__ a, int64_t ra, const uint8_t* __restrict__ b, int64_t rb, int K,
                     int Kp, uint8_t* __restrict__ out) {
   pdl_trigger();
   pdl_wait();
-  const int chunks = Kp / 16;
-  const int64_t n = (ra + rb) * chunks;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const int64_t row = i / chunks;
-    const int k0 = (int)(i - row * chunks) * 16;
-    const uint8_t* src = row < ra ? a + row * K : b + (row - ra) * K;
-    uint32_t w[4] = {0, 0, 0, 0};
+  const int lane = threadIdx.x & 31, warps = gridDim.x * 8;
+  for (int64_t row = blockIdx.x * 8 + (threadIdx.x >> 5); row < ra + rb; row += warps) {
+    const bool of_a = row < ra;
+    const uint8_t* lo = of_a ? a : b;
+    const uint8_t* hi = lo + (of_a ? ra : rb) * K;  // the operand's bytes, and no others, are read
+    const uint8_t* src = lo + (of_a ? row : row - ra) * K;
+    auto word = [&](const uint8_t* p) -> uint32_t {
+      if (p >= lo && p + 4 <= hi) return __ldg(reinterpret_cast<const uint32_t*>(p));
+      uint32_t w = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (k0 + j < K) w[j >> 2] |= (uint32_t)__ldg(src + k0 + j) << (8 * (j & 3));
-    reinterpret_cast<uint4*>(out)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int j = 0; j < 4; ++j)
+        if (p + j >= lo && p + j < hi) w |= (uint32_t)__ldg(p + j) << (8 * j);
+      return w;
+    };
+    for (int k = lane * 16; k < Kp; k += 512) {
+      const uint8_t* p = src + k;
+      const uint32_t off = (uint32_t)((uintptr_t)p & 3);
+      p -= off;
+      uint32_t w[5];
+#pragma unroll
+      for (int j = 0; j < 5; ++j) w[j] = word(p + 4 * j);
+      const int left = K - k;  // bytes of the row from here on
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = __funnelshift_r(w[j], w[j + 1], 8 * off);
+        const int n = left - 4 * j;
+        if (n < 4) w[j] &= n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+      }
+      *reinterpret_cast<uint4*>(out + row * Kp + k) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 }
 
-// Features of a pair's tile, 0: the kernel for few tokens.
-int wide_features(int64_t M, int64_t N) {
-  if (M <= 128) return 0;
-  const int64_t m = cdiv(M, 256);
-  if (m * cdiv(N, 256) >= kSMs / 2) return 256;
-  return m * cdiv(N, 128) >= kSMs / 4 ? 128 : 0;
+// How a product is cut: tokens a CTA (0: CTA pairs) and K splits.
+struct Cut {
+  int nt, splits;
+};
+
+// Up to 64 tokens the smallest tile that holds them all, so that few tokens pay an MMA of
+// their width, and K splits while they fill the SMs, as many as the root of twice the
+// stages at most (more shorten the stages' time / splits and lengthen the sum).  Beyond,
+// what costs least by the times that the kernels took (microseconds): a stage of a 128 x
+// 128 tile 0.42 alone on an SM and 0.53 for two, of a 128 x 64 tile 0.33 and 0.40, of a
+// pair's 256 x 256 tile 0.38; 6 or 8 around them, 4.5 to join splits, which have to win by
+// a fifth.  E.g. (auto / the other kernels' best): 160 x 4096 x 11008 18.8 / 22.5, 256 x
+// 11008 x 4096 23.4 / 28.8, 700 x 4096 x 11008 32.9 / 39.4, 2000 x 2048 x 2048 14.5 /
+// 16.4.  Splits stop at 256 CTAs: clusters of more do not all fit at once.
+Cut cut_of(int64_t M, int64_t N, int64_t ksteps, bool pairs) {
+  const int64_t ft = cdiv(N, BM);
+  if (M <= 64) {
+    const int nt = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    int64_t splits = 2 * kSMs / ft;
+    if (splits > ksteps / 2) splits = ksteps / 2;
+    if (splits > kMaxSplit) splits = kMaxSplit;
+    while (splits * splits > 2 * ksteps) --splits;
+    return {nt, (int)(splits < 1 ? 1 : splits)};
+  }
+  Cut best = {0, 1};
+  double least = pairs ? 8.0 + 0.38 * ksteps * cdiv(cdiv(M, 256) * cdiv(N, 256), kSMs / 2) : 1e30;
+  for (int nt = 64; nt <= 128; nt += 64) {
+    double whole = 0.0;
+    for (int s = 1; s <= kMaxSplit && (s == 1 || 2 * s <= ksteps); ++s) {
+      const int64_t ctas = ft * cdiv(M, nt) * s;
+      if (s > 1 && ctas > 256) break;
+      const double stage = nt == 64 ? (ctas <= kSMs ? 0.33 : 0.40) : (ctas <= kSMs ? 0.42 : 0.53);
+      const double t = 6.0 + stage * cdiv(ksteps, s) * cdiv(ctas, 2 * kSMs) + (s > 1 ? 4.5 : 0.0);
+      if (s == 1) whole = t;
+      if (t < least && (s == 1 || t < 0.8 * whole)) {
+        least = t;
+        best = {nt, s};
+      }
+    }
+  }
+  return best;
 }
 
 template <typename OutT>
 int dispatch(const void* fcodes, const void* tcodes, int64_t ldk, Args& a, cudaStream_t st) {
-  const int64_t ft = cdiv(a.N, BM);
   CUtensorMap tf, tt;
-  // whole TMA lines of the output, 16-byte groups of scales and bias
+  // pairs write whole TMA lines, and read scales and bias by 16 bytes
   const bool lines = a.N % (16 / (int)sizeof(OutT)) == 0 && (uintptr_t)a.out % 16 == 0 &&
                      ((uintptr_t)a.sf | (uintptr_t)a.bias) % 16 == 0;
-  const int bn = wide_features(a.M, a.N);
-  if (lines && bn) {
+  const Cut cut = cut_of(a.M, a.N, a.ksteps, lines);
+  if (cut.nt == 0) {
     CUtensorMap to;
     const bool half = sizeof(OutT) == 2;
-    if (!encode_tmap_2d(&tf, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, fcodes, (uint64_t)ldk, (uint64_t)a.N, BK, bn / 2,
+    if (!encode_tmap_2d(&tf, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, fcodes, (uint64_t)ldk, (uint64_t)a.N, BK, wide::BN / 2,
                         CU_TENSOR_MAP_SWIZZLE_128B) ||
         !encode_tmap_2d(&tt, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, tcodes, (uint64_t)ldk, (uint64_t)a.M, BK, 128,
                         CU_TENSOR_MAP_SWIZZLE_128B) ||
@@ -596,15 +651,10 @@ int dispatch(const void* fcodes, const void* tcodes, int64_t ldk, Args& a, cudaS
                         sizeof(OutT), a.out, (uint64_t)a.N, (uint64_t)a.M, 128 / sizeof(OutT), 32,
                         CU_TENSOR_MAP_SWIZZLE_128B))
       return MXB_E_CUDA;
-    return bn == 256 ? wide::launch<256, OutT>(tf, tt, to, a, st) : wide::launch<128, OutT>(tf, tt, to, a, st);
+    return wide::launch<OutT>(tf, tt, to, a, st);
   }
-  const int nt = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
-  const int64_t tiles = ft * cdiv(a.M, nt);
-  int64_t splits = (nt >= 128 ? kSMs : 2 * kSMs) / tiles;
-  if (splits > a.ksteps / 2) splits = a.ksteps / 2;
-  if (splits > kMaxSplit) splits = kMaxSplit;
-  while (splits * splits > 2 * (int64_t)a.ksteps) --splits;
-  a.splits = (int)(splits < 1 ? 1 : splits);
+  const int nt = cut.nt;
+  a.splits = cut.splits;
   if (!encode_tmap_2d(&tf, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, fcodes, (uint64_t)ldk, (uint64_t)a.N, BK, BM,
                       CU_TENSOR_MAP_SWIZZLE_128B) ||
       !encode_tmap_2d(&tt, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, tcodes, (uint64_t)ldk, (uint64_t)a.M, BK, nt,
@@ -663,8 +713,8 @@ int mxb_int8_matmul(const void* a_codes, const float* a_scales, int a_scale_step
     const size_t need = mxb_int8_matmul_workspace_size(M, K, N, 0);
     if (need > 0) {
       if (!workspace || workspace_bytes < need) return MXB_E_WORKSPACE;
-      const int64_t blocks = cdiv((M + N) * (ldk / 16), 256);
-      MXB_CUDA_TRY(launch_pdl(i8g::pad_rows_kernel, dim3((unsigned)(blocks < 16 * kSMs ? blocks : 16 * kSMs)),
+      const int64_t blocks = cdiv(M + N, 8);
+      MXB_CUDA_TRY(launch_pdl(i8g::pad_rows_kernel, dim3((unsigned)(blocks < 8 * kSMs ? blocks : 8 * kSMs)),
                               256, 0, st, static_cast<const uint8_t*>(a_codes), M,
                               static_cast<const uint8_t*>(b_codes), N, (int)K, (int)ldk,
                               static_cast<uint8_t*>(workspace)));
