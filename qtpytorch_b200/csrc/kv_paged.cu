@@ -140,6 +140,11 @@ __global__ void __launch_bounds__(kThreads)
 // 4 * 2^-24 of the row's largest value, so only the values within 2^-20 of the
 // largest and those whose quotient comes within m 2^-20 of a border between two
 // codes are turned again in 64 bits.
+//
+// 16384 tokens of 32 + 8 heads of 128 dims, bf16 into int4 (215 MB): 55 us = 3.9 TB/s, at
+// two thirds of the issue slots; 61 us with divisions for a row's token, 89 with one row
+// of queries in flight and 64-bit strides.  More rows in flight (more registers, fewer
+// blocks) were slower, 48 registers a thread no faster.  32 tokens: 4.1 us.
 struct Rotary {
   const int64_t* pos;  // [axes][axis_stride]
   int64_t axis_stride;
