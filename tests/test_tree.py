@@ -127,6 +127,28 @@ def test_tree_attention(dtype, dim, page, heads, group, T, lengths, prefix):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["int8d", "int4d"])
+@pytest.mark.parametrize("dim,page,heads,group,T,lengths,prefix", [
+    # short sequences of many rows, a unit a CTA: empty ones, shorter than their trees
+    (128, 64, 2, 4, 16, [0, 3, 16, 17, 300, 900, 128, 127] * 5, 0), (64, 16, 2, 8, 12, [12, 0, 500, 5] * 10, 0),
+    (64, 32, 4, 4, 40, [40, 41, 0, 170, 39] * 5, 90), (128, 128, 1, 8, 16, [16, 250] * 40, 0),
+    # 25 to 63 rows in groups of the decode kernel
+    (128, 16, 2, 4, 10, [600, 10, 0, 33] * 8, 0), (64, 32, 2, 4, 7, [640, 700, 9] * 9, 50),
+    (128, 64, 4, 8, 5, [1500] * 5, 0)])
+def test_many_units(dtype, dim, page, heads, group, T, lengths, prefix):
+    run(dtype, dim, page, heads, group, T, lengths, prefix)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_more_sequences_than_a_warp_adds_up(prefix):
+    """The list of tiles of more than 512 sequences, one of them long."""
+    lengths = [8 + i % 9 for i in range(700)]
+    lengths[3], lengths[650], lengths[100], lengths[699] = 1500, 300, 0, 2
+    run("int4d", 64, 16, 1, 8, 8, lengths, prefix)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["int8d", "int4d"])
 @pytest.mark.parametrize("group,T,lengths,prefix", [(4, 5, [70, 5, 0], 0), (8, 40, [40, 300], 0), (4, 5, [70, 5, 0], 50),
                                                     (8, 40, [39, 300], 50), (2, 64, [3000, 64], 0)])
 def test_masks_that_leave_rows_empty(dtype, group, T, lengths, prefix):
