@@ -517,7 +517,7 @@ int mxb_tree_attention(const void* q, int64_t B, int64_t T, int heads, int group
  * (host memory, their sum rot / 2).
  *   q      [T][q_heads][dim] under its strides (all strides in elements, below 2^31),
  *          or q_heads 0; q_out contiguous,
- *          of the input's type, written for skipped tokens too
+ *          of the input's type, written for skipped tokens too, not over q
  *   k, v   as for mxb_kv_write; a key's codes and scale are those of the
  *          rotation in 64 bits rounded to fp32
  */
@@ -540,7 +540,7 @@ int mxb_kv_append(const void* q, const void* k, const void* v, int x_dtype, int6
  *                residual may be NULL
  *   weight       [d] of w_dtype (MXB_F32 / MXB_BF16)
  *   codes        int8 [rows][d], scales fp32 [rows]
- *   sum          [rows][d] of x_dtype, h rounded, or NULL
+ *   sum          [rows][d] of x_dtype, h rounded, or NULL; not over x or residual
  */
 int mxb_rms_norm_quantize(const void* x, const void* residual, int x_dtype, int64_t rows, int64_t d,
                           int64_t x_stride, int64_t residual_stride, const void* weight, int w_dtype,

@@ -622,6 +622,7 @@ Cut cut_of(int64_t M, int64_t N, int64_t ksteps, bool pairs) {
   Cut best = {0, 1};
   double least = pairs ? 8.0 + 0.38 * ksteps * cdiv(cdiv(M, 256) * cdiv(N, 256), kSMs / 2) : 1e30;
   for (int nt = 64; nt <= 128; nt += 64) {
+    if (cdiv(M, nt) > 65535) continue;  // gridDim.y
     double whole = 0.0;
     for (int s = 1; s <= kMaxSplit && (s == 1 || 2 * s <= ksteps); ++s) {
       const int64_t ctas = ft * cdiv(M, nt) * s;

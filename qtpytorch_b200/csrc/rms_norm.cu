@@ -13,7 +13,7 @@
 // their product); where it comes within twice that of a border between two codes
 // it is found again in 64 bits from x, r and w, whose sums and products 64 bits
 // hold.  That meets 1 value in 8000.  The largest u is found in 64 bits too, among
-// those within 2^-22 of the fp32 one.  Rows that hold infinities or NaN, or whose
+// those within 2^-21 of the fp32 one.  Rows that hold infinities or NaN, or whose
 // values leave the range in which all this holds, take a slow path in 64 bits.
 //
 // One pass over HBM: a row stays in the registers of its block, 8 NC values a
@@ -368,6 +368,13 @@ extern "C" int mxb_rms_norm_quantize(const void* x, const void* residual, int x_
   if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)sum) % xa || (uintptr_t)weight % wa ||
       (uintptr_t)scales % 4)
     return MXB_E_ALIGN;
+  // x and the residual are read again after the sum is written
+  auto meets = [&](const void* p, int64_t stride) {
+    const uintptr_t lo = (uintptr_t)p, hi = lo + (uintptr_t)((rows - 1) * stride + d) * xa;
+    return p && sum && lo < (uintptr_t)sum + (uintptr_t)(rows * d) * xa && (uintptr_t)sum < hi;
+  };
+  if (x_stride < 0 || residual_stride < 0) return MXB_E_SHAPE;
+  if (meets(x, x_stride) || meets(residual, residual_stride)) return MXB_E_ARG;
   const NormArgs a = {x, residual, weight, rows, d, x_stride, residual_stride, eps, static_cast<int8_t*>(codes),
                       scales, sum};
   cudaStream_t st = static_cast<cudaStream_t>(stream);

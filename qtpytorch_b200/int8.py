@@ -181,7 +181,8 @@ class int8_linear(nn.Module):
             scales = scales.expand(self.out_features).contiguous()
         self.register_buffer("weight_codes", codes[:weight._mx_n].view(self.out_features, self.in_features))
         self.register_buffer("weight_scales", scales)
-        self.register_buffer("bias", None if bias is None else bias.detach().float())
+        bias = _bias(None if bias is None else bias.detach(), self.out_features, codes.device, "int8_linear")
+        self.register_buffer("bias", bias)
 
     @classmethod
     def from_linear(cls, linear: nn.Linear, out_dtype: torch.dtype = torch.bfloat16) -> "int8_linear":
@@ -222,10 +223,16 @@ class int8_linear(nn.Module):
         a = _operand(x, K, "int8_linear")
         L.require_cuda(a[0], "int8_linear")
         codes = self.weight_codes
-        if codes.device != a[0].device:
+        scales, bias = self.weight_scales, self.bias
+        if codes.device != a[0].device or scales.device != codes.device:
             raise ValueError("int8_linear: activations and weight on different devices")
+        # buffers that were assigned since
+        if codes.dtype != torch.int8 or codes.shape != (N, K) or scales.dtype != torch.float32 or scales.shape != (N,):
+            raise ValueError(f"int8_linear: int8 codes [{N}, {K}] and fp32 scales [{N}], got {codes.dtype} "
+                             f"{tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")
+        bias = _bias(bias, N, codes.device, "int8_linear")
         out = torch.empty((*shape[:-1], N), dtype=self.out_dtype, device=codes.device)
-        return _product(a, (codes, self.weight_scales, 1), shape[:-1].numel(), K, N, self.bias, out)
+        return _product(a, (codes.contiguous(), scales.contiguous(), 1), shape[:-1].numel(), K, N, bias, out)
 
     def extra_repr(self):
         return f"in={self.in_features}, out={self.out_features}, bias={self.bias is not None}"

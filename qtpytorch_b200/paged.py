@@ -138,7 +138,8 @@ class paged_kv_cache:
         ``sections`` (pairs of each axis, up to four, in order) positions are
         [axes, T], one row an axis.  Angles are found in 64 bits; a key's codes and
         scale are those of its rotation in 64 bits rounded to fp32.  The queries of
-        skipped tokens are rotated too.  No gradient."""
+        skipped tokens are rotated too.  Slots of one call must be distinct.  No
+        gradient."""
         dev = self._cuda("paged_kv_cache.append")
         H, D = self.n_heads, self.head_dim
         if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (H, D) or slots.shape != k.shape[:1]:

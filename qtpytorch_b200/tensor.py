@@ -35,12 +35,16 @@ _STRICT = os.environ.get("MX_STRICT", "0") == "1"
 _placeholders: dict = {}
 
 
-def _placeholder(device: torch.device) -> torch.Tensor:
+def _placeholder(packed: torch.Tensor) -> torch.Tensor:
     """What stands behind the wrapper itself: an fp32 scalar that nothing reads or
-    writes, one a device."""
+    writes, one a device.  Inference and fake tensors get one of their own kind."""
+    device = packed.device
+    if type(packed) is not torch.Tensor or packed.is_inference():
+        return torch.empty((), dtype=torch.float32, device=device)
     t = _placeholders.get(device)
     if t is None:
-        t = torch.empty((), dtype=torch.float32, device=device)
+        with torch.inference_mode(False):
+            t = torch.empty((), dtype=torch.float32, device=device)
         # a capture's allocations belong to its graph
         if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
             _placeholders[device] = t
@@ -52,7 +56,7 @@ class mx_tensor(torch.Tensor):
 
     def __new__(cls, packed: torch.Tensor, scales: torch.Tensor, mx_dtype: mx_dtype,
                 orig_shape, n: int, block: int = 128, requires_grad: bool = False):
-        inst = torch.Tensor._make_subclass(cls, _placeholder(packed.device), False)
+        inst = torch.Tensor._make_subclass(cls, _placeholder(packed), False)
         inst._mx_packed = packed
         inst._mx_scales = scales
         inst._mx_dtype = get_mx_dtype(mx_dtype)

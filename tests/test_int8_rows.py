@@ -31,6 +31,10 @@ def test_argument_errors_need_no_gpu():
     assert norm(x=odd) == -3 and norm(r=odd) == -3 and norm(h=odd) == -3 and norm(w=odd) == -3
     assert norm(scales=ctypes.c_void_p(34)) == -3 and norm(dt=0, x=ctypes.c_void_p(34)) == -3
     assert norm(rows=0) == 0
+    # the sum lies over neither of its terms (rows 64 apart: 2 x 128 bytes of bf16)
+    assert norm(h=P) == -6 and norm(h=ctypes.c_void_p(32 + 254)) == -6
+    far = ctypes.c_void_p(4096)
+    assert norm(r=far, h=far) == -6 and norm(r=far, h=ctypes.c_void_p(4096 - 254)) == -6
 
     def product(a=P, sa=P, sta=1, b=P, sb=P, stb=1, M=2, K=64, N=3, bias=None, out=P, od=1, ws=None, n=0):
         return lib.mxb_int8_matmul(a, sa, sta, b, sb, stb, M, K, N, bias, out, od, ws, n, None)
@@ -93,6 +97,59 @@ def test_linear_module_casts_and_copies():
     assert one.weight_scales.shape == (3,)
     with pytest.raises(ValueError):
         lin(fake(2, 9))
+
+
+def test_linear_module_checks_its_buffers():
+    strided = torch.arange(6.0)[::2]
+    assert torch.equal(mxb.int8_linear(fake(3, 8), strided).bias, strided)
+    for bad in (torch.ones(2), torch.ones(3, 1), torch.ones(()), torch.ones(3, device="meta")):
+        with pytest.raises(ValueError):
+            mxb.int8_linear(fake(3, 8), bad)
+
+
+def test_codes_made_in_inference_mode_leave_later_ones_usable():
+    def inference(t):  # of the wrapper itself
+        with torch._C.DisableTorchFunctionSubclass():
+            return t.is_inference()
+
+    with torch.inference_mode():
+        fake(2, 8)
+    later = fake(2, 8)
+    assert not inference(later)
+    with torch.inference_mode():
+        assert not inference(mxb.mx_tensor(later.packed, later.mx_scales, mxb.int8d, (2, 8), 16, 8))
+        assert inference(fake(2, 8))
+    assert not inference(fake(2, 8))
+
+
+@pytest.mark.gpu
+def test_linear_module_with_assigned_buffers():
+    lin = mxb.int8_linear.from_linear(torch.nn.Linear(64, 24, device="cuda"))
+    x = rows(1, 5, 64)
+    want = lin(x)
+    state = {k: v.clone() for k, v in lin.state_dict().items()}
+    wide = torch.zeros(48, device="cuda")
+    wide[::2] = state["bias"]
+    lin.bias = wide[::2]  # in steps
+    assert torch.equal(lin(x), want)
+    lin.bias = state["bias"].double()
+    assert torch.equal(lin(x), want)
+    lin.weight_codes = state["weight_codes"].t().contiguous().t()
+    assert torch.equal(lin(x), want)
+    for name, bad in (("bias", state["bias"][:23]), ("bias", state["bias"].cpu()),
+                      ("weight_scales", state["weight_scales"].bfloat16()),
+                      ("weight_scales", state["weight_scales"][:23]), ("weight_scales", state["weight_scales"].cpu()),
+                      ("weight_codes", state["weight_codes"][:23]), ("weight_codes", state["weight_codes"].short())):
+        for k, v in {**state, name: bad}.items():
+            setattr(lin, k, v)
+        with pytest.raises(ValueError):
+            lin(x)
+    for k, v in state.items():
+        setattr(lin, k, v)
+    assert torch.equal(lin(x), want)
+    assert lin(x[:0]).shape == (0, 24) and torch.equal(lin(x[0]), want[0])
+    with torch.inference_mode():
+        assert torch.equal(lin(x), want)
 
 
 # ── norm ─────────────────────────────────────────────────────────────────────
@@ -213,6 +270,34 @@ def test_norm_refusals_on_the_device():
             mxb.rms_norm_quantize(x, w, **kw)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d,dtype", [(8, 4096, torch.bfloat16), (500, 1000, torch.float32), (700, 512, torch.bfloat16)])
+def test_norm_repeats_on_any_stream_and_in_a_graph(n, d, dtype):
+    x, r, w = rows(1, n, d).to(dtype), rows(2, n, d).to(dtype), 1 + 0.1 * rows(3, d, loud=False)
+    want, sum_ = mxb.rms_norm_quantize(x, w, residual=r)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [mxb.rms_norm_quantize(x, w, residual=r) for _ in range(10)]
+    here = [mxb.rms_norm_quantize(x, w, residual=r) for _ in range(10)]
+    torch.cuda.synchronize()
+    for q, s in got + here:
+        assert torch.equal(q.packed, want.packed) and torch.equal(q.mx_scales, want.mx_scales)
+        assert torch.equal(s, sum_)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q, s = mxb.rms_norm_quantize(x, w, residual=r)
+        y = q.dequantize()
+    x0 = x.clone()
+    x.copy_(r)
+    graph.replay()
+    other, _ = mxb.rms_norm_quantize(x, w, residual=r)
+    assert torch.equal(q.packed, other.packed) and torch.equal(y, other.dequantize())
+    x.copy_(x0)
+    graph.replay()
+    assert torch.equal(q.packed, want.packed) and torch.equal(s, sum_) and torch.equal(y, want.dequantize())
+
+
 # ── product ──────────────────────────────────────────────────────────────────
 def operand(n, k, seed, block=None, full=False):
     g = torch.Generator("cuda").manual_seed(seed)
@@ -311,6 +396,40 @@ def test_product_repeats_on_any_stream_and_in_a_graph():
         z.zero_()
         graph.replay()
         assert torch.equal(y, want) and torch.equal(z, want2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k,n", [(2048, 2048, 2048), (2305, 1000, 2184)])
+def test_product_of_many_tokens(out, m, k, n):
+    """The kernel of CTA pairs: two at once on two streams, in a graph, one scale for all,
+    and the operands that it leaves to the other one (scales and bias in steps of 4 bytes)."""
+    a, b = operand(m, k, 1), operand(n, k, 2, full=True)
+    bias = torch.randn(n, generator=torch.Generator("cuda").manual_seed(1), device="cuda")
+    want = product_ref(a, b, bias, out)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ys = [mxb.int8_matmul(a, b, bias=bias, out_dtype=out) for _ in range(5)]
+    ys += [mxb.int8_matmul(a, b, bias=bias, out_dtype=out) for _ in range(5)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in ys)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = mxb.int8_matmul(a, b, bias=bias, out_dtype=out)
+    for _ in range(2):
+        y.zero_()
+        graph.replay()
+        assert torch.equal(y, want)
+    off = torch.empty(n + 1, device="cuda")[1:]
+    assert torch.equal(mxb.int8_matmul(a, b, bias=off.copy_(bias), out_dtype=out), want)
+    at = torch.empty(n + 1, device="cuda")[1:].copy_(b.mx_scales)
+    moved = mxb.mx_tensor(b.packed, at, mxb.int8d, (n, k), n * k, k)
+    assert torch.equal(mxb.int8_matmul(a, moved, bias=bias, out_dtype=out), want)
+    one = mxb.mx_tensor(b.packed, b.mx_scales[:1], mxb.int8d, (n, k), n * k, n * k)
+    for p, q in ((a, one), (mxb.mx_tensor(a.packed, a.mx_scales[5:6], mxb.int8d, (m, k), m * k, m * k), b)):
+        assert torch.equal(mxb.int8_matmul(p, q, out_dtype=out), product_ref(p, q, None, out))
+    assert L.load().mxb_device_error(1) == 0
 
 
 @pytest.mark.gpu
