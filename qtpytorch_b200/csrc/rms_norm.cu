@@ -17,9 +17,12 @@
 // values leave the range in which all this holds, take a slow path in 64 bits.
 //
 // One pass over HBM: a row stays in the registers of its block, 8 NC values a
-// thread.  4096 x 8192 bf16 with a residual (235 MB): 51 us = 4.6 TB/s with three rows an
-// SM; 109 us where each correction in 64 bits stood in line and two fitted.  8 x 4096:
-// 3.0 us; 1001 x 1999 fp32, value by value: 9 us, 13 with 32 values a thread.
+// thread.  What bounds it beside HBM is the issue of its instructions and the chain of a
+// row (two reductions, two barriers).  4096 x 8192 bf16 with a residual (235 MB): 43 us =
+// 5.4 TB/s in pairs of values with four rows an SM, 51 one value at a time with three, 109
+// where each correction in 64 bits stood in line.  Rows copied to shared memory ahead of
+// their turn by blocks that stay: 50.  8 x 4096: 3.0 us; 1001 x 1999 fp32, value by value:
+// 9 us, 13 with 32 values a thread.
 #include "mxb_common.cuh"
 #include "mxb_internal.h"
 
@@ -40,33 +43,31 @@ struct Raw8<float> {
     a = __ldg(reinterpret_cast<const float4*>(p));
     b = __ldg(reinterpret_cast<const float4*>(p) + 1);
   }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  __device__ __forceinline__ void get(uint64_t (&v)[4]) const {
+    v[0] = pack2(a.x, a.y); v[1] = pack2(a.z, a.w);
+    v[2] = pack2(b.x, b.y); v[3] = pack2(b.z, b.w);
   }
 };
 template <>
 struct Raw8<__nv_bfloat16> {
   uint4 r;
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { r = __ldg(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
+  __device__ __forceinline__ void get(uint64_t (&v)[4]) const {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    for (int i = 0; i < 4; ++i) v[i] = pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
   }
 };
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+__device__ __forceinline__ void store8(float* p, const uint64_t (&v)[4]) {
+  reinterpret_cast<ulonglong2*>(p)[0] = make_ulonglong2(v[0], v[1]);
+  reinterpret_cast<ulonglong2*>(p)[1] = make_ulonglong2(v[2], v[3]);
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const uint64_t (&v)[4]) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    const float2 f = unpack2(v[i]);
+    const __nv_bfloat162 t = __floats2bfloat162_rn(f.x, f.y);
     w[i] = *reinterpret_cast<const uint32_t*>(&t);
   }
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -140,6 +141,142 @@ __device__ __noinline__ void row_in_64_bits(const Row<InT, WT>& row, double eps,
   if (t == 0) *scale = ok ? (float)(den / root / 127.0) : __int_as_float(0x7fc00000);
 }
 
+__device__ __forceinline__ float nan_max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// A row's sum of squares and largest |u|: the warp's, then the block's.
+template <bool WARP>
+__device__ __forceinline__ void reduce(float& ssq, float& top, Shared& sm, int t, int n) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
+    top = nan_max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  if constexpr (!WARP) {
+    if ((t & 31) == 0) {
+      sm.ssq[t >> 5] = ssq;
+      sm.top[t >> 5] = top;
+    }
+    __syncthreads();
+    const int lane = t & 31, warps = n >> 5;
+    ssq = lane < warps ? sm.ssq[lane] : 0.0f;
+    top = lane < warps ? sm.top[lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
+      top = nan_max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+  }
+}
+
+// Squares and products in the range in which fp32 holds them to 2^-24, the largest y
+// above what the scale's lower bound asks for.
+__device__ __forceinline__ bool in_range(float ssq, float top, float inv_d, double eps) {
+  const float root = sqrtf(fmaf(ssq, inv_d, (float)eps));
+  return ssq >= 1e-30f && ssq <= 1e37f && top >= 1e-30f && top <= 1e37f && top >= 1.01e-12f * root;
+}
+
+// Value j of a thread's chunk c.
+template <bool VEC>
+__device__ __forceinline__ int index_of(int c, int j, int t, int n) {
+  return VEC ? (c * n + t) * 8 + j : (c * 8 + j) * n + t;
+}
+// Elements that need 64 bits: a bit each, so that there is one place that reads them again.
+template <bool VEC>
+__device__ __forceinline__ int index_of_bit(uint32_t bits, int t, int n) {
+  const int b = __ffs(bits) - 1;
+  return index_of<VEC>(b >> 3, b & 7, t, n);
+}
+
+// 8 values of h taken into the sum of squares; u and its largest.
+__device__ __forceinline__ void take8(const uint64_t (&xv)[4], const uint64_t (&wv)[4], uint64_t (&u)[4],
+                                      uint64_t& ssq, float& top) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    ssq = ffma2(xv[j], xv[j], ssq);
+    u[j] = fmul2(xv[j], wv[j]);
+    const float2 v = unpack2(u[j]);
+    top = nan_max3(top, fabsf(v.x), fabsf(v.y));
+  }
+}
+
+// The largest |u| in 64 bits of this thread's, whose largest in fp32 is `mine`: of those
+// that fp32 cannot tell from the row's largest.
+template <int NC, bool VEC, typename RowT>
+__device__ __forceinline__ double largest(const uint64_t (&u)[NC][4], float mine, float top, const RowT& row, int t,
+                                          int n) {
+  const float near_top = top * (1.0f - 0x1p-21f);
+  double most = 0.0;
+  if (mine >= near_top) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = unpack2(u[c][j]);
+        bits |= fabsf(v.x) >= near_top ? 1u << (8 * c + 2 * j) : 0u;
+        bits |= fabsf(v.y) >= near_top ? 2u << (8 * c + 2 * j) : 0u;
+      }
+    for (; bits; bits &= bits - 1) most = fmax(most, fabs(row.u64(index_of_bit<VEC>(bits, t, n))));
+  }
+  return most;
+}
+
+// Codes and scale.
+template <int NC, bool VEC, typename RowT>
+__device__ __forceinline__ void put_codes(const uint64_t (&u)[NC][4], double most, float ssq, double eps,
+                                          const RowT& row, int t, int n, int8_t* code, float* scale) {
+  constexpr float kNear = 0.5f - 127.0f * 0x1p-21f, kRound = 12582912.0f;  // 1.5 * 2^23
+  const int d = row.d;
+  const float factor = __fdiv_rn(127.0f, (float)most);
+  const uint64_t f2 = pack2(factor, factor), r2 = pack2(kRound, kRound), minus = pack2(-1.0f, -1.0f);
+  float far = 0.0f;  // largest distance from the code taken
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    uint32_t q[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t v = fmul2(u[c][j], f2), k = fadd2(v, r2);
+      const float2 off = unpack2(fadd2(v, ffma2(k, minus, r2))), kk = unpack2(k);
+      q[2 * j] = __float_as_uint(kk.x);  // the code in the low byte
+      q[2 * j + 1] = __float_as_uint(kk.y);
+      far = fmaxf(fmaxf(far, fabsf(off.x)), fabsf(off.y));
+    }
+    if constexpr (VEC) {
+      uint32_t p[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        p[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040),
+                           0x5410);
+      if (index_of<VEC>(c, 0, t, n) < d)
+        *reinterpret_cast<uint2*>(code + index_of<VEC>(c, 0, t, n)) = make_uint2(p[0], p[1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (index_of<VEC>(c, j, t, n) < d) code[index_of<VEC>(c, j, t, n)] = (int8_t)q[j];
+    }
+  }
+  if (far > kNear) {  // over what this thread has just stored
+    uint32_t bits = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = unpack2(fmul2(u[c][j], f2));
+        bits |= fabsf(v.x - rintf(v.x)) > kNear ? 1u << (8 * c + 2 * j) : 0u;
+        bits |= fabsf(v.y - rintf(v.y)) > kNear ? 2u << (8 * c + 2 * j) : 0u;
+      }
+    for (; bits; bits &= bits - 1) {
+      const int i = index_of_bit<VEC>(bits, t, n);
+      code[i] = (int8_t)__double2int_rn(__ddiv_rn(127.0 * row.u64(i), most));
+    }
+  }
+  if (t == 0) *scale = (float)(most / sqrt((double)ssq / d + eps) / 127.0);
+}
+
 // WARP: a warp a row, kWarpRows of them a block; otherwise a block of up to MAX
 // threads a row, MIN of them on an SM.
 template <typename InT, typename WT, int NC, int MAX, int MIN, bool VEC, bool WARP>
@@ -161,10 +298,10 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : MAX, MIN)
     row_in_64_bits(row, eps, t, n, &sm, code, scales + at, ho);
     return;
   }
-  // value j of chunk c
-  auto index = [&](int c, int j) { return VEC ? (c * n + t) * 8 + j : (c * 8 + j) * n + t; };
-  float u[NC][8];
-  float ssq = 0.0f, top = 0.0f;
+  auto index = [&](int c, int j) { return index_of<VEC>(c, j, t, n); };
+  uint64_t u[NC][4];
+  uint64_t sq2 = 0;
+  float top = 0.0f;
   if constexpr (VEC) {
     // x and r of the whole row on their way at once; as many registers as u takes after
     Raw8<InT> xr[NC], rr[NC];
@@ -179,88 +316,52 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : MAX, MIN)
       if (index(c, 0) < d) {
         Raw8<WT> wr;
         wr.load(w + index(c, 0));
-        float h[8], v[8];
+        uint64_t h[4], v[4];
         xr[c].get(h);
         if (r) {
           rr[c].get(v);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) h[j] = __fadd_rn(h[j], v[j]);
+          for (int j = 0; j < 4; ++j) h[j] = fadd2(h[j], v[j]);
         }
         if (ho) store8(ho + index(c, 0), h);
         wr.get(v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          ssq = fmaf(h[j], h[j], ssq);
-          u[c][j] = __fmul_rn(h[j], v[j]);
-          top = amax_step(top, u[c][j]);
-        }
+        take8(h, v, u[c], sq2, top);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) u[c][j] = 0.0f;
+        for (int j = 0; j < 4; ++j) u[c][j] = 0;
       }
     }
   } else {
-    float h[NC][8];
+    uint64_t h[NC][4];
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = index(c, j);
-        h[c][j] = i < d ? row.h32(i) : 0.0f;
-        u[c][j] = i < d ? load_as_f32(w, i) : 0.0f;
+      for (int j = 0; j < 4; ++j) {
+        const int i0 = index(c, 2 * j), i1 = index(c, 2 * j + 1);
+        h[c][j] = pack2(i0 < d ? row.h32(i0) : 0.0f, i1 < d ? row.h32(i1) : 0.0f);
+        u[c][j] = pack2(i0 < d ? load_as_f32(w, i0) : 0.0f, i1 < d ? load_as_f32(w, i1) : 0.0f);
       }
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int c = 0; c < NC; ++c) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (ho && index(c, j) < d) store1(ho + index(c, j), h[c][j]);
-        ssq = fmaf(h[c][j], h[c][j], ssq);
-        u[c][j] = index(c, j) < d ? __fmul_rn(h[c][j], u[c][j]) : 0.0f;
-        top = amax_step(top, u[c][j]);
+      for (int j = 0; j < 4; ++j) {
+        const int i0 = index(c, 2 * j), i1 = index(c, 2 * j + 1);
+        const float2 v = unpack2(h[c][j]);
+        if (ho && i0 < d) store1(ho + i0, v.x);
+        if (ho && i1 < d) store1(ho + i1, v.y);
       }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
-    top = nan_max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  }
-  if constexpr (!WARP) {
-    if ((t & 31) == 0) {
-      sm.ssq[t >> 5] = ssq;
-      sm.top[t >> 5] = top;
-    }
-    __syncthreads();
-    const int lane = t & 31, warps = n >> 5;
-    ssq = lane < warps ? sm.ssq[lane] : 0.0f;
-    top = lane < warps ? sm.top[lane] : 0.0f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
-      top = nan_max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      take8(h[c], u[c], u[c], sq2, top);
     }
   }
-  // squares and products in the range in which fp32 holds them to 2^-24, the
-  // largest y above what the scale's lower bound asks for
-  const float root32 = sqrtf(fmaf(ssq, inv_d, (float)eps));
-  const bool fast = ssq >= 1e-30f && ssq <= 1e37f && top >= 1e-30f && top <= 1e37f && top >= 1.01e-12f * root32;
-  if (!fast) {  // the same for the whole row
+  const float mine = top;
+  const float2 sq = unpack2(sq2);
+  float ssq = sq.x + sq.y;
+  reduce<WARP>(ssq, top, sm, t, n);
+  if (!in_range(ssq, top, inv_d, eps)) {  // the same for the whole row
     row_in_64_bits<InT, WT>(row, eps, t, n, &sm, code, scales + at, nullptr);
     return;
   }
-  // Elements that need 64 bits: a bit each, so that there is one place that reads them again.
-  auto of_bit = [&](uint32_t bits) {
-    const int b = __ffs(bits) - 1;
-    return index(b >> 3, b & 7);
-  };
-  // ── the largest |u| in 64 bits, of those that fp32 cannot tell from it ──
-  const float near_top = top * (1.0f - 0x1p-21f);
-  double most = 0.0;
-  uint32_t bits = 0;
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) bits |= fabsf(u[c][j]) >= near_top ? 1u << (8 * c + j) : 0u;
-  for (; bits; bits &= bits - 1) most = fmax(most, fabs(row.u64(of_bit(bits))));
+  double most = largest<NC, VEC>(u, mine, top, row, t, n);
   if constexpr (WARP) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -270,36 +371,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : MAX, MIN)
     __syncthreads();
     most = __longlong_as_double((long long)sm.most);
   }
-  const float factor = __fdiv_rn(127.0f, (float)most);
-  constexpr float kNear = 0.5f - 127.0f * 0x1p-21f, kRound = 12582912.0f;  // 1.5 * 2^23
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    uint32_t q[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float v = __fmul_rn(u[c][j], factor), k = __fadd_rn(v, kRound);
-      q[j] = __float_as_uint(k);  // the code in the low byte
-      bits |= fabsf(v - __fadd_rn(k, -kRound)) > kNear ? 1u << (8 * c + j) : 0u;
-    }
-    if constexpr (VEC) {
-      uint32_t p[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        p[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040),
-                           0x5410);
-      if (index(c, 0) < d) *reinterpret_cast<uint2*>(code + index(c, 0)) = make_uint2(p[0], p[1]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (index(c, j) < d) code[index(c, j)] = (int8_t)q[j];
-    }
-  }
-  // over what this thread has just stored
-  for (; bits; bits &= bits - 1) {
-    const int i = of_bit(bits);
-    code[i] = (int8_t)__double2int_rn(__ddiv_rn(127.0 * row.u64(i), most));
-  }
-  if (t == 0) scales[at] = (float)(most / sqrt((double)ssq / d + eps) / 127.0);
+  put_codes<NC, VEC>(u, most, ssq, eps, row, t, n, code, scales + at);
 }
 
 struct NormArgs {
@@ -337,9 +409,13 @@ int by_size(const NormArgs& a, cudaStream_t st) {
   if ((a.rows <= 2 * kSMs || !VEC) && threads(1) <= 1024)
     return launch<InT, WT, 1, 1024, 1, VEC, false>(a, threads(1), st);
   if constexpr (VEC) {
-    if (threads(4) <= 256) return launch<InT, WT, 4, 256, 3, VEC, false>(a, threads(4), st);
+    // 64 registers a thread hold a row of bf16 on its way and its u, of fp32 they do not
+    // (80 bytes of spills; 4096 x 4096 with a residual 50 us, 44 with three rows an SM)
+    constexpr int kRows = sizeof(InT) == 2 ? 4 : 3;
+    if (threads(4) <= 256) return launch<InT, WT, 4, 256, kRows, VEC, false>(a, threads(4), st);
   }
-  if (threads(4) <= 512) return launch<InT, WT, 4, 512, 1, VEC, false>(a, threads(4), st);
+  if (threads(4) <= 512)
+    return launch<InT, WT, 4, 512, VEC && sizeof(InT) == 2 ? 2 : 1, VEC, false>(a, threads(4), st);
   return launch<InT, WT, 4, 1024, 1, VEC, false>(a, threads(4), st);
 }
 
