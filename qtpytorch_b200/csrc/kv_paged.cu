@@ -16,6 +16,8 @@
 #include "mxb_common.cuh"
 #include "mxb_internal.h"
 
+#include <type_traits>
+
 using namespace mxb;
 
 namespace {
@@ -141,10 +143,12 @@ __global__ void __launch_bounds__(kThreads)
 // largest and those whose quotient comes within m 2^-20 of a border between two
 // codes are turned again in 64 bits.
 //
-// 16384 tokens of 32 + 8 heads of 128 dims, bf16 into int4 (215 MB): 55 us = 3.9 TB/s, at
-// two thirds of the issue slots; 61 us with divisions for a row's token, 89 with one row
-// of queries in flight and 64-bit strides.  More rows in flight (more registers, fewer
-// blocks) were slower, 48 registers a thread no faster.  32 tokens: 4.1 us.
+// 16384 tokens of 32 + 8 heads of 128 dims, bf16 into int4 (353 MB): 88 us = 4.0 TB/s; 95
+// with 8 values of a query row a lane, one at a time, 52 of them without queries (of those
+// 1 for the angles, 4 for what 64 bits decide): the chain of a row of keys (its load, three
+// reductions, two reciprocals) at 32 warps an SM.  Keys loaded a row ahead (76 registers,
+// three blocks) 98, more query rows in flight slower, 48 registers no faster.  32 tokens:
+// 4.1 us.
 struct Rotary {
   const int64_t* pos;  // [axes][axis_stride]
   int64_t axis_stride;
@@ -202,6 +206,27 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
       make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
+// Eight bf16 values as they lie in memory (16-byte aligned), in pairs.
+struct Raw8 {
+  uint4 r;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { r = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void get(uint64_t (&v)[4]) const {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+};
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const uint64_t (&v)[4]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2(v[i]);
+    const __nv_bfloat162 t = __floats2bfloat162_rn(f.x, f.y);
+    w[i] = *reinterpret_cast<const uint32_t*>(&t);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // cos and sin of an angle in 64 bits, however large: in turns, as a product and its
 // rounding error, so that the whole turns leave exactly.
 __device__ __forceinline__ void turn64(double angle, double& c, double& s) {
@@ -220,7 +245,9 @@ __device__ __forceinline__ int64_t offset_of(int t, int ts, int h, int hs) {
   return (int64_t)t * ts + (int64_t)h * hs;
 }
 
-template <typename InT, int BITS, int D, bool ILV>
+// Q16: a lane takes 16 values of a query row in pairs (bf16, aligned, whole runs of 8
+// pairs), otherwise 8.
+template <typename InT, int BITS, int D, bool ILV, bool Q16>
 __global__ void __launch_bounds__(kThreads)
     kv_append_kernel(const AppendRows a, const Rotary ro, int TB, const int64_t* __restrict__ slots,
                      int64_t n_slots, int page_shift, InT* __restrict__ q_out, uint8_t* __restrict__ kc,
@@ -228,8 +255,8 @@ __global__ void __launch_bounds__(kThreads)
                      int* __restrict__ err) {
   constexpr int L = D / 8, kRows = kThreads / L;
   constexpr float m = BITS == 8 ? 127.0f : 7.0f;
-  __shared__ float4 hi[kAppendTokens][D / 4];  // (cos, sin) of two pairs
-  __shared__ float4 lo[kAppendTokens][D / 4];
+  __shared__ float4 hi[kAppendTokens][D / 4];  // cosines and sines of two pairs
+  __shared__ float4 lo[kAppendTokens][D / 4];  // (cos, sin) of two pairs
   pdl_trigger();
   pdl_wait();
   const int64_t t0 = (int64_t)blockIdx.x * TB;
@@ -238,25 +265,34 @@ __global__ void __launch_bounds__(kThreads)
   // this lane's two runs of four values, and whether they turn
   const bool turns = part < ro.pairs / 4;
   const int oa = ILV || !turns ? part * 8 : part * 4, ob = ILV || !turns ? oa + 4 : ro.pairs + part * 4;
-  // rows of queries, kU of them in flight; the first while the angles are found
-  constexpr int kU = 4;
   const InT* q = static_cast<const InT*>(a.q) + t0 * a.q_ts;
   const InT* k = static_cast<const InT*>(a.k) + t0 * a.k_ts;
   const InT* v = static_cast<const InT*>(a.v) + t0 * a.v_ts + part * 8;
-  Raw4<InT> qa[kU], qb[kU];
+  // rows of queries, kU of them in flight; the first while the angles are found
+  constexpr int QE = Q16 ? 8 : 4, QL = D / (2 * QE), kQRows = kThreads / QL, kU = 16 / QE;
+  const int q_part = threadIdx.x % QL;
+  const bool q_turns = q_part < ro.pairs / QE;
+  const int qa = q_part * (ILV || !q_turns ? 2 * QE : QE), qb = ILV || !q_turns ? qa + QE : ro.pairs + qa;
+  using Raw = std::conditional_t<Q16, Raw8, Raw4<InT>>;
+  Raw ra[kU], rb[kU];
   auto load_q = [&](int u0) {
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
-      const int u = u0 + i * kRows;
+      const int u = u0 + i * kQRows;
       if (u < q_rows) {
         const int t = token_of(u, a.Hq);
         const InT* p = q + offset_of(t, a.q_ts, u - t * a.Hq, a.q_hs);
-        qa[i].load(p + oa, a.vec);
-        qb[i].load(p + ob, a.vec);
+        if constexpr (Q16) {
+          ra[i].load(p + qa);
+          rb[i].load(p + qb);
+        } else {
+          ra[i].load(p + qa, a.vec);
+          rb[i].load(p + qb, a.vec);
+        }
       }
     }
   };
-  int u0 = threadIdx.x / L;
+  int u0 = threadIdx.x / QL;
   load_q(u0);
   q_out += t0 * a.Hq * D;
   for (int i = threadIdx.x; i < tokens * ro.pairs; i += kThreads) {
@@ -265,7 +301,9 @@ __global__ void __launch_bounds__(kThreads)
     double c, s;
     turn64(__dmul_rn((double)ro.pos[axis * ro.axis_stride + t0 + t], (double)__ldg(ro.inv_freq + p)), c, s);
     const float ch = (float)c, sh = (float)s;
-    reinterpret_cast<float2*>(hi[t])[p] = make_float2(ch, sh);
+    float* at = reinterpret_cast<float*>(&hi[t][p >> 1]) + (p & 1);
+    at[0] = ch;
+    at[2] = sh;
     reinterpret_cast<float2*>(lo[t])[p] = make_float2((float)(c - (double)ch), (float)(s - (double)sh));
   }
   __syncthreads();
@@ -275,8 +313,8 @@ __global__ void __launch_bounds__(kThreads)
   auto turn = [&](int t, const float (&x)[8], float (&y)[8], float (&cs)[8]) {
     if (turns) {
       const float4 c0 = hi[t][part * 2], c1 = hi[t][part * 2 + 1];
-      cs[0] = c0.x; cs[1] = c0.y; cs[2] = c0.z; cs[3] = c0.w;
-      cs[4] = c1.x; cs[5] = c1.y; cs[6] = c1.z; cs[7] = c1.w;
+      cs[0] = c0.x; cs[1] = c0.z; cs[2] = c0.y; cs[3] = c0.w;
+      cs[4] = c1.x; cs[5] = c1.z; cs[6] = c1.y; cs[7] = c1.w;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float v0 = x[first(j)], v1 = x[second(j)], c = cs[2 * j], s = cs[2 * j + 1];
@@ -288,25 +326,49 @@ __global__ void __launch_bounds__(kThreads)
       for (int j = 0; j < 8; ++j) y[j] = x[j];
     }
   };
-  auto get8 = [](const Raw4<InT>& r0, const Raw4<InT>& r1, float (&x)[8]) {
+  [[maybe_unused]] auto get8 = [](const Raw4<InT>& r0, const Raw4<InT>& r1, float (&x)[8]) {
     r0.get(*reinterpret_cast<float (*)[4]>(x));
     r1.get(*reinterpret_cast<float (*)[4]>(x + 4));
   };
   while (u0 < q_rows) {
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
-      const int u = u0 + i * kRows;
+      const int u = u0 + i * kQRows;
       if (u < q_rows) {
         const int t = token_of(u, a.Hq);
-        float x[8], y[8], cs[8];
-        get8(qa[i], qb[i], x);
-        turn(t, x, y, cs);
         InT* o = q_out + u * D;  // u counts a token's heads in their order
-        store4(o + oa, *reinterpret_cast<float (*)[4]>(y));
-        store4(o + ob, *reinterpret_cast<float (*)[4]>(y + 4));
+        if constexpr (Q16) {
+          uint64_t x0[4], x1[4];
+          ra[i].get(x0);
+          rb[i].get(x1);
+          if (q_turns) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float4 f = hi[t][q_part * 4 + j];
+              if constexpr (ILV) {  // two pairs lie in x0[2 j], x0[2 j + 1], then in x1
+                uint64_t* x = j < 2 ? x0 + 2 * j : x1 + 2 * j - 4;
+                const float2 v0 = unpack2(x[0]), v1 = unpack2(x[1]);
+                x[0] = pack2(fmaf(v0.x, f.x, -__fmul_rn(v0.y, f.z)), fmaf(v0.x, f.z, __fmul_rn(v0.y, f.x)));
+                x[1] = pack2(fmaf(v1.x, f.y, -__fmul_rn(v1.y, f.w)), fmaf(v1.x, f.w, __fmul_rn(v1.y, f.y)));
+              } else {
+                const uint64_t c = pack2(f.x, f.y), s = pack2(f.z, f.w), ns = pack2(-f.z, -f.w), v0 = x0[j];
+                x0[j] = ffma2(v0, c, fmul2(x1[j], ns));
+                x1[j] = ffma2(v0, s, fmul2(x1[j], c));
+              }
+            }
+          }
+          store8(o + qa, x0);
+          store8(o + qb, x1);
+        } else {
+          float x[8], y[8], cs[8];
+          get8(ra[i], rb[i], x);
+          turn(t, x, y, cs);
+          store4(o + qa, *reinterpret_cast<float (*)[4]>(y));
+          store4(o + qb, *reinterpret_cast<float (*)[4]>(y + 4));
+        }
       }
     }
-    u0 += kU * kRows;
+    u0 += kU * kQRows;
     load_q(u0);
   }
   // keys, with the values beside them; a warp goes through its loop as one
@@ -342,6 +404,7 @@ __global__ void __launch_bounds__(kThreads)
       top = amax_step(top, y[j]);
       top_v = amax_step(top_v, w[j]);
     }
+    const float mine = top;
 #pragma unroll
     for (int o = L >> 1; o > 0; o >>= 1) {
       top = nan_max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -350,9 +413,11 @@ __global__ void __launch_bounds__(kThreads)
     if (ro.pairs > 0) {
       const float near_top = top * (1.0f - 0x1p-20f);
       float best = 0.0f;
+      if (!(mine < near_top)) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (!(fabsf(y[j]) < near_top)) best = amax_step(best, turns ? again(j) : y[j]);
+        for (int j = 0; j < 8; ++j)
+          if (!(fabsf(y[j]) < near_top)) best = amax_step(best, turns ? again(j) : y[j]);
+      }
 #pragma unroll
       for (int o = L >> 1; o > 0; o >>= 1) best = nan_max(best, __shfl_xor_sync(0xffffffffu, best, o));
       top = best;
@@ -366,13 +431,22 @@ __global__ void __launch_bounds__(kThreads)
     put_row<BITS, D>(w, top_v, r, part, vc, vs);
     const float si = __fmul_rn(__frcp_rn(nan_max(top, 1e-12f)), m);
     const bool ok = si > 0.0f && si <= 3.4028235e38f;  // no infinity or NaN in the row
-    uint32_t c[8];
+    float far = 0.0f;  // largest distance from a whole number
+    constexpr float kNear = 0.5f - m * 0x1p-20f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      float v = __fmul_rn(y[j], si);
-      if (turns && fabsf(v - rintf(v)) > 0.5f - m * 0x1p-20f) v = __fmul_rn(again(j), si);
-      c[j] = ok ? __float_as_uint(__fadd_rn(v, 12582912.0f)) & (BITS == 8 ? 255u : 15u) : 0u;
+      w[j] = __fmul_rn(y[j], si);
+      far = fmaxf(far, fabsf(w[j] - rintf(w[j])));
     }
+    if (turns && far > kNear) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (fabsf(w[j] - rintf(w[j])) > kNear) w[j] = __fmul_rn(again(j), si);
+    }
+    uint32_t c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      c[j] = ok ? __float_as_uint(__fadd_rn(w[j], 12582912.0f)) & (BITS == 8 ? 255u : 15u) : 0u;
     uint8_t* dst = kc + r * (D * BITS / 8);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -520,7 +594,13 @@ int append_t(const AppendArgs& a, cudaStream_t st) {
     MXB_LAUNCH_CHECK();
     return MXB_OK;
   };
-  return a.interleaved ? go(kv_append_kernel<InT, BITS, D, true>) : go(kv_append_kernel<InT, BITS, D, false>);
+  if constexpr (sizeof(InT) == 2) {
+    if (r.vec && a.ro.pairs % 8 == 0)
+      return a.interleaved ? go(kv_append_kernel<InT, BITS, D, true, true>)
+                           : go(kv_append_kernel<InT, BITS, D, false, true>);
+  }
+  return a.interleaved ? go(kv_append_kernel<InT, BITS, D, true, false>)
+                       : go(kv_append_kernel<InT, BITS, D, false, false>);
 }
 
 struct ReadArgs {
