@@ -300,11 +300,45 @@ struct Tile {
   const float* slot;
   uint32_t s, o;        // TMEM: S (P over it) and O of this warp's rows
   bool first;           // no O yet
-  int key0, hist;       // first key of the tile; keys before the tree
-  int T;                // tokens of the tree
-  const uint8_t* mask;  // the sequence's
-  int64_t mask_t;
 };
+
+// Which of a lane's scores of a tile that reaches the tree are hidden by the masks of its
+// rows: bit 4 i + 2 k + e of a word of 32 keys for key 8 i + 2 (lane % 4) + e of row 8 k +
+// lane / 4.  key0: the tile's first key, from the tree's first one on.
+__device__ __forceinline__ uint4 tree_bits(int key0, int T, const uint8_t* mask, int64_t mask_t, const int (&tok)[2]) {
+  const uint8_t* row[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) row[k] = mask + min(tok[k], T - 1) * mask_t;
+  uint4 all = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t bits = 0;
+    const int k0 = key0 + 32 * c + 2 * (threadIdx.x & 3);
+    if (key0 + 32 * c + 32 > 0) {
+      // all bytes at once, those of other places are not looked at
+      uint32_t seen[4][2][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) seen[i][k][e] = __ldg(row[k] + max(min(k0 + 8 * i + e, T - 1), 0));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int at = k0 + 8 * i + e;
+            const bool off = at >= 0 && (at >= T || tok[k] >= T || seen[i][k][e] == 0u);
+            bits |= (off ? 1u : 0u) << (4 * i + 2 * k + e);
+          }
+    }
+    all = make_uint4(all.y, all.z, all.w, bits);  // four turns: each word in its place
+  }
+  __syncwarp();
+  return all;
+}
 
 // Multiplies the D columns of O, and with them the P of `pieces` pieces of this tile,
 // of the lane's rows by 2^x, in place.
@@ -345,49 +379,20 @@ __device__ __noinline__ void rescale(uint32_t o_at, uint32_t s_at, bool has_o, i
 // is not unrolled: three roles share the instruction cache, and four pieces in a row,
 // the next one's S on its way, took 304 us where the loop takes 245.
 template <int D>
-__device__ __forceinline__ void softmax_tile(Rows& r, const Tile& g, const float (&rowf)[2], const int (&tok)[2]) {
+__device__ __forceinline__ void softmax_tile(Rows& r, const Tile& g, const float (&rowf)[2], uint4 hidden) {
   const float* head = g.slot + 2 * KT;
   const float lcn = head[0];
   const bool wide = __float_as_uint(head[1]) != 0u;
-  uint4 hidden = *reinterpret_cast<const uint4*>(head + 4);
+  const uint4 gone = *reinterpret_cast<const uint4*>(head + 4);
   const int lane = threadIdx.x & 31;
-  if (__builtin_expect(g.key0 + KT > g.hist || (hidden.x | hidden.y | hidden.z | hidden.w), 0)) {
-    // from keys that are hidden to which of a lane's scores are: bit 4 i + 2 k + e of a
-    // word for key 8 i + 2 (lane % 4) + e of row 8 k + lane / 4
-    const uint8_t* mask[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) mask[k] = g.mask + min(tok[k], g.T - 1) * g.mask_t;
-#pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-      const uint32_t gone = hidden.x;
+  if (__builtin_expect((gone.x | gone.y | gone.z | gone.w) != 0u, 0)) {  // for both rows of a lane
+    auto of = [&](uint32_t w) -> uint32_t {
       uint32_t bits = 0;
-      if (gone != 0u || g.key0 + 32 * c + 32 > g.hist) {
-        // the tree's own keys, as far as the row's mask names them: all bytes at once, those
-        // of other places are not looked at
-        uint32_t seen[4][2][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int at = g.key0 + 32 * c + 8 * i + 2 * (lane & 3) + e - g.hist;
-              seen[i][k][e] = __ldg(mask[k] + max(min(at, g.T - 1), 0));
-            }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int j = 8 * i + 2 * (lane & 3) + e, at = g.key0 + 32 * c + j - g.hist;
-              const bool off = (gone >> j & 1u) || (at >= 0 && (at >= g.T || tok[k] >= g.T || seen[i][k][e] == 0u));
-              bits |= (off ? 1u : 0u) << (4 * i + 2 * k + e);
-            }
-      }
-      hidden = make_uint4(hidden.y, hidden.z, hidden.w, bits);  // four turns: each word in its place
-    }
-    __syncwarp();
+      for (int i = 0; i < 4; ++i) bits |= (w >> (8 * i + 2 * (lane & 3)) & 3u) * 5u << (4 * i);
+      return bits;
+    };
+    hidden = make_uint4(hidden.x | of(gone.x), hidden.y | of(gone.y), hidden.z | of(gone.z), hidden.w | of(gone.w));
   }
   if (g.first) {
 #pragma unroll
@@ -954,21 +959,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         Tile tile;
         tile.s = t_s(g) + lane_sel;
         tile.o = t_o(g) + lane_sel;
-        tile.hist = at.len - a.T;
-        tile.T = a.T;
-        tile.mask = a.tree + (int64_t)at.b * a.tree_b;
-        tile.mask_t = a.tree_t;
+        const int hist = at.len - a.T;  // keys before the tree
+        const uint8_t* mask = a.tree + (int64_t)at.b * a.tree_b;
         const int i0 = MT == 2 ? 0 : g, di = MT == 2 ? 1 : 2;
         for (int i = i0; i < n && ok; i += di, ++step) {
-          const int j = j0 + i;
+          const int j = j0 + i, key0 = (at.t_lo + i) * KT - hist;
+          uint4 hidden = make_uint4(0u, 0u, 0u, 0u);
+          // while the codes are on their way
+          if (__builtin_expect(key0 + KT > 0, 0)) hidden = tree_bits(key0, a.T, mask, a.tree_t, tok);
           ok = mbar_sleep_warp_to(&bars->scready[j & 3], (j >> 2) & 1, kErrTimeoutFull, a.err) &&
                mbar_sleep_warp_to(&bars->sready[g], step & 1, kErrTimeoutTmemFull, a.err);
           if (!ok) break;
           tc_fence_after();
           tile.slot = slots + (j & 3) * kSlotF;
           tile.first = i < di;
-          tile.key0 = (at.t_lo + i) * KT;
-          softmax_tile<D>(r, tile, rowf, tok);
+          softmax_tile<D>(r, tile, rowf, hidden);
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->pready[g]);
         }

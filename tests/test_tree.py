@@ -139,6 +139,20 @@ def test_many_units(dtype, dim, page, heads, group, T, lengths, prefix):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("group,T", [(1, 4), (8, 40)])
+def test_no_keys_at_all(group, T):
+    for B, prefix in ((2, 0), (60, 0), (2, 30)):
+        run("int8d", 64, 16, 2, group, T, [0] * B, prefix)
+    q, c, table, n, rest, _, _ = run("int8d", 64, 16, 2, group, T, [T, 2 * T], 0)
+    mask = trees(2, T, 0)
+    o, lse = mxb.paged_attention(q[:0], c, table[:0], n[:0], return_lse=True, tree_mask=mask[:0])
+    assert o.shape == (0, T, 2 * group, 64) and lse.shape == (0, T, 2 * group)
+    assert mxb.paged_attention(q[:, :0], c, table, n, tree_mask=mask[:, :0, :0]).shape == (2, 0, 2 * group, 64)
+    o, lse = mxb.paged_attention(q, c, table[:, :0], n * 0, return_lse=True, tree_mask=mask)  # no pages
+    assert not o.any() and bool((lse == float("-inf")).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("prefix", [0, 40])
 def test_more_sequences_than_a_warp_adds_up(prefix):
     """The list of tiles of more than 512 sequences, one of them long."""
