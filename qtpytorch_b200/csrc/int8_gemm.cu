@@ -92,6 +92,17 @@ __device__ __forceinline__ int4 ld_cluster_i4(uint32_t saddr, uint32_t rank) {
   return v;
 }
 
+// N columns of the accumulator.  A half of a 16- or 32-token tile is 8 or 16 columns of the
+// 32 allocated: 32 at once would read past them.
+template <int N>
+__device__ __forceinline__ void acc_ld(uint32_t taddr, uint32_t (&r)[N]) {
+  if constexpr (N == 8) tmem_ld8(taddr, r);
+  else if constexpr (N == 16) tmem_ld16(taddr, r);
+  else tmem_ld32(taddr, r);
+  tmem_wait_ld();
+  tmem_landed(r);
+}
+
 template <int NT, typename OutT>
 __global__ void __launch_bounds__(kThreads, 2)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_f,
@@ -174,6 +185,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   const bool epi = warp >= 2;
   const int q = warp & 3, half = (warp - 2) >> 2;  // TMEM lane quarter, column half
   constexpr int kPer = NT >= 64 ? 32 : NT / 2;     // columns per tcgen05.ld
+  constexpr int kLoads = NT >= 64 ? NT / 64 : 1;   // of them a half
+  static_assert(NT / 2 + kLoads * kPer <= kAcc, "columns outside the allocation");
   OutT* out = static_cast<OutT*>(a.out);
   if (a.splits == 1) {
     if (epi && mbar_wait_warp_to(&bars->acc, 0, kErrTimeoutDone, a.err)) {
@@ -182,13 +195,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       const float sf = n < a.N ? a.sf[(int64_t)n * a.sf_step] : 0.0f;
       const float bv = a.bias && n < a.N ? a.bias[n] : 0.0f;
 #pragma unroll
-      for (int cb = 0; cb < (NT >= 64 ? NT / 64 : 1); ++cb) {
+      for (int cb = 0; cb < kLoads; ++cb) {
         const int c0 = half * (NT / 2) + cb * kPer;
         if (m0 + c0 >= a.M) break;
-        uint32_t r[32];
-        tmem_ld32(tbase + ((uint32_t)(q * 32) << 16) + c0, r);
-        tmem_wait_ld();
-        tmem_landed(r);
+        uint32_t r[kPer];
+        acc_ld(tbase + ((uint32_t)(q * 32) << 16) + c0, r);
         if (n < a.N) {
           OutT* o = out + (size_t)(m0 + c0) * a.N + n;
           const float* st = a.st + (int64_t)(m0 + c0) * a.st_step;
@@ -205,13 +216,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (epi && nk > 0 && mbar_wait_warp_to(&bars->acc, 0, kErrTimeoutDone, a.err)) {
       tc_fence_after();
 #pragma unroll
-      for (int cb = 0; cb < (NT >= 64 ? NT / 64 : 1); ++cb) {
+      for (int cb = 0; cb < kLoads; ++cb) {
         const int c0 = half * (NT / 2) + cb * kPer;
         if (m0 + c0 >= a.M) break;
-        uint32_t r[32];
-        tmem_ld32(tbase + ((uint32_t)(q * 32) << 16) + c0, r);
-        tmem_wait_ld();
-        tmem_landed(r);
+        uint32_t r[kPer];
+        acc_ld(tbase + ((uint32_t)(q * 32) << 16) + c0, r);
 #pragma unroll
         for (int j = 0; j < kPer; ++j) part[(c0 + j) * BM + q * 32 + lane] = (int)r[j];
       }

@@ -473,3 +473,28 @@ def test_norm_into_linear():
     # the scale is off by 2^-19, the roundings of the product are three of 2^-24 and one of 2^-8
     assert bool(((y.double() - ref).abs() <= (2.0 ** -8 + 2.0 ** -18) * ref.abs()).all())
     assert torch.equal(h2, x + h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k,n", [(9, 128, 128), (16, 4096, 384), (17, 96, 640), (25, 8192, 256), (32, 256, 40000),
+                                   (12, 2048, 19000)])
+def test_product_of_narrow_tiles_beside_others(out, m, k, n):
+    """Tiles of 16 and 32 tokens, with and without splits, while other products hold
+    accumulators on the same SMs."""
+    a, b = operand(m, k, 1), operand(n, k, 2, full=True)
+    c, e = operand(100, 1024, 3), operand(900, 1024, 4)
+    want, want2 = product_ref(a, b, None, out), product_ref(c, e, None, out)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    ys, zs = [], []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(8):
+        for s in streams[:2]:
+            with torch.cuda.stream(s):
+                ys.append(mxb.int8_matmul(a, b, out_dtype=out))
+        with torch.cuda.stream(streams[2]):
+            zs.append(mxb.int8_matmul(c, e, out_dtype=out))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in ys) and all(torch.equal(z, want2) for z in zs)
+    assert L.load().mxb_device_error(1) == 0
