@@ -32,23 +32,15 @@ from .dtypes import get_mx_dtype, mx_dtype, optimal_output_dtype
 _STRICT = os.environ.get("MX_STRICT", "0") == "1"
 
 
-_placeholders: dict = {}
-
-
 def _placeholder(packed: torch.Tensor) -> torch.Tensor:
     """What stands behind the wrapper itself: an fp32 scalar that nothing reads or
-    writes, one a device.  Inference and fake tensors get one of their own kind."""
-    device = packed.device
-    if type(packed) is not torch.Tensor or packed.is_inference():
-        return torch.empty((), dtype=torch.float32, device=device)
-    t = _placeholders.get(device)
-    if t is None:
+    writes, each wrapper's own (a shared one ties their version counters together, and
+    stays a fake or a dead functorch tensor where the first was made under such a mode).
+    An inference tensor where the codes are one."""
+    if torch.is_inference_mode_enabled() and not packed.is_inference():
         with torch.inference_mode(False):
-            t = torch.empty((), dtype=torch.float32, device=device)
-        # a capture's allocations belong to its graph
-        if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
-            _placeholders[device] = t
-    return t
+            return torch.empty((), dtype=torch.float32, device=packed.device)
+    return torch.empty((), dtype=torch.float32, device=packed.device)
 
 
 class mx_tensor(torch.Tensor):

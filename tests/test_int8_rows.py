@@ -6,6 +6,9 @@ for equality; the reference's counterpart of the product is ``fused_int8_linear`
 import copy
 import ctypes
 import io
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -498,3 +501,67 @@ def test_product_of_narrow_tiles_beside_others(out, m, k, n):
     torch.cuda.synchronize()
     assert all(torch.equal(y, want) for y in ys) and all(torch.equal(z, want2) for z in zs)
     assert L.load().mxb_device_error(1) == 0
+
+
+def plain_use(t):
+    """Of the wrapper itself."""
+    with torch._C.DisableTorchFunctionSubclass():
+        return t.detach().untyped_storage().data_ptr(), t._version
+
+
+@pytest.mark.parametrize("mode", ["fake", "grad", "jvp", "functionalize"])
+def test_first_codes_made_under_a_mode_leave_later_ones_usable(mode):
+    code = """if True:
+    import sys, torch
+    import qtpytorch_b200 as mxb
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    codes, scales = torch.zeros(16, dtype=torch.int8), torch.ones(2)
+    def make():
+        return mxb.mx_tensor(codes, scales, mxb.int8d, (2, 8), 16, 8)
+    def inside(x):
+        make()
+        return x.sum()
+    def fake(x):
+        with FakeTensorMode():
+            try:
+                make()
+            except RuntimeError:  # real codes have no wrapper there
+                pass
+    modes = dict(fake=fake, grad=torch.func.grad(inside), functionalize=torch.func.functionalize(inside),
+                 jvp=lambda x: torch.func.jvp(inside, (x,), (x,)))
+    modes[sys.argv[1]](torch.ones(3))
+    t = make()
+    with torch._C.DisableTorchFunctionSubclass():
+        t = t.detach()
+        assert not torch._is_functional_tensor(t)
+        t.untyped_storage().data_ptr()
+    """
+    subprocess.run([sys.executable, "-W", "ignore", "-c", code, mode], check=True, timeout=300,
+                   cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+
+def test_wrappers_share_neither_memory_nor_versions():
+    a, b = fake(2, 8), fake(2, 8)
+    assert plain_use(a)[0] != plain_use(b)[0]
+    with torch._C.DisableTorchFunctionSubclass():
+        a.zero_()
+    assert plain_use(a)[1] == 1 and plain_use(b)[1] == 0
+
+    class keep(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w):
+            ctx.save_for_backward(w)
+            return 2 * x
+
+        @staticmethod
+        def backward(ctx, g):
+            assert ctx.saved_tensors[0].shape == (2, 8)
+            return 2 * g, None
+
+    x = torch.ones(2, requires_grad=True)
+    y = keep.apply(x, b)
+    with torch._C.DisableTorchFunctionSubclass():
+        a.zero_()
+    y.sum().backward()
+    assert torch.equal(x.grad, torch.full((2,), 2.0))
