@@ -27,6 +27,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import _lib as L
 from . import int8, ops
 from .dtypes import get_mx_dtype, mx_dtype
 from .tensor import mx_tensor
@@ -104,6 +105,7 @@ def fused_int8_linear(x: mx_tensor, weight: mx_tensor, bias: Optional[torch.Tens
         sw = _kblock_scales(weight, N, K, kb)
         if xd.bits == 8 and kb == K and K <= int8.MAX_K and x.device == weight.device:
             # one scale a token and a channel: the same sums and roundings, not cut into K-blocks
+            L.require_cuda(x._mx_packed, "fused_int8_linear")
             out = torch.empty(M, N, dtype=torch.float32, device=x._mx_packed.device)
             int8._product((x._mx_packed.contiguous(), sx, 1), (weight._mx_packed.contiguous(), sw, 1), M, K, N,
                           None, out)

@@ -565,3 +565,9 @@ def test_wrappers_share_neither_memory_nor_versions():
         a.zero_()
     y.sum().backward()
     assert torch.equal(x.grad, torch.full((2,), 2.0))
+
+
+def test_fused_int8_linear_refuses_the_cpu():
+    for block in (None, 4):  # a scale a row, and blocks of K
+        with pytest.raises(L.MxbError):
+            mxb.fused_int8_linear(fake(2, 8, block), fake(3, 8, block))
