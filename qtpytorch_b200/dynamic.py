@@ -106,7 +106,9 @@ def fused_int8_linear(x: mx_tensor, weight: mx_tensor, bias: Optional[torch.Tens
         if xd.bits == 8 and kb == K and K <= int8.MAX_K and x.device == weight.device:
             # one scale a token and a channel: the same sums and roundings, not cut into K-blocks
             L.require_cuda(x._mx_packed, "fused_int8_linear")
-            out = torch.empty(M, N, dtype=torch.float32, device=x._mx_packed.device)
+            dev = x._mx_packed.device
+            sx, sw = sx.to(dev), sw.to(dev)
+            out = torch.empty(M, N, dtype=torch.float32, device=dev)
             int8._product((x._mx_packed.contiguous(), sx, 1), (weight._mx_packed.contiguous(), sw, 1), M, K, N,
                           None, out)
         else:

@@ -571,3 +571,12 @@ def test_fused_int8_linear_refuses_the_cpu():
     for block in (None, 4):  # a scale a row, and blocks of K
         with pytest.raises(L.MxbError):
             mxb.fused_int8_linear(fake(2, 8, block), fake(3, 8, block))
+
+
+@pytest.mark.gpu
+def test_fused_int8_linear_takes_scales_from_the_host():
+    a, b = operand(5, 96, 1), operand(7, 96, 2)
+    want = product_ref(a, b, None, torch.float32)
+    for p, q in ((a, mxb.mx_tensor(b.packed, b.mx_scales.cpu(), mxb.int8d, (7, 96), 672, 96)),
+                 (mxb.mx_tensor(a.packed, a.mx_scales.cpu(), mxb.int8d, (5, 96), 480, 96), b)):
+        assert torch.equal(mxb.fused_int8_linear(p, q), want)
