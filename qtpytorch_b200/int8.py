@@ -97,7 +97,11 @@ def _operand(t: mx_tensor, K: int, what: str) -> Tuple[torch.Tensor, torch.Tenso
     if not (dt.is_int and dt.bits == 8 and dt.variant == ""):
         raise NotImplementedError(f"{what} takes int8 codes, not {dt.name}")
     codes, scales = t._mx_packed, t._mx_scales
-    rows = t._mx_n // K if K else 0
+    n = t._mx_orig_shape.numel()
+    if t._mx_n != n or codes.numel() * codes.element_size() < n or scales.device != codes.device:
+        raise ValueError(f"{what} takes whole tensors: {n} codes for {tuple(t._mx_orig_shape)} and their scales on one "
+                         f"device, got {codes.numel()} on {codes.device} (n = {t._mx_n}) and scales on {scales.device}")
+    rows = n // K if K else 0
     if t._mx_block == K and scales.numel() == rows:
         step = 1
     elif scales.numel() == 1:

@@ -573,6 +573,23 @@ def test_fused_int8_linear_refuses_the_cpu():
             mxb.fused_int8_linear(fake(2, 8, block), fake(3, 8, block))
 
 
+def test_operands_that_are_not_whole_are_refused():
+    """Before any device is looked at: their addresses would go to a kernel as they are."""
+    codes, ones = torch.zeros(24, dtype=torch.int8), torch.ones(3)
+    good = fake(3, 8)
+    for bad in (mxb.mx_tensor(codes, ones.to("meta"), mxb.int8d, (3, 8), 24, 8),  # scales elsewhere
+                mxb.mx_tensor(codes[:23], ones, mxb.int8d, (3, 8), 24, 8),        # a code short
+                mxb.mx_tensor(codes, ones, mxb.int8d, (6, 8), 24, 8),             # another shape
+                mxb.mx_tensor(codes, ones[:1], mxb.int8d, (3, 8), 48, 48)):
+        for a, b in ((good, bad), (bad, good)):
+            with pytest.raises(ValueError):
+                mxb.int8_matmul(a, b)
+        with pytest.raises(ValueError):
+            mxb.int8_linear(bad)
+        with pytest.raises(ValueError):
+            mxb.int8_linear(good)(bad)
+
+
 @pytest.mark.gpu
 def test_fused_int8_linear_takes_scales_from_the_host():
     a, b = operand(5, 96, 1), operand(7, 96, 2)
