@@ -1188,7 +1188,8 @@ int attention(const void* q, int64_t B, int64_t T, int heads, int group, int dim
   if ((int64_t)p.tiles_own * heads > 65535 || (int64_t)p.tiles_pre * heads > 65535 ||
       (p.splits_pre > 0 && p.nt_pre == 0 && cdiv(pre_rows, prefix_rows_per_cta(pre_rows)) > 65535) ||
       B * heads * p.tiles_own > INT32_MAX || B * T * heads * group > INT32_MAX ||
-      (int64_t)heads * p.tiles_own * (width * page / p.tile_own + 1) > INT32_MAX)
+      (int64_t)heads * p.tiles_own * (width * page / p.tile_own + 1) > INT32_MAX ||
+      (p.tensor && width * page > INT32_MAX - 4 * kTreeKeys))  // its positions are 32 bits, a tile further
     return MXB_E_SHAPE;
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return MXB_E_WORKSPACE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -29,6 +29,21 @@ def test_argument_errors_need_no_gpu():
     assert attend(B=0) == 0 and attend(T=0) == 0 and attend(B=0, mask=None) == 0
 
 
+def test_histories_that_32_bit_positions_do_not_hold_are_refused():
+    """A length within a tile of 2^31 wraps where it is rounded up to tiles of 128 keys.
+    Shapes are looked at before the workspace, so that no call gets further than that."""
+    lib, p = L.load(), ctypes.c_void_p(32)
+
+    def attend(T, group, keys, page=16):
+        return lib.mxb_tree_attention(p, 1, T, 2, group, 128, p, p, p, p, 4, page, 8, p, keys // page, p, None, 0, 0,
+                                      p, T * T, T, 0.1, p, None, None, 0, None)
+
+    most = 2 ** 31 - 1 - 512
+    assert attend(64, 4, 2 ** 31 - 80) == -1 and attend(64, 1, most + 16) == -1
+    assert attend(64, 4, most) == -7 and attend(64, 4, most, 1024) == -7
+    assert attend(3, 4, 2 ** 31 - 80) == -7 and attend(3, 4, 2 ** 31 - 64) == -1  # few rows: tiles of 32
+
+
 @pytest.mark.gpu
 def test_refusals_on_the_device():
     c = mxb.paged_kv_cache(4, 2, 64, "int8d", 16)
