@@ -534,7 +534,8 @@ int mxb_kv_append(const void* q, const void* k, const void* v, int x_dtype, int6
 /*
  * Root-mean-square norm of rows into int8 codes: h = x (+ residual), y = h * weight
  * / sqrt(mean(h^2) + eps), scale = max(amax|y|, 1e-12) / 127, code = y / scale
- * rounded to the nearest, ties to even, as exact arithmetic gives it (a row with an
+ * rounded to the nearest, ties to even, as 64 bits give it: rint(127 u / amax|u|) with
+ * h, u = h * weight, 127 u and the quotient each rounded to a double (a row with an
  * infinity or NaN: codes 0, scale NaN).
  *   x, residual  [rows][d] of x_dtype, rows x_stride / residual_stride apart;
  *                residual may be NULL

@@ -8,11 +8,12 @@
 // of squares and its largest u are found in the same pass and the codes need one
 // reduction, not two.
 //
-// The codes are the ones of exact arithmetic.  The fp32 quotient is off by less
-// than 127 * 2^-22 (h, u and the factor 127 / amax are rounded once each, as is
-// their product); where it comes within twice that of a border between two codes
-// it is found again in 64 bits from x, r and w, whose sums and products 64 bits
-// hold.  That meets 1 value in 8000.  The largest u is found in 64 bits too, among
+// The codes are the ones of this formula in 64 bits.  The fp32 quotient is off by at
+// most 127 * 5 * 2^-24 (h, u, amax, the factor 127 / amax and the product with it are
+// rounded once each); where it comes within 127 * 2^-21 of a border between two codes
+// it is found again in 64 bits from x, r and w.  There h, u and 127 u are rounded to 53
+// bits, which hold them unless the terms lie far apart (0.5 + 2^-60 of a largest 127
+// is a tie).  That meets 1 value in 8000.  The largest u is found in 64 bits too, among
 // those within 2^-21 of the fp32 one.  Rows that hold infinities or NaN, or whose
 // values leave the range in which all this holds, take a slow path in 64 bits.
 //

@@ -44,9 +44,10 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: Optional[
         h = x + residual,  y = h * weight / sqrt(mean(h^2) + eps)
 
     with scale = max(amax|y|, 1e-12) / 127 and code = y / scale to the nearest, ties
-    to even, as exact arithmetic gives it.  x and residual fp32 or bf16 as they are
-    (other and mixed types through fp32), weight [d] likewise.  With ``residual``
-    returns (codes, h), h in x's type.  A row with an infinity or NaN has codes of 0
+    to even, as 64 bits give it: 127 u / amax|u| of u = h * weight, each step rounded to
+    a double (a quotient that lies closer to a tie than that is taken for one).  x and
+    residual fp32 or bf16 as they are (other and mixed types through fp32), weight [d]
+    likewise.  With ``residual`` returns (codes, h), h in x's type.  A row with an infinity or NaN has codes of 0
     and a scale of NaN.  No gradient."""
     L.require_cuda(x, "rms_norm_quantize")
     if x.dim() < 1:

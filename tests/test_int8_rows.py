@@ -597,3 +597,18 @@ def test_fused_int8_linear_takes_scales_from_the_host():
     for p, q in ((a, mxb.mx_tensor(b.packed, b.mx_scales.cpu(), mxb.int8d, (7, 96), 672, 96)),
                  (mxb.mx_tensor(a.packed, a.mx_scales.cpu(), mxb.int8d, (5, 96), 480, 96), b)):
         assert torch.equal(mxb.fused_int8_linear(p, q), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 2048, 40000])
+def test_norm_codes_are_those_of_64_bits(d):
+    """A residual too small for a double's sum makes a tie, as the documentation says; one
+    that it holds does not."""
+    x = torch.zeros(3, d, device="cuda")
+    x[:, 0], x[:, 1], x[:, 2] = 127.0, 0.5, 2.5
+    r = torch.zeros_like(x)
+    r[0, 1:3], r[1, 1:3] = 2.0 ** -60, 2.0 ** -40
+    for t in (torch.float32, torch.bfloat16):
+        q, _ = mxb.rms_norm_quantize(x.to(t), torch.ones(d, device="cuda", dtype=t), residual=r.to(t))
+        assert q.packed.view(3, d)[:, :3].tolist() == [[127, 0, 2], [127, 1, 3], [127, 0, 2]]
+        check_norm(x.to(t), torch.ones(d, device="cuda", dtype=t), r.to(t))
