@@ -552,8 +552,9 @@ int mxb_rms_norm_quantize(const void* x, const void* residual, int x_dtype, int6
 size_t mxb_int8_matmul_workspace_size(int64_t M, int64_t K, int64_t N, int aligned);
 
 /*
- * C[m][n] = fl(fl(P sa[m]) sb[n]) (+ bias[n]), P the exact integer product of int8
- * codes a [M][K] and b [N][K], K at most 131071.
+ * C[m][n] = fl(fl(fl(fl(P) sa[m]) sb[n]) + bias[n]), then rounded to the output's
+ * type: fl rounds to fp32 (P past 2^24 too), P is the exact integer product of int8
+ * codes a [M][K] and b [N][K], K at most 131071.  Without a bias 0 is added (no -0).
  *   a_scales, b_scales  fp32, one a row (step 1) or one for all (step 0)
  *   bias                fp32 [N] or NULL
  *   out                 [M][N] MXB_F32 or MXB_BF16

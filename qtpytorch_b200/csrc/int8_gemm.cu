@@ -3,9 +3,9 @@
 //   C[m, n] = sa[m] sb[n] sum_k a[m, k] b[n, k] (+ bias[n])
 //
 // The sum is the tensor core's exact int32 (kind::i8), so neither the split of K
-// nor the tiles change a result; the epilogue rounds fl(fl(P sa) sb), the order of
-// the framework's other integer products, then adds the bias and rounds to the
-// output's type.
+// nor the tiles change a result; the epilogue rounds fl(fl(fl(P) sa) sb) to fp32 step by
+// step, the order of the framework's other integer products, then adds the bias
+// (rounded to fp32 as well) and rounds to the output's type.
 #include "mxb_common.cuh"
 #include "mxb_internal.h"
 

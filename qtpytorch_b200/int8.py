@@ -135,8 +135,9 @@ def _product(a, b, M: int, K: int, N: int, bias: Optional[torch.Tensor], out: to
 def int8_matmul(a: mx_tensor, b: mx_tensor, bias: Optional[torch.Tensor] = None,
                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """a [..., K] @ b [N, K]^T (+ bias [N]) of int8 codes with one scale a row (or one
-    for all): the exact integer sum, times a's scale, times b's, each rounded to fp32,
-    then the bias, rounded once to ``out_dtype`` (bf16 or fp32).  K at most 131071.  No
+    for all): the exact integer sum, times a's scale, times b's, plus the bias, each step
+    (the sum itself past 2^24, too) rounded to fp32, the result to ``out_dtype`` (bf16 or
+    fp32).  K at most 131071.  No
     gradient."""
     if not isinstance(a, mx_tensor) or not isinstance(b, mx_tensor):
         raise TypeError("int8_matmul takes two mx_tensors")

@@ -612,3 +612,28 @@ def test_norm_codes_are_those_of_64_bits(d):
         q, _ = mxb.rms_norm_quantize(x.to(t), torch.ones(d, device="cuda", dtype=t), residual=r.to(t))
         assert q.packed.view(3, d)[:, :3].tolist() == [[127, 0, 2], [127, 1, 3], [127, 0, 2]]
         check_norm(x.to(t), torch.ones(d, device="cuda", dtype=t), r.to(t))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(3, 40), (300, 128), (2048, 2048)])
+def test_product_rounds_sums_past_24_bits(m, n):
+    """Each step of the documented formula by itself, P = 2^24 + 3 among the sums."""
+    k = 4096
+    code = torch.zeros(k, dtype=torch.int8, device="cuda")
+    code[:2047] = 127
+    p = int((code.long() ** 2).sum())  # under 2^25, and no multiple of 2
+    a = code.repeat(m, 1)
+    a[1:, 2047:] = torch.randint(-127, 128, (m - 1, k - 2047), generator=torch.Generator().manual_seed(3)).to(a)
+    b = code.repeat(n, 1)
+    b[:, 4095] = torch.arange(n) % 100
+    sa, sb = (0.1 + torch.rand(x, generator=torch.Generator().manual_seed(x)).cuda() for x in (m, n))
+    assert p > 1 << 24 and p % 2 == 1
+    bias = torch.linspace(-3, 3, n, device="cuda")
+    qa, qb = (mxb.mx_tensor(t.reshape(-1), s, mxb.int8d, t.shape, t.numel(), k) for t, s in ((a, sa), (b, sb)))
+    y = mxb.int8_matmul(qa, qb, bias=bias, out_dtype=torch.float32)
+    exact = torch.mm(a.double(), b.double().t())
+    one = exact.to(torch.float32)
+    assert bool((one.double() != exact).any())
+    two = (one.double() * sa.double()[:, None]).to(torch.float32)
+    three = (two.double() * sb.double()).to(torch.float32)
+    assert torch.equal(y, (three.double() + bias.double()).to(torch.float32))
