@@ -617,7 +617,12 @@ struct Cut {
 // pair's 256 x 256 tile 0.38; 6 or 8 around them, 4.5 to join splits, which have to win by
 // a fifth.  E.g. (auto / the other kernels' best): 160 x 4096 x 11008 18.8 / 22.5, 256 x
 // 11008 x 4096 23.4 / 28.8, 700 x 4096 x 11008 32.9 / 39.4, 2000 x 2048 x 2048 14.5 /
-// 16.4.  Splits stop at 256 CTAs: clusters of more do not all fit at once.
+// 16.4.
+//
+// Clusters have to fit all at once: one too many starts when the first ones have gone (1 x
+// 4096 x 4736, weights from HBM: 37 clusters of 8 11.2 us, of 6 7.7).  Two CTAs an SM, the
+// SMs of a cluster in one GPC: 148 clusters of 2 fit, 91 of 3, 71, 55, 45, 37 and 33 of 4
+// to 8 (90 of 3 11.7 us, of 2 12.5; 96 of 3 17.2).  So threes stop at 270 CTAs, more at 256.
 Cut cut_of(int64_t M, int64_t N, int64_t ksteps, bool pairs) {
   const int64_t ft = cdiv(N, BM);
   if (M <= 64) {
@@ -626,6 +631,7 @@ Cut cut_of(int64_t M, int64_t N, int64_t ksteps, bool pairs) {
     if (splits > ksteps / 2) splits = ksteps / 2;
     if (splits > kMaxSplit) splits = kMaxSplit;
     while (splits * splits > 2 * ksteps) --splits;
+    while (splits > 2 && ft * splits > (splits == 3 ? 270 : 256)) --splits;
     return {nt, (int)(splits < 1 ? 1 : splits)};
   }
   Cut best = {0, 1};

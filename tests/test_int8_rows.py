@@ -637,3 +637,11 @@ def test_product_rounds_sums_past_24_bits(m, n):
     two = (one.double() * sa.double()[:, None]).to(torch.float32)
     three = (two.double() * sb.double()).to(torch.float32)
     assert torch.equal(y, (three.double() + bias.double()).to(torch.float32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 4736), (30, 4000, 4700), (64, 8192, 4992), (2, 4096, 11520), (7, 4096, 11648),
+                                   (1, 4096, 4224), (20, 4096, 7000), (1, 2048, 18944)])
+def test_product_of_as_many_splits_as_clusters_fit(m, k, n):
+    a, b = operand(m, k, 1), operand(n, k, 2, full=True)
+    assert torch.equal(mxb.int8_matmul(a, b), product_ref(a, b, None, torch.bfloat16))
