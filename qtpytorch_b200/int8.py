@@ -20,7 +20,7 @@ import torch.nn as nn
 
 from . import _lib as L
 from .dtypes import get_mx_dtype
-from .tensor import mx_tensor
+from .tensor import mx_tensor, plain
 
 _IO = {torch.float32: L.F32, torch.bfloat16: L.BF16}
 _INT8 = get_mx_dtype("int8d")
@@ -49,6 +49,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: Optional[
     residual fp32 or bf16 as they are (other and mixed types through fp32), weight [d]
     likewise.  With ``residual`` returns (codes, h), h in x's type.  A row with an infinity or NaN has codes of 0
     and a scale of NaN.  No gradient."""
+    x, weight, residual = plain(x), plain(weight), plain(residual)
     L.require_cuda(x, "rms_norm_quantize")
     if x.dim() < 1:
         raise ValueError("rms_norm_quantize: x needs at least one dim")
@@ -162,6 +163,7 @@ def int8_matmul(a: mx_tensor, b: mx_tensor, bias: Optional[torch.Tensor] = None,
 def _bias(bias: Optional[torch.Tensor], N: int, dev: torch.device, what: str) -> Optional[torch.Tensor]:
     if bias is None:
         return None
+    bias = plain(bias)
     if bias.shape != (N,) or bias.device != dev:
         raise ValueError(f"{what}: bias must be [{N}] on {dev}")
     return bias if bias.dtype == torch.float32 and bias.is_contiguous() else bias.float().contiguous()

@@ -191,6 +191,12 @@ def _device_arg(args, kwargs):
     return None
 
 
+def plain(t):
+    """A tensor whose memory holds its values: a quantized one is dequantized (its own
+    ``data_ptr`` and ``stride`` are those of a copy that is gone when they return)."""
+    return t.dequantize() if isinstance(t, mx_tensor) else t
+
+
 def _rebuild_mx(packed, scales, dtype_name, shape, n, block):
     return mx_tensor(packed, scales, get_mx_dtype(dtype_name), shape, n, block)
 

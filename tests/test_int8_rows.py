@@ -645,3 +645,15 @@ def test_product_rounds_sums_past_24_bits(m, n):
 def test_product_of_as_many_splits_as_clusters_fit(m, k, n):
     a, b = operand(m, k, 1), operand(n, k, 2, full=True)
     assert torch.equal(mxb.int8_matmul(a, b), product_ref(a, b, None, torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_quantized_tensors_are_taken_by_their_values():
+    x, r, w, bias = (mxb.mx_tensor.quantize(rows(i, *s), "int8d", 64)
+                     for i, s in enumerate([(40, 512), (40, 512), (512,), (24,)]))
+    got, h = mxb.rms_norm_quantize(x, w, residual=r)
+    want, h2 = mxb.rms_norm_quantize(x.dequantize(), w.dequantize(), residual=r.dequantize())
+    assert torch.equal(got.packed, want.packed) and torch.equal(got.mx_scales, want.mx_scales) and torch.equal(h, h2)
+    a, b = operand(5, 64, 1), operand(24, 64, 2)
+    assert torch.equal(mxb.int8_matmul(a, b, bias=bias), mxb.int8_matmul(a, b, bias=bias.dequantize()))
+    assert torch.equal(mxb.int8_linear(b, bias)(a), mxb.int8_matmul(a, b, bias=bias.dequantize()))
