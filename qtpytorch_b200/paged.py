@@ -26,6 +26,7 @@ import torch
 
 from . import _lib as L
 from .dtypes import get_mx_dtype, mx_dtype
+from .tensor import plain
 
 _IO = {torch.float32: L.F32, torch.bfloat16: L.BF16}
 
@@ -106,6 +107,7 @@ class paged_kv_cache:
         head strides) into ``slots`` [T]; a negative slot skips its token.
         The slots of one call must be distinct."""
         dev = self._cuda("paged_kv_cache.write")
+        k, v = plain(k), plain(v)
         H, D = self.n_heads, self.head_dim
         if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (H, D) or slots.shape != k.shape[:1]:
             raise ValueError(f"write: k and v must be [T, {H}, {D}] and slots [T]; got "
@@ -141,6 +143,7 @@ class paged_kv_cache:
         skipped tokens are rotated too.  Slots of one call must be distinct.  No
         gradient."""
         dev = self._cuda("paged_kv_cache.append")
+        k, v, q, inv_freq = plain(k), plain(v), plain(q), plain(inv_freq)
         H, D = self.n_heads, self.head_dim
         if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (H, D) or slots.shape != k.shape[:1]:
             raise ValueError(f"append: k and v must be [T, {H}, {D}] and slots [T]; got "

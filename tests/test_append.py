@@ -231,3 +231,21 @@ def test_append_on_another_stream_and_in_a_graph():
         got = e.append(k, v, slots, pos, f, q=q)
     graph.replay()
     assert same(c, e) and torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_quantized_keys_values_and_queries_are_taken_by_their_values():
+    """Outputs of the packed product are such tensors."""
+    g = torch.Generator("cuda").manual_seed(0)
+    q, k, v = (mxb.mx_tensor.quantize(torch.randn(20, n, 64, generator=g, device="cuda"), "int8d", 64)
+               for n in (4, 2, 2))
+    slots, pos = torch.arange(20, device="cuda"), torch.arange(20, device="cuda") + 5
+    freq = 10000.0 ** (-torch.arange(32, device="cuda") / 32)
+    made = []
+    for f in (lambda t: t, lambda t: t.dequantize()):
+        c = mxb.paged_kv_cache(2, 2, 64, "int8d", 16)
+        out = c.append(f(k), f(v), slots, pos, freq, q=f(q))
+        d = mxb.paged_kv_cache(2, 2, 64, "int8d", 16)
+        d.write(f(k), f(v), slots)
+        made.append((out, c.k_codes, c.k_scales, c.v_codes, c.v_scales, d.k_codes, d.v_codes))
+    assert all(torch.equal(x, y) for x, y in zip(*made))
