@@ -541,7 +541,8 @@ int mxb_kv_append(const void* q, const void* k, const void* v, int x_dtype, int6
  *                residual may be NULL
  *   weight       [d] of w_dtype (MXB_F32 / MXB_BF16)
  *   codes        int8 [rows][d], scales fp32 [rows]
- *   sum          [rows][d] of x_dtype, h rounded, or NULL; not over x or residual
+ *   sum          [rows][d] of x_dtype, h rounded, or NULL
+ * No output lies over an input.
  */
 int mxb_rms_norm_quantize(const void* x, const void* residual, int x_dtype, int64_t rows, int64_t d,
                           int64_t x_stride, int64_t residual_stride, const void* weight, int w_dtype,

@@ -445,13 +445,19 @@ extern "C" int mxb_rms_norm_quantize(const void* x, const void* residual, int x_
   if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)sum) % xa || (uintptr_t)weight % wa ||
       (uintptr_t)scales % 4)
     return MXB_E_ALIGN;
-  // x and the residual are read again after the sum is written
-  auto meets = [&](const void* p, int64_t stride) {
-    const uintptr_t lo = (uintptr_t)p, hi = lo + (uintptr_t)((rows - 1) * stride + d) * xa;
-    return p && sum && lo < (uintptr_t)sum + (uintptr_t)(rows * d) * xa && (uintptr_t)sum < hi;
-  };
   if (x_stride < 0 || residual_stride < 0) return MXB_E_SHAPE;
-  if (meets(x, x_stride) || meets(residual, residual_stride)) return MXB_E_ARG;
+  // the inputs are read again after codes and sum are written
+  auto meets = [&](const void* p, int64_t n, uintptr_t size) {
+    const uintptr_t lo = (uintptr_t)p, hi = lo + (uintptr_t)n * size;
+    auto over = [&](const void* out, uintptr_t bytes) {
+      return p && out && lo < (uintptr_t)out + bytes && (uintptr_t)out < hi;
+    };
+    return over(sum, (uintptr_t)(rows * d) * xa) || over(codes, (uintptr_t)(rows * d)) ||
+           over(scales, (uintptr_t)rows * 4);
+  };
+  if (meets(x, (rows - 1) * x_stride + d, xa) || meets(residual, (rows - 1) * residual_stride + d, xa) ||
+      meets(weight, d, wa))
+    return MXB_E_ARG;
   const NormArgs a = {x, residual, weight, rows, d, x_stride, residual_stride, eps, static_cast<int8_t*>(codes),
                       scales, sum};
   cudaStream_t st = static_cast<cudaStream_t>(stream);

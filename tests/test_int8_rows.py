@@ -657,3 +657,18 @@ def test_quantized_tensors_are_taken_by_their_values():
     a, b = operand(5, 64, 1), operand(24, 64, 2)
     assert torch.equal(mxb.int8_matmul(a, b, bias=bias), mxb.int8_matmul(a, b, bias=bias.dequantize()))
     assert torch.equal(mxb.int8_linear(b, bias)(a), mxb.int8_matmul(a, b, bias=bias.dequantize()))
+
+
+def test_norm_outputs_over_its_inputs_are_refused():
+    """Values next to a border are read again after the codes are written."""
+    lib = L.load()
+
+    def norm(x, r, w, codes, scales, h, rows=2, d=64):
+        x, r, w, codes, scales, h = (ctypes.c_void_p(p) if p else None for p in (x, r, w, codes, scales, h))
+        return lib.mxb_rms_norm_quantize(x, r, 1, rows, d, 64, 64, w, 1, 1e-6, codes, scales, h, None)
+
+    # x, residual: 256 bytes each; weight 128; codes 128, scales 8, sum 256
+    at = dict(x=0x1000, r=0x2000, w=0x3000, codes=0x4000, scales=0x5000, h=0x6000)
+    for over in (dict(codes=0x1000), dict(codes=0x10ff), dict(codes=0x0f81), dict(codes=0x2000), dict(codes=0x307f),
+                 dict(scales=0x10fc), dict(scales=0x1ffc), dict(scales=0x3000), dict(h=0x2f02), dict(h=0x20fe)):
+        assert norm(**{**at, **over}) == -6, over
