@@ -51,8 +51,9 @@ __device__ __forceinline__ float scaled(int p, float st, float sf, float bias) {
 // MMA of N = 16, and a warp of the epilogue holds 32 adjacent features of a token,
 // which leave as one run.  One CTA owns a 128 x NT tile or, with split K, one of
 // `splits` ranges of it; those CTAs form a cluster and add their partial tiles
-// over distributed shared memory.  1 token, 4096 -> 11008 (45 MB): 11.5 us a call, about 5
-// of them the start and the end of a launch; 77 tokens, 2000 -> 1000: 7.5 us.
+// over distributed shared memory.  1 token, 4096 -> 11008 (45 MB): 11.4 us a call in a graph
+// over the weights of ten layers = 4.0 TB/s from HBM, 8.8 over one that stays in L2; about 5
+// of them are the start and the end of a launch.  77 tokens, 2000 -> 1000: 8.4 us.
 //   warp 0     TMA producer;  warp 1  TMEM allocation and MMAs;
 //   warps 2-9  epilogue
 constexpr int BM = 128;
@@ -292,10 +293,10 @@ int launch(const CUtensorMap& tf, const CUtensorMap& tt, const Args& a, cudaStre
 //   warp 1      MMAs (the leader's);  warps 2, 3  TMEM allocation, idle;
 //   warps 4-11  epilogue: a thread a token and half of the columns; 32 tokens x 128
 //               bytes leave as one TMA store from shared memory.
-// 4096 tokens, 8192 -> 8192: 177 us cold = 3.1 POP/s (292 on 128 x 128 tiles), 206 held,
-// where the power limit holds the clock down; 2048 tokens, 4096 -> 11008: 68 and 79 us
-// (344 tiles for 74 pairs).  1024 x 8192 x 8192: 55 us, tensor pipe 61 % (128 tiles, two
-// rounds), each operand read from HBM once.
+// 4096 tokens, 8192 -> 8192: 174 us in short runs = 3.2 POP/s (292 on 128 x 128 tiles), 194
+// to 203 by box where the power limit holds the clock down; 2048 tokens, 4096 -> 11008: 65
+// and 75 to 78 us (344 tiles for 74 pairs).  1024 x 8192 x 8192: 55 to 59 us, tensor pipe
+// 61 % (128 tiles, two rounds), each operand read from HBM once.
 namespace wide {
 
 constexpr int kEpi = 8;

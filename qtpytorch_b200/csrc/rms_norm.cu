@@ -15,7 +15,8 @@
 // bits, which hold them unless the terms lie far apart (0.5 + 2^-60 of a largest 127
 // is a tie).  That meets 1 value in 8000.  The largest u is found in 64 bits too, among
 // those within 2^-21 of the fp32 one.  Rows that hold infinities or NaN, or whose
-// values leave the range in which all this holds, take a slow path in 64 bits.
+// values leave the range in which all this holds, rows of zeros among them, take a slow
+// path in 64 bits (4096 x 8192 bf16 with a residual: every second row zero 155 us, all 247).
 //
 // One pass over HBM: a row stays in the registers of its block, 8 NC values a
 // thread.  What bounds it beside HBM is the issue of its instructions and the chain of a
