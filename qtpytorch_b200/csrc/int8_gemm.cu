@@ -294,7 +294,7 @@ int launch(const CUtensorMap& tf, const CUtensorMap& tt, const Args& a, cudaStre
 //   warps 4-11  epilogue: a thread a token and half of the columns; 32 tokens x 128
 //               bytes leave as one TMA store from shared memory.
 // 4096 tokens, 8192 -> 8192: 174 us in short runs = 3.2 POP/s (292 on 128 x 128 tiles), 194
-// to 203 by box where the power limit holds the clock down; 2048 tokens, 4096 -> 11008: 65
+// to 203 by machine where the power limit holds the clock down; 2048 tokens, 4096 -> 11008: 65
 // and 75 to 78 us (344 tiles for 74 pairs).  1024 x 8192 x 8192: 55 to 59 us, tensor pipe
 // 61 % (128 tiles, two rounds), each operand read from HBM once.
 namespace wide {
